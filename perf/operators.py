@@ -312,7 +312,7 @@ def plain_sample(s):
 def plain_reserve(refs, table, lens, grow, page):
     have, want = (lens + page - 1) // page, (lens + grow + page - 1) // page
     col = torch.arange(table.shape[1], device=table.device)[None]
-    fresh = (col >= have[:, None]) & (col < want[:, None])
+    fresh = (col >= have[:, None]) & (col < want[:, None]) & (table < 0)
     rank = fresh.reshape(-1).long().cumsum(0) - 1
     free = torch.sort((refs != 0).long(), stable=True)[1]
     ids = free[rank.clamp(min=0)].reshape(fresh.shape).int()
