@@ -305,7 +305,8 @@ def plain_sample(s):
     by_index = torch.zeros_like(w).scatter_(1, order, w)
     r = torch.floor(s["uniform"].double() * total.double()).long()
     token = (by_index.cumsum(1) <= r[:, None]).sum(1).clamp(max=vocab - 1)
-    prob = by_index.gather(1, token[:, None])[:, 0].float() / total.float()
+    share = torch.zeros_like(x).scatter_(1, order, e).gather(1, token[:, None])[:, 0]
+    prob = share / (total.float() * 2.0 ** -40)
     return dict(token=token.int(), prob=prob, kept=keep.sum(1).int())
 
 
