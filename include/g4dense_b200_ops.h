@@ -89,6 +89,135 @@ G4B_API int g4b_sample_token(const float* logits, int vocab, float temperature, 
 /* out4 = {N, K, grid CTAs at M=5, split-K slots per row group} */
 G4B_API int g4b_qmat_info(const g4b_qmat* q, int* out4);
 
+/* ---------------------------------------------------------------------------------------------
+ * Batched tree verification over a paged K/V cache. The reference verifies one sequence's chain of
+ * drafts over a contiguous ring (src/speculator.cpp, src/kv_cache.cpp) and has no counterpart of
+ * these; they are what a server needs to run the same round for many sequences at once, each with
+ * a tree of drafts:
+ *
+ *   g4b_tree_attention   every layer: the nodes over their sequence's pages and their ancestors
+ *   g4b_sample_rows      one token per node from its logits row and a given uniform number
+ *   g4b_tree_accept      the path along the drawn tokens
+ *   g4b_pages_reserve    pages for the accepted rows
+ *   g4b_pages_commit     the accepted nodes' K/V rows into those pages
+ *   g4b_pages_fork / _free / _compact / _copy   sharing, releasing and moving pages
+ *
+ * A round needs no host synchronization: lengths, counts and tables stay on the device. All calls
+ * are asynchronous on `stream`, allocate nothing, and can be captured in a CUDA graph. Array
+ * arguments are device memory; indices that a call finds out of range on the device are skipped,
+ * never followed. Calls that write a `status` word leave the state as it was when it is not 0. */
+
+typedef enum { G4B_BF16 = 0, G4B_FP16 = 1, G4B_FP32 = 2 } g4b_dtype;
+
+/* Attention of drafted trees. Sequence s has cu_nodes[s + 1] - cu_nodes[s] nodes (0 to max_nodes),
+ * node 0 its pending token, and lens[s] cached tokens, position j of which is row j % page_size of
+ * page table[s][j / page_size]. Node i sits at position lens[s] + depth[i] and sees every cached
+ * key and those nodes j of its own sequence whose bit (j % 32) is set in word j / 32 of its mask
+ * row; a window w > 0 hides keys w or more positions before the node. With one node per sequence
+ * this is decoding attention; with a lower-triangular mask, a chunk of a prompt.
+ *   out[i][h] = sum_j p_j v_j[h / g],  p = softmax_j(scale * q[i][h] . k_j[h / g]),  g = heads / kv_heads
+ * A node that sees no key gets zeros. Values behind a hidden key, past lens[s] in a page, or in
+ * another sequence are never used, whatever they are (NaN and infinities included). Softmax and
+ * sums are fp32; the probabilities are rounded to the cache's type before the product with V.
+ * head_dim 64, 128, 256 or 512; page_size a multiple of 8; max_nodes 1..256; dtype G4B_BF16 or
+ * G4B_FP16 for q, K, V and out alike; pointers 16-byte aligned, strides multiples of 8 elements. */
+typedef struct g4b_tree_attention_args {
+    const void* q;            /* [n_tokens][heads][head_dim] */
+    const void* k_pool;       /* [n_pages][page_size][kv_heads][head_dim] */
+    const void* v_pool;
+    const void* k_new;        /* [n_tokens][kv_heads][head_dim]: the nodes' own keys and values */
+    const void* v_new;
+    void* out;                /* [n_tokens][heads][head_dim] */
+    const int32_t* table;     /* [n_seqs][table_width] */
+    const int32_t* lens;      /* [n_seqs] */
+    const int32_t* cu_nodes;  /* [n_seqs + 1] */
+    const uint32_t* mask;     /* [n_tokens][mask_words], mask_words >= (max_nodes + 31) / 32 */
+    const int32_t* depth;     /* [n_tokens]; may be NULL when window is 0 */
+    void* workspace;          /* g4b_tree_attention_workspace() bytes, used by one stream at a time */
+    size_t workspace_bytes;
+    int64_t q_stride, out_stride, new_stride;  /* elements from one token to the next */
+    int64_t page_stride;                       /* elements from one page of a pool to the next */
+    int n_seqs, n_tokens, max_nodes, n_pages, page_size, table_width, mask_words;
+    int heads, kv_heads, head_dim, window, dtype;
+    float scale;
+} g4b_tree_attention_args;
+/* 0 when the shape is not supported. */
+G4B_API size_t g4b_tree_attention_workspace(int max_nodes, int heads, int kv_heads, int head_dim);
+G4B_API int g4b_tree_attention(const g4b_tree_attention_args* args, void* stream);
+
+/* One token per logits row. With l the row, m its maximum and T = temperature[r], entries are
+ * weighted exp((l - m) / T), held as whole multiples of 2^-40 so that sums are exact and the draw
+ * does not depend on their order. In descending order of l (ties to the lower index) the kept
+ * entries are the top_k[r] first (0: all), of those the smallest prefix that holds top_p[r] of
+ * their mass (1: all), of those the ones whose weight is at least min_p[r] of the maximum's. The
+ * token is the first kept entry in index order at which the running kept mass exceeds uniform[r]
+ * times the whole. temperature <= 0 picks the maximum. NaN and -inf are never kept; a row without
+ * any other entry gives token -1, probability 0. prob (may be NULL) receives the token's share of
+ * the kept mass, kept (may be NULL) their number. Any of temperature, top_k, top_p and min_p may
+ * be NULL (1, 0, 1, 0). Differs from g4b_sample_token, which keeps the reference's order and its
+ * 256-entry bound. vocab 1..262144; stride in elements; dtype any g4b_dtype. One kernel launch. */
+G4B_API int g4b_sample_rows(const void* logits, int dtype, int rows, int vocab, int64_t stride,
+                            const float* uniform, const float* temperature, const int32_t* top_k,
+                            const float* top_p, const float* min_p, int32_t* token, float* prob, int32_t* kept,
+                            void* stream);
+
+/* Walks each sequence's tree: from node 0 to the lowest child whose token is the one drawn at the
+ * current node (sampled[]), as long as there is one. parents[i] is relative to the sequence's
+ * first node, and smaller than i. path[s] receives the accepted nodes (relative, -1 behind the
+ * last; at most path_width), count[s] their number, next[s] the token drawn at the last of them,
+ * which becomes the next round's pending token. A sequence without nodes gets count 0, next -1.
+ * At most 256 nodes a sequence. */
+G4B_API int g4b_tree_accept(const int32_t* tokens, const int32_t* parents, const int32_t* sampled,
+                            const int32_t* cu_nodes, int n_seqs, int n_tokens, int32_t* path, int path_width,
+                            int32_t* count, int32_t* next, void* stream);
+
+/* A pool of pages: n_planes planes (one per layer's K and V) of n_pages pages of page_size rows of
+ * row_bytes bytes. Base and strides multiples of 16 bytes; the rows of one page are contiguous. */
+typedef struct g4b_page_pool {
+    void* base;
+    int64_t plane_stride, page_stride; /* bytes */
+    int n_planes, n_pages, page_size, row_bytes;
+} g4b_page_pool;
+
+/* The keeping of n_seqs (up to 4096) sequences' pages: refs [n_pages] counts how many sequences hold
+ * a page (0: free), table [n_seqs][table_width] lists each sequence's pages (-1: none), lens
+ * [n_seqs] its tokens. Each call reads refs, table and lens and writes refs_out, table_out and
+ * lens_out (those it changes), which may be the same arrays. New pages are the free pages of lowest
+ * id, in (sequence, position) order: results depend on the state alone. status: 0 done, 1 too few
+ * free pages, 2 more pages than the table row holds (or a negative length), 3 a bad sequence index,
+ * 4 a page id out of range in the table; the outputs then equal the inputs. */
+typedef struct g4b_page_tables {
+    const int32_t *refs, *table, *lens;
+    int32_t *refs_out, *table_out, *lens_out;
+    int n_pages, n_seqs, table_width, page_size;
+} g4b_page_tables;
+
+/* Fills the empty table entries that sequence s needs to hold lens[s] + grow[s] tokens. */
+G4B_API int g4b_pages_reserve(const g4b_page_tables* t, const int32_t* grow, int32_t* status, void* stream);
+/* dst[i] (an empty sequence, named once) becomes a continuation of src[i]: full pages are shared, a
+ * partial last page is copied to a page of its own in every plane, so each sequence only ever
+ * writes rows of pages that it alone holds. */
+G4B_API int g4b_pages_fork(const g4b_page_pool* pool, const g4b_page_tables* t, const int32_t* src,
+                           const int32_t* dst, int n, int32_t* status, void* stream);
+/* Releases the pages of the n sequences seqs[] and empties them. */
+G4B_API int g4b_pages_free(const g4b_page_tables* t, const int32_t* seqs, int n, void* stream);
+/* Moves live pages so that they fill ids 0 .. live - 1: the k-th live page at or past `live` goes to
+ * the k-th free page before it. moves [1 + 2 * n_pages] receives their number and the (from, to)
+ * pairs, -1 behind them. lens is not read. */
+G4B_API int g4b_pages_compact(const g4b_page_pool* pool, const g4b_page_tables* t, int32_t* moves, void* stream);
+/* Page src[i] of one pool to page dst[i] of another (same planes, page_size and row_bytes), or of
+ * the same one when no page is both a source and a destination. */
+G4B_API int g4b_pages_copy(const g4b_page_pool* from, const g4b_page_pool* to, const int32_t* src,
+                           const int32_t* dst, int n, void* stream);
+/* Writes rows [n_planes][n_tokens][row_bytes] (plane stride rows_plane_stride bytes) of sequence s's
+ * nodes path[s][0 .. count[s]) (NULL path: the first count[s]) at positions lens[s] onwards of its
+ * pages, and lens_out[s] = lens[s] + count[s]. status (may be NULL) is g4b_pages_reserve's: nothing
+ * is committed unless it is 0. */
+G4B_API int g4b_pages_commit(const g4b_page_pool* pool, const int32_t* table, int table_width, const int32_t* lens,
+                             int n_seqs, const void* rows, int64_t rows_plane_stride, int n_tokens,
+                             const int32_t* cu_nodes, const int32_t* path, int path_width, const int32_t* count,
+                             const int32_t* status, int32_t* lens_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2,13 +2,17 @@
 // verify GEMM on caller-owned device buffers.
 #include "g4dense_b200_ops.h"
 
+#include <climits>
 #include <cstdio>
 #include <mutex>
 #include <string>
 
 #include "common.cuh"
 #include "kernels.h"
+#include "pages.h"
 #include "pgemm.h"
+#include "sample_rows.h"
+#include "tree_attn.h"
 #include "vgemm.h"
 
 namespace {
@@ -289,6 +293,203 @@ int g4b_sample_token(const float* logits, int vocab, float temperature, float to
     const cudaError_t e = g4b_sample_launch(logits, vocab, temperature, top_p, top_k, seed, workspace, out_token,
                                             static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? 0 : fail(e, "g4b_sample_token");
+}
+
+// ---------------------------------------------------------------- tree verification, paged cache
+
+size_t g4b_tree_attention_workspace(int max_nodes, int heads, int kv_heads, int head_dim) {
+    if (max_nodes < 1 || max_nodes > 256 || kv_heads < 1 || heads < kv_heads || heads % kv_heads ||
+        (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512))
+        return 0;
+    return g4b::tree_attn_workspace(max_nodes, heads, kv_heads, head_dim);
+}
+
+int g4b_tree_attention(const g4b_tree_attention_args* x, void* stream) {
+    if (!x) return fail_msg("g4b_tree_attention: null arguments");
+    const size_t need = g4b_tree_attention_workspace(x->max_nodes, x->heads, x->kv_heads, x->head_dim);
+    if (!need)
+        return fail_msg("g4b_tree_attention: max_nodes must be 1..256, heads a multiple of kv_heads and head_dim 64, "
+                        "128, 256 or 512");
+    if (x->dtype != G4B_BF16 && x->dtype != G4B_FP16)
+        return fail_msg("g4b_tree_attention: dtype must be G4B_BF16 or G4B_FP16");
+    if (x->n_seqs < 0 || x->n_tokens < 0 || x->n_pages < 1 || x->table_width < 1 || x->window < 0)
+        return fail_msg("g4b_tree_attention: negative or empty sizes");
+    if (x->page_size < 8 || x->page_size % 8 || (int64_t)x->page_size * x->table_width > INT32_MAX - 1024)
+        return fail_msg("g4b_tree_attention: page_size must be a multiple of 8, and page_size * table_width fit 31 bits");
+    if (x->mask_words < (x->max_nodes + 31) / 32)
+        return fail_msg("g4b_tree_attention: mask_words must hold max_nodes bits");
+    const int64_t row = (int64_t)x->kv_heads * x->head_dim, qrow = (int64_t)x->heads * x->head_dim;
+    if (x->q_stride < qrow || x->out_stride < qrow || x->new_stride < row || x->page_stride < row * x->page_size ||
+        ((x->q_stride | x->out_stride | x->new_stride | x->page_stride) & 7))
+        return fail_msg("g4b_tree_attention: strides must cover a row and be multiples of 8 elements");
+    if (x->n_seqs == 0 || x->n_tokens == 0) return 0;
+    if (!x->q || !x->k_pool || !x->v_pool || !x->k_new || !x->v_new || !x->out || !x->table || !x->lens ||
+        !x->cu_nodes || !x->mask || !x->workspace || (x->window && !x->depth))
+        return fail_msg("g4b_tree_attention: null pointer");
+    if ((reinterpret_cast<uintptr_t>(x->q) | reinterpret_cast<uintptr_t>(x->k_pool) |
+         reinterpret_cast<uintptr_t>(x->v_pool) | reinterpret_cast<uintptr_t>(x->k_new) |
+         reinterpret_cast<uintptr_t>(x->v_new) | reinterpret_cast<uintptr_t>(x->out) |
+         reinterpret_cast<uintptr_t>(x->workspace)) & 15)
+        return fail_msg("g4b_tree_attention: q, K, V, out and workspace must be 16-byte aligned");
+    if (x->workspace_bytes < need) return fail_msg("g4b_tree_attention: workspace too small");
+    g4b::TreeAttnArgs a{};
+    a.q = x->q;
+    a.k_pool = x->k_pool;
+    a.v_pool = x->v_pool;
+    a.k_new = x->k_new;
+    a.v_new = x->v_new;
+    a.out = x->out;
+    a.table = x->table;
+    a.lens = x->lens;
+    a.cu = x->cu_nodes;
+    a.mask = x->mask;
+    a.depth = x->depth;
+    a.work = x->workspace;
+    a.q_stride = x->q_stride;
+    a.page_stride = x->page_stride;
+    a.new_stride = x->new_stride;
+    a.out_stride = x->out_stride;
+    a.seqs = x->n_seqs;
+    a.n_tokens = x->n_tokens;
+    a.max_nodes = x->max_nodes;
+    a.pages = x->n_pages;
+    a.page_size = x->page_size;
+    a.width = x->table_width;
+    a.mask_words = x->mask_words;
+    a.heads = x->heads;
+    a.kv_heads = x->kv_heads;
+    a.dim = x->head_dim;
+    a.window = x->window;
+    a.bf16 = x->dtype == G4B_BF16;
+    a.scale = x->scale;
+    const cudaError_t e = g4b::tree_attn_launch(a, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : fail(e, "g4b_tree_attention");
+}
+
+int g4b_sample_rows(const void* logits, int dtype, int rows, int vocab, int64_t stride, const float* uniform,
+                    const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                    int32_t* token, float* prob, int32_t* kept, void* stream) {
+    if (dtype < G4B_BF16 || dtype > G4B_FP32 || rows < 0 || rows > (1 << 26) || vocab < 1 ||
+        vocab > g4b::kSampleRowsVocab || stride < vocab)
+        return fail_msg("g4b_sample_rows: bad arguments (dtype bf16, fp16 or fp32, vocab 1..262144, stride >= vocab)");
+    if (rows == 0) return 0;
+    if (!logits || !uniform || !token) return fail_msg("g4b_sample_rows: null pointer");
+    if (reinterpret_cast<uintptr_t>(logits) % (dtype == G4B_FP32 ? 4 : 2))
+        return fail_msg("g4b_sample_rows: logits are not aligned to their type");
+    g4b::SampleRowsArgs a{logits, uniform, temperature, top_k, top_p, min_p, token, prob, kept, stride, rows, vocab, dtype};
+    const cudaError_t e = g4b::sample_rows_launch(a, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : fail(e, "g4b_sample_rows");
+}
+
+int g4b_tree_accept(const int32_t* tokens, const int32_t* parents, const int32_t* sampled, const int32_t* cu_nodes,
+                    int n_seqs, int n_tokens, int32_t* path, int path_width, int32_t* count, int32_t* next,
+                    void* stream) {
+    if (n_seqs < 0 || n_tokens < 0 || path_width < 1) return fail_msg("g4b_tree_accept: bad sizes");
+    if (n_seqs == 0) return 0;
+    if (!cu_nodes || !path || !count || !next || (n_tokens && (!tokens || !parents || !sampled)))
+        return fail_msg("g4b_tree_accept: null pointer");
+    const cudaError_t e = g4b::tree_accept(tokens, parents, sampled, cu_nodes, n_seqs, n_tokens, path, path_width,
+                                           count, next, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : fail(e, "g4b_tree_accept");
+}
+
+namespace {
+const char* bad_pool(const g4b_page_pool* p) {
+    if (!p || !p->base) return "null pool";
+    if (p->n_planes < 1 || p->n_pages < 1 || p->n_pages > (1 << 24) || p->page_size < 1 || p->row_bytes < 16)
+        return "pool sizes must be positive (at most 2^24 pages)";
+    if ((reinterpret_cast<uintptr_t>(p->base) & 15) || (p->row_bytes & 15) || (p->plane_stride & 15) ||
+        (p->page_stride & 15))
+        return "pool base, strides and row_bytes must be multiples of 16 bytes";
+    if (p->page_stride < (int64_t)p->page_size * p->row_bytes) return "page_stride must cover a page";
+    return nullptr;
+}
+const char* bad_tables(const g4b_page_tables* t, bool lens, bool lens_out) {
+    if (!t || !t->refs || !t->table || !t->refs_out || !t->table_out || (lens && !t->lens) ||
+        (lens_out && !t->lens_out))
+        return "null tables";
+    if (t->n_pages < 1 || t->n_pages > (1 << 24) || t->n_seqs < 1 || t->n_seqs > g4b::kMaxPageSeqs ||
+        t->table_width < 1 || t->page_size < 1 || (int64_t)t->table_width * t->page_size > INT32_MAX)
+        return "sizes out of range (1..4096 sequences, at most 2^24 pages, table_width * page_size in 31 bits)";
+    return nullptr;
+}
+g4b::PagePool pool_of(const g4b_page_pool* p) {
+    return {static_cast<char*>(p->base), p->plane_stride, p->page_stride, p->n_planes, p->n_pages, p->page_size,
+            p->row_bytes};
+}
+g4b::PageTables tables_of(const g4b_page_tables* t) {
+    return {t->refs, t->table, t->lens, t->refs_out, t->table_out, t->lens_out, t->n_pages, t->n_seqs,
+            t->table_width, t->page_size};
+}
+int bad(const char* call, const char* why) {
+    g_err = std::string(call) + ": " + why;
+    return (int)cudaErrorInvalidValue;
+}
+}  // namespace
+
+int g4b_pages_reserve(const g4b_page_tables* t, const int32_t* grow, int32_t* status, void* stream) {
+    if (const char* why = bad_tables(t, true, false)) return bad("g4b_pages_reserve", why);
+    if (!grow || !status) return bad("g4b_pages_reserve", "null pointer");
+    const cudaError_t e = g4b::pages_reserve(tables_of(t), grow, status, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : fail(e, "g4b_pages_reserve");
+}
+
+int g4b_pages_fork(const g4b_page_pool* pool, const g4b_page_tables* t, const int32_t* src, const int32_t* dst, int n,
+                   int32_t* status, void* stream) {
+    if (const char* why = bad_pool(pool)) return bad("g4b_pages_fork", why);
+    if (const char* why = bad_tables(t, true, true)) return bad("g4b_pages_fork", why);
+    if (n < 0 || n > g4b::kMaxPageSeqs || !status || (n && (!src || !dst)))
+        return bad("g4b_pages_fork", "null pointer or more than 4096 forks");
+    if (pool->n_pages != t->n_pages || pool->page_size != t->page_size)
+        return bad("g4b_pages_fork", "pool and tables differ in pages or page_size");
+    const cudaError_t e = g4b::pages_fork(pool_of(pool), tables_of(t), src, dst, n, status, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : fail(e, "g4b_pages_fork");
+}
+
+int g4b_pages_free(const g4b_page_tables* t, const int32_t* seqs, int n, void* stream) {
+    if (const char* why = bad_tables(t, true, true)) return bad("g4b_pages_free", why);
+    if (n < 0 || (n && !seqs)) return bad("g4b_pages_free", "null pointer");
+    const cudaError_t e = g4b::pages_free(tables_of(t), seqs, n, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : fail(e, "g4b_pages_free");
+}
+
+int g4b_pages_compact(const g4b_page_pool* pool, const g4b_page_tables* t, int32_t* moves, void* stream) {
+    if (const char* why = bad_pool(pool)) return bad("g4b_pages_compact", why);
+    if (const char* why = bad_tables(t, false, false)) return bad("g4b_pages_compact", why);
+    if (!moves) return bad("g4b_pages_compact", "null pointer");
+    if (pool->n_pages != t->n_pages) return bad("g4b_pages_compact", "pool and tables differ in pages");
+    const cudaError_t e = g4b::pages_compact(pool_of(pool), tables_of(t), moves, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : fail(e, "g4b_pages_compact");
+}
+
+int g4b_pages_copy(const g4b_page_pool* from, const g4b_page_pool* to, const int32_t* src, const int32_t* dst, int n,
+                   void* stream) {
+    if (const char* why = bad_pool(from)) return bad("g4b_pages_copy", why);
+    if (const char* why = bad_pool(to)) return bad("g4b_pages_copy", why);
+    if (from->n_planes != to->n_planes || from->page_size != to->page_size || from->row_bytes != to->row_bytes)
+        return bad("g4b_pages_copy", "the pools differ in planes, page_size or row_bytes");
+    if (n < 0 || (n && (!src || !dst))) return bad("g4b_pages_copy", "null pointer");
+    if (n == 0) return 0;
+    const cudaError_t e = g4b::pages_copy(pool_of(from), pool_of(to), src, dst, n, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : fail(e, "g4b_pages_copy");
+}
+
+int g4b_pages_commit(const g4b_page_pool* pool, const int32_t* table, int table_width, const int32_t* lens, int n_seqs,
+                     const void* rows, int64_t rows_plane_stride, int n_tokens, const int32_t* cu_nodes,
+                     const int32_t* path, int path_width, const int32_t* count, const int32_t* status,
+                     int32_t* lens_out, void* stream) {
+    if (const char* why = bad_pool(pool)) return bad("g4b_pages_commit", why);
+    if (n_seqs < 0 || n_seqs > g4b::kMaxPageSeqs || table_width < 1 || n_tokens < 0 || (path && path_width < 1))
+        return bad("g4b_pages_commit", "sizes out of range");
+    if (n_seqs == 0) return 0;
+    if (!table || !lens || !cu_nodes || !count || !lens_out || (n_tokens && !rows))
+        return bad("g4b_pages_commit", "null pointer");
+    if ((reinterpret_cast<uintptr_t>(rows) & 15) || (rows_plane_stride & 15))
+        return bad("g4b_pages_commit", "rows and their plane stride must be multiples of 16 bytes");
+    const cudaError_t e = g4b::pages_commit(pool_of(pool), table, table_width, lens, n_seqs,
+                                            static_cast<const char*>(rows), rows_plane_stride, n_tokens, cu_nodes, path,
+                                            path_width, count, status, lens_out, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : fail(e, "g4b_pages_commit");
 }
 
 int g4b_qmat_check_error(g4b_qmat* q) {

@@ -34,9 +34,50 @@ def lib():
         L.g4b_gemv_int8.argtypes = [_vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, _vp]
         L.g4b_attn_gate.argtypes = [_vp, _vp, _vp] + [ctypes.c_int] * 5 + [_vp]
         L.g4b_qmat_check_error.argtypes = [_vp]
+        _bind_tree(L)
         _bind_engine(L)
         _lib = L
     return _lib
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """g4b_tree_attention_args (include/g4dense_b200_ops.h)."""
+    _fields_ = ([(n, _vp) for n in ("q", "k_pool", "v_pool", "k_new", "v_new", "out", "table", "lens", "cu_nodes",
+                                    "mask", "depth", "workspace")] + [("workspace_bytes", ctypes.c_size_t)] +
+                [(n, ctypes.c_int64) for n in ("q_stride", "out_stride", "new_stride", "page_stride")] +
+                [(n, ctypes.c_int) for n in ("n_seqs", "n_tokens", "max_nodes", "n_pages", "page_size", "table_width",
+                                             "mask_words", "heads", "kv_heads", "head_dim", "window", "dtype")] +
+                [("scale", ctypes.c_float)])
+
+
+class PagePool(ctypes.Structure):
+    """g4b_page_pool (include/g4dense_b200_ops.h)."""
+    _fields_ = [("base", _vp), ("plane_stride", ctypes.c_int64), ("page_stride", ctypes.c_int64),
+                ("n_planes", ctypes.c_int), ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("row_bytes", ctypes.c_int)]
+
+
+class PageTables(ctypes.Structure):
+    """g4b_page_tables (include/g4dense_b200_ops.h)."""
+    _fields_ = ([(n, _vp) for n in ("refs", "table", "lens", "refs_out", "table_out", "lens_out")] +
+                [(n, ctypes.c_int) for n in ("n_pages", "n_seqs", "table_width", "page_size")])
+
+
+def _bind_tree(L):
+    """Binds the tree-verification and paged-cache operators (include/g4dense_b200_ops.h)."""
+    i, i64 = ctypes.c_int, ctypes.c_int64
+    pool, tables = ctypes.POINTER(PagePool), ctypes.POINTER(PageTables)
+    L.g4b_tree_attention_workspace.restype = ctypes.c_size_t
+    L.g4b_tree_attention_workspace.argtypes = [i, i, i, i]
+    L.g4b_tree_attention.argtypes = [ctypes.POINTER(TreeAttentionArgs), _vp]
+    L.g4b_sample_rows.argtypes = [_vp, i, i, i, i64] + [_vp] * 9
+    L.g4b_tree_accept.argtypes = [_vp] * 4 + [i, i, _vp, i, _vp, _vp, _vp]
+    L.g4b_pages_reserve.argtypes = [tables, _vp, _vp, _vp]
+    L.g4b_pages_fork.argtypes = [pool, tables, _vp, _vp, i, _vp, _vp]
+    L.g4b_pages_free.argtypes = [tables, _vp, i, _vp]
+    L.g4b_pages_compact.argtypes = [pool, tables, _vp, _vp]
+    L.g4b_pages_copy.argtypes = [pool, pool, _vp, _vp, i, _vp]
+    L.g4b_pages_commit.argtypes = [pool, _vp, i, _vp, i, _vp, i64, i, _vp, _vp, i, _vp, _vp, _vp, _vp]
 
 
 class EngineConfig(ctypes.Structure):
@@ -170,6 +211,214 @@ def sample_token(logits, temperature, top_p, top_k, seed, workspace, out, stream
     of sample_workspace_bytes()."""
     _check(lib().g4b_sample_token(_dptr(logits), logits.numel(), temperature, top_p, top_k, seed & (2**64 - 1),
                                   _dptr(workspace), _dptr(out), _stream(stream)), "g4b_sample_token")
+
+_DTYPES = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2}  # g4b_dtype
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _ints(name, t, shape=None, optional=False):
+    """Device pointer of a contiguous int32 CUDA tensor of the given shape."""
+    if t is None and optional:
+        return None
+    _need(t.is_cuda and str(t.dtype) == "torch.int32" and t.is_contiguous(), f"{name}: a contiguous int32 CUDA tensor")
+    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, expected {tuple(shape or ())}")
+    return _dptr(t)
+
+
+def _floats(name, t, shape):
+    if t is None:
+        return None
+    _need(t.is_cuda and str(t.dtype) == "torch.float32" and t.is_contiguous() and tuple(t.shape) == tuple(shape),
+          f"{name}: a contiguous float32 CUDA tensor of shape {tuple(shape)}")
+    return _dptr(t)
+
+
+def tree_mask(parents, words=None):
+    """Mask words and depths of one tree from its parents (parents[i] < i, -1 for a root): (mask
+    [n][words] int32, depth [n] int32) numpy arrays for tree_attention, node i seeing itself and its
+    ancestors."""
+    n = len(parents)
+    words = words or max(1, (n + 31) // 32)
+    mask, depth = np.zeros((n, words), np.uint32), np.zeros(n, np.int32)
+    for i, p in enumerate(parents):
+        _need(-1 <= p < i, f"tree_mask: parent {p} of node {i}")
+        if p >= 0:
+            mask[i] = mask[p]
+            depth[i] = depth[p] + 1
+        mask[i, i // 32] |= np.uint32(1 << (i % 32))
+    return mask.view(np.int32), depth
+
+
+def tree_attention_workspace(max_nodes, heads, kv_heads, head_dim):
+    """Bytes of workspace tree_attention needs (ValueError for a shape it does not support)."""
+    n = int(lib().g4b_tree_attention_workspace(max_nodes, heads, kv_heads, head_dim))
+    _need(n, f"tree_attention: max_nodes {max_nodes} (1..256), heads {heads} (a multiple of {kv_heads}), head_dim "
+             f"{head_dim} (64, 128, 256 or 512)")
+    return n
+
+
+def tree_attention(q, k_pool, v_pool, table, lens, k_new, v_new, cu_nodes, mask, out, workspace, *, max_nodes, scale,
+                   depth=None, window=0, stream=None):
+    """Attention of drafted-token trees over a paged K/V cache (g4b_tree_attention). q, out
+    [tokens][heads][dim]; k_pool, v_pool [pages][page_size][kv_heads][dim]; k_new, v_new
+    [tokens][kv_heads][dim], all bf16 or all fp16 torch CUDA tensors (token and page strides
+    honoured); table [seqs][width], lens [seqs], cu_nodes [seqs + 1], mask [tokens][words], depth
+    [tokens] int32; workspace a byte tensor of tree_attention_workspace()."""
+    _need(q.dim() == 3 and k_pool.dim() == 4 and k_new.dim() == 3, "tree_attention: q and k_new 3-d, pools 4-d")
+    tokens, heads, dim = q.shape
+    pages, page_size, kv_heads, _ = k_pool.shape
+    dtype = _DTYPES.get(str(q.dtype), -1)
+    _need(dtype in (0, 1), f"tree_attention: dtype {q.dtype} (bfloat16 or float16)")
+    for name, t, shape in (("q", q, (tokens, heads, dim)), ("out", out, (tokens, heads, dim)),
+                           ("k_pool", k_pool, (pages, page_size, kv_heads, dim)),
+                           ("v_pool", v_pool, (pages, page_size, kv_heads, dim)),
+                           ("k_new", k_new, (tokens, kv_heads, dim)), ("v_new", v_new, (tokens, kv_heads, dim))):
+        _need(t.is_cuda and t.dtype == q.dtype and tuple(t.shape) == shape,
+              f"tree_attention: {name} has to be a {q.dtype} CUDA tensor of shape {shape}")
+        inner = t.stride()[1:]
+        want, n = [], 1
+        for size in reversed(shape[1:]):
+            want.insert(0, n)
+            n *= size
+        _need(all(w == s or d == 1 for w, s, d in zip(want, inner, shape[1:])),
+              f"tree_attention: {name} has to be contiguous but for its first dimension")
+    _need(tokens <= 1 or k_new.stride(0) == v_new.stride(0), "tree_attention: k_new and v_new differ in their strides")
+    _need(pages <= 1 or k_pool.stride(0) == v_pool.stride(0), "tree_attention: the pools differ in their strides")
+    seqs, row = lens.numel(), kv_heads * dim
+    a = TreeAttentionArgs()
+    a.table = _ints("table", table, (seqs, table.shape[-1]))
+    a.lens = _ints("lens", lens, (seqs,))
+    a.cu_nodes = _ints("cu_nodes", cu_nodes, (seqs + 1,))
+    a.mask = _ints("mask", mask, (tokens, mask.shape[-1]))
+    a.depth = _ints("depth", depth, (tokens,), optional=True)
+    _need(not window or depth is not None, "tree_attention: a window needs the nodes' depths")
+    a.q, a.k_pool, a.v_pool, a.k_new, a.v_new = map(_dptr, (q, k_pool, v_pool, k_new, v_new))
+    a.out, a.workspace, a.workspace_bytes = _dptr(out), _dptr(workspace), workspace.numel() * workspace.element_size()
+    a.q_stride = q.stride(0) if tokens > 1 else heads * dim
+    a.out_stride = out.stride(0) if tokens > 1 else heads * dim
+    a.new_stride = k_new.stride(0) if tokens > 1 else row
+    a.page_stride = k_pool.stride(0) if pages > 1 else row * page_size
+    a.n_seqs, a.n_tokens, a.max_nodes, a.n_pages, a.page_size = seqs, tokens, max_nodes, pages, page_size
+    a.table_width, a.mask_words = table.shape[1], mask.shape[1]
+    a.heads, a.kv_heads, a.head_dim, a.window, a.dtype, a.scale = heads, kv_heads, dim, window, dtype, scale
+    _check(lib().g4b_tree_attention(ctypes.byref(a), _stream(stream)), "g4b_tree_attention")
+
+
+def sample_rows(logits, uniform, token, prob=None, kept=None, temperature=None, top_k=None, top_p=None, min_p=None,
+                stream=None):
+    """One token per row of logits [rows][vocab] (bf16, fp16 or fp32; row stride honoured) into token
+    [rows] int32, from uniform [rows] float32 in [0, 1), with per-row temperature, top_p, min_p
+    (float32) and top_k (int32) where given (g4b_sample_rows). prob [rows] float32 and kept [rows]
+    int32 receive the token's share of the kept mass and the number of kept entries."""
+    _need(logits.is_cuda and logits.dim() == 2 and logits.stride(1) in (1,) or logits.shape[-1] == 1,
+          "sample_rows: logits [rows][vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    dtype = _DTYPES.get(str(logits.dtype), -1)
+    _need(dtype >= 0, f"sample_rows: dtype {logits.dtype} (bfloat16, float16 or float32)")
+    _need(uniform is not None, "sample_rows: uniform numbers are needed")
+    _check(lib().g4b_sample_rows(_dptr(logits), dtype, rows, vocab, logits.stride(0) if rows > 1 else vocab,
+                                 _floats("uniform", uniform, (rows,)), _floats("temperature", temperature, (rows,)),
+                                 _ints("top_k", top_k, (rows,), optional=True), _floats("top_p", top_p, (rows,)),
+                                 _floats("min_p", min_p, (rows,)), _ints("token", token, (rows,)),
+                                 _floats("prob", prob, (rows,)), _ints("kept", kept, (rows,), optional=True),
+                                 _stream(stream)), "g4b_sample_rows")
+
+
+def tree_accept(tokens, parents, sampled, cu_nodes, path, count, next_token, stream=None):
+    """Walks each tree along the drawn tokens (g4b_tree_accept): path [seqs][width], count [seqs] and
+    next_token [seqs] from tokens, parents, sampled [nodes] and cu_nodes [seqs + 1], all int32."""
+    n, seqs = tokens.numel(), cu_nodes.numel() - 1
+    _check(lib().g4b_tree_accept(_ints("tokens", tokens, (n,)), _ints("parents", parents, (n,)),
+                                 _ints("sampled", sampled, (n,)), _ints("cu_nodes", cu_nodes, (seqs + 1,)), seqs, n,
+                                 _ints("path", path, (seqs, path.shape[-1])), path.shape[-1],
+                                 _ints("count", count, (seqs,)), _ints("next_token", next_token, (seqs,)),
+                                 _stream(stream)), "g4b_tree_accept")
+
+
+def _pool(pool):
+    """g4b_page_pool of a CUDA tensor [planes][pages][page_size][...] with contiguous pages."""
+    _need(pool.is_cuda and pool.dim() >= 4, "pool: a CUDA tensor [planes][pages][page_size][row...]")
+    size = pool.element_size()
+    row = 1
+    for d in pool.shape[3:]:
+        row *= d
+    _need(pool[0, 0].is_contiguous(), "pool: the rows of a page have to be contiguous")
+    planes, pages, page_size = pool.shape[:3]
+    page_stride = (pool.stride(1) if pages > 1 else page_size * row) * size
+    plane_stride = (pool.stride(0) if planes > 1 else pages * page_size * row) * size
+    return PagePool(pool.data_ptr(), plane_stride, page_stride, planes, pages, page_size, row * size)
+
+
+def _tables(refs, table, lens, refs_out, table_out, lens_out, page_size):
+    pages, (seqs, width) = refs.numel(), table.shape
+    t = PageTables()
+    t.refs, t.table = _ints("refs", refs, (pages,)), _ints("table", table, (seqs, width))
+    t.refs_out, t.table_out = _ints("refs_out", refs_out, (pages,)), _ints("table_out", table_out, (seqs, width))
+    t.lens = _ints("lens", lens, (seqs,), optional=True)
+    t.lens_out = _ints("lens_out", lens_out, (seqs,), optional=True)
+    t.n_pages, t.n_seqs, t.table_width, t.page_size = pages, seqs, width, page_size
+    return t
+
+
+def pages_reserve(refs, table, lens, grow, page_size, refs_out, table_out, status, stream=None):
+    """Pages for grow[s] more tokens of every sequence (g4b_pages_reserve). int32 CUDA tensors: refs
+    [pages], table [seqs][width], lens, grow [seqs], status [1]; the outputs may be the inputs."""
+    t = _tables(refs, table, lens, refs_out, table_out, None, page_size)
+    _check(lib().g4b_pages_reserve(ctypes.byref(t), _ints("grow", grow, (lens.numel(),)), _ints("status", status, (1,)),
+                                   _stream(stream)), "g4b_pages_reserve")
+
+
+def pages_fork(pool, refs, table, lens, src, dst, refs_out, table_out, lens_out, status, stream=None):
+    """Sequences dst[i] become continuations of src[i] (g4b_pages_fork): full pages shared, a partial
+    last page copied. pool [planes][pages][page_size][row...]."""
+    t, p = _tables(refs, table, lens, refs_out, table_out, lens_out, pool.shape[2]), _pool(pool)
+    _check(lib().g4b_pages_fork(ctypes.byref(p), ctypes.byref(t), _ints("src", src, (src.numel(),)),
+                                _ints("dst", dst, (src.numel(),)), src.numel(), _ints("status", status, (1,)),
+                                _stream(stream)), "g4b_pages_fork")
+
+
+def pages_free(refs, table, lens, seqs, page_size, refs_out, table_out, lens_out, stream=None):
+    """Releases the pages of the sequences seqs[] and empties them (g4b_pages_free)."""
+    t = _tables(refs, table, lens, refs_out, table_out, lens_out, page_size)
+    _check(lib().g4b_pages_free(ctypes.byref(t), _ints("seqs", seqs, (seqs.numel(),)), seqs.numel(), _stream(stream)),
+           "g4b_pages_free")
+
+
+def pages_compact(pool, refs, table, refs_out, table_out, moves, stream=None):
+    """Moves live pages to the front of the pool (g4b_pages_compact); moves [1 + 2 * pages] int32
+    receives their number and the (from, to) pairs."""
+    t, p = _tables(refs, table, None, refs_out, table_out, None, pool.shape[2]), _pool(pool)
+    _check(lib().g4b_pages_compact(ctypes.byref(p), ctypes.byref(t), _ints("moves", moves, (1 + 2 * refs.numel(),)),
+                                   _stream(stream)), "g4b_pages_compact")
+
+
+def pages_copy(pool, to_pool, src, dst, stream=None):
+    """Page src[i] of pool to page dst[i] of to_pool, in every plane (g4b_pages_copy)."""
+    a, b = _pool(pool), _pool(to_pool)
+    _check(lib().g4b_pages_copy(ctypes.byref(a), ctypes.byref(b), _ints("src", src, (src.numel(),)),
+                                _ints("dst", dst, (src.numel(),)), src.numel(), _stream(stream)), "g4b_pages_copy")
+
+
+def pages_commit(pool, table, lens, rows, cu_nodes, path, count, lens_out, status=None, stream=None):
+    """Writes the accepted nodes' rows [planes][tokens][row...] into their sequences' pages and the
+    new lengths into lens_out (g4b_pages_commit). path None: the first count[s] rows."""
+    p, seqs, tokens = _pool(pool), lens.numel(), rows.shape[1]
+    _need(rows.is_cuda and rows.dtype == pool.dtype and rows.shape[0] == pool.shape[0] and
+          tuple(rows.shape[2:]) == tuple(pool.shape[3:]) and (tokens == 0 or rows[0].is_contiguous()),
+          "pages_commit: rows have to be [planes][tokens][row...] of the pool's type")
+    stride = rows.stride(0) * rows.element_size() if rows.shape[0] > 1 else p.row_bytes * tokens
+    _check(lib().g4b_pages_commit(ctypes.byref(p), _ints("table", table, (seqs, table.shape[-1])), table.shape[-1],
+                                  _ints("lens", lens, (seqs,)), seqs, _dptr(rows), stride, tokens,
+                                  _ints("cu_nodes", cu_nodes, (seqs + 1,)),
+                                  None if path is None else _ints("path", path, (seqs, path.shape[-1])),
+                                  0 if path is None else path.shape[-1], _ints("count", count, (seqs,)),
+                                  _ints("status", status, (1,), optional=True), _ints("lens_out", lens_out, (seqs,)),
+                                  _stream(stream)), "g4b_pages_commit")
+
 
 
 class QMat:
