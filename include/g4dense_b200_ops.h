@@ -119,7 +119,7 @@ typedef enum { G4B_BF16 = 0, G4B_FP16 = 1, G4B_FP32 = 2 } g4b_dtype;
  * A node that sees no key gets zeros. Values behind a hidden key, past lens[s] in a page, or in
  * another sequence are never used, whatever they are (NaN and infinities included). Softmax and
  * sums are fp32; the probabilities are rounded to the cache's type before the product with V.
- * head_dim 64, 128, 256 or 512; page_size a multiple of 8; max_nodes 1..256; dtype G4B_BF16 or
+ * scale > 0; head_dim 64, 128, 256 or 512; page_size a multiple of 8; max_nodes 1..256; dtype G4B_BF16 or
  * G4B_FP16 for q, K, V and out alike; pointers 16-byte aligned, strides multiples of 8 elements. */
 typedef struct g4b_tree_attention_args {
     const void* q;            /* [n_tokens][heads][head_dim] */
@@ -132,7 +132,7 @@ typedef struct g4b_tree_attention_args {
     const int32_t* lens;      /* [n_seqs] */
     const int32_t* cu_nodes;  /* [n_seqs + 1] */
     const uint32_t* mask;     /* [n_tokens][mask_words], mask_words >= (max_nodes + 31) / 32 */
-    const int32_t* depth;     /* [n_tokens]; may be NULL when window is 0 */
+    const int32_t* depth;     /* [n_tokens], below the tree's node count; may be NULL when window is 0 */
     void* workspace;          /* g4b_tree_attention_workspace() bytes, used by one stream at a time */
     size_t workspace_bytes;
     int64_t q_stride, out_stride, new_stride;  /* elements from one token to the next */
@@ -144,6 +144,9 @@ typedef struct g4b_tree_attention_args {
 /* 0 when the shape is not supported. */
 G4B_API size_t g4b_tree_attention_workspace(int max_nodes, int heads, int kv_heads, int head_dim);
 G4B_API int g4b_tree_attention(const g4b_tree_attention_args* args, void* stream);
+/* Synchronizes and reports whether a launch on this device hit a bounded-wait timeout since the
+ * last call. */
+G4B_API int g4b_tree_attention_check_error(void);
 
 /* One token per logits row. With l the row, m its maximum and T = temperature[r], entries are
  * weighted exp((l - m) / T), held as whole multiples of 2^-40 so that sums are exact and the draw

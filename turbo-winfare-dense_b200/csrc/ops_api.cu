@@ -322,6 +322,7 @@ int g4b_tree_attention(const g4b_tree_attention_args* x, void* stream) {
     if (x->q_stride < qrow || x->out_stride < qrow || x->new_stride < row || x->page_stride < row * x->page_size ||
         ((x->q_stride | x->out_stride | x->new_stride | x->page_stride) & 7))
         return fail_msg("g4b_tree_attention: strides must cover a row and be multiples of 8 elements");
+    if (!(x->scale > 0.f) || x->scale > 1e30f) return fail_msg("g4b_tree_attention: scale must be positive");
     if (x->n_seqs == 0 || x->n_tokens == 0) return 0;
     if (!x->q || !x->k_pool || !x->v_pool || !x->k_new || !x->v_new || !x->out || !x->table || !x->lens ||
         !x->cu_nodes || !x->mask || !x->workspace || (x->window && !x->depth))
@@ -364,6 +365,13 @@ int g4b_tree_attention(const g4b_tree_attention_args* x, void* stream) {
     a.scale = x->scale;
     const cudaError_t e = g4b::tree_attn_launch(a, (cudaStream_t)stream);
     return e == cudaSuccess ? 0 : fail(e, "g4b_tree_attention");
+}
+
+int g4b_tree_attention_check_error(void) {
+    const int e = g4b::tree_attn_error();
+    if (e < 0) return fail(cudaGetLastError(), "g4b_tree_attention_check_error");
+    if (e) return fail_msg("g4b_tree_attention: a bounded wait gave up (keys or values never arrived)");
+    return 0;
 }
 
 int g4b_sample_rows(const void* logits, int dtype, int rows, int vocab, int64_t stride, const float* uniform,

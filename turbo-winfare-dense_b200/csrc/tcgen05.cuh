@@ -1,8 +1,8 @@
 // Thin inline-PTX wrappers for the sm_100a 5th-generation tensor core (tcgen05): tensor-memory
 // allocation, the MMA with its accumulator in tensor memory (TMEM), completion tracking through
-// mbarriers, and TMEM <-> register moves. Only the forms the prefill GEMM and the long-context
-// attention use are wrapped: cta_group::1, kind::f16 (fp16 or bf16 inputs, fp32 accumulate), B
-// from shared memory, A from shared (K- or MN-major) or tensor memory.
+// mbarriers, and TMEM <-> register moves. Only the forms the prefill GEMM, the long-context
+// attention and the tree attention use are wrapped: cta_group::1, kind::f16 (fp16 or bf16 inputs, fp32 accumulate), B
+// from shared memory (K- or MN-major), A from shared (K- or MN-major) or tensor memory.
 //
 // TMEM addresses are (lane << 16) | column. A warp may only touch the 32 lanes of its
 // quadrant, lanes 32 * (warp % 4) .. +31.
@@ -106,6 +106,14 @@ __device__ __forceinline__ void st16(uint32_t taddr, const float (&v)[16]) {
         "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15]))
         : "memory");
 }
+// 8 consecutive 32-bit columns of this thread's lane. Warp-collective; follow with wait_st().
+__device__ __forceinline__ void st8(uint32_t taddr, const float (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+                 "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+                 "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
+                 "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
+                 : "memory");
+}
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Shared-memory matrix descriptor of a K-major operand tile in the canonical 128-byte-swizzled
@@ -139,6 +147,16 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool a_mn) {
            | ((a_mn ? 1u : 0u) << 15)       // A major-ness (0: K-major)
            | ((uint32_t)(N >> 3) << 17)     // N / 8
            | ((uint32_t)(M >> 4) << 24);    // M / 16
+}
+
+// Instruction descriptor for kind::f16 with A and B both bf16 or both fp16, fp32 D, M x N; a_mn,
+// b_mn: that operand is MN-major.
+__host__ __device__ constexpr uint32_t idesc_16(int M, int N, bool bf16, bool a_mn, bool b_mn) {
+    return (1u << 4)                                               // D format: f32
+           | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10)    // A, B format
+           | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16)   // major-ness (0: K-major)
+           | ((uint32_t)(N >> 3) << 17)                            // N / 8
+           | ((uint32_t)(M >> 4) << 24);                           // M / 16
 }
 
 // Instruction descriptor for kind::f16: fp16 A and B (both K-major), fp32 D, M x N.

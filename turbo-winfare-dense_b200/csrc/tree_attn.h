@@ -27,5 +27,6 @@ struct TreeAttnArgs {
 
 size_t tree_attn_workspace(int max_nodes, int heads, int kv_heads, int dim);
 cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st);
+int tree_attn_error();  // synchronizes; nonzero when a bounded wait gave up since the last call
 
 }  // namespace g4b

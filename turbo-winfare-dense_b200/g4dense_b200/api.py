@@ -70,6 +70,7 @@ def _bind_tree(L):
     L.g4b_tree_attention_workspace.restype = ctypes.c_size_t
     L.g4b_tree_attention_workspace.argtypes = [i, i, i, i]
     L.g4b_tree_attention.argtypes = [ctypes.POINTER(TreeAttentionArgs), _vp]
+    L.g4b_tree_attention_check_error.argtypes = []
     L.g4b_sample_rows.argtypes = [_vp, i, i, i, i64] + [_vp] * 9
     L.g4b_tree_accept.argtypes = [_vp] * 4 + [i, i, _vp, i, _vp, _vp, _vp]
     L.g4b_pages_reserve.argtypes = [tables, _vp, _vp, _vp]
@@ -306,6 +307,11 @@ def tree_attention(q, k_pool, v_pool, table, lens, k_new, v_new, cu_nodes, mask,
     a.table_width, a.mask_words = table.shape[1], mask.shape[1]
     a.heads, a.kv_heads, a.head_dim, a.window, a.dtype, a.scale = heads, kv_heads, dim, window, dtype, scale
     _check(lib().g4b_tree_attention(ctypes.byref(a), _stream(stream)), "g4b_tree_attention")
+
+
+def tree_attention_check_error():
+    """Synchronizes; raises when a tree_attention launch hit a bounded-wait timeout."""
+    _check(lib().g4b_tree_attention_check_error(), "g4b_tree_attention_check_error")
 
 
 def sample_rows(logits, uniform, token, prob=None, kept=None, temperature=None, top_k=None, top_p=None, min_p=None,
