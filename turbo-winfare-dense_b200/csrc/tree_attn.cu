@@ -18,9 +18,9 @@
 // Per tile, S^T[key][row] = K Q^T and O^T[dim][row] += V^T P^T: with the keys and the dimensions on
 // the 128-lane side of the MMA the row count is its N, so a tree of 5 nodes costs N = 16 and not a
 // padded 128. Roles:
-//   * warp 0 streams K of tile t + 1, then V of tile t, through a ring of 32 KB slots (128 keys x
+//   * one warp streams K of tile t + 1, then V of tile t, through a ring of 32 KB slots (128 keys x
 //     128 dims) by TMA: one box per (page part, 64 dims), swizzled as the MMA reads it;
-//   * warp 1 (one thread) issues the MMAs, S^T into two alternating TMEM buffers;
+//   * one thread of another issues the MMAs, S^T into two alternating TMEM buffers;
 //   * two groups of four warps take half of the rows each, a thread one key of all its rows: they
 //     hold the softmax in fp32, write P^T (rounded to the cache's type, 8 rows a store) and, when a
 //     row's score exceeds its reference maximum by more than 8 (in powers of two), move the
@@ -49,20 +49,45 @@ namespace g4b {
 namespace {
 
 constexpr int kKeys = 128;           // keys per tile: the M of S^T
-constexpr int kThreads = 384;        // producer, MMA, two idle warps, 8 softmax warps
-constexpr int kSoftWarps = 8;
+constexpr int kSoftWarps = 8;        // warps 0 .. 7
+constexpr int kProducer = 8, kIssuer = 9, kScheduler = 10;
+constexpr int kThreads = 384;        // the last warp only gives up registers
+// Registers a thread: 168 at launch; 256 x 216 + 128 x 72 is the same total.
+constexpr int kSoftRegs = 216, kOtherRegs = 72;
 constexpr uint32_t kBoxBytes = kKeys * 128;  // 128 keys x 64 dims of 16 bits
 constexpr int kMaxSlots = 8;
+constexpr int kParts = 4;            // parts the scheduler is ahead
 constexpr int kTreeBox = 16;         // node rows per TMA box
 constexpr float kUnset = 1e30f;      // negated reference of a row that has seen no key
 constexpr float kLazy = 8.f;         // a reference moves when a score exceeds it by 2^8
 constexpr size_t kSmemLimit = 232448;
+// What starting and finishing an item costs, in tiles, when the shares are cut.
+constexpr int kItemCost = 2;
 
 __device__ int g_tree_err;  // set when a bounded wait gives up
+
+// A part of an item: tiles t0 .. t1 - 1 of (sequence b, K/V head h, row group g).
+struct Part {
+    int b, h, g, t0, t1;
+    int len, first, n, start, base, pre, tiles;
+    // Keys of tile i up to its last one any row may see, whether some rows start inside it, and
+    // whether some keys are hidden from some row.
+    __device__ __forceinline__ int keys(int i) const {
+        return min(kKeys, i < pre ? len - (base + i * kKeys) : n - (i - pre) * kKeys);
+    }
+    __device__ __forceinline__ bool windowed(int window, int i) const {
+        return window && i < pre && base + i * kKeys < start + n - 1;
+    }
+    __device__ __forceinline__ bool edge(int window, int i) const {
+        return i >= pre || keys(i) < kKeys || windowed(window, i) || base + i * kKeys < start;
+    }
+};
 
 struct Ctl {
     uint64_t full[kMaxSlots], empty[kMaxSlots];
     uint64_t s_full[2], s_free[2];
+    uint64_t part_full[kParts], part_free[kParts];
+    Part part[kParts];
     uint64_t q_ready, p_full, o_done, v_ready[4], v_fix[4], done;
     uint32_t tmem_base;
     int abort, poison;
@@ -75,6 +100,7 @@ struct Ctl {
     float red[4][128];
     int start[128];      // first cached position a row sees
     int depth[128];
+    int tok[128], hd[128];  // a row's token and its head's offset in elements
     uint32_t mask[8][128];
 };
 
@@ -103,8 +129,9 @@ struct Seq {
     int pre, tiles, groups;
 };
 
-__device__ __forceinline__ Seq load_seq(const Params& p, int b) {
-    Seq s;
+// The kernel's roles share this code out of line, here and below: inlined everywhere it would not
+// fit the instruction cache, which costs more than the calls.
+__device__ __noinline__ void load_seq(const Params& p, int b, Seq& s) {
     const int gqa = p.heads / p.kv_heads;
     s.first = min(max(p.cu[b], 0), p.n_tokens);
     s.n = min(min(max(p.cu[b + 1] - s.first, 0), p.n_tokens - s.first), p.max_nodes);
@@ -114,7 +141,6 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int b) {
     s.pre = s.start < s.len ? (s.len - s.base + kKeys - 1) / kKeys : 0;
     s.tiles = s.n ? s.pre + (s.n + kKeys - 1) / kKeys : 0;
     s.groups = (s.n * gqa + p.N - 1) / p.N;
-    return s;
 }
 
 // Sum of the block's values, to every thread.
@@ -126,82 +152,112 @@ __device__ __forceinline__ long long block_total(long long v, long long* red) {
     if (lane == 0) red[w] = v;
     __syncthreads();
     long long t = 0;
+#pragma unroll 1
     for (int i = 0; i < nw; ++i) t += red[i];
     return t;
 }
 
-__device__ __forceinline__ long long seq_tiles(const Params& p, int b) {
-    const Seq s = load_seq(p, b);
-    return (long long)s.tiles * s.groups * p.kv_heads;
+// An item is as long as its tiles and kItemCost more, ahead of them.
+__device__ __forceinline__ long long seq_units(const Params& p, int b) {
+    Seq s;
+    load_seq(p, b, s);
+    return s.tiles ? (long long)(s.tiles + kItemCost) * s.groups * p.kv_heads : 0;
 }
 
 __device__ __forceinline__ long long share_begin(long long total, int grid, int c) { return total * c / grid; }
 
-// Walks the parts of items in this block's share.
-struct Walk {
-    Seq s;
-    int b, h, g, t;
-    long long pos, end;
-    int t0, t1;  // the part: tiles t0 .. t1 - 1 of item (b, h, g)
-    __device__ void open(const Params& p, const Ctl& c) {
-        pos = c.begin;
-        end = c.end;
-        b = c.seq0;
-        if (pos >= end) return;
-        s = load_seq(p, b);
-        const long long per = (long long)s.tiles * s.groups;
-        h = (int)(c.rem0 / per);
-        const long long r = c.rem0 % per;
-        g = (int)(r / s.tiles);
-        t = (int)(r % s.tiles);
-    }
-    __device__ bool next(const Params& p) {
-        if (pos >= end) return false;
-        if (t == s.tiles) {
-            t = 0;
-            if (++g == s.groups) {
-                g = 0;
-                if (++h == p.kv_heads) {
-                    h = 0;
-                    do s = load_seq(p, ++b);
-                    while (s.tiles == 0);
-                }
-            }
+// A place in the ring of slots and the parity of its current use.
+struct Place {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void step(int slots) {
+        if (++slot == slots) {
+            slot = 0;
+            phase ^= 1;
         }
-        t0 = t;
-        t1 = (int)min((long long)s.tiles, t0 + (end - pos));
-        pos += t1 - t0;
-        t = t1;
-        return true;
-    }
-    // Keys of tile i up to its last one any row may see, and whether some of them are hidden from
-    // some row.
-    __device__ __forceinline__ int keys(int i) const {
-        return i < s.pre ? min(kKeys, s.len - (s.base + i * kKeys)) : min(kKeys, s.n - (i - s.pre) * kKeys);
-    }
-    __device__ __forceinline__ bool windowed(const Params& p, int i) const {  // rows start inside the tile
-        return p.window && i < s.pre && s.base + i * kKeys < s.start + s.n - 1;
-    }
-    __device__ __forceinline__ bool edge(const Params& p, int i) const {
-        return i >= s.pre || keys(i) < kKeys || windowed(p, i) || s.base + i * kKeys < s.start;
     }
 };
 
+// Bounded wait that also gives up as soon as another warp of the block has.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
     const uint64_t t0 = global_ns();
-    while (!mbar_try_wait_sleep(bar, parity, 1000000u)) {
-        if (*abort) return false;
-        if (global_ns() - t0 > kWaitLimitNs) {
+#pragma unroll 1
+    while (!mbar_try_wait_sleep(bar, parity, 1000000u))
+        if (*abort || global_ns() - t0 > kWaitLimitNs) {
             *abort = 1;
-            atomicExch(&g_tree_err, 1);
             return false;
         }
-    }
     return true;
 }
 
+// Writes down the parts of this block's share, one by one; t0 = t1 ends them.
+__device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* abort) {
+    Place at;
+    long long pos = c.begin;
+    const long long end = c.end;
+    Seq s;
+    int b = 0, h = 0, g = 0, u = 0;
+    if (pos < end) {
+        b = c.seq0;
+        load_seq(p, b, s);
+        const long long item = s.tiles + kItemCost, r = c.rem0 % (item * s.groups);
+        h = (int)(c.rem0 / (item * s.groups));
+        g = (int)(r / item);
+        u = (int)(r % item);
+    }
+#pragma unroll 1
+    while (true) {
+        int t0 = 0, t1 = 0;
+#pragma unroll 1
+        while (pos < end && t0 == t1) {
+            const int item = s.tiles + kItemCost;
+            if (u == item) {
+                u = 0;
+                if (++g == s.groups) {
+                    g = 0;
+                    if (++h == p.kv_heads) {
+                        h = 0;
+                        do load_seq(p, ++b, s);
+                        while (s.tiles == 0);
+                    }
+                }
+                continue;
+            }
+            const int v = (int)min((long long)item, u + (end - pos));
+            pos += v - u;
+            t0 = max(0, u - kItemCost);
+            t1 = max(0, v - kItemCost);
+            u = v;
+        }
+        if (!wait(&c.part_free[at.slot], at.phase ^ 1, abort)) return;
+        c.part[at.slot] = Part{b, h, g, t0, t1, s.len, s.first, s.n, s.start, s.base, s.pre, s.tiles};
+        mbar_arrive(&c.part_full[at.slot]);
+        if (t0 == t1) return;
+        at.step(kParts);
+    }
+}
+
+// The next part, for a warp (or its one thread); false at the end.
+__device__ __forceinline__ bool next_part(Ctl& c, Place& at, Part& w, bool leader, volatile int* abort) {
+    if (!wait(&c.part_full[at.slot], at.phase, abort)) return false;
+    w = c.part[at.slot];
+    if (leader) mbar_arrive(&c.part_free[at.slot]);
+    at.step(kParts);
+    return w.t0 < w.t1;
+}
+
 __device__ __forceinline__ void group_bar(int grp) { asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory"); }
+// The AND over the 256 threads of the softmax warps.
+__device__ __forceinline__ bool all_256(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.and.pred q, 3, 256, p;\n selp.u32 %0, 1, 0, q;\n}"
+        : "=r"(r)
+        : "r"((uint32_t)v)
+        : "memory");
+    return r != 0;
+}
 __device__ __forceinline__ bool group_or(int grp, bool v) {
     uint32_t r;
     asm volatile(
@@ -212,19 +268,32 @@ __device__ __forceinline__ bool group_or(int grp, bool v) {
     return r != 0;
 }
 
-__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+__device__ __forceinline__ void tma_3d(void* dst, uint64_t map, int x, int y, int z, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
         "[%5];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
-__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+__device__ __forceinline__ void tma_4d(void* dst, uint64_t map, int x, int y, int z, int w, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
         "[%6];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
         : "memory");
+}
+
+// 8 or 16 consecutive tensor-memory columns of this thread's lane.
+__device__ __forceinline__ void load16(uint32_t ta, bool both, float (&v)[16]) {
+    if (both) {
+        tc::ld16(ta, v);
+    } else {
+        float h[8];
+        tc::ld8(ta, h);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = h[j];
+    }
+    tc::wait_ld();
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -253,78 +322,77 @@ __device__ __forceinline__ bool not_finite(uint16_t v) {
     return kBf16 ? (v & 0x7f80) == 0x7f80 : (v & 0x7c00) == 0x7c00;
 }
 
-// Reduce-scatter of per-lane values v[0 .. P) (P a power of two, 8 .. 64) over the warp: each step
-// sends the half the lane gives away. Afterwards the lane holds max(1, P / 32) reduced values in
-// v[0 ..], of rows scatter_row<P>(lane) onwards (for P < 32 several lanes hold the same row).
-template <int P, bool kMax>
-__device__ __forceinline__ void reduce_scatter(float (&v)[P], int lane) {
+// Reduce-scatter of eight per-lane values over the warp: each of three exchanges sends the half the
+// lane gives away, two more finish the four lanes that share a row. Lane 4 r + (0 .. 3) ends with
+// row r's reduction in v[0].
+template <bool kMax>
+__device__ __forceinline__ void reduce_scatter8(float (&v)[8], int lane) {
     auto op = [](float a, float b) { return kMax ? fmaxf(a, b) : a + b; };
-    int bit = 16;
 #pragma unroll
-    for (int n = P / 2; n >= 1 && bit >= 1; n >>= 1, bit >>= 1) {
+    for (int n = 4, bit = 16; n >= 1; n >>= 1, bit >>= 1) {
         const bool up = lane & bit;
 #pragma unroll
-        for (int i = 0; i < P / 2; ++i)
+        for (int i = 0; i < 4; ++i)
             if (i < n) {
                 const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
                 v[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, bit));
             }
     }
-#pragma unroll
-    for (int k = 2; k >= 1; k >>= 1)
-        if (k <= bit) v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], k));
+    v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 2));
+    v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 1));
 }
-template <int P>
-__device__ __forceinline__ int scatter_row(int lane) {
-    int r = 0, bit = 16;
-#pragma unroll
-    for (int n = P / 2; n >= 1 && bit >= 1; n >>= 1, bit >>= 1)
-        if (lane & bit) r += n;
-    return r;
-}
-
-__host__ __device__ constexpr int pow2_at_least(int n) { return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : 64; }
 
 // Whether row r of the part sees key k (0 .. 127) of tile i.
-__device__ __forceinline__ bool sees(const Params& p, const Walk& w, const Ctl& c, int i, int k, int r) {
-    if (i < w.s.pre) {
-        const int j = w.s.base + i * kKeys + k;
-        return j < w.s.len && j >= c.start[r];
+__device__ __forceinline__ bool sees(const Params& p, const Part& w, const Ctl& c, int i, int k, int r) {
+    if (i < w.pre) {
+        const int j = w.base + i * kKeys + k;
+        return j < w.len && j >= c.start[r];
     }
-    const int j = (i - w.s.pre) * kKeys + k;
-    if (j >= w.s.n || !((c.mask[j >> 5][r] >> (j & 31)) & 1)) return false;
-    return !p.window || c.depth[r] - min(max(p.depth[w.s.first + j], 0), w.s.n - 1) < p.window;
+    const int j = (i - w.pre) * kKeys + k;
+    if (j >= w.n || !((c.mask[j >> 5][r] >> (j & 31)) & 1)) return false;
+    return !p.window || c.depth[r] - min(max(p.depth[w.first + j], 0), w.n - 1) < p.window;
 }
 
-// Address of V's row for key k of tile i (null: no such row).
-template <int D>
-__device__ __noinline__ const uint16_t* v_row(const Params& p, const Walk& w, int i, int k) {
-    if (i < w.s.pre) {
-        const int j = w.s.base + i * kKeys + k;
-        if (j < w.s.start || j >= w.s.len) return nullptr;
+// V's row for key k of tile i (null: no such row).
+__device__ const uint16_t* v_row(const Params& p, const Part& w, int i, int k, int dim) {
+    if (i < w.pre) {
+        const int j = w.base + i * kKeys + k;
+        if (j < w.start || j >= w.len) return nullptr;
         const int page = p.table[(long long)w.b * p.width + j / p.page_size];
         if (page < 0 || page >= p.pages) return nullptr;
         return reinterpret_cast<const uint16_t*>(p.v_pool) + page * p.page_stride +
-               ((long long)(j % p.page_size) * p.kv_heads + w.h) * D;
+               ((long long)(j % p.page_size) * p.kv_heads + w.h) * dim;
     }
-    const int j = (i - w.s.pre) * kKeys + k;
-    if (j >= w.s.n) return nullptr;
-    return reinterpret_cast<const uint16_t*>(p.v_new) + (w.s.first + j) * p.new_stride + w.h * D;
+    const int j = (i - w.pre) * kKeys + k;
+    if (j >= w.n) return nullptr;
+    return reinterpret_cast<const uint16_t*>(p.v_new) + (w.first + j) * p.new_stride + w.h * dim;
 }
 
-// The infinities and NaN that were taken out of this part's V tiles, added to the outputs v of rows
-// r0 .. r0 + 7 in dimension d.
-template <int D, bool kBf16>
-__device__ __noinline__ void add_poison(const Params& p, const Walk& w, const Ctl& c, int d, int r0, float (&v)[8]) {
+// What the infinities and NaN taken out of this part's V tiles add to row r in dimension d.
+template <bool kBf16>
+__device__ __noinline__ float poison_of(const Params& p, Part w, const Ctl& c, int dim, int d, int r) {
+    float sum = 0.f;
     for (int i = w.t0; i < w.t1; ++i) {
-        if (!(i >= w.s.pre || w.windowed(p, i))) continue;
+        if (!(i >= w.pre || w.windowed(p.window, i))) continue;
         for (int k = 0; k < w.keys(i); ++k) {
-            const uint16_t* row = v_row<D>(p, w, i, k);
-            if (!row || !not_finite<kBf16>(row[d])) continue;
-            for (int j = 0; j < 8; ++j)
-                if (sees(p, w, c, i, k, r0 + j)) v[j] += unpack1<kBf16>(row[d]);
+            const uint16_t* row = v_row(p, w, i, k, dim);
+            if (row && not_finite<kBf16>(row[d]) && sees(p, w, c, i, k, r)) sum += unpack1<kBf16>(row[d]);
         }
     }
+    return sum;
+}
+
+// Takes infinities and NaN out of eight values; whether there were any.
+template <bool kBf16>
+__device__ __forceinline__ bool clean(uint4& v) {
+    bool dirty = false;
+    uint32_t* x = &v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (not_finite<kBf16>((uint16_t)x[i])) x[i] &= 0xffff0000u, dirty = true;
+        if (not_finite<kBf16>((uint16_t)(x[i] >> 16))) x[i] &= 0x0000ffffu, dirty = true;
+    }
+    return dirty;
 }
 
 // kNH: the most rows a softmax group takes (N / 2 of them are used, a multiple of 8).
@@ -348,17 +416,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
+#pragma unroll 1
         for (int s = 0; s < slots; ++s) {
             mbar_init(&c.full[s], 1);
             mbar_init(&c.empty[s], 1);
         }
+#pragma unroll 1
         for (int b = 0; b < 2; ++b) {
             mbar_init(&c.s_full[b], 1);
             mbar_init(&c.s_free[b], kSoftWarps);
         }
+#pragma unroll 1
+        for (int i = 0; i < kParts; ++i) {
+            mbar_init(&c.part_full[i], 1);
+            mbar_init(&c.part_free[i], kSoftWarps + 2);
+        }
         mbar_init(&c.q_ready, kSoftWarps);
         mbar_init(&c.p_full, kSoftWarps);
         mbar_init(&c.o_done, 1);
+#pragma unroll 1
         for (int i = 0; i < 4; ++i) {
             mbar_init(&c.v_ready[i], 1);
             mbar_init(&c.v_fix[i], kSoftWarps);
@@ -368,11 +444,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         c.poison = 0;
         mbar_init_fence();
     }
-    if (warp == 1) tc::alloc(&c.tmem_base, p.tmem_cols);
+    if (warp == kIssuer) tc::alloc(&c.tmem_base, p.tmem_cols);
 
-    // This block's share of all tiles.
+    // This block's share of all units.
     long long mine = 0;
-    for (int b = threadIdx.x; b < p.seqs; b += kThreads) mine += seq_tiles(p, b);
+#pragma unroll 1
+    for (int b = threadIdx.x; b < p.seqs; b += kThreads) mine += seq_units(p, b);
     const long long total = block_total(mine, c.scan);
     const long long begin = share_begin(total, gridDim.x, blockIdx.x), end = share_begin(total, gridDim.x, blockIdx.x + 1);
     if (threadIdx.x == 0) {
@@ -380,9 +457,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         c.end = end;
     }
     long long before = 0;
+#pragma unroll 1
     for (int b0 = 0; warp == 0 && begin < end && b0 < p.seqs; b0 += 32) {
         const int b = b0 + lane;
-        const long long mt = b < p.seqs ? seq_tiles(p, b) : 0;
+        const long long mt = b < p.seqs ? seq_units(p, b) : 0;
         long long x = mt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -404,126 +482,152 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t o_col = 2 * (uint32_t)N;  // S^T buffers, then the O^T tiles of 128 dims
     pdl_launch_dependents();
 
-    Walk w;
-    w.open(p, c);
-    if (warp == 0) {
+    if (warp == kProducer) {
         // ------------------------------------------------------------------ producer
-        int q = 0;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        Part w;
+        Place at, list;
+        int used = 0;
         bool ok = true;
         const int kb = lane & 15, half = lane >> 4;  // up to 16 key boxes, two halves of 64 dims
-        auto ids = [&](int i) {  // page of this lane's key box in tile i
-            const int j = w.s.base + i * kKeys + kb * p.box;
-            return i < w.s.pre && kb * p.box < kKeys && j < w.s.len ? p.table[(long long)w.b * p.width + j / p.page_size] : -1;
-        };
-        auto load = [&](const CUtensorMap* pool, const CUtensorMap* fresh, int i, int page) {
-            const bool old = i < w.s.pre;
-            const int rows = old ? p.box : kTreeBox;
-            const int boxes = (w.keys(i) + rows - 1) / rows;
-            const bool mine = kb < boxes && half < kHalves;
-            const int j = w.s.base + i * kKeys + kb * p.box;
-            for (int ci = 0; ci < kChunks && ok; ++ci, ++q) {
-                const int slot = q % slots;
-                if (q >= slots) ok = wait(&c.empty[slot], ((q / slots) + 1) & 1, abort);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
-                if (lane == 0) mbar_expect_tx(&c.full[slot], (uint32_t)(boxes * rows) * 128 * kHalves);
-                __syncwarp();
-                if (mine) {
-                    unsigned char* dst = ring + slot * kSlotBytes + half * kBoxBytes + kb * rows * 128;
-                    const int x = 128 * ci + 64 * half;
-                    // A page id out of range is an out-of-range coordinate: the box reads as zeros.
-                    if (old) tma_4d(dst, pool, x, w.h, j % p.page_size, page < 0 ? p.pages : page, &c.full[slot]);
-                    else tma_3d(dst, fresh, x, w.h, w.s.first + (i - w.s.pre) * kKeys + kb * kTreeBox, &c.full[slot]);
+        const uint64_t kd = reinterpret_cast<uint64_t>(&kmap), vd = reinterpret_cast<uint64_t>(&vmap);
+        const uint64_t knd = reinterpret_cast<uint64_t>(&knmap), vnd = reinterpret_cast<uint64_t>(&vnmap);
+#pragma unroll 1
+        while (ok) {
+            ok = next_part(c, list, w, false, abort);
+            ok = __all_sync(0xffffffffu, ok);  // every lane has its copy
+            if (lane == 0) mbar_arrive(&c.part_free[(list.slot + kParts - 1) % kParts]);
+            if (!ok) break;
+            const int32_t* row = p.table + (long long)w.b * p.width;
+            auto ids = [&](int i) {  // page of this lane's key box in tile i
+                const int j = w.base + i * kKeys + kb * p.box;
+                return i < w.pre && kb * p.box < kKeys && j < w.len ? row[j / p.page_size] : -1;
+            };
+            int id0 = -1, id1 = ids(w.t0), id2 = -1;
+#pragma unroll 1
+            for (int st = 2 * w.t0; st <= 2 * w.t1 + 1 && ok; ++st) {  // K of tile i = st / 2, then V of tile i - 1
+                const bool is_v = st & 1;
+                const int tile = is_v ? (st >> 1) - 1 : st >> 1;
+                if (!is_v) id2 = tile + 1 < w.t1 ? ids(tile + 1) : -1;
+                const int page = is_v ? id0 : id1;
+                if (is_v) {
+                    id0 = id1;
+                    id1 = id2;
+                }
+                if (tile < w.t0 || tile >= w.t1) continue;
+                const bool old = tile < w.pre;
+                const int rows = old ? p.box : kTreeBox, boxes = (w.keys(tile) + rows - 1) / rows;
+                const int j = w.base + tile * kKeys + kb * p.box;
+                // A page id out of range is an out-of-range coordinate: the box reads as zeros.
+                const int z = old ? j % p.page_size : w.first + (tile - w.pre) * kKeys + kb * kTreeBox;
+                const int pg = page < 0 ? p.pages : page;
+                const uint64_t map = old ? (is_v ? vd : kd) : (is_v ? vnd : knd);
+                const bool mine = kb < boxes && half < kHalves;
+#pragma unroll 1
+                for (int ci = 0; ci < kChunks; ++ci) {
+                    ok = wait(&c.empty[at.slot], at.phase ^ 1, abort);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(&c.full[at.slot], (uint32_t)(boxes * rows) * 128 * kHalves);
+                    __syncwarp();
+                    if (mine) {
+                        unsigned char* dst = ring + at.slot * kSlotBytes + half * kBoxBytes + kb * rows * 128;
+                        const int x = 128 * ci + 64 * half;
+                        if (old) tma_4d(dst, map, x, w.h, z, pg, &c.full[at.slot]);
+                        else tma_3d(dst, map, x, w.h, z, &c.full[at.slot]);
+                    }
+                    at.step(slots);
+                    ++used;
                 }
             }
-        };
-        while (ok && w.next(p)) {
-            int id0 = -1, id1 = ids(w.t0);
-            for (int i = w.t0; i <= w.t1 && ok; ++i) {
-                const int id2 = i + 1 < w.t1 ? ids(i + 1) : -1;
-                if (i < w.t1) load(&kmap, &knmap, i, id1);
-                if (i > w.t0 && ok) load(&vmap, &vnmap, i - 1, id0);
-                id0 = id1;
-                id1 = id2;
-            }
         }
-        // Every issued copy lands before the block can exit.
-        if (lane == 0)
-            for (int i = max(0, q - slots); i < q; ++i)
-                if (!mbar_wait(&c.full[i % slots], (i / slots) & 1)) atomicExch(&g_tree_err, 1);
-    } else if (warp == 1) {
-        // ------------------------------------------------------------------ MMA issuer
+        // Every issued copy lands before the block can exit: the last use of each slot.
         if (lane == 0) {
+#pragma unroll 1
+            for (int i = max(0, used - slots); i < used; ++i)
+                if (!mbar_wait(&c.full[i % slots], (i / slots) & 1)) *abort = 1;
+        }
+    } else if (warp == kIssuer) {
+        // ------------------------------------------------------------------ MMA issuer
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (lane == 0) {
+            Part w;
+            Place list;
             const uint32_t id_s = tc::idesc_16(kKeys, N, kBf16, false, false);
             const uint32_t id_o = tc::idesc_16(128, N, kBf16, true, true);
-            const uint32_t q_addr = smem_u32(qs), p_addr = smem_u32(ps), r_addr = smem_u32(ring);
-            const uint32_t blk = (uint32_t)N * 128;
-            int q = 0, tile = 0, otile = 0, part = 0, fix = 0;
+            // Descriptors of the ring's first slot, of Q and of P; other places add their distance in
+            // 16-byte units.
+            const uint64_t k_desc = tc::desc_sw128(smem_u32(ring)), v_desc = tc::desc_sw128_mn(smem_u32(ring), kBoxBytes, 1024);
+            const uint64_t q_desc = tc::desc_sw128(smem_u32(qs)), p_desc = tc::desc_sw128_mn(smem_u32(ps), kBoxBytes, 1024);
+            const uint32_t blk = (uint32_t)N * 8;  // one 64-dim block of Q
+            Place at;
+            int tile = 0, otile = 0, part = 0, fix = 0;
             bool ok = true;
-            auto issue_s = [&]() {
-                const int b = tile & 1;
-                if (tile >= 2 && !wait(&c.s_free[b], ((tile >> 1) - 1) & 1, abort)) return false;
-                for (int ci = 0; ci < kChunks; ++ci, ++q) {
-                    const int slot = q % slots;
-                    if (!wait(&c.full[slot], (q / slots) & 1, abort)) return false;
-                    tc::fence_after_sync();
-                    const uint32_t sa = r_addr + slot * kSlotBytes;
-#pragma unroll
-                    for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            tc::mma_ss(tmem + b * N, tc::desc_sw128(sa + h * kBoxBytes + kk * 32),
-                                       tc::desc_sw128(q_addr + (uint32_t)(2 * ci + h) * blk + kk * 32), id_s,
-                                       (ci | h | kk) ? 1u : 0u);
-                    tc::commit(&c.empty[slot]);
-                }
-                tc::commit(&c.s_full[b]);
-                ++tile;
-                return true;
-            };
-            auto issue_o = [&](int i) {
-                if (!wait(&c.p_full, otile & 1, abort)) return false;
-                tc::fence_after_sync();
-                const int steps = (w.keys(i) + 15) >> 4;
-                const bool edge = w.edge(p, i);
-                for (int ci = 0; ci < kChunks; ++ci, ++q) {
-                    const int slot = q % slots;
-                    if (!wait(&c.full[slot], (q / slots) & 1, abort)) return false;
-                    if (edge) {  // the softmax warps clean the chunk first
-                        mbar_arrive(&c.v_ready[ci]);
-                        if (!wait(&c.v_fix[ci], fix & 1, abort)) return false;
-                    }
-                    tc::fence_after_sync();
-                    const uint32_t sa = r_addr + slot * kSlotBytes;
-                    for (int kk = 0; kk < steps; ++kk)
-                        // V^T rows are the slot's dims, two 64-dim boxes apart (with D = 64 the lanes
-                        // 64 .. 127 multiply whatever follows in shared memory, and are never read).
-                        tc::mma_ss(tmem + o_col + ci * N, tc::desc_sw128_mn(sa + kk * 2048, kBoxBytes, 1024),
-                                   tc::desc_sw128_mn(p_addr + kk * 2048, kBoxBytes, 1024), id_o,
-                                   (i > w.t0 || kk > 0) ? 1u : 0u);
-                    tc::commit(&c.empty[slot]);
-                }
-                tc::commit(&c.o_done);
-                fix += edge;
-                ++otile;
-                return true;
-            };
-            while (ok && w.next(p)) {
+#pragma unroll 1
+            while (ok && next_part(c, list, w, true, abort)) {
                 ok = wait(&c.q_ready, part++ & 1, abort);
-                if (ok) {
-                    tc::fence_after_sync();
-                    ok = issue_s();
+                tc::fence_after_sync();
+                // S of tile i, then O of tile i - 1.
+#pragma unroll 1
+                for (int i = w.t0; i <= w.t1 && ok; ++i) {
+                    if (i < w.t1) {
+                        const int b = tile & 1;
+                        if (tile >= 2) ok = wait(&c.s_free[b], ((tile >> 1) - 1) & 1, abort);
+#pragma unroll 1
+                        for (int ci = 0; ci < kChunks && ok; ++ci) {
+                            ok = wait(&c.full[at.slot], at.phase, abort);
+                            tc::fence_after_sync();
+                            const uint64_t a = k_desc + at.slot * (kSlotBytes >> 4), q = q_desc + 2 * ci * blk;
+#pragma unroll
+                            for (int kk = 0; kk < 4 * kHalves; ++kk)
+                                tc::mma_ss(tmem + b * N, a + (kk >> 2) * (kBoxBytes >> 4) + (kk & 3) * 2,
+                                           q + (kk >> 2) * blk + (kk & 3) * 2, id_s, (ci | kk) ? 1u : 0u);
+                            tc::commit(&c.empty[at.slot]);
+                            at.step(slots);
+                        }
+                        tc::commit(&c.s_full[b]);
+                        ++tile;
+                    }
+                    if (i > w.t0 && ok) {
+                        ok = wait(&c.p_full, otile & 1, abort);
+                        tc::fence_after_sync();
+                        const int steps = (w.keys(i - 1) + 15) >> 4;
+                        const bool edge = w.edge(p.window, i - 1);
+#pragma unroll 1
+                        for (int ci = 0; ci < kChunks && ok; ++ci) {
+                            ok = wait(&c.full[at.slot], at.phase, abort);
+                            if (edge) {  // the softmax warps clean the chunk first
+                                mbar_arrive(&c.v_ready[ci]);
+                                ok = wait(&c.v_fix[ci], fix & 1, abort);
+                            }
+                            tc::fence_after_sync();
+                            const uint64_t a = v_desc + at.slot * (kSlotBytes >> 4);
+                            // V^T rows are the slot's dims, two 64-dim boxes apart (with D = 64 the lanes
+                            // 64 .. 127 multiply whatever follows in shared memory, and are never read).
+#pragma unroll 2
+                            for (int kk = 0; kk < steps; ++kk)
+                                tc::mma_ss(tmem + o_col + ci * N, a + kk * 128, p_desc + kk * 128, id_o,
+                                           (i - 1 > w.t0 || kk > 0) ? 1u : 0u);
+                            tc::commit(&c.empty[at.slot]);
+                            at.step(slots);
+                        }
+                        tc::commit(&c.o_done);
+                        fix += edge;
+                        ++otile;
+                    }
                 }
-                for (int i = w.t0; i < w.t1 && ok; ++i) ok = (i + 1 >= w.t1 || issue_s()) && issue_o(i);
             }
             tc::commit(&c.done);  // every MMA has completed before tensor memory is freed
-            if (!mbar_wait(&c.done, 0)) atomicExch(&g_tree_err, 1);
+            if (!mbar_wait(&c.done, 0)) *abort = 1;
         }
-    } else if (warp >= 4) {
+    } else if (warp < kSoftWarps) {
         // ------------------------------------------------------------------ softmax
-        constexpr int kP = pow2_at_least(kNH);
-        const int sw = warp - 4, grp = sw >> 2, qd = sw & 3;
-        const int tid = sw * 32 + lane, gt = tid & 127;   // 0..255; 0..127 in the group
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+        Part w;
+        Place list;
+        constexpr int kCh = kNH == 64 ? 32 : kNH;         // rows whose scores are in registers at once
+        const int grp = warp >> 2, qd = warp & 3;
+        const int tid = threadIdx.x, gt = tid & 127;      // 0..255; 0..127 in the group
         const int key = qd * 32 + lane;                   // TMEM lane
         const int r0 = grp * nh;                          // the group's rows r0 .. r0 + nh - 1
         const uint32_t lanes = (uint32_t)(qd * 32) << 16;
@@ -533,28 +637,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         float l[kNH];
         // After a wait that gave up, these warps go on (on meaningless values) to the end of the share:
         // none of them may leave while others stand at a barrier of the group.
-        while (w.next(p)) {
+#pragma unroll 1
+        while (true) {
+            const bool more = all_256(next_part(c, list, w, false, abort));
+            if (lane == 0) mbar_arrive(&c.part_free[(list.slot + kParts - 1) % kParts]);
+            if (!more) break;
             // Rows of this part: r -> node (g N + r) / gqa, query head h gqa + (g N + r) % gqa.
-            const int R = min(N, w.s.n * gqa - w.g * N);
+            const int R = min(N, w.n * gqa - w.g * N);
             if (tid < N) {
-                const int node = min((w.g * N + tid) / gqa, w.s.n - 1), tok = w.s.first + node;
-                const int dep = p.window ? min(max(p.depth[tok], 0), w.s.n - 1) : 0;
+                const int row = w.g * N + tid, node = min(row / gqa, w.n - 1), tok = w.first + node;
+                c.tok[tid] = tok;
+                c.hd[tid] = (w.h * gqa + row % gqa) * D;
+                const int dep = p.window ? min(max(p.depth[tok], 0), w.n - 1) : 0;
                 c.nref[tid] = kUnset;
                 c.depth[tid] = dep;
-                c.start[tid] = p.window ? max(0, w.s.len + dep - p.window + 1) : 0;
-                for (int i = 0; i * 32 < w.s.n; ++i) c.mask[i][tid] = p.mask[(long long)tok * p.mask_words + i];
+                c.start[tid] = p.window ? max(0, w.len + dep - p.window + 1) : 0;
+#pragma unroll 1
+                for (int i = 0; i * 32 < w.n; ++i) c.mask[i][tid] = p.mask[(long long)tok * p.mask_words + i];
             }
             if (tid == 0) c.poison = 0;
+            asm volatile("bar.sync 3, 256;" ::: "memory");
             // The queries, into the MMA's K-major layout (S of the part before has completed).
-            for (int e = tid; e < N * (D / 8); e += 256) {
-                const int r = e / (D / 8), ch = e % (D / 8);
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < R) {
-                    const int row = w.g * N + r;
-                    v = __ldg(reinterpret_cast<const uint4*>(
-                                  p.q + 2 * ((w.s.first + row / gqa) * p.q_stride + (w.h * gqa + row % gqa) * D)) + ch);
+            constexpr int kRowsAt = 256 / (D / 8);  // rows the 256 threads load at once
+            const int ch = tid % (D / 8);
+#pragma unroll 1
+            for (int rb = tid / (D / 8); rb < N; rb += 8 * kRowsAt) {
+                uint4 v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int r = rb + k * kRowsAt;
+                    v[k] = make_uint4(0, 0, 0, 0);
+                    if (r < R) v[k] = __ldg(reinterpret_cast<const uint4*>(p.q + 2 * (c.tok[r] * p.q_stride + c.hd[r])) + ch);
                 }
-                *reinterpret_cast<uint4*>(qs + (size_t)(ch >> 3) * N * 128 + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int r = rb + k * kRowsAt;
+                    if (r < N) *reinterpret_cast<uint4*>(qs + (size_t)(ch >> 3) * N * 128 + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v[k];
+                }
             }
             fence_proxy_async();
             asm volatile("bar.sync 3, 256;" ::: "memory");
@@ -562,61 +681,62 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int r = 0; r < kNH; ++r) l[r] = 0.f;
 
+#pragma unroll 1
             for (int i = w.t0; i < w.t1; ++i, ++tile) {
                 const int b = tile & 1;
+                const uint32_t st = tmem + lanes + b * N + r0;
                 wait(&c.s_full[b], (tile >> 1) & 1, abort);
-                tc::fence_after_sync();
-                float s[kNH];
-#pragma unroll
-                for (int e = 0; e < kNH / 8; ++e)
-                    if (8 * e < nh) {
-                        float v[8];
-                        tc::ld8(tmem + lanes + b * N + r0 + 8 * e, v);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) s[8 * e + j] = v[j];
-                    }
-                tc::wait_ld();
-                tc::fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&c.s_free[b]);
-                const bool edge = w.edge(p, i);
+                tc::fence_after_sync();
+                const bool edge = w.edge(p.window, i);
                 if (edge) {
-                    if (i < w.s.pre) {
-                        const int j = w.s.base + i * kKeys + key;
+                    // Hidden scores become -inf, in tensor memory.
+                    const bool old = i < w.pre;
+                    const int j = old ? w.base + i * kKeys + key : (i - w.pre) * kKeys + key;
+                    const int near = !old && p.window && j < w.n ? min(max(p.depth[w.first + j], 0), w.n - 1) + p.window : INT_MAX;
+                    const bool in = j < (old ? w.len : w.n);
+                    const uint32_t* word = c.mask[old ? 0 : (i - w.pre) * 4 + qd];
+#pragma unroll 1
+                    for (int e = 0; e < nh; e += 8) {
+                        float v[8];
+                        tc::ld8(st + e, v);
+                        tc::wait_ld();
 #pragma unroll
-                        for (int r = 0; r < kNH; ++r)
-                            if (r < nh && !(j < w.s.len && j >= c.start[r0 + r])) s[r] = -INFINITY;
-                    } else {
-                        const int j = (i - w.s.pre) * kKeys + key;
-                        const int word = (i - w.s.pre) * 4 + qd;
-                        const int near = p.window && j < w.s.n
-                                             ? min(max(p.depth[w.s.first + j], 0), w.s.n - 1) + p.window
-                                             : INT_MAX;
-#pragma unroll
-                        for (int r = 0; r < kNH; ++r)
-                            if (r < nh && !(j < w.s.n && ((c.mask[word][r0 + r] >> lane) & 1) && c.depth[r0 + r] < near))
-                                s[r] = -INFINITY;
+                        for (int k = 0; k < 8; ++k) {
+                            const int r = r0 + e + k;
+                            if (!(in && (old ? j >= c.start[r] : ((word[r] >> lane) & 1) && c.depth[r] < near))) v[k] = -INFINITY;
+                        }
+                        tc::st8(st + e, v);
                     }
+                    tc::wait_st();
                 }
-                // Does a score exceed its row's reference by more than kLazy?
+                // First look: does a score exceed its row's reference by more than kLazy? The scores
+                // stay in tensor memory and are read again for the exponentials, which leaves the
+                // registers to the row sums.
                 float over = -INFINITY;
+#pragma unroll 1
+                for (int f = 0; f < nh; f += 16) {
+                    float v[16];
+                    const bool both = f + 8 < nh;
+                    load16(st + f, both, v);
 #pragma unroll
-                for (int r = 0; r < kNH; r += 4)
-                    if (r < nh) {
-                        const float4 f = *reinterpret_cast<const float4*>(&c.nref[r0 + r]);
-                        over = fmaxf(fmaxf(over, fmaf(s[r], p.c, f.x)), fmaf(s[r + 1], p.c, f.y));
-                        over = fmaxf(fmaxf(over, fmaf(s[r + 2], p.c, f.z)), fmaf(s[r + 3], p.c, f.w));
-                    }
-                bool waited = false;
+                    for (int r = 0; r < 16; r += 4)
+                        if (r < 8 || both) {
+                            const float4 n = *reinterpret_cast<const float4*>(&c.nref[r0 + f + r]);
+                            over = fmaxf(over, fmaxf(fmaf(v[r], p.c, n.x), fmaf(v[r + 1], p.c, n.y)));
+                            over = fmaxf(over, fmaxf(fmaf(v[r + 2], p.c, n.z), fmaf(v[r + 3], p.c, n.w)));
+                        }
+                }
+                bool waited = tile == 0;
                 if (group_or(grp, over > kLazy)) {
-                    float m[kP];
-#pragma unroll
-                    for (int r = 0; r < kP; ++r) m[r] = r < kNH && r < nh ? s[r] * p.c : -INFINITY;
-                    reduce_scatter<kP, true>(m, lane);
-                    const int at = scatter_row<kP>(lane);
-#pragma unroll
-                    for (int j = 0; j < (kP > 32 ? 2 : 1); ++j)
-                        if (at + j < nh) c.red[qd][r0 + at + j] = m[j];
+#pragma unroll 1
+                    for (int e = 0; e < nh; e += 8) {
+                        float m[8];
+                        tc::ld8(st + e, m);
+                        tc::wait_ld();
+                        reduce_scatter8<true>(m, lane);
+                        c.red[qd][r0 + e + (lane >> 2)] = m[0] * p.c;
+                    }
                     group_bar(grp);
                     if (gt < nh) {
                         const int r = r0 + gt;
@@ -631,64 +751,87 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     group_bar(grp);
 #pragma unroll
-                    for (int r = 0; r < kNH; ++r)
-                        if (r < nh) l[r] *= c.corr[r0 + r];
+                    for (int r = 0; r < kNH; r += 4)
+                        if (r < nh) {
+                            const float4 f = *reinterpret_cast<const float4*>(&c.corr[r0 + r]);
+                            l[r] *= f.x;
+                            l[r + 1] *= f.y;
+                            l[r + 2] *= f.z;
+                            l[r + 3] *= f.w;
+                        }
                     if (i > w.t0) {
                         wait(&c.o_done, (tile - 1) & 1, abort);
+                        __syncwarp();
                         waited = true;
                         tc::fence_after_sync();
 #pragma unroll 1
-                        for (int ci = 0; ci < kChunks; ++ci)
-#pragma unroll 1
-                            for (int e = 0; e < nh; e += 8) {
-                                float v[8];
-                                const uint32_t ta = tmem + lanes + o_col + ci * N + r0 + e;
-                                tc::ld8(ta, v);
-                                tc::wait_ld();
+                        for (int e = 0; e < kChunks * nh; e += 8) {
+                            const int ci = e / nh, f = e - ci * nh;
+                            float v[8];
+                            const uint32_t ta = tmem + lanes + o_col + ci * N + r0 + f;
+                            tc::ld8(ta, v);
+                            tc::wait_ld();
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) v[j] *= c.corr[r0 + e + j];
-                                tc::st8(ta, v);
-                            }
+                            for (int j = 0; j < 8; ++j) v[j] *= c.corr[r0 + f + j];
+                            tc::st8(ta, v);
+                        }
                         tc::wait_st();
                     }
                 }
+                uint32_t pk[kNH / 2];
 #pragma unroll
-                for (int r = 0; r < kNH; r += 4)
-                    if (r < nh) {
-                        const float4 f = *reinterpret_cast<const float4*>(&c.nref[r0 + r]);
-                        s[r] = exp2_approx(fmaf(s[r], p.c, f.x));
-                        s[r + 1] = exp2_approx(fmaf(s[r + 1], p.c, f.y));
-                        s[r + 2] = exp2_approx(fmaf(s[r + 2], p.c, f.z));
-                        s[r + 3] = exp2_approx(fmaf(s[r + 3], p.c, f.w));
-                        l[r] += s[r];
-                        l[r + 1] += s[r + 1];
-                        l[r + 2] += s[r + 2];
-                        l[r + 3] += s[r + 3];
+                for (int f = 0; f < kNH; f += kCh)
+                    if (f < nh) {
+                        float s[kCh];
+#pragma unroll
+                        for (int e = 0; e < kCh; e += 8)
+                            if (f + e < nh) {
+                                float v[8];
+                                tc::ld8(st + f + e, v);
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) s[e + j] = v[j];
+                            }
+                        tc::wait_ld();
+                        if (f + kCh >= nh) {
+                            tc::fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&c.s_free[b]);
+                        }
+#pragma unroll
+                        for (int r = 0; r < kCh; r += 4)
+                            if (f + r < nh) {
+                                const float4 n = *reinterpret_cast<const float4*>(&c.nref[r0 + f + r]);
+                                const float e0 = exp2_approx(fmaf(s[r], p.c, n.x)), e1 = exp2_approx(fmaf(s[r + 1], p.c, n.y));
+                                const float e2 = exp2_approx(fmaf(s[r + 2], p.c, n.z)), e3 = exp2_approx(fmaf(s[r + 3], p.c, n.w));
+                                l[f + r] += e0;
+                                l[f + r + 1] += e1;
+                                l[f + r + 2] += e2;
+                                l[f + r + 3] += e3;
+                                pk[(f + r) / 2] = pack2<kBf16>(e0, e1);
+                                pk[(f + r) / 2 + 1] = pack2<kBf16>(e2, e3);
+                            }
                     }
                 // P V of the tile before has read the buffer.
-                if (tile > 0 && !waited) wait(&c.o_done, (tile - 1) & 1, abort);
+                if (!waited) wait(&c.o_done, (tile - 1) & 1, abort);
                 const uint32_t prow = key * 128;
 #pragma unroll
                 for (int e = 0; e < kNH / 8; ++e)
                     if (8 * e < nh) {
                         const int r = r0 + 8 * e;
-                        uint4 v;
-                        v.x = pack2<kBf16>(s[8 * e], s[8 * e + 1]);
-                        v.y = pack2<kBf16>(s[8 * e + 2], s[8 * e + 3]);
-                        v.z = pack2<kBf16>(s[8 * e + 4], s[8 * e + 5]);
-                        v.w = pack2<kBf16>(s[8 * e + 6], s[8 * e + 7]);
-                        *reinterpret_cast<uint4*>(ps + (r >> 6) * kBoxBytes + prow + ((((r & 63) >> 3) ^ (key & 7)) << 4)) = v;
+                        *reinterpret_cast<uint4*>(ps + (r >> 6) * kBoxBytes + prow + ((((r & 63) >> 3) ^ (key & 7)) << 4)) =
+                            make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
                     }
                 fence_proxy_async();
                 tc::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.p_full);
-                // Ring slots of this tile's V, in the producer's order: K(t0), then K(i + 1), V(i).
-                const int vq = q + (i - w.t0) * 2 * kChunks + (i + 1 < w.t1 ? 2 : 1) * kChunks;
                 if (edge) {
-                    const int rows = (w.keys(i) + 15) & ~15;
-                    const bool scan = i >= w.s.pre || w.windowed(p, i);
-                    const int lead = i < w.s.pre ? w.s.start - (w.s.base + i * kKeys) : 0;  // keys before every row's
+                    // Ring slots of this tile's V, in the producer's order: K(t0), then K(i + 1), V(i).
+                    const int vq = q + (i - w.t0) * 2 * kChunks + (i + 1 < w.t1 ? 2 : 1) * kChunks;
+                    const int keys = w.keys(i), rows = (keys + 15) & ~15;
+                    const bool scan = i >= w.pre || w.windowed(p.window, i);
+                    const int lead = i < w.pre ? w.start - (w.base + i * kKeys) : 0;  // keys before every row's
+#pragma unroll 1
                     for (int ci = 0; ci < kChunks; ++ci) {
                         const int slot = (vq + ci) % slots;
                         // v_ready first: the slot may still be a use behind, and a parity cannot tell a
@@ -696,23 +839,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                         wait(&c.v_ready[ci], fix & 1, abort);
                         wait(&c.full[slot], ((vq + ci) / slots) & 1, abort);
                         unsigned char* base = ring + slot * kSlotBytes;
+#pragma unroll 1
                         for (int e = tid; e < rows * 8 * kHalves; e += 256) {
-                            const int k = e / (8 * kHalves), ch = e % (8 * kHalves);
-                            uint4* at = reinterpret_cast<uint4*>(base + (ch >> 3) * kBoxBytes + k * 128 + (ch & 7) * 16);
-                            if (k >= w.keys(i) || k < lead) {
+                            const int k = e / (8 * kHalves), cc = e % (8 * kHalves);
+                            uint4* at = reinterpret_cast<uint4*>(base + (cc >> 3) * kBoxBytes + k * 128 + (cc & 7) * 16);
+                            if (k >= keys || k < lead) {
                                 *at = make_uint4(0, 0, 0, 0);
                             } else if (scan) {
                                 uint4 v = *at;
-                                bool dirty = false;
-                                auto clean = [&](uint32_t& x) {
-                                    if (not_finite<kBf16>((uint16_t)x)) x &= 0xffff0000u, dirty = true;
-                                    if (not_finite<kBf16>((uint16_t)(x >> 16))) x &= 0x0000ffffu, dirty = true;
-                                };
-                                clean(v.x);
-                                clean(v.y);
-                                clean(v.z);
-                                clean(v.w);
-                                if (dirty) {
+                                if (clean<kBf16>(v)) {
                                     *at = v;
                                     c.poison = 1;
                                 }
@@ -728,17 +863,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             q += (w.t1 - w.t0) * 2 * kChunks;
 
             // The part's result: sums over the keys, then O^T.
-            float m[kP];
-#pragma unroll
-            for (int r = 0; r < kP; ++r) m[r] = r < kNH ? l[r < kNH ? r : 0] : 0.f;
-            reduce_scatter<kP, false>(m, lane);
-            const int at = scatter_row<kP>(lane);
             group_bar(grp);
 #pragma unroll
-            for (int j = 0; j < (kP > 32 ? 2 : 1); ++j)
-                if (at + j < nh) c.red[qd][r0 + at + j] = m[j];
+            for (int r = 0; r < kNH; r += 8)
+                if (r < nh) {
+                    float m[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) m[j] = l[r + j];
+                    reduce_scatter8<false>(m, lane);
+                    c.red[qd][r0 + r + (lane >> 2)] = m[0];
+                }
             group_bar(grp);
-            const bool whole = w.t0 == 0 && w.t1 == w.s.tiles;
+            const bool whole = w.t1 - w.t0 == w.tiles;
             const int slot = 2 * blockIdx.x + (first_part ? 0 : 1);
             first_part = false;
             if (gt < nh) {
@@ -748,38 +884,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!whole) p.ml[(long long)slot * N + r] = make_float2(c.nref[r] == kUnset ? -INFINITY : -c.nref[r], sum);
             }
             wait(&c.o_done, (tile - 1) & 1, abort);
+            __syncwarp();
             tc::fence_after_sync();
             asm volatile("bar.sync 3, 256;" ::: "memory");  // also: every thread's poison flag
             const bool poison = c.poison != 0;
+            const int held = min(nh, R - r0);               // the group's rows that exist
 #pragma unroll 1
             for (int ci = 0; ci < kChunks; ++ci) {
                 const int d = 128 * ci + key;
+                uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + d;
+                float* part = p.part + ((long long)slot * N + r0) * D + d;
 #pragma unroll 1
-                for (int e = 0; e < nh && r0 + e < R; e += 8) {
+                for (int e = 0; e < held; e += 8) {
                     float v[8];
                     tc::ld8(tmem + lanes + o_col + ci * N + r0 + e, v);
                     tc::wait_ld();
                     if (D == 64 && key >= 64) continue;
-                    if (poison) add_poison<D, kBf16>(p, w, c, d, r0 + e, v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int r = r0 + e + j, row = w.g * N + r;
-                        if (r >= R) break;
-                        if (whole)
-                            reinterpret_cast<uint16_t*>(p.out)[(w.s.first + row / gqa) * p.out_stride +
-                                                               (w.h * gqa + row % gqa) * D + d] = pack1<kBf16>(v[j] * c.inv[r]);
-                        else
-                            __stcg(p.part + ((long long)slot * N + r) * D + d, v[j]);
+                        if (e + j >= held) break;
+                        const int r = r0 + e + j;
+                        if (poison) v[j] += poison_of<kBf16>(p, w, c, D, d, r);
+                        if (whole) out[c.tok[r] * p.out_stride + c.hd[r]] = pack1<kBf16>(v[j] * c.inv[r]);
+                        else __stcg(part + (e + j) * D, v[j]);
                     }
                 }
             }
             tc::fence_before_sync();
             asm volatile("bar.sync 3, 256;" ::: "memory");  // the row state is free for the next part
         }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kScheduler && lane == 0) schedule(p, c, abort);
     }
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == 1) {
+    if (threadIdx.x == 0 && *abort) atomicExch(&g_tree_err, 1);
+    if (warp == kIssuer) {
         tc::fence_after_sync();
         tc::dealloc(tmem, p.tmem_cols);
     }
@@ -795,11 +936,12 @@ __global__ void __launch_bounds__(32 * kJoinRows) tree_attn_join_kernel(const __
     pdl_wait();
     const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads, lane = threadIdx.x & 31;
     const int gqa = p.heads / p.kv_heads;
-    const Seq s = load_seq(p, b);
+    Seq s;
+    load_seq(p, b, s);
     if (s.n * gqa <= (int)blockIdx.y * kJoinRows) return;
     long long before = 0, all = 0;
     for (int i = threadIdx.x; i < p.seqs; i += 32 * kJoinRows) {
-        const long long t = seq_tiles(p, i);
+        const long long t = seq_units(p, i);
         all += t;
         if (i < b) before += t;
     }
@@ -808,10 +950,11 @@ __global__ void __launch_bounds__(32 * kJoinRows) tree_attn_join_kernel(const __
     const int row = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
     if (row >= s.n * gqa) return;
     const int g = row / p.N, r = row % p.N;
-    const long long a = before + ((long long)h * s.groups + g) * s.tiles, z = a + s.tiles;
+    const int item = s.tiles + kItemCost;
+    const long long a = before + ((long long)h * s.groups + g) * item, z = a + item;
     const auto block_of = [&](long long x) { return (int)(((x + 1) * p.grid - 1) / all); };
-    const int c0 = block_of(a), c1 = block_of(z - 1);
-    if (c0 == c1 && share_begin(all, p.grid, c0) <= a && share_begin(all, p.grid, c0 + 1) >= z) return;
+    const int c0 = block_of(a + kItemCost), c1 = block_of(z - 1);  // the blocks of its first and last tile
+    if (c0 == c1) return;
     const auto slot_of = [&](int c) { return (long long)(2 * c + (share_begin(all, p.grid, c) < a ? 1 : 0)); };
     float top = -INFINITY;
     for (int c = c0 + lane; c <= c1; c += 32) {
