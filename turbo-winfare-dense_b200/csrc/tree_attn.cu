@@ -63,6 +63,8 @@ constexpr float kLazy = 8.f;         // a reference moves when a score exceeds i
 constexpr size_t kSmemLimit = 232448;
 // What starting and finishing an item costs, in tiles, when the shares are cut.
 constexpr int kItemCost = 2;
+// Items of at most this many tiles are not split, which saves the second kernel.
+constexpr int kWholeTiles = 6;
 
 __device__ int g_tree_err;  // set when a bounded wait gives up
 
@@ -91,18 +93,34 @@ struct Ctl {
     uint64_t q_ready, p_full, o_done, v_ready[4], v_fix[4], done;
     uint32_t tmem_base;
     int abort, poison;
-    int seq0;            // where this block's share starts
-    long long rem0, begin, end;
-    long long scan[kThreads / 32 + 1];
-    float nref[128];     // negated reference maximum of a row, in powers of two
+    int seq0, rem0, begin, end;  // this block's share and where in which sequence it starts
+    int scan[kThreads / 32 + 1];
     float corr[128];     // factor of a row's sum and output when its reference moves
     float inv[128];
     float red[4][128];
-    int start[128];      // first cached position a row sees
-    int depth[128];
     int tok[128], hd[128];  // a row's token and its head's offset in elements
-    uint32_t mask[8][128];
 };
+
+// What a part's rows carry, twice: the next part's is set up before the current one is written out.
+struct Rows {
+    long long* out;   // offset of the row's output in elements
+    float* nref;      // negated reference maximum of a row, in powers of two
+    int* start;       // first cached position a row sees
+    int* depth;
+    uint32_t* mask;   // [words][N]
+};
+constexpr int kRowBytes = 8 + 4 * 3;
+__host__ __device__ constexpr size_t rows_bytes(int N, int words) { return (size_t)2 * N * (kRowBytes + 4 * words); }
+__device__ __forceinline__ Rows rows_of(unsigned char* base, int N, int words, int par) {
+    unsigned char* b = base + par * (N * (kRowBytes + 4 * words));
+    Rows r;
+    r.out = reinterpret_cast<long long*>(b);
+    r.nref = reinterpret_cast<float*>(b + N * 8);
+    r.start = reinterpret_cast<int*>(b + N * 12);
+    r.depth = reinterpret_cast<int*>(b + N * 16);
+    r.mask = reinterpret_cast<uint32_t*>(b + N * 20);
+    return r;
+}
 
 struct Params {
     const char* q;
@@ -118,7 +136,7 @@ struct Params {
     float2* ml;    // [2 x blocks][N]
     long long q_stride, out_stride, page_stride, new_stride;  // elements
     int seqs, n_tokens, max_nodes, pages, page_size, width, mask_words, heads, kv_heads, window;
-    int N, slots, box, grid, tmem_cols;
+    int N, words, slots, box, grid, tmem_cols, whole;
     float c;       // scale * log2(e)
 };
 
@@ -144,27 +162,30 @@ __device__ __noinline__ void load_seq(const Params& p, int b, Seq& s) {
 }
 
 // Sum of the block's values, to every thread.
-__device__ __forceinline__ long long block_total(long long v, long long* red) {
+__device__ __forceinline__ int block_total(int v, int* red) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    v = warp_sum_int(v);
     __syncthreads();
     if (lane == 0) red[w] = v;
     __syncthreads();
-    long long t = 0;
+    int t = 0;
 #pragma unroll 1
     for (int i = 0; i < nw; ++i) t += red[i];
     return t;
 }
 
-// An item is as long as its tiles and kItemCost more, ahead of them.
-__device__ __forceinline__ long long seq_units(const Params& p, int b) {
+// An item is as long as its tiles and kItemCost more, ahead of them; 1 where items stay whole.
+__device__ __forceinline__ int item_units(const Params& p, const Seq& s) { return p.whole ? 1 : s.tiles + kItemCost; }
+__device__ __forceinline__ int seq_units(const Params& p, int b) {
     Seq s;
     load_seq(p, b, s);
-    return s.tiles ? (long long)(s.tiles + kItemCost) * s.groups * p.kv_heads : 0;
+    return s.tiles ? item_units(p, s) * s.groups * p.kv_heads : 0;
 }
 
-__device__ __forceinline__ long long share_begin(long long total, int grid, int c) { return total * c / grid; }
+// First unit of block c when `total` units are dealt to `grid` blocks.
+__device__ __forceinline__ int share_begin(int total, int grid, int c) {
+    return total / grid * c + total % grid * c / grid;
+}
 
 // A place in the ring of slots and the parity of its current use.
 struct Place {
@@ -194,24 +215,24 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
 // Writes down the parts of this block's share, one by one; t0 = t1 ends them.
 __device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* abort) {
     Place at;
-    long long pos = c.begin;
-    const long long end = c.end;
+    int pos = c.begin;
+    const int end = c.end;
     Seq s;
     int b = 0, h = 0, g = 0, u = 0;
     if (pos < end) {
         b = c.seq0;
         load_seq(p, b, s);
-        const long long item = s.tiles + kItemCost, r = c.rem0 % (item * s.groups);
-        h = (int)(c.rem0 / (item * s.groups));
-        g = (int)(r / item);
-        u = (int)(r % item);
+        const int item = item_units(p, s), r = c.rem0 % (item * s.groups);
+        h = c.rem0 / (item * s.groups);
+        g = r / item;
+        u = r % item;
     }
 #pragma unroll 1
     while (true) {
         int t0 = 0, t1 = 0;
 #pragma unroll 1
         while (pos < end && t0 == t1) {
-            const int item = s.tiles + kItemCost;
+            const int item = item_units(p, s);
             if (u == item) {
                 u = 0;
                 if (++g == s.groups) {
@@ -224,10 +245,10 @@ __device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* 
                 }
                 continue;
             }
-            const int v = (int)min((long long)item, u + (end - pos));
+            const int v = min(item, u + (end - pos));
             pos += v - u;
-            t0 = max(0, u - kItemCost);
-            t1 = max(0, v - kItemCost);
+            t0 = p.whole ? 0 : max(0, u - kItemCost);
+            t1 = p.whole ? s.tiles : max(0, v - kItemCost);
             u = v;
         }
         if (!wait(&c.part_free[at.slot], at.phase ^ 1, abort)) return;
@@ -343,13 +364,13 @@ __device__ __forceinline__ void reduce_scatter8(float (&v)[8], int lane) {
 }
 
 // Whether row r of the part sees key k (0 .. 127) of tile i.
-__device__ __forceinline__ bool sees(const Params& p, const Part& w, const Ctl& c, int i, int k, int r) {
+__device__ __forceinline__ bool sees(const Params& p, const Part& w, const Rows& c, int i, int k, int r) {
     if (i < w.pre) {
         const int j = w.base + i * kKeys + k;
         return j < w.len && j >= c.start[r];
     }
     const int j = (i - w.pre) * kKeys + k;
-    if (j >= w.n || !((c.mask[j >> 5][r] >> (j & 31)) & 1)) return false;
+    if (j >= w.n || !((c.mask[(j >> 5) * p.N + r] >> (j & 31)) & 1)) return false;
     return !p.window || c.depth[r] - min(max(p.depth[w.first + j], 0), w.n - 1) < p.window;
 }
 
@@ -370,7 +391,7 @@ __device__ const uint16_t* v_row(const Params& p, const Part& w, int i, int k, i
 
 // What the infinities and NaN taken out of this part's V tiles add to row r in dimension d.
 template <bool kBf16>
-__device__ __noinline__ float poison_of(const Params& p, Part w, const Ctl& c, int dim, int d, int r) {
+__device__ __noinline__ float poison_of(const Params& p, Part w, Rows c, int dim, int d, int r) {
     float sum = 0.f;
     for (int i = w.t0; i < w.t1; ++i) {
         if (!(i >= w.pre || w.windowed(p.window, i))) continue;
@@ -382,19 +403,13 @@ __device__ __noinline__ float poison_of(const Params& p, Part w, const Ctl& c, i
     return sum;
 }
 
-// Takes infinities and NaN out of eight values; whether there were any.
+// Whether any of eight values is an infinity or NaN: adding one to an all-ones exponent carries into
+// the sign's place.
 template <bool kBf16>
-__device__ __forceinline__ bool clean(uint4& v) {
-    bool dirty = false;
-    uint32_t* x = &v.x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (not_finite<kBf16>((uint16_t)x[i])) x[i] &= 0xffff0000u, dirty = true;
-        if (not_finite<kBf16>((uint16_t)(x[i] >> 16))) x[i] &= 0x0000ffffu, dirty = true;
-    }
-    return dirty;
+__device__ __forceinline__ bool any_not_finite(const uint4& v) {
+    constexpr uint32_t kExp = kBf16 ? 0x7f807f80u : 0x7c007c00u, kOne = kBf16 ? 0x00800080u : 0x04000400u;
+    return (((v.x & kExp) + kOne) | ((v.y & kExp) + kOne) | ((v.z & kExp) + kOne) | ((v.w & kExp) + kOne)) & 0x80008000u;
 }
-
 // kNH: the most rows a softmax group takes (N / 2 of them are used, a multiple of 8).
 template <int D, int kNH, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -411,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     unsigned char* ring = sm;
     unsigned char* qs = ring + slots * kSlotBytes;             // [D / 64][N rows][64 dims]
     unsigned char* ps = qs + (D / 64) * N * 128;               // [N / 64][128 keys][64 rows]
-    Ctl& c = *reinterpret_cast<Ctl*>(ps + ((N + 63) / 64) * kBoxBytes);
+    unsigned char* rows_at = ps + ((N + 63) / 64) * kBoxBytes;  // row state
+    Ctl& c = *reinterpret_cast<Ctl*>(rows_at + rows_bytes(N, p.words));
     volatile int* abort = &c.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -447,33 +463,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kIssuer) tc::alloc(&c.tmem_base, p.tmem_cols);
 
     // This block's share of all units.
-    long long mine = 0;
+    int mine = 0;
 #pragma unroll 1
     for (int b = threadIdx.x; b < p.seqs; b += kThreads) mine += seq_units(p, b);
-    const long long total = block_total(mine, c.scan);
-    const long long begin = share_begin(total, gridDim.x, blockIdx.x), end = share_begin(total, gridDim.x, blockIdx.x + 1);
-    if (threadIdx.x == 0) {
-        c.begin = begin;
-        c.end = end;
-    }
-    long long before = 0;
+    const int total = block_total(mine, c.scan);
+    if (warp == 0) {
+        const int begin = share_begin(total, gridDim.x, blockIdx.x), end = share_begin(total, gridDim.x, blockIdx.x + 1);
+        if (lane == 0) {
+            c.begin = begin;
+            c.end = end;
+        }
+        int before = 0;
 #pragma unroll 1
-    for (int b0 = 0; warp == 0 && begin < end && b0 < p.seqs; b0 += 32) {
-        const int b = b0 + lane;
-        const long long mt = b < p.seqs ? seq_units(p, b) : 0;
-        long long x = mt;
+        for (int b0 = 0; begin < end && b0 < p.seqs && before <= begin; b0 += 32) {
+            const int b = b0 + lane;
+            const int mt = b < p.seqs ? seq_units(p, b) : 0;
+            int x = mt;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const int at = before + x - mt;
+            if (mt > 0 && begin >= at && begin < at + mt) {
+                c.seq0 = b;
+                c.rem0 = begin - at;
+            }
+            before += __shfl_sync(0xffffffffu, x, 31);
         }
-        const long long at = before + x - mt;
-        if (mt > 0 && begin >= at && begin < at + mt) {
-            c.seq0 = b;
-            c.rem0 = begin - at;
-        }
-        before += __shfl_sync(0xffffffffu, x, 31);
-        if (before > begin) break;
     }
     tc::fence_before_sync();
     __syncthreads();
@@ -632,30 +649,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int r0 = grp * nh;                          // the group's rows r0 .. r0 + nh - 1
         const uint32_t lanes = (uint32_t)(qd * 32) << 16;
         const int gqa = p.heads / p.kv_heads;
-        int tile = 0, q = 0, fix = 0;  // tiles, ring slots (as the producer counts them), edge tiles so far
+        int tile = 0, q = 0, fix = 0, par = 0;  // tiles, ring slots (as the producer counts them), edge tiles so far
         bool first_part = true;
         float l[kNH];
-        // After a wait that gave up, these warps go on (on meaningless values) to the end of the share:
-        // none of them may leave while others stand at a barrier of the group.
-#pragma unroll 1
-        while (true) {
+        // The next part's rows and queries; false at the end. All 256 threads come here together.
+        auto stage = [&](Part& w) {
             const bool more = all_256(next_part(c, list, w, false, abort));
             if (lane == 0) mbar_arrive(&c.part_free[(list.slot + kParts - 1) % kParts]);
-            if (!more) break;
+            if (!more) return false;
             // Rows of this part: r -> node (g N + r) / gqa, query head h gqa + (g N + r) % gqa.
+            const Rows rs = rows_of(rows_at, N, p.words, par ^ 1);
             const int R = min(N, w.n * gqa - w.g * N);
+            int dep = 0, tok = 0;
+            uint32_t word[8];
             if (tid < N) {
-                const int row = w.g * N + tid, node = min(row / gqa, w.n - 1), tok = w.first + node;
+                const int row = w.g * N + tid, hd = (w.h * gqa + row % gqa) * D;
+                tok = w.first + min(row / gqa, w.n - 1);
                 c.tok[tid] = tok;
-                c.hd[tid] = (w.h * gqa + row % gqa) * D;
-                const int dep = p.window ? min(max(p.depth[tok], 0), w.n - 1) : 0;
-                c.nref[tid] = kUnset;
-                c.depth[tid] = dep;
-                c.start[tid] = p.window ? max(0, w.len + dep - p.window + 1) : 0;
-#pragma unroll 1
-                for (int i = 0; i * 32 < w.n; ++i) c.mask[i][tid] = p.mask[(long long)tok * p.mask_words + i];
+                c.hd[tid] = hd;
+                rs.out[tid] = tok * p.out_stride + hd;
+                rs.nref[tid] = kUnset;
+                if (p.window) dep = p.depth[tok];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) word[i] = i * 32 < w.n ? p.mask[(long long)tok * p.mask_words + i] : 0;
             }
-            if (tid == 0) c.poison = 0;
             asm volatile("bar.sync 3, 256;" ::: "memory");
             // The queries, into the MMA's K-major layout (S of the part before has completed).
             constexpr int kRowsAt = 256 / (D / 8);  // rows the 256 threads load at once
@@ -675,9 +692,85 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (r < N) *reinterpret_cast<uint4*>(qs + (size_t)(ch >> 3) * N * 128 + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v[k];
                 }
             }
+            if (tid < N) {
+                dep = min(max(dep, 0), w.n - 1);
+                rs.depth[tid] = dep;
+                rs.start[tid] = p.window ? max(0, w.len + dep - p.window + 1) : 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i * 32 < w.n) rs.mask[i * N + tid] = word[i];
+            }
             fence_proxy_async();
             asm volatile("bar.sync 3, 256;" ::: "memory");
             if (lane == 0) mbar_arrive(&c.q_ready);
+            return true;
+        };
+        // After a wait that gave up, these warps go on (on meaningless values) to the end of the share:
+        // none of them may leave while others stand at a barrier of the group.
+        // The next part's queries go in before a part's output is written: its first scores are computed
+        // meanwhile.
+        int slot = 0;
+        bool open = false, whole = false;
+#pragma unroll 1
+        while (true) {
+            Part following;
+            const bool more = stage(following);
+            if (open) {
+                wait(&c.o_done, (tile - 1) & 1, abort);
+                __syncwarp();
+                tc::fence_after_sync();
+                const Rows rs = rows_of(rows_at, N, p.words, par);
+                const int held = min(nh, min(N, w.n * gqa - w.g * N) - r0);  // the group's rows that exist
+                const uint32_t ot = tmem + lanes + o_col + r0;
+                if (c.poison) {  // set before the staging's barriers, cleared after them
+#pragma unroll 1
+                    for (int ci = 0; ci < kChunks; ++ci)
+#pragma unroll 1
+                        for (int f = 0; f < held; f += 8) {
+                            float v[8];
+                            tc::ld8(ot + ci * N + f, v);
+                            tc::wait_ld();
+                            if (128 * ci + key < D)
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) v[j] += poison_of<kBf16>(p, w, rs, D, 128 * ci + key, r0 + f + j);
+                            __syncwarp();
+                            tc::st8(ot + ci * N + f, v);
+                        }
+                    tc::wait_st();
+                }
+#pragma unroll 1
+                for (int ci = 0; ci < kChunks; ++ci) {
+                    const int d = 128 * ci + key;
+                    uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + d;
+                    float* part = p.part + ((long long)slot * N + r0) * D + d;
+#pragma unroll 1
+                    for (int f = 0; f < held; f += 32) {
+                        float v[4][8];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (f + 8 * e < nh) tc::ld8(ot + ci * N + f + 8 * e, v[e]);
+                        tc::wait_ld();
+                        if (D == 64 && key >= 64) continue;
+                        if (whole) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (f + j < held) out[rs.out[r0 + f + j]] = pack1<kBf16>(v[j >> 3][j & 7] * c.inv[r0 + f + j]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (f + j < held) __stcg(part + (f + j) * D, v[j >> 3][j & 7]);
+                        }
+                    }
+                }
+                tc::fence_before_sync();
+                asm volatile("bar.sync 3, 256;" ::: "memory");  // every thread is done with poison and inv
+            }
+            if (!more) break;
+            open = true;
+            w = following;
+            par ^= 1;
+            const Rows rs = rows_of(rows_at, N, p.words, par);
+            if (tid == 0) c.poison = 0;
 #pragma unroll
             for (int r = 0; r < kNH; ++r) l[r] = 0.f;
 
@@ -693,20 +786,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // Hidden scores become -inf, in tensor memory.
                     const bool old = i < w.pre;
                     const int j = old ? w.base + i * kKeys + key : (i - w.pre) * kKeys + key;
-                    const int near = !old && p.window && j < w.n ? min(max(p.depth[w.first + j], 0), w.n - 1) + p.window : INT_MAX;
                     const bool in = j < (old ? w.len : w.n);
-                    const uint32_t* word = c.mask[old ? 0 : (i - w.pre) * 4 + qd];
+                    const int near = p.window && in && !old ? min(max(p.depth[w.first + j], 0), w.n - 1) + p.window : INT_MAX;
+                    const uint32_t* word = rs.mask + (old ? 0 : (i - w.pre) * 4 + qd) * N + r0;
+                    const int* depth = rs.depth + r0;
+                    const int* start = rs.start + r0;
 #pragma unroll 1
-                    for (int e = 0; e < nh; e += 8) {
+                    for (int f = 0; f < nh; f += 8) {
                         float v[8];
-                        tc::ld8(st + e, v);
+                        tc::ld8(st + f, v);
+                        int a[8], d[8];
+                        if (old) {
+                            *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(start + f);
+                            *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(start + f + 4);
+                        } else {
+                            *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(word + f);
+                            *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(word + f + 4);
+                        }
+                        *reinterpret_cast<int4*>(d) = *reinterpret_cast<const int4*>(depth + f);
+                        *reinterpret_cast<int4*>(d + 4) = *reinterpret_cast<const int4*>(depth + f + 4);
                         tc::wait_ld();
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            const int r = r0 + e + k;
-                            if (!(in && (old ? j >= c.start[r] : ((word[r] >> lane) & 1) && c.depth[r] < near))) v[k] = -INFINITY;
+                            const bool seen = old ? j >= a[k] : (((unsigned)a[k] >> lane) & 1u) & (unsigned)(d[k] < near);
+                            v[k] = in & seen ? v[k] : -INFINITY;
                         }
-                        tc::st8(st + e, v);
+                        tc::st8(st + f, v);
                     }
                     tc::wait_st();
                 }
@@ -722,7 +827,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int r = 0; r < 16; r += 4)
                         if (r < 8 || both) {
-                            const float4 n = *reinterpret_cast<const float4*>(&c.nref[r0 + f + r]);
+                            const float4 n = *reinterpret_cast<const float4*>(&rs.nref[r0 + f + r]);
                             over = fmaxf(over, fmaxf(fmaf(v[r], p.c, n.x), fmaf(v[r + 1], p.c, n.y)));
                             over = fmaxf(over, fmaxf(fmaf(v[r + 2], p.c, n.z), fmaf(v[r + 3], p.c, n.w)));
                         }
@@ -730,22 +835,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bool waited = tile == 0;
                 if (group_or(grp, over > kLazy)) {
 #pragma unroll 1
-                    for (int e = 0; e < nh; e += 8) {
-                        float m[8];
-                        tc::ld8(st + e, m);
+                    for (int f = 0; f < nh; f += 32) {
+                        float m[4][8];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (f + 8 * e < nh) tc::ld8(st + f + 8 * e, m[e]);
                         tc::wait_ld();
-                        reduce_scatter8<true>(m, lane);
-                        c.red[qd][r0 + e + (lane >> 2)] = m[0] * p.c;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (f + 8 * e < nh) {
+                                reduce_scatter8<true>(m[e], lane);
+                                c.red[qd][r0 + f + 8 * e + (lane >> 2)] = m[e][0] * p.c;
+                            }
                     }
                     group_bar(grp);
                     if (gt < nh) {
                         const int r = r0 + gt;
                         const float top = fmaxf(fmaxf(c.red[0][r], c.red[1][r]), fmaxf(c.red[2][r], c.red[3][r]));
-                        const float old = c.nref[r];
+                        const float old = rs.nref[r];
                         float f = 1.f;
                         if (top > -INFINITY && (old == kUnset || top + old > kLazy)) {
                             f = old == kUnset ? 0.f : exp2_approx(-old - top);
-                            c.nref[r] = -top;
+                            rs.nref[r] = -top;
                         }
                         c.corr[r] = f;
                     }
@@ -765,10 +876,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                         waited = true;
                         tc::fence_after_sync();
 #pragma unroll 1
-                        for (int e = 0; e < kChunks * nh; e += 8) {
-                            const int ci = e / nh, f = e - ci * nh;
+                        for (int f = 0, ta = tmem + lanes + o_col + r0, ci = 0; ci < kChunks; f += 8, ta += 8) {
+                            if (f == nh) {
+                                f = 0;
+                                ta += N - nh;
+                                if (++ci == kChunks) break;
+                            }
                             float v[8];
-                            const uint32_t ta = tmem + lanes + o_col + ci * N + r0 + f;
                             tc::ld8(ta, v);
                             tc::wait_ld();
 #pragma unroll
@@ -800,7 +914,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int r = 0; r < kCh; r += 4)
                             if (f + r < nh) {
-                                const float4 n = *reinterpret_cast<const float4*>(&c.nref[r0 + f + r]);
+                                const float4 n = *reinterpret_cast<const float4*>(&rs.nref[r0 + f + r]);
                                 const float e0 = exp2_approx(fmaf(s[r], p.c, n.x)), e1 = exp2_approx(fmaf(s[r + 1], p.c, n.y));
                                 const float e2 = exp2_approx(fmaf(s[r + 2], p.c, n.z)), e3 = exp2_approx(fmaf(s[r + 3], p.c, n.w));
                                 l[f + r] += e0;
@@ -840,17 +954,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                         wait(&c.full[slot], ((vq + ci) / slots) & 1, abort);
                         unsigned char* base = ring + slot * kSlotBytes;
 #pragma unroll 1
-                        for (int e = tid; e < rows * 8 * kHalves; e += 256) {
-                            const int k = e / (8 * kHalves), cc = e % (8 * kHalves);
-                            uint4* at = reinterpret_cast<uint4*>(base + (cc >> 3) * kBoxBytes + k * 128 + (cc & 7) * 16);
-                            if (k >= keys || k < lead) {
-                                *at = make_uint4(0, 0, 0, 0);
-                            } else if (scan) {
-                                uint4 v = *at;
-                                if (clean<kBf16>(v)) {
-                                    *at = v;
-                                    c.poison = 1;
+                        for (int e = tid; e < rows * 8 * kHalves; e += 4 * 256) {
+                            uint4 v[4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                const int x = e + u * 256, k = x / (8 * kHalves), cc = x % (8 * kHalves);
+                                uint4* at = reinterpret_cast<uint4*>(base + (cc >> 3) * kBoxBytes + k * 128 + (cc & 7) * 16);
+                                v[u] = make_uint4(0, 0, 0, 0);
+                                if (k < rows) {
+                                    if (k >= keys || k < lead) *at = make_uint4(0, 0, 0, 0);
+                                    else if (scan) v[u] = *at;
                                 }
+                            }
+                            uint32_t dirty = 0;
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) dirty |= (uint32_t)any_not_finite<kBf16>(v[u]) << u;
+#pragma unroll 1
+                            for (int u = 0; dirty; ++u, dirty >>= 1) {
+                                if (!(dirty & 1)) continue;
+                                const int x = e + u * 256;
+                                uint16_t* h = reinterpret_cast<uint16_t*>(base + (x % (8 * kHalves) >> 3) * kBoxBytes +
+                                                                          x / (8 * kHalves) * 128 + (x & 7) * 16);
+#pragma unroll 1
+                                for (int y = 0; y < 8; ++y)
+                                    if (not_finite<kBf16>(h[y])) h[y] = 0;
+                                c.poison = 1;
                             }
                         }
                         fence_proxy_async();
@@ -874,44 +1002,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     c.red[qd][r0 + r + (lane >> 2)] = m[0];
                 }
             group_bar(grp);
-            const bool whole = w.t1 - w.t0 == w.tiles;
-            const int slot = 2 * blockIdx.x + (first_part ? 0 : 1);
+            whole = w.t1 - w.t0 == w.tiles;
+            slot = 2 * blockIdx.x + (first_part ? 0 : 1);
             first_part = false;
             if (gt < nh) {
                 const int r = r0 + gt;
                 const float sum = (c.red[0][r] + c.red[1][r]) + (c.red[2][r] + c.red[3][r]);
                 c.inv[r] = sum != 0.f ? 1.f / sum : 0.f;
-                if (!whole) p.ml[(long long)slot * N + r] = make_float2(c.nref[r] == kUnset ? -INFINITY : -c.nref[r], sum);
+                if (!whole) p.ml[(long long)slot * N + r] = make_float2(rs.nref[r] == kUnset ? -INFINITY : -rs.nref[r], sum);
             }
-            wait(&c.o_done, (tile - 1) & 1, abort);
-            __syncwarp();
-            tc::fence_after_sync();
-            asm volatile("bar.sync 3, 256;" ::: "memory");  // also: every thread's poison flag
-            const bool poison = c.poison != 0;
-            const int held = min(nh, R - r0);               // the group's rows that exist
-#pragma unroll 1
-            for (int ci = 0; ci < kChunks; ++ci) {
-                const int d = 128 * ci + key;
-                uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + d;
-                float* part = p.part + ((long long)slot * N + r0) * D + d;
-#pragma unroll 1
-                for (int e = 0; e < held; e += 8) {
-                    float v[8];
-                    tc::ld8(tmem + lanes + o_col + ci * N + r0 + e, v);
-                    tc::wait_ld();
-                    if (D == 64 && key >= 64) continue;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        if (e + j >= held) break;
-                        const int r = r0 + e + j;
-                        if (poison) v[j] += poison_of<kBf16>(p, w, c, D, d, r);
-                        if (whole) out[c.tok[r] * p.out_stride + c.hd[r]] = pack1<kBf16>(v[j] * c.inv[r]);
-                        else __stcg(part + (e + j) * D, v[j]);
-                    }
-                }
-            }
-            tc::fence_before_sync();
-            asm volatile("bar.sync 3, 256;" ::: "memory");  // the row state is free for the next part
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -932,16 +1031,16 @@ constexpr int kJoinRows = 8;
 // sum_s 2^(m_s - M) l_s. A warp per row, kJoinRows rows a block; grid (seqs x kv_heads, row blocks).
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(32 * kJoinRows) tree_attn_join_kernel(const __grid_constant__ Params p) {
-    __shared__ long long red[32];
+    __shared__ int red[32];
     pdl_wait();
     const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads, lane = threadIdx.x & 31;
     const int gqa = p.heads / p.kv_heads;
     Seq s;
     load_seq(p, b, s);
     if (s.n * gqa <= (int)blockIdx.y * kJoinRows) return;
-    long long before = 0, all = 0;
+    int before = 0, all = 0;
     for (int i = threadIdx.x; i < p.seqs; i += 32 * kJoinRows) {
-        const long long t = seq_units(p, i);
+        const int t = seq_units(p, i);
         all += t;
         if (i < b) before += t;
     }
@@ -951,8 +1050,14 @@ __global__ void __launch_bounds__(32 * kJoinRows) tree_attn_join_kernel(const __
     if (row >= s.n * gqa) return;
     const int g = row / p.N, r = row % p.N;
     const int item = s.tiles + kItemCost;
-    const long long a = before + ((long long)h * s.groups + g) * item, z = a + item;
-    const auto block_of = [&](long long x) { return (int)(((x + 1) * p.grid - 1) / all); };
+    const int a = before + (h * s.groups + g) * item, z = a + item;
+    // Block that holds unit x: an estimate, corrected.
+    const auto block_of = [&](int x) {
+        int c = min(p.grid - 1, (int)((float)x / (float)all * (float)p.grid));
+        while (c > 0 && share_begin(all, p.grid, c) > x) --c;
+        while (c + 1 < p.grid && share_begin(all, p.grid, c + 1) <= x) ++c;
+        return c;
+    };
     const int c0 = block_of(a + kItemCost), c1 = block_of(z - 1);  // the blocks of its first and last tile
     if (c0 == c1) return;
     const auto slot_of = [&](int c) { return (long long)(2 * c + (share_begin(all, p.grid, c) < a ? 1 : 0)); };
@@ -1016,14 +1121,15 @@ int rows_per_item(int max_nodes, int gqa, int dim) {
 }
 
 struct Shape {
-    int N, slots, tmem;
+    int N, words, slots, tmem;
     size_t smem;
 };
 Shape shape_for(int max_nodes, int gqa, int dim) {
     Shape s;
     s.N = rows_per_item(max_nodes, gqa, dim);
     const size_t slot = (dim == 64 ? 1 : 2) * kBoxBytes;
-    const size_t rest = 1024 + (size_t)s.N * dim * 2 + (size_t)((s.N + 63) / 64) * kBoxBytes + sizeof(Ctl);
+    s.words = (max_nodes + 31) / 32;
+    const size_t rest = 1024 + (size_t)s.N * dim * 2 + (size_t)((s.N + 63) / 64) * kBoxBytes + rows_bytes(s.N, s.words) + sizeof(Ctl);
     s.slots = (int)std::min<size_t>(kMaxSlots, (kSmemLimit - rest) / slot);
     s.smem = rest + s.slots * slot;
     const int cols = s.N * (2 + std::max(1, dim / 128));
@@ -1062,7 +1168,7 @@ cudaError_t run(const CUtensorMap* maps, const Params& p, const Shape& sh, cudaS
         attr = true;
     }
     cudaError_t e = launch(kern, dim3(p.grid), dim3(kThreads), sh.smem, st, false, maps[0], maps[1], maps[2], maps[3], p);
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || p.whole) return e;
     const int rows = p.max_nodes * (p.heads / p.kv_heads);
     return launch(tree_attn_join_kernel<D, kBf16>, dim3(p.seqs * p.kv_heads, (rows + kJoinRows - 1) / kJoinRows),
                   dim3(32 * kJoinRows), 0, st, true, p);
@@ -1120,10 +1226,16 @@ cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
     p.kv_heads = a.kv_heads;
     p.window = a.window;
     p.N = sh.N;
+    p.words = sh.words;
     p.slots = sh.slots;
     p.tmem_cols = sh.tmem;
     // The largest power of two that divides a page, so that a box never crosses one.
     p.box = std::min(kKeys, a.page_size & -a.page_size);
+    const long long tiles = ((long long)a.width * a.page_size + kKeys - 1) / kKeys + 1 + (a.max_nodes + kKeys - 1) / kKeys;
+    const long long items = (long long)a.seqs * a.kv_heads * ((a.max_nodes * (a.heads / a.kv_heads) + sh.N - 1) / sh.N);
+    if (items * (tiles + kItemCost) > INT32_MAX) return cudaErrorInvalidConfiguration;  // units are counted in 32 bits
+    p.whole = tiles <= kWholeTiles;
+    if (p.whole) p.grid = (int)std::min<long long>(p.grid, items);
     p.c = a.scale * 1.4426950408889634f;
     const cuuint64_t row = (cuuint64_t)a.dim * 2, D = a.dim, H = a.kv_heads;
     const cuuint64_t pool_dims[4] = {D, H, (cuuint64_t)a.page_size, (cuuint64_t)a.pages};
