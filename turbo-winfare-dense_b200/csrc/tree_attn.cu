@@ -21,7 +21,7 @@
 //   * one warp streams K of tile t + 1, then V of tile t, through a ring of 32 KB slots (128 keys x
 //     128 dims) by TMA: one box per (page part, 64 dims), swizzled as the MMA reads it;
 //   * one thread of another issues the MMAs, S^T into two alternating TMEM buffers;
-//   * two groups of four warps take half of the rows each, a thread one key of all its rows: they
+//   * four groups of four warps take a quarter of the rows each, a thread one key of all its rows: they
 //     hold the softmax in fp32, write P^T (rounded to the cache's type, 8 rows a store) and, when a
 //     row's score exceeds its reference maximum by more than 8 (in powers of two), move the
 //     reference and rescale that row of O^T in TMEM. In between only a vote of the group is needed,
@@ -49,11 +49,11 @@ namespace g4b {
 namespace {
 
 constexpr int kKeys = 128;           // keys per tile: the M of S^T
-constexpr int kSoftWarps = 8;        // warps 0 .. 7
-constexpr int kProducer = 8, kIssuer = 9, kScheduler = 10;
-constexpr int kThreads = 384;        // the last warp only gives up registers
-// Registers a thread: 168 at launch; 256 x 216 + 128 x 72 is the same total.
-constexpr int kSoftRegs = 216, kOtherRegs = 72;
+constexpr int kSoftWarps = 16;       // warps 0 .. 15, four groups of four
+constexpr int kProducer = 16, kIssuer = 17, kScheduler = 18;  // and 19, the cleaner
+constexpr int kThreads = 640;
+// Registers a thread: 96 at launch; 512 x 104 + 128 x 64 is the same total.
+constexpr int kSoftRegs = 104, kOtherRegs = 64;
 constexpr uint32_t kBoxBytes = kKeys * 128;  // 128 keys x 64 dims of 16 bits
 constexpr int kMaxSlots = 8;
 constexpr int kParts = 4;            // parts the scheduler is ahead
@@ -85,20 +85,19 @@ struct Part {
     }
 };
 
-struct Ctl {
+struct alignas(16) Ctl {
     uint64_t full[kMaxSlots], empty[kMaxSlots];
     uint64_t s_full[2], s_free[2];
     uint64_t part_full[kParts], part_free[kParts];
     Part part[kParts];
-    uint64_t q_ready, p_full, o_done, v_ready[4], v_fix[4], done;
+    uint64_t q_ready[2], q_free, rows_free[2], p_full, o_done, v_ready[4], v_fix[4], done;
     uint32_t tmem_base;
-    int abort, poison;
+    int abort, poison[2];
     int seq0, rem0, begin, end;  // this block's share and where in which sequence it starts
     int scan[kThreads / 32 + 1];
-    float corr[128];     // factor of a row's sum and output when its reference moves
-    float inv[128];
-    float red[4][128];
-    int tok[128], hd[128];  // a row's token and its head's offset in elements
+    alignas(16) float corr[128];  // factor of a row's sum and output when its reference moves
+    alignas(16) float inv[128];
+    alignas(16) float red[4][128];
 };
 
 // What a part's rows carry, twice: the next part's is set up before the current one is written out.
@@ -212,8 +211,10 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
     return true;
 }
 
-// Writes down the parts of this block's share, one by one; t0 = t1 ends them.
-__device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* abort) {
+// Writes down the parts of this block's share, one by one (t0 = t1 ends them), and hands each to
+// ready(part). One warp.
+template <class Ready>
+__device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* abort, Ready ready) {
     Place at;
     int pos = c.begin;
     const int end = c.end;
@@ -251,10 +252,13 @@ __device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* 
             t1 = p.whole ? s.tiles : max(0, v - kItemCost);
             u = v;
         }
-        if (!wait(&c.part_free[at.slot], at.phase ^ 1, abort)) return;
-        c.part[at.slot] = Part{b, h, g, t0, t1, s.len, s.first, s.n, s.start, s.base, s.pre, s.tiles};
-        mbar_arrive(&c.part_full[at.slot]);
-        if (t0 == t1) return;
+        if (!__all_sync(0xffffffffu, wait(&c.part_free[at.slot], at.phase ^ 1, abort))) return;
+        const Part part{b, h, g, t0, t1, s.len, s.first, s.n, s.start, s.base, s.pre, s.tiles};
+        if ((threadIdx.x & 31) == 0) {
+            c.part[at.slot] = part;
+            mbar_arrive(&c.part_full[at.slot]);
+        }
+        if (t0 == t1 || !ready(part)) return;
         at.step(kParts);
     }
 }
@@ -269,11 +273,11 @@ __device__ __forceinline__ bool next_part(Ctl& c, Place& at, Part& w, bool leade
 }
 
 __device__ __forceinline__ void group_bar(int grp) { asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory"); }
-// The AND over the 256 threads of the softmax warps.
-__device__ __forceinline__ bool all_256(bool v) {
+// The AND over the threads of the softmax warps.
+__device__ __forceinline__ bool all_groups(bool v) {
     uint32_t r;
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.and.pred q, 3, 256, p;\n selp.u32 %0, 1, 0, q;\n}"
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.and.pred q, 5, 512, p;\n selp.u32 %0, 1, 0, q;\n}"
         : "=r"(r)
         : "r"((uint32_t)v)
         : "memory");
@@ -315,6 +319,10 @@ __device__ __forceinline__ void load16(uint32_t ta, bool both, float (&v)[16]) {
         for (int j = 0; j < 8; ++j) v[j] = h[j];
     }
     tc::wait_ld();
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -410,7 +418,7 @@ __device__ __forceinline__ bool any_not_finite(const uint4& v) {
     constexpr uint32_t kExp = kBf16 ? 0x7f807f80u : 0x7c007c00u, kOne = kBf16 ? 0x00800080u : 0x04000400u;
     return (((v.x & kExp) + kOne) | ((v.y & kExp) + kOne) | ((v.z & kExp) + kOne) | ((v.w & kExp) + kOne)) & 0x80008000u;
 }
-// kNH: the most rows a softmax group takes (N / 2 of them are used, a multiple of 8).
+// kNH: the most rows a softmax group takes.
 template <int D, int kNH, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -420,9 +428,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kChunks = D == 64 ? 1 : D / 128;          // slots per K or V tile
     constexpr uint32_t kSlotBytes = kHalves * kBoxBytes;
     extern __shared__ unsigned char smem_raw[];
-    unsigned char* sm = reinterpret_cast<unsigned char*>(
-        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    const int N = p.N, nh = N >> 1, slots = p.slots;
+    // An offset, not a rounded pointer: the compiler still sees shared memory, and uses its 32-bit
+    // addresses and instructions.
+    unsigned char* sm = smem_raw + (-smem_u32(smem_raw) & 1023u);
+    const int N = p.N, slots = p.slots;
     unsigned char* ring = sm;
     unsigned char* qs = ring + slots * kSlotBytes;             // [D / 64][N rows][64 dims]
     unsigned char* ps = qs + (D / 64) * N * 128;               // [N / 64][128 keys][64 rows]
@@ -445,19 +454,23 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int i = 0; i < kParts; ++i) {
             mbar_init(&c.part_full[i], 1);
-            mbar_init(&c.part_free[i], kSoftWarps + 2);
+            mbar_init(&c.part_free[i], kSoftWarps + 3);
         }
-        mbar_init(&c.q_ready, kSoftWarps);
+        mbar_init(&c.q_free, 1);
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&c.q_ready[i], 1);
+            mbar_init(&c.rows_free[i], kSoftWarps);
+        }
         mbar_init(&c.p_full, kSoftWarps);
         mbar_init(&c.o_done, 1);
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
             mbar_init(&c.v_ready[i], 1);
-            mbar_init(&c.v_fix[i], kSoftWarps);
+            mbar_init(&c.v_fix[i], 1);
         }
         mbar_init(&c.done, 1);
         c.abort = 0;
-        c.poison = 0;
         mbar_init_fence();
     }
     if (warp == kIssuer) tc::alloc(&c.tmem_base, p.tmem_cols);
@@ -567,73 +580,106 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == kIssuer) {
         // ------------------------------------------------------------------ MMA issuer
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (lane == 0) {
-            Part w;
-            Place list;
-            const uint32_t id_s = tc::idesc_16(kKeys, N, kBf16, false, false);
-            const uint32_t id_o = tc::idesc_16(128, N, kBf16, true, true);
-            // Descriptors of the ring's first slot, of Q and of P; other places add their distance in
-            // 16-byte units.
-            const uint64_t k_desc = tc::desc_sw128(smem_u32(ring)), v_desc = tc::desc_sw128_mn(smem_u32(ring), kBoxBytes, 1024);
-            const uint64_t q_desc = tc::desc_sw128(smem_u32(qs)), p_desc = tc::desc_sw128_mn(smem_u32(ps), kBoxBytes, 1024);
-            const uint32_t blk = (uint32_t)N * 8;  // one 64-dim block of Q
-            Place at;
-            int tile = 0, otile = 0, part = 0, fix = 0;
-            bool ok = true;
+        // The whole warp walks the loops, one lane issues: what the instructions need is the same in
+        // every lane and can stay in uniform registers.
+        const bool leader = tc::elect();
+        Part w;
+        Place list;
+        const uint32_t id_s = tc::idesc_16(kKeys, N, kBf16, false, false);
+        const uint32_t id_o = tc::idesc_16(128, N, kBf16, true, true);
+        // Descriptors of the ring's first slot, of Q and of P; other places add their distance in
+        // 16-byte units.
+        const uint64_t k_desc = tc::desc_sw128(smem_u32(ring)), v_desc = tc::desc_sw128_mn(smem_u32(ring), kBoxBytes, 1024);
+        const uint64_t q_desc = tc::desc_sw128(smem_u32(qs)), p_desc = tc::desc_sw128_mn(smem_u32(ps), kBoxBytes, 1024);
+        const uint32_t blk = (uint32_t)N * 8;  // one 64-dim block of Q
+        // V chunks that fit the ring beside nothing else: the cleaning of an edge tile's first ones
+        // can start before its P is there.
+        const int ahead = min(kChunks, slots);
+        Place at;
+        int tile = 0, otile = 0, part = 0, fix = 0;
+        bool ok = true;
 #pragma unroll 1
-            while (ok && next_part(c, list, w, true, abort)) {
-                ok = wait(&c.q_ready, part++ & 1, abort);
-                tc::fence_after_sync();
-                // S of tile i, then O of tile i - 1.
+        while (ok) {
+            ok = __all_sync(0xffffffffu, next_part(c, list, w, false, abort));
+            if (leader) mbar_arrive(&c.part_free[(list.slot + kParts - 1) % kParts]);
+            if (!ok) break;
+            const int t0 = __shfl_sync(0xffffffffu, w.t0, 0), t1 = __shfl_sync(0xffffffffu, w.t1, 0);
+            ok = __all_sync(0xffffffffu, wait(&c.q_ready[part & 1], (part >> 1) & 1, abort));
+            ++part;
+            // S of tile i, then O of tile i - 1.
 #pragma unroll 1
-                for (int i = w.t0; i <= w.t1 && ok; ++i) {
-                    if (i < w.t1) {
-                        const int b = tile & 1;
-                        if (tile >= 2) ok = wait(&c.s_free[b], ((tile >> 1) - 1) & 1, abort);
+            for (int i = t0; i <= t1 && ok; ++i) {
+                if (i < t1) {
+                    const int b = tile & 1;
+                    if (tile >= 2) ok = wait(&c.s_free[b], ((tile >> 1) - 1) & 1, abort);
 #pragma unroll 1
-                        for (int ci = 0; ci < kChunks && ok; ++ci) {
-                            ok = wait(&c.full[at.slot], at.phase, abort);
-                            tc::fence_after_sync();
-                            const uint64_t a = k_desc + at.slot * (kSlotBytes >> 4), q = q_desc + 2 * ci * blk;
+                    for (int ci = 0; ci < kChunks; ++ci) {
+                        ok = ok && wait(&c.full[at.slot], at.phase, abort);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc::fence_after_sync();
+                        const uint64_t a = k_desc + at.slot * (kSlotBytes >> 4), q = q_desc + 2 * ci * blk;
+                        if (leader) {
 #pragma unroll
                             for (int kk = 0; kk < 4 * kHalves; ++kk)
                                 tc::mma_ss(tmem + b * N, a + (kk >> 2) * (kBoxBytes >> 4) + (kk & 3) * 2,
                                            q + (kk >> 2) * blk + (kk & 3) * 2, id_s, (ci | kk) ? 1u : 0u);
                             tc::commit(&c.empty[at.slot]);
-                            at.step(slots);
                         }
+                        at.step(slots);
+                    }
+                    if (leader) {
                         tc::commit(&c.s_full[b]);
-                        ++tile;
+                        if (i + 1 == t1) tc::commit(&c.q_free);
                     }
-                    if (i > w.t0 && ok) {
-                        ok = wait(&c.p_full, otile & 1, abort);
-                        tc::fence_after_sync();
-                        const int steps = (w.keys(i - 1) + 15) >> 4;
-                        const bool edge = w.edge(p.window, i - 1);
+                    ++tile;
+                }
+                if (i > t0 && ok) {
+                    const int steps = __shfl_sync(0xffffffffu, (w.keys(i - 1) + 15) >> 4, 0);
+                    const bool edge = w.edge(p.window, i - 1);
+                    Place look = at;
 #pragma unroll 1
-                        for (int ci = 0; ci < kChunks && ok; ++ci) {
-                            ok = wait(&c.full[at.slot], at.phase, abort);
-                            if (edge) {  // the softmax warps clean the chunk first
-                                mbar_arrive(&c.v_ready[ci]);
-                                ok = wait(&c.v_fix[ci], fix & 1, abort);
-                            }
-                            tc::fence_after_sync();
-                            const uint64_t a = v_desc + at.slot * (kSlotBytes >> 4);
-                            // V^T rows are the slot's dims, two 64-dim boxes apart (with D = 64 the lanes
-                            // 64 .. 127 multiply whatever follows in shared memory, and are never read).
-#pragma unroll 2
-                            for (int kk = 0; kk < steps; ++kk)
-                                tc::mma_ss(tmem + o_col + ci * N, a + kk * 128, p_desc + kk * 128, id_o,
-                                           (i - 1 > w.t0 || kk > 0) ? 1u : 0u);
-                            tc::commit(&c.empty[at.slot]);
-                            at.step(slots);
-                        }
-                        tc::commit(&c.o_done);
-                        fix += edge;
-                        ++otile;
+                    for (int ci = 0; ci < ahead && edge; ++ci) {
+                        ok = ok && wait(&c.full[look.slot], look.phase, abort);
+                        if (leader) mbar_arrive(&c.v_ready[ci]);
+                        look.step(slots);
                     }
+                    ok = ok && wait(&c.p_full, otile & 1, abort);
+#pragma unroll 1
+                    for (int ci = 0; ci < kChunks; ++ci) {
+                        ok = ok && wait(&c.full[at.slot], at.phase, abort);
+                        if (edge) {  // cleaned first
+                            if (ci >= ahead && leader) mbar_arrive(&c.v_ready[ci]);
+                            ok = ok && wait(&c.v_fix[ci], fix & 1, abort);
+                        }
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc::fence_after_sync();
+                        const uint64_t a = v_desc + at.slot * (kSlotBytes >> 4);
+                        const uint32_t d = tmem + o_col + ci * N, more = i - 1 > t0 ? 1u : 0u;
+                        // V^T rows are the slot's dims, two 64-dim boxes apart (with D = 64 the lanes
+                        // 64 .. 127 multiply whatever follows in shared memory, and are never read).
+                        if (leader) {
+                            if (steps == 8) {
+#pragma unroll
+                                for (int kk = 0; kk < 8; ++kk)
+                                    tc::mma_ss(d, a + kk * 128, p_desc + kk * 128, id_o, kk ? 1u : more);
+                            } else {
+#pragma unroll 1
+                                for (int kk = 0; kk < steps; ++kk)
+                                    tc::mma_ss(d, a + kk * 128, p_desc + kk * 128, id_o, kk ? 1u : more);
+                            }
+                            tc::commit(&c.empty[at.slot]);
+                        }
+                        at.step(slots);
+                    }
+                    if (leader) tc::commit(&c.o_done);
+                    fix += edge;
+                    ++otile;
                 }
             }
+        }
+        if (leader) {
             tc::commit(&c.done);  // every MMA has completed before tensor memory is freed
             if (!mbar_wait(&c.done, 0)) *abort = 1;
         }
@@ -642,135 +688,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         Part w;
         Place list;
-        constexpr int kCh = kNH == 64 ? 32 : kNH;         // rows whose scores are in registers at once
         const int grp = warp >> 2, qd = warp & 3;
-        const int tid = threadIdx.x, gt = tid & 127;      // 0..255; 0..127 in the group
+        const int gt = threadIdx.x & 127;                 // place in the group
         const int key = qd * 32 + lane;                   // TMEM lane
-        const int r0 = grp * nh;                          // the group's rows r0 .. r0 + nh - 1
+        // The group's rows r0 .. r0 + nh - 1, in eights; with few rows some groups have none.
+        const int r0 = (N >> 3) * grp / 4 * 8, nh = (N >> 3) * (grp + 1) / 4 * 8 - r0;
         const uint32_t lanes = (uint32_t)(qd * 32) << 16;
         const int gqa = p.heads / p.kv_heads;
-        int tile = 0, q = 0, fix = 0, par = 0;  // tiles, ring slots (as the producer counts them), edge tiles so far
-        bool first_part = true;
+        int tile = 0;
         float l[kNH];
-        // The next part's rows and queries; false at the end. All 256 threads come here together.
-        auto stage = [&](Part& w) {
-            const bool more = all_256(next_part(c, list, w, false, abort));
-            if (lane == 0) mbar_arrive(&c.part_free[(list.slot + kParts - 1) % kParts]);
-            if (!more) return false;
-            // Rows of this part: r -> node (g N + r) / gqa, query head h gqa + (g N + r) % gqa.
-            const Rows rs = rows_of(rows_at, N, p.words, par ^ 1);
-            const int R = min(N, w.n * gqa - w.g * N);
-            int dep = 0, tok = 0;
-            uint32_t word[8];
-            if (tid < N) {
-                const int row = w.g * N + tid, hd = (w.h * gqa + row % gqa) * D;
-                tok = w.first + min(row / gqa, w.n - 1);
-                c.tok[tid] = tok;
-                c.hd[tid] = hd;
-                rs.out[tid] = tok * p.out_stride + hd;
-                rs.nref[tid] = kUnset;
-                if (p.window) dep = p.depth[tok];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) word[i] = i * 32 < w.n ? p.mask[(long long)tok * p.mask_words + i] : 0;
-            }
-            asm volatile("bar.sync 3, 256;" ::: "memory");
-            // The queries, into the MMA's K-major layout (S of the part before has completed).
-            constexpr int kRowsAt = 256 / (D / 8);  // rows the 256 threads load at once
-            const int ch = tid % (D / 8);
-#pragma unroll 1
-            for (int rb = tid / (D / 8); rb < N; rb += 8 * kRowsAt) {
-                uint4 v[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int r = rb + k * kRowsAt;
-                    v[k] = make_uint4(0, 0, 0, 0);
-                    if (r < R) v[k] = __ldg(reinterpret_cast<const uint4*>(p.q + 2 * (c.tok[r] * p.q_stride + c.hd[r])) + ch);
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int r = rb + k * kRowsAt;
-                    if (r < N) *reinterpret_cast<uint4*>(qs + (size_t)(ch >> 3) * N * 128 + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v[k];
-                }
-            }
-            if (tid < N) {
-                dep = min(max(dep, 0), w.n - 1);
-                rs.depth[tid] = dep;
-                rs.start[tid] = p.window ? max(0, w.len + dep - p.window + 1) : 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i * 32 < w.n) rs.mask[i * N + tid] = word[i];
-            }
-            fence_proxy_async();
-            asm volatile("bar.sync 3, 256;" ::: "memory");
-            if (lane == 0) mbar_arrive(&c.q_ready);
-            return true;
-        };
         // After a wait that gave up, these warps go on (on meaningless values) to the end of the share:
         // none of them may leave while others stand at a barrier of the group.
-        // The next part's queries go in before a part's output is written: its first scores are computed
-        // meanwhile.
-        int slot = 0;
-        bool open = false, whole = false;
 #pragma unroll 1
-        while (true) {
-            Part following;
-            const bool more = stage(following);
-            if (open) {
-                wait(&c.o_done, (tile - 1) & 1, abort);
-                __syncwarp();
-                tc::fence_after_sync();
-                const Rows rs = rows_of(rows_at, N, p.words, par);
-                const int held = min(nh, min(N, w.n * gqa - w.g * N) - r0);  // the group's rows that exist
-                const uint32_t ot = tmem + lanes + o_col + r0;
-                if (c.poison) {  // set before the staging's barriers, cleared after them
-#pragma unroll 1
-                    for (int ci = 0; ci < kChunks; ++ci)
-#pragma unroll 1
-                        for (int f = 0; f < held; f += 8) {
-                            float v[8];
-                            tc::ld8(ot + ci * N + f, v);
-                            tc::wait_ld();
-                            if (128 * ci + key < D)
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) v[j] += poison_of<kBf16>(p, w, rs, D, 128 * ci + key, r0 + f + j);
-                            __syncwarp();
-                            tc::st8(ot + ci * N + f, v);
-                        }
-                    tc::wait_st();
-                }
-#pragma unroll 1
-                for (int ci = 0; ci < kChunks; ++ci) {
-                    const int d = 128 * ci + key;
-                    uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + d;
-                    float* part = p.part + ((long long)slot * N + r0) * D + d;
-#pragma unroll 1
-                    for (int f = 0; f < held; f += 32) {
-                        float v[4][8];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (f + 8 * e < nh) tc::ld8(ot + ci * N + f + 8 * e, v[e]);
-                        tc::wait_ld();
-                        if (D == 64 && key >= 64) continue;
-                        if (whole) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (f + j < held) out[rs.out[r0 + f + j]] = pack1<kBf16>(v[j >> 3][j & 7] * c.inv[r0 + f + j]);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (f + j < held) __stcg(part + (f + j) * D, v[j >> 3][j & 7]);
-                        }
-                    }
-                }
-                tc::fence_before_sync();
-                asm volatile("bar.sync 3, 256;" ::: "memory");  // every thread is done with poison and inv
-            }
+        for (int part = 0;; ++part) {
+            const bool more = all_groups(next_part(c, list, w, false, abort));
+            if (lane == 0) mbar_arrive(&c.part_free[(list.slot + kParts - 1) % kParts]);
             if (!more) break;
-            open = true;
-            w = following;
-            par ^= 1;
-            const Rows rs = rows_of(rows_at, N, p.words, par);
-            if (tid == 0) c.poison = 0;
+            const Rows rs = rows_of(rows_at, N, p.words, part & 1);
+            wait(&c.q_ready[part & 1], (part >> 1) & 1, abort);
 #pragma unroll
             for (int r = 0; r < kNH; ++r) l[r] = 0.f;
 
@@ -835,18 +770,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bool waited = tile == 0;
                 if (group_or(grp, over > kLazy)) {
 #pragma unroll 1
-                    for (int f = 0; f < nh; f += 32) {
-                        float m[4][8];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (f + 8 * e < nh) tc::ld8(st + f + 8 * e, m[e]);
+                    for (int f = 0; f < nh; f += 16) {
+                        float m[2][8];
+                        const bool both = f + 8 < nh;
+                        tc::ld8(st + f, m[0]);
+                        if (both) tc::ld8(st + f + 8, m[1]);
                         tc::wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (f + 8 * e < nh) {
-                                reduce_scatter8<true>(m[e], lane);
-                                c.red[qd][r0 + f + 8 * e + (lane >> 2)] = m[e][0] * p.c;
-                            }
+                        reduce_scatter8<true>(m[0], lane);
+                        c.red[qd][r0 + f + (lane >> 2)] = m[0][0] * p.c;
+                        if (both) {
+                            reduce_scatter8<true>(m[1], lane);
+                            c.red[qd][r0 + f + 8 + (lane >> 2)] = m[1][0] * p.c;
+                        }
                     }
                     group_bar(grp);
                     if (gt < nh) {
@@ -894,29 +829,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 uint32_t pk[kNH / 2];
 #pragma unroll
-                for (int f = 0; f < kNH; f += kCh)
+                for (int f = 0; f < kNH; f += 16)
                     if (f < nh) {
-                        float s[kCh];
+                        float v[16];
+                        load16(st + f, kNH > 8 && f + 8 < nh, v);
 #pragma unroll
-                        for (int e = 0; e < kCh; e += 8)
-                            if (f + e < nh) {
-                                float v[8];
-                                tc::ld8(st + f + e, v);
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) s[e + j] = v[j];
-                            }
-                        tc::wait_ld();
-                        if (f + kCh >= nh) {
-                            tc::fence_before_sync();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&c.s_free[b]);
-                        }
-#pragma unroll
-                        for (int r = 0; r < kCh; r += 4)
-                            if (f + r < nh) {
+                        for (int r = 0; r < 16; r += 4)
+                            if (f + r < kNH && f + r < nh) {
                                 const float4 n = *reinterpret_cast<const float4*>(&rs.nref[r0 + f + r]);
-                                const float e0 = exp2_approx(fmaf(s[r], p.c, n.x)), e1 = exp2_approx(fmaf(s[r + 1], p.c, n.y));
-                                const float e2 = exp2_approx(fmaf(s[r + 2], p.c, n.z)), e3 = exp2_approx(fmaf(s[r + 3], p.c, n.w));
+                                const float e0 = exp2_approx(fmaf(v[r], p.c, n.x)), e1 = exp2_approx(fmaf(v[r + 1], p.c, n.y));
+                                const float e2 = exp2_approx(fmaf(v[r + 2], p.c, n.z)), e3 = exp2_approx(fmaf(v[r + 3], p.c, n.w));
                                 l[f + r] += e0;
                                 l[f + r + 1] += e1;
                                 l[f + r + 2] += e2;
@@ -925,6 +847,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 pk[(f + r) / 2 + 1] = pack2<kBf16>(e2, e3);
                             }
                     }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&c.s_free[b]);
                 // P V of the tile before has read the buffer.
                 if (!waited) wait(&c.o_done, (tile - 1) & 1, abort);
                 const uint32_t prow = key * 128;
@@ -939,56 +864,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.p_full);
-                if (edge) {
-                    // Ring slots of this tile's V, in the producer's order: K(t0), then K(i + 1), V(i).
-                    const int vq = q + (i - w.t0) * 2 * kChunks + (i + 1 < w.t1 ? 2 : 1) * kChunks;
-                    const int keys = w.keys(i), rows = (keys + 15) & ~15;
-                    const bool scan = i >= w.pre || w.windowed(p.window, i);
-                    const int lead = i < w.pre ? w.start - (w.base + i * kKeys) : 0;  // keys before every row's
-#pragma unroll 1
-                    for (int ci = 0; ci < kChunks; ++ci) {
-                        const int slot = (vq + ci) % slots;
-                        // v_ready first: the slot may still be a use behind, and a parity cannot tell a
-                        // phase from the one two before it.
-                        wait(&c.v_ready[ci], fix & 1, abort);
-                        wait(&c.full[slot], ((vq + ci) / slots) & 1, abort);
-                        unsigned char* base = ring + slot * kSlotBytes;
-#pragma unroll 1
-                        for (int e = tid; e < rows * 8 * kHalves; e += 4 * 256) {
-                            uint4 v[4];
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                const int x = e + u * 256, k = x / (8 * kHalves), cc = x % (8 * kHalves);
-                                uint4* at = reinterpret_cast<uint4*>(base + (cc >> 3) * kBoxBytes + k * 128 + (cc & 7) * 16);
-                                v[u] = make_uint4(0, 0, 0, 0);
-                                if (k < rows) {
-                                    if (k >= keys || k < lead) *at = make_uint4(0, 0, 0, 0);
-                                    else if (scan) v[u] = *at;
-                                }
-                            }
-                            uint32_t dirty = 0;
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) dirty |= (uint32_t)any_not_finite<kBf16>(v[u]) << u;
-#pragma unroll 1
-                            for (int u = 0; dirty; ++u, dirty >>= 1) {
-                                if (!(dirty & 1)) continue;
-                                const int x = e + u * 256;
-                                uint16_t* h = reinterpret_cast<uint16_t*>(base + (x % (8 * kHalves) >> 3) * kBoxBytes +
-                                                                          x / (8 * kHalves) * 128 + (x & 7) * 16);
-#pragma unroll 1
-                                for (int y = 0; y < 8; ++y)
-                                    if (not_finite<kBf16>(h[y])) h[y] = 0;
-                                c.poison = 1;
-                            }
-                        }
-                        fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&c.v_fix[ci]);
-                    }
-                    ++fix;
-                }
             }
-            q += (w.t1 - w.t0) * 2 * kChunks;
 
             // The part's result: sums over the keys, then O^T.
             group_bar(grp);
@@ -1002,19 +878,190 @@ __global__ void __launch_bounds__(kThreads, 1)
                     c.red[qd][r0 + r + (lane >> 2)] = m[0];
                 }
             group_bar(grp);
-            whole = w.t1 - w.t0 == w.tiles;
-            slot = 2 * blockIdx.x + (first_part ? 0 : 1);
-            first_part = false;
+            const bool whole = w.t1 - w.t0 == w.tiles;
+            const int slot = 2 * blockIdx.x + (part ? 1 : 0);
             if (gt < nh) {
                 const int r = r0 + gt;
                 const float sum = (c.red[0][r] + c.red[1][r]) + (c.red[2][r] + c.red[3][r]);
                 c.inv[r] = sum != 0.f ? 1.f / sum : 0.f;
                 if (!whole) p.ml[(long long)slot * N + r] = make_float2(rs.nref[r] == kUnset ? -INFINITY : -rs.nref[r], sum);
             }
+            group_bar(grp);
+            wait(&c.o_done, (tile - 1) & 1, abort);
+            __syncwarp();
+            tc::fence_after_sync();
+            const int held = min(nh, min(N, w.n * gqa - w.g * N) - r0);  // the group's rows that exist
+            const uint32_t ot = tmem + lanes + o_col + r0;
+            if (*(volatile int*)&c.poison[part & 1]) {
+#pragma unroll 1
+                for (int ci = 0; ci < kChunks; ++ci)
+#pragma unroll 1
+                    for (int f = 0; f < held; f += 8) {
+                        float v[8];
+                        tc::ld8(ot + ci * N + f, v);
+                        tc::wait_ld();
+                        if (128 * ci + key < D)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[j] += poison_of<kBf16>(p, w, rs, D, 128 * ci + key, r0 + f + j);
+                        __syncwarp();
+                        tc::st8(ot + ci * N + f, v);
+                    }
+                tc::wait_st();
+            }
+#pragma unroll 1
+            for (int ci = 0; ci < kChunks; ++ci) {
+                const int d = 128 * ci + key;
+                uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + d;
+                float* dst = p.part + ((long long)slot * N + r0) * D + d;
+#pragma unroll 1
+                for (int f = 0; f < held; f += 16) {
+                    float v[16];
+                    load16(ot + ci * N + f, f + 8 < nh, v);
+                    if (D == 64 && key >= 64) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (f + j < held) out[rs.out[r0 + f + j]] = pack1<kBf16>(v[j] * c.inv[r0 + f + j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (f + j < held) __stcg(dst + (f + j) * D, v[j]);
+                    }
+                }
+            }
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c.rows_free[part & 1]);
         }
-    } else {
+    } else if (warp == kScheduler) {
+        // ------------------------------------------------------------------ scheduler
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (warp == kScheduler && lane == 0) schedule(p, c, abort);
+        // Deals the parts out, and sets up each part's rows and queries while the one before is worked on.
+        const int gqa = p.heads / p.kv_heads;
+        int part = 0;
+        schedule(p, c, abort, [&](const Part& w) {
+            const int par = part & 1;
+            const Rows rs = rows_of(rows_at, N, p.words, par);
+            const int R = min(N, w.n * gqa - w.g * N);
+            bool ok = part < 2 || wait(&c.rows_free[par], ((part >> 1) - 1) & 1, abort);
+            // Rows of a part: r -> node (g N + r) / gqa, query head h gqa + (g N + r) % gqa.
+#pragma unroll 1
+            for (int r = lane; r < N; r += 32) {
+                const int row = w.g * N + r, tok = w.first + min(row / gqa, w.n - 1);
+                rs.out[r] = tok * p.out_stride + (w.h * gqa + row % gqa) * D;
+                rs.nref[r] = kUnset;
+                const int dep = p.window ? min(max(p.depth[tok], 0), w.n - 1) : 0;
+                rs.depth[r] = dep;
+                rs.start[r] = p.window ? max(0, w.len + dep - p.window + 1) : 0;
+#pragma unroll 1
+                for (int i = 0; i * 32 < w.n; ++i) rs.mask[i * N + r] = p.mask[(long long)tok * p.mask_words + i];
+            }
+            if (lane == 0) c.poison[par] = 0;
+            // The queries, into the MMA's K-major layout, once S of the part before has completed.
+            ok = ok && (part == 0 || wait(&c.q_free, (part - 1) & 1, abort));
+            ++part;
+            if (!__all_sync(0xffffffffu, ok)) return false;
+            constexpr int kLanes = D / 8 < 32 ? D / 8 : 32;      // lanes on one row, 16 bytes each
+            const uint32_t q_at = smem_u32(qs);
+            const int step = 32 / kLanes, ch = lane % kLanes;
+            int r = lane / kLanes, node = (w.g * N + r) / gqa, hd = (w.g * N + r) % gqa;
+#pragma unroll 1
+            for (; r < N; r += step) {
+                const uint32_t dst = q_at + r * 128 + ((ch & 7) ^ (r & 7)) * 16;
+                if (r < R) {
+                    const char* src = p.q + 2 * ((w.first + node) * p.q_stride + (w.h * gqa + hd) * D + ch * 8);
+#pragma unroll
+                    for (int k = 0; k < D / 8 / kLanes; ++k)
+                        cp_async16(dst + ((ch >> 3) + k * (kLanes / 8)) * N * 128, src + k * kLanes * 16);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < D / 8 / kLanes; ++k)
+                        *reinterpret_cast<uint4*>(qs + (dst - q_at) + ((ch >> 3) + k * (kLanes / 8)) * N * 128) = make_uint4(0, 0, 0, 0);
+                }
+                hd += step;
+                while (hd >= gqa) {
+                    hd -= gqa;
+                    ++node;
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c.q_ready[par]);
+            return true;
+        });
+    } else {
+        // ------------------------------------------------------------------ cleaner
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        // In tiles with hidden keys, V's rows that no row may see become zeros (they may hold anything,
+        // and 0 x NaN is NaN); rows that only some see lose their infinities and NaN, which are noted and
+        // added to those rows' outputs.
+        Part w;
+        Place list;
+        int q = 0, fix = 0;  // ring slots, as the producer counts them, and edge tiles so far
+        bool ok = true;
+#pragma unroll 1
+        for (int part = 0; ok; ++part) {
+            ok = __all_sync(0xffffffffu, next_part(c, list, w, false, abort));
+            if (lane == 0) mbar_arrive(&c.part_free[(list.slot + kParts - 1) % kParts]);
+            if (!ok) break;
+#pragma unroll 1
+            for (int i = w.t0; i < w.t1; ++i) {
+                if (!w.edge(p.window, i)) continue;
+                // V(i) comes after K(t0) .. K(i + 1) and V(t0) .. V(i - 1).
+                const int vq = q + (i - w.t0) * 2 * kChunks + (i + 1 < w.t1 ? 2 : 1) * kChunks;
+                const int keys = w.keys(i), rows = (keys + 15) & ~15;
+                const bool scan = i >= w.pre || w.windowed(p.window, i);
+                const int lead = i < w.pre ? w.start - (w.base + i * kKeys) : 0;  // keys before every row's
+#pragma unroll 1
+                for (int ci = 0; ci < kChunks && ok; ++ci) {
+                    // v_ready first: the slot may still be a use behind, and a parity cannot tell a phase
+                    // from the one two before it.
+                    ok = wait(&c.v_ready[ci], fix & 1, abort) && wait(&c.full[(vq + ci) % slots], ((vq + ci) / slots) & 1, abort);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    unsigned char* base = ring + (vq + ci) % slots * kSlotBytes;
+                    const int from = scan ? 0 : max(0, keys) * 8 * kHalves;
+                    if (!scan)
+#pragma unroll 1
+                        for (int e = lane; e < lead * 8 * kHalves; e += 32)
+                            *reinterpret_cast<uint4*>(base + (e % (8 * kHalves) >> 3) * kBoxBytes + e / (8 * kHalves) * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+                    for (int e = from + lane; e < rows * 8 * kHalves; e += 8 * 32) {
+                        uint4 v[8];
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const int x = e + u * 32, k = x / (8 * kHalves), cc = x % (8 * kHalves);
+                            uint4* at = reinterpret_cast<uint4*>(base + (cc >> 3) * kBoxBytes + k * 128 + (cc & 7) * 16);
+                            v[u] = make_uint4(0, 0, 0, 0);
+                            if (k < rows) {
+                                if (k >= keys || k < lead) *at = make_uint4(0, 0, 0, 0);
+                                else v[u] = *at;
+                            }
+                        }
+                        uint32_t dirty = 0;
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) dirty |= (uint32_t)any_not_finite<kBf16>(v[u]) << u;
+#pragma unroll 1
+                        for (int u = 0; dirty; ++u, dirty >>= 1) {
+                            if (!(dirty & 1)) continue;
+                            const int x = e + u * 32;
+                            uint16_t* h = reinterpret_cast<uint16_t*>(base + (x % (8 * kHalves) >> 3) * kBoxBytes +
+                                                                      x / (8 * kHalves) * 128 + (x & 7) * 16);
+#pragma unroll 1
+                            for (int y = 0; y < 8; ++y)
+                                if (not_finite<kBf16>(h[y])) h[y] = 0;
+                            c.poison[part & 1] = 1;
+                        }
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&c.v_fix[ci]);
+                }
+                ++fix;
+            }
+            q += (w.t1 - w.t0) * 2 * kChunks;
+        }
     }
     tc::fence_before_sync();
     __syncthreads();
@@ -1176,12 +1223,11 @@ cudaError_t run(const CUtensorMap* maps, const Params& p, const Shape& sh, cudaS
 
 template <int D, bool kBf16>
 cudaError_t run_rows(const CUtensorMap* maps, const Params& p, const Shape& sh, cudaStream_t st) {
-    const int nh = sh.N / 2;
-    if (nh <= 8) return run<D, 8, kBf16>(maps, p, sh, st);
-    if (nh <= 16) return run<D, 16, kBf16>(maps, p, sh, st);
-    if (nh <= 32) return run<D, 32, kBf16>(maps, p, sh, st);
-    if constexpr (D == 512) return run<D, 40, kBf16>(maps, p, sh, st);
-    else return run<D, 64, kBf16>(maps, p, sh, st);
+    const int units = (sh.N / 8 + 3) / 4;  // rows of the largest softmax group, in eights
+    if (units <= 1) return run<D, 8, kBf16>(maps, p, sh, st);
+    if (units <= 2) return run<D, 16, kBf16>(maps, p, sh, st);
+    if constexpr (D == 512) return run<D, 24, kBf16>(maps, p, sh, st);
+    else return run<D, 32, kBf16>(maps, p, sh, st);
 }
 
 template <int D>
