@@ -57,7 +57,8 @@ constexpr int kSoftRegs = 104, kOtherRegs = 64;
 constexpr uint32_t kBoxBytes = kKeys * 128;  // 128 keys x 64 dims of 16 bits
 constexpr int kMaxSlots = 8;
 constexpr int kParts = 4;            // parts the scheduler is ahead
-constexpr int kTreeBox = 16;         // node rows per TMA box
+constexpr int kTreeBox = 8;          // node rows per TMA box: the swizzle's eight
+constexpr int kPageBox = 32;         // and at most so many cached rows
 constexpr float kUnset = 1e30f;      // negated reference of a row that has seen no key
 constexpr float kLazy = 8.f;         // a reference moves when a score exceeds it by 2^8
 constexpr size_t kSmemLimit = 232448;
@@ -65,23 +66,24 @@ constexpr size_t kSmemLimit = 232448;
 constexpr int kItemCost = 2;
 // Items of at most this many tiles are not split, which saves the second kernel.
 constexpr int kWholeTiles = 6;
+constexpr int kFewSeqs = 64;
 
 __device__ int g_tree_err;  // set when a bounded wait gives up
 
 // A part of an item: tiles t0 .. t1 - 1 of (sequence b, K/V head h, row group g).
 struct Part {
     int b, h, g, t0, t1;
+    // The part's keys stand in a line: `pre` cached ones from position `base` on (whole boxes, the last
+    // of them may pass the sequence's end), then the nodes. Tile i is places 128 i .. 128 i + 127.
     int len, first, n, start, base, pre, tiles;
-    // Keys of tile i up to its last one any row may see, whether some rows start inside it, and
-    // whether some keys are hidden from some row.
-    __device__ __forceinline__ int keys(int i) const {
-        return min(kKeys, i < pre ? len - (base + i * kKeys) : n - (i - pre) * kKeys);
-    }
+    // Places of tile i up to its last node.
+    __device__ __forceinline__ int keys(int i) const { return min(kKeys, pre + n - i * kKeys); }
+    // Whether some rows' windows start inside the tile, and whether some places are hidden from some row.
     __device__ __forceinline__ bool windowed(int window, int i) const {
-        return window && i < pre && base + i * kKeys < start + n - 1;
+        return window && i * kKeys < pre && base + i * kKeys < start + n - 1;
     }
     __device__ __forceinline__ bool edge(int window, int i) const {
-        return i >= pre || keys(i) < kKeys || windowed(window, i) || base + i * kKeys < start;
+        return (i + 1) * kKeys > len - base || base + i * kKeys < start || windowed(window, i);
     }
 };
 
@@ -93,8 +95,7 @@ struct alignas(16) Ctl {
     uint64_t q_ready[2], q_free, rows_free[2], p_full, o_done, v_ready[4], v_fix[4], done;
     uint32_t tmem_base;
     int abort, poison[2];
-    int seq0, rem0, begin, end;  // this block's share and where in which sequence it starts
-    int scan[kThreads / 32 + 1];
+    int scan[kThreads / 32];      // units of each warp's run of sequences
     alignas(16) float corr[128];  // factor of a row's sum and output when its reference moves
     alignas(16) float inv[128];
     alignas(16) float red[4][128];
@@ -142,8 +143,8 @@ struct Params {
 // One sequence's share of the work.
 struct Seq {
     int len, first, n;   // cached tokens, first node, nodes
-    int start, base;     // first cached position any node may see, and the first tile's
-    int pre, tiles, groups;
+    int start, base;     // first cached position any node may see, and the first in the line of keys
+    int pre, tiles, groups;  // cached places in that line, tiles, row groups
 };
 
 // The kernel's roles share this code out of line, here and below: inlined everywhere it would not
@@ -154,9 +155,14 @@ __device__ __noinline__ void load_seq(const Params& p, int b, Seq& s) {
     s.n = min(min(max(p.cu[b + 1] - s.first, 0), p.n_tokens - s.first), p.max_nodes);
     s.len = min(max(p.lens[b], 0), p.width * p.page_size);
     s.start = p.window ? max(0, s.len - p.window + 1) : 0;
-    s.base = s.start / p.box * p.box;
-    s.pre = s.start < s.len ? (s.len - s.base + kKeys - 1) / kKeys : 0;
-    s.tiles = s.n ? s.pre + (s.n + kKeys - 1) / kKeys : 0;
+    if (s.start < s.len) {
+        s.base = s.start / p.box * p.box;
+        s.pre = (s.len - s.base + p.box - 1) / p.box * p.box;
+    } else {
+        s.base = s.start = s.len;
+        s.pre = 0;
+    }
+    s.tiles = s.n ? (s.pre + s.n + kKeys - 1) / kKeys : 0;
     s.groups = (s.n * gqa + p.N - 1) / p.N;
 }
 
@@ -216,17 +222,50 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
 template <class Ready>
 __device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* abort, Ready ready) {
     Place at;
-    int pos = c.begin;
-    const int end = c.end;
+    const int lane = threadIdx.x & 31;
+    // This block's share of all units, and where it starts: skip whole runs, then sequences.
+    int total = 0, first = 0, per = p.seqs, runs = 1;
+    if (p.seqs > kFewSeqs) {
+        runs = kThreads / 32;
+        per = (p.seqs + runs - 1) / runs;
+        total = warp_sum_int(lane < runs ? c.scan[lane] : 0);
+    } else {
+#pragma unroll 1
+        for (int b = lane; b < p.seqs; b += 32) total += seq_units(p, b);
+        total = warp_sum_int(total);
+    }
+    int pos = share_begin(total, gridDim.x, blockIdx.x), before = 0;
+    const int end = share_begin(total, gridDim.x, blockIdx.x + 1);
+#pragma unroll 1
+    for (; runs > 1 && before + c.scan[first] <= pos && first + 1 < runs; ++first) before += c.scan[first];
+    first *= per;
     Seq s;
     int b = 0, h = 0, g = 0, u = 0;
     if (pos < end) {
-        b = c.seq0;
+#pragma unroll 1
+        for (int b0 = first; b0 < p.seqs; b0 += 32) {
+            const int units = b0 + lane < p.seqs ? seq_units(p, b0 + lane) : 0;
+            int x = units;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, pos < before + x);
+            if (hit) {
+                const int who = __ffs(hit) - 1;
+                b = b0 + who;
+                u = pos - before - __shfl_sync(0xffffffffu, x - units, who);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, x, 31);
+        }
         load_seq(p, b, s);
-        const int item = item_units(p, s), r = c.rem0 % (item * s.groups);
-        h = c.rem0 / (item * s.groups);
-        g = r / item;
-        u = r % item;
+        const int item = item_units(p, s);
+        h = u / (item * s.groups);
+        u -= h * item * s.groups;
+        g = u / item;
+        u -= g * item;
     }
 #pragma unroll 1
     while (true) {
@@ -371,30 +410,26 @@ __device__ __forceinline__ void reduce_scatter8(float (&v)[8], int lane) {
     v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 1));
 }
 
-// Whether row r of the part sees key k (0 .. 127) of tile i.
-__device__ __forceinline__ bool sees(const Params& p, const Part& w, const Rows& c, int i, int k, int r) {
-    if (i < w.pre) {
-        const int j = w.base + i * kKeys + k;
-        return j < w.len && j >= c.start[r];
-    }
-    const int j = (i - w.pre) * kKeys + k;
+// Whether row r of the part sees place x of its line of keys.
+__device__ __forceinline__ bool sees(const Params& p, const Part& w, const Rows& c, int x, int r) {
+    if (x < w.pre) return w.base + x < w.len && w.base + x >= c.start[r];
+    const int j = x - w.pre;
     if (j >= w.n || !((c.mask[(j >> 5) * p.N + r] >> (j & 31)) & 1)) return false;
     return !p.window || c.depth[r] - min(max(p.depth[w.first + j], 0), w.n - 1) < p.window;
 }
 
-// V's row for key k of tile i (null: no such row).
-__device__ const uint16_t* v_row(const Params& p, const Part& w, int i, int k, int dim) {
-    if (i < w.pre) {
-        const int j = w.base + i * kKeys + k;
+// V's row at place x (null: no such row).
+__device__ const uint16_t* v_row(const Params& p, const Part& w, int x, int dim) {
+    if (x < w.pre) {
+        const int j = w.base + x;
         if (j < w.start || j >= w.len) return nullptr;
         const int page = p.table[(long long)w.b * p.width + j / p.page_size];
         if (page < 0 || page >= p.pages) return nullptr;
         return reinterpret_cast<const uint16_t*>(p.v_pool) + page * p.page_stride +
                ((long long)(j % p.page_size) * p.kv_heads + w.h) * dim;
     }
-    const int j = (i - w.pre) * kKeys + k;
-    if (j >= w.n) return nullptr;
-    return reinterpret_cast<const uint16_t*>(p.v_new) + (w.first + j) * p.new_stride + w.h * dim;
+    if (x - w.pre >= w.n) return nullptr;
+    return reinterpret_cast<const uint16_t*>(p.v_new) + (w.first + x - w.pre) * p.new_stride + w.h * dim;
 }
 
 // What the infinities and NaN taken out of this part's V tiles add to row r in dimension d.
@@ -402,10 +437,11 @@ template <bool kBf16>
 __device__ __noinline__ float poison_of(const Params& p, Part w, Rows c, int dim, int d, int r) {
     float sum = 0.f;
     for (int i = w.t0; i < w.t1; ++i) {
-        if (!(i >= w.pre || w.windowed(p.window, i))) continue;
-        for (int k = 0; k < w.keys(i); ++k) {
-            const uint16_t* row = v_row(p, w, i, k, dim);
-            if (row && not_finite<kBf16>(row[d]) && sees(p, w, c, i, k, r)) sum += unpack1<kBf16>(row[d]);
+        if (!w.edge(p.window, i)) continue;
+        for (int x = i * kKeys; x < i * kKeys + w.keys(i); ++x) {
+            if (x < w.pre && !w.windowed(p.window, i)) continue;  // seen by all: still in the product
+            const uint16_t* row = v_row(p, w, x, dim);
+            if (row && not_finite<kBf16>(row[d]) && sees(p, w, c, x, r)) sum += unpack1<kBf16>(row[d]);
         }
     }
     return sum;
@@ -475,35 +511,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (warp == kIssuer) tc::alloc(&c.tmem_base, p.tmem_cols);
 
-    // This block's share of all units.
-    int mine = 0;
+    // With few sequences the scheduling warp adds them up by itself, below; with many each warp adds a run.
+    if (p.seqs > kFewSeqs) {
+        const int per = (p.seqs + kThreads / 32 - 1) / (kThreads / 32);
+        int mine = 0;
 #pragma unroll 1
-    for (int b = threadIdx.x; b < p.seqs; b += kThreads) mine += seq_units(p, b);
-    const int total = block_total(mine, c.scan);
-    if (warp == 0) {
-        const int begin = share_begin(total, gridDim.x, blockIdx.x), end = share_begin(total, gridDim.x, blockIdx.x + 1);
-        if (lane == 0) {
-            c.begin = begin;
-            c.end = end;
-        }
-        int before = 0;
-#pragma unroll 1
-        for (int b0 = 0; begin < end && b0 < p.seqs && before <= begin; b0 += 32) {
-            const int b = b0 + lane;
-            const int mt = b < p.seqs ? seq_units(p, b) : 0;
-            int x = mt;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            const int at = before + x - mt;
-            if (mt > 0 && begin >= at && begin < at + mt) {
-                c.seq0 = b;
-                c.rem0 = begin - at;
-            }
-            before += __shfl_sync(0xffffffffu, x, 31);
-        }
+        for (int b = warp * per + lane; b < min(p.seqs, (warp + 1) * per); b += 32) mine += seq_units(p, b);
+        mine = warp_sum_int(mine);
+        if (lane == 0) c.scan[warp] = mine;
     }
     tc::fence_before_sync();
     __syncthreads();
@@ -529,9 +544,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(&c.part_free[(list.slot + kParts - 1) % kParts]);
             if (!ok) break;
             const int32_t* row = p.table + (long long)w.b * p.width;
-            auto ids = [&](int i) {  // page of this lane's key box in tile i
-                const int j = w.base + i * kKeys + kb * p.box;
-                return i < w.pre && kb * p.box < kKeys && j < w.len ? row[j / p.page_size] : -1;
+            // Boxes of tile i: cached rows, then nodes; one of up to 16 is this lane's.
+            auto cached = [&](int i) { return min(kKeys, max(0, w.pre - i * kKeys)) / p.box; };
+            auto ids = [&](int i) {  // its page
+                return kb < cached(i) ? row[(w.base + i * kKeys + kb * p.box) / p.page_size] : -1;
             };
             int id0 = -1, id1 = ids(w.t0), id2 = -1;
 #pragma unroll 1
@@ -545,26 +561,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                     id1 = id2;
                 }
                 if (tile < w.t0 || tile >= w.t1) continue;
-                const bool old = tile < w.pre;
-                const int rows = old ? p.box : kTreeBox, boxes = (w.keys(tile) + rows - 1) / rows;
-                const int j = w.base + tile * kKeys + kb * p.box;
+                const int nc = cached(tile), from = nc * p.box, nn = max(0, w.keys(tile) - from + kTreeBox - 1) / kTreeBox;
+                const bool old = kb < nc, mine = kb < nc + nn && half < kHalves;
+                const int at_row = old ? kb * p.box : from + (kb - nc) * kTreeBox;
+                const int x = tile * kKeys + at_row;
                 // A page id out of range is an out-of-range coordinate: the box reads as zeros.
-                const int z = old ? j % p.page_size : w.first + (tile - w.pre) * kKeys + kb * kTreeBox;
+                const int z = old ? (w.base + x) % p.page_size : w.first + x - w.pre;
                 const int pg = page < 0 ? p.pages : page;
                 const uint64_t map = old ? (is_v ? vd : kd) : (is_v ? vnd : knd);
-                const bool mine = kb < boxes && half < kHalves;
+                const uint32_t bytes = (uint32_t)(from + nn * kTreeBox) * 128 * kHalves;
 #pragma unroll 1
                 for (int ci = 0; ci < kChunks; ++ci) {
                     ok = wait(&c.empty[at.slot], at.phase ^ 1, abort);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    if (lane == 0) mbar_expect_tx(&c.full[at.slot], (uint32_t)(boxes * rows) * 128 * kHalves);
+                    if (lane == 0) mbar_expect_tx(&c.full[at.slot], bytes);
                     __syncwarp();
                     if (mine) {
-                        unsigned char* dst = ring + at.slot * kSlotBytes + half * kBoxBytes + kb * rows * 128;
-                        const int x = 128 * ci + 64 * half;
-                        if (old) tma_4d(dst, map, x, w.h, z, pg, &c.full[at.slot]);
-                        else tma_3d(dst, map, x, w.h, z, &c.full[at.slot]);
+                        unsigned char* dst = ring + at.slot * kSlotBytes + half * kBoxBytes + at_row * 128;
+                        const int d = 128 * ci + 64 * half;
+                        if (old) tma_4d(dst, map, d, w.h, z, pg, &c.full[at.slot]);
+                        else tma_3d(dst, map, d, w.h, z, &c.full[at.slot]);
                     }
                     at.step(slots);
                     ++used;
@@ -719,31 +736,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const bool edge = w.edge(p.window, i);
                 if (edge) {
                     // Hidden scores become -inf, in tensor memory.
-                    const bool old = i < w.pre;
-                    const int j = old ? w.base + i * kKeys + key : (i - w.pre) * kKeys + key;
+                    const int x = i * kKeys + key;
+                    const bool old = x < w.pre;
+                    const int j = old ? w.base + x : x - w.pre;
                     const bool in = j < (old ? w.len : w.n);
                     const int near = p.window && in && !old ? min(max(p.depth[w.first + j], 0), w.n - 1) + p.window : INT_MAX;
-                    const uint32_t* word = rs.mask + (old ? 0 : (i - w.pre) * 4 + qd) * N + r0;
+                    // What a row is asked: its first position, or the node's word of its mask.
+                    const int* ask = old || !in ? rs.start + r0 : reinterpret_cast<const int*>(rs.mask) + (j >> 5) * N + r0;
                     const int* depth = rs.depth + r0;
-                    const int* start = rs.start + r0;
 #pragma unroll 1
                     for (int f = 0; f < nh; f += 8) {
                         float v[8];
                         tc::ld8(st + f, v);
                         int a[8], d[8];
-                        if (old) {
-                            *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(start + f);
-                            *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(start + f + 4);
-                        } else {
-                            *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(word + f);
-                            *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(word + f + 4);
-                        }
+                        *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(ask + f);
+                        *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(ask + f + 4);
                         *reinterpret_cast<int4*>(d) = *reinterpret_cast<const int4*>(depth + f);
                         *reinterpret_cast<int4*>(d + 4) = *reinterpret_cast<const int4*>(depth + f + 4);
                         tc::wait_ld();
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            const bool seen = old ? j >= a[k] : (((unsigned)a[k] >> lane) & 1u) & (unsigned)(d[k] < near);
+                            const bool seen = old ? j >= a[k] : (((unsigned)a[k] >> (j & 31)) & 1u) & (unsigned)(d[k] < near);
                             v[k] = in & seen ? v[k] : -INFINITY;
                         }
                         tc::st8(st + f, v);
@@ -1010,9 +1023,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!w.edge(p.window, i)) continue;
                 // V(i) comes after K(t0) .. K(i + 1) and V(t0) .. V(i - 1).
                 const int vq = q + (i - w.t0) * 2 * kChunks + (i + 1 < w.t1 ? 2 : 1) * kChunks;
-                const int keys = w.keys(i), rows = (keys + 15) & ~15;
-                const bool scan = i >= w.pre || w.windowed(p.window, i);
-                const int lead = i < w.pre ? w.start - (w.base + i * kKeys) : 0;  // keys before every row's
+                // Nobody's rows: before every window, from the sequence's end to its first node, past the
+                // last node. Rows that some see and others do not: where windows start, and the nodes.
+                const int keys = w.keys(i), at = w.base + i * kKeys, nodes = min(kKeys, max(0, w.pre - i * kKeys));
+                const int held = min(nodes, max(0, w.len - at));
+                const int lead = max(0, min(held, w.start - at));
+                const int mixed = p.window ? min(held, max(lead, w.start + w.n - 1 - at)) : lead;
 #pragma unroll 1
                 for (int ci = 0; ci < kChunks && ok; ++ci) {
                     // v_ready first: the slot may still be a use behind, and a parity cannot tell a phase
@@ -1021,23 +1037,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     unsigned char* base = ring + (vq + ci) % slots * kSlotBytes;
-                    const int from = scan ? 0 : max(0, keys) * 8 * kHalves;
-                    if (!scan)
+                    const auto zero = [&](int k0, int k1) {
 #pragma unroll 1
-                        for (int e = lane; e < lead * 8 * kHalves; e += 32)
-                            *reinterpret_cast<uint4*>(base + (e % (8 * kHalves) >> 3) * kBoxBytes + e / (8 * kHalves) * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        for (int e = k0 * 8 * kHalves + lane; e < k1 * 8 * kHalves; e += 32)
+                            *reinterpret_cast<uint4*>(base + (e % (8 * kHalves) >> 3) * kBoxBytes + e / (8 * kHalves) * 128 +
+                                                      (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    };
+                    zero(0, lead);
+                    zero(held, nodes);
+                    zero(keys, (keys + 15) & ~15);
 #pragma unroll 1
-                    for (int e = from + lane; e < rows * 8 * kHalves; e += 8 * 32) {
+                    for (int e = lead * 8 * kHalves + lane; e < keys * 8 * kHalves; e += 8 * 32) {
+                        if (e >= mixed * 8 * kHalves && e + 7 * 32 < nodes * 8 * kHalves) continue;
                         uint4 v[8];
 #pragma unroll
                         for (int u = 0; u < 8; ++u) {
                             const int x = e + u * 32, k = x / (8 * kHalves), cc = x % (8 * kHalves);
-                            uint4* at = reinterpret_cast<uint4*>(base + (cc >> 3) * kBoxBytes + k * 128 + (cc & 7) * 16);
                             v[u] = make_uint4(0, 0, 0, 0);
-                            if (k < rows) {
-                                if (k >= keys || k < lead) *at = make_uint4(0, 0, 0, 0);
-                                else v[u] = *at;
-                            }
+                            if (k < mixed || (k >= nodes && k < keys)) v[u] = *reinterpret_cast<const uint4*>(base + (cc >> 3) * kBoxBytes + k * 128 + (cc & 7) * 16);
                         }
                         uint32_t dirty = 0;
 #pragma unroll
@@ -1276,8 +1293,8 @@ cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
     p.slots = sh.slots;
     p.tmem_cols = sh.tmem;
     // The largest power of two that divides a page, so that a box never crosses one.
-    p.box = std::min(kKeys, a.page_size & -a.page_size);
-    const long long tiles = ((long long)a.width * a.page_size + kKeys - 1) / kKeys + 1 + (a.max_nodes + kKeys - 1) / kKeys;
+    p.box = std::min(kPageBox, a.page_size & -a.page_size);
+    const long long tiles = ((long long)a.width * a.page_size + 2 * kPageBox + a.max_nodes + kKeys - 1) / kKeys;
     const long long items = (long long)a.seqs * a.kv_heads * ((a.max_nodes * (a.heads / a.kv_heads) + sh.N - 1) / sh.N);
     if (items * (tiles + kItemCost) > INT32_MAX) return cudaErrorInvalidConfiguration;  // units are counted in 32 bits
     p.whole = tiles <= kWholeTiles;
