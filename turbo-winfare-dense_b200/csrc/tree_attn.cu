@@ -61,7 +61,7 @@ constexpr int kTreeBox = 8;          // node rows per TMA box: the swizzle's eig
 constexpr int kPageBox = 32;         // and at most so many cached rows
 constexpr float kUnset = 1e30f;      // negated reference of a row that has seen no key
 constexpr float kLazy = 8.f;         // a reference moves when a score exceeds it by 2^8
-constexpr size_t kSmemLimit = 232448;
+constexpr size_t kSmemLimit = 232448 - 2048;  // leaves room for a block of the second kernel
 // What starting and finishing an item costs, in tiles, when the shares are cut.
 constexpr int kItemCost = 2;
 // Items of at most this many tiles are not split, which saves the second kernel.
@@ -122,6 +122,20 @@ __device__ __forceinline__ Rows rows_of(unsigned char* base, int N, int words, i
     return r;
 }
 
+// Division of a whole number below 2^31 by one fixed at launch: with s = ceil(log2 d) and m =
+// floor(2^32 (2^s - d) / d) + 1, n / d = (n + mulhi(m, n)) >> s (Granlund and Montgomery).
+struct Div {
+    uint32_t d, m, s;
+    __device__ __forceinline__ int quot(int n) const { return (int)((__umulhi(m, (uint32_t)n) + (uint32_t)n) >> s); }
+    __device__ __forceinline__ int rem(int n) const { return n - quot(n) * (int)d; }
+};
+Div make_div(int d) {
+    Div x{(uint32_t)d, 0, 0};
+    while ((1ll << x.s) < d) ++x.s;
+    x.m = (uint32_t)((((1ull << x.s) - (unsigned)d) << 32) / (unsigned)d + 1);
+    return x;
+}
+
 struct Params {
     const char* q;
     char* out;
@@ -135,8 +149,9 @@ struct Params {
     float* part;   // [2 x blocks][N][dim]
     float2* ml;    // [2 x blocks][N]
     long long q_stride, out_stride, page_stride, new_stride;  // elements
-    int seqs, n_tokens, max_nodes, pages, page_size, width, mask_words, heads, kv_heads, window;
-    int N, words, slots, box, grid, tmem_cols, whole;
+    int seqs, n_tokens, max_nodes, pages, page_size, width, mask_words, kv_heads, window;
+    int N, words, slots, box, box_log, tmem_cols, whole, gqa;
+    Div by_rows, by_gqa, by_page, by_grid;  // N, gqa, page_size and the number of blocks
     float c;       // scale * log2(e)
 };
 
@@ -147,23 +162,23 @@ struct Seq {
     int pre, tiles, groups;  // cached places in that line, tiles, row groups
 };
 
-// The kernel's roles share this code out of line, here and below: inlined everywhere it would not
-// fit the instruction cache, which costs more than the calls.
-__device__ __noinline__ void load_seq(const Params& p, int b, Seq& s) {
-    const int gqa = p.heads / p.kv_heads;
-    s.first = min(max(p.cu[b], 0), p.n_tokens);
-    s.n = min(min(max(p.cu[b + 1] - s.first, 0), p.n_tokens - s.first), p.max_nodes);
-    s.len = min(max(p.lens[b], 0), p.width * p.page_size);
+// The sequence's numbers as they stand in memory, within their bounds, and what follows from them.
+__device__ __forceinline__ void read_seq(const Params& p, int b, Seq& s) {
+    const int from = p.cu[b], to = p.cu[b + 1], len = p.lens[b];
+    s.first = min(max(from, 0), p.n_tokens);
+    s.n = min(min(max(to - s.first, 0), p.n_tokens - s.first), p.max_nodes);
+    s.len = min(max(len, 0), p.width * p.page_size);
+}
+__device__ __forceinline__ void derive_seq(const Params& p, Seq& s) {
     s.start = p.window ? max(0, s.len - p.window + 1) : 0;
-    if (s.start < s.len) {
-        s.base = s.start / p.box * p.box;
-        s.pre = (s.len - s.base + p.box - 1) / p.box * p.box;
-    } else {
+    s.base = s.start >> p.box_log << p.box_log;
+    s.pre = (s.len - s.base + p.box - 1) >> p.box_log << p.box_log;
+    if (s.start >= s.len) {
         s.base = s.start = s.len;
         s.pre = 0;
     }
     s.tiles = s.n ? (s.pre + s.n + kKeys - 1) / kKeys : 0;
-    s.groups = (s.n * gqa + p.N - 1) / p.N;
+    s.groups = p.by_rows.quot(s.n * p.gqa + p.N - 1);
 }
 
 // Sum of the block's values, to every thread.
@@ -181,15 +196,20 @@ __device__ __forceinline__ int block_total(int v, int* red) {
 
 // An item is as long as its tiles and kItemCost more, ahead of them; 1 where items stay whole.
 __device__ __forceinline__ int item_units(const Params& p, const Seq& s) { return p.whole ? 1 : s.tiles + kItemCost; }
-__device__ __forceinline__ int seq_units(const Params& p, int b) {
-    Seq s;
-    load_seq(p, b, s);
+__device__ __forceinline__ int seq_units(const Params& p, const Seq& s) {
     return s.tiles ? item_units(p, s) * s.groups * p.kv_heads : 0;
 }
+__device__ __forceinline__ int seq_units(const Params& p, int b) {
+    Seq s;
+    read_seq(p, b, s);
+    derive_seq(p, s);
+    return seq_units(p, s);
+}
 
-// First unit of block c when `total` units are dealt to `grid` blocks.
-__device__ __forceinline__ int share_begin(int total, int grid, int c) {
-    return total / grid * c + total % grid * c / grid;
+// First unit of block c when `total` units are dealt to the grid's blocks.
+__device__ __forceinline__ int share_begin(const Params& p, int total, int c) {
+    const int q = p.by_grid.quot(total);
+    return q * c + p.by_grid.quot((total - q * (int)p.by_grid.d) * c);
 }
 
 // A place in the ring of slots and the parity of its current use.
@@ -225,26 +245,36 @@ __device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* 
     const int lane = threadIdx.x & 31;
     // This block's share of all units, and where it starts: skip whole runs, then sequences.
     int total = 0, first = 0, per = p.seqs, runs = 1;
+    Seq mine{};
     if (p.seqs > kFewSeqs) {
         runs = kThreads / 32;
         per = (p.seqs + runs - 1) / runs;
         total = warp_sum_int(lane < runs ? c.scan[lane] : 0);
     } else {
 #pragma unroll 1
-        for (int b = lane; b < p.seqs; b += 32) total += seq_units(p, b);
+        for (int b = lane; b < p.seqs; b += 32) {
+            read_seq(p, b, mine);
+            derive_seq(p, mine);
+            total += seq_units(p, mine);
+        }
         total = warp_sum_int(total);
     }
-    int pos = share_begin(total, gridDim.x, blockIdx.x), before = 0;
-    const int end = share_begin(total, gridDim.x, blockIdx.x + 1);
+    int pos = share_begin(p, total, blockIdx.x), before = 0;
+    const int end = share_begin(p, total, blockIdx.x + 1);
 #pragma unroll 1
     for (; runs > 1 && before + c.scan[first] <= pos && first + 1 < runs; ++first) before += c.scan[first];
     first *= per;
-    Seq s;
+    Seq s{};
     int b = 0, h = 0, g = 0, u = 0;
     if (pos < end) {
 #pragma unroll 1
         for (int b0 = first; b0 < p.seqs; b0 += 32) {
-            const int units = b0 + lane < p.seqs ? seq_units(p, b0 + lane) : 0;
+            if (p.seqs > 32) {
+                mine = Seq{};
+                if (b0 + lane < p.seqs) read_seq(p, b0 + lane, mine);
+                derive_seq(p, mine);
+            }
+            const int units = seq_units(p, mine);
             int x = units;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -256,11 +286,14 @@ __device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* 
                 const int who = __ffs(hit) - 1;
                 b = b0 + who;
                 u = pos - before - __shfl_sync(0xffffffffu, x - units, who);
+                s.first = __shfl_sync(0xffffffffu, mine.first, who);
+                s.n = __shfl_sync(0xffffffffu, mine.n, who);
+                s.len = __shfl_sync(0xffffffffu, mine.len, who);
                 break;
             }
             before += __shfl_sync(0xffffffffu, x, 31);
         }
-        load_seq(p, b, s);
+        derive_seq(p, s);
         const int item = item_units(p, s);
         h = u / (item * s.groups);
         u -= h * item * s.groups;
@@ -279,8 +312,10 @@ __device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* 
                     g = 0;
                     if (++h == p.kv_heads) {
                         h = 0;
-                        do load_seq(p, ++b, s);
-                        while (s.tiles == 0);
+                        do {
+                            read_seq(p, ++b, s);
+                            derive_seq(p, s);
+                        } while (s.tiles == 0);
                     }
                 }
                 continue;
@@ -476,37 +511,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int* abort = &c.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    if (threadIdx.x == 0) {
-#pragma unroll 1
-        for (int s = 0; s < slots; ++s) {
-            mbar_init(&c.full[s], 1);
-            mbar_init(&c.empty[s], 1);
-        }
-#pragma unroll 1
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(&c.s_full[b], 1);
-            mbar_init(&c.s_free[b], kSoftWarps);
-        }
-#pragma unroll 1
-        for (int i = 0; i < kParts; ++i) {
-            mbar_init(&c.part_full[i], 1);
-            mbar_init(&c.part_free[i], kSoftWarps + 3);
-        }
-        mbar_init(&c.q_free, 1);
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&c.q_ready[i], 1);
-            mbar_init(&c.rows_free[i], kSoftWarps);
-        }
-        mbar_init(&c.p_full, kSoftWarps);
-        mbar_init(&c.o_done, 1);
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(&c.v_ready[i], 1);
-            mbar_init(&c.v_fix[i], 1);
-        }
-        mbar_init(&c.done, 1);
-        c.abort = 0;
+    if (warp == 0) {  // a lane or two per kind of barrier: one after another they take a microsecond
+        const auto init = [&](int from, int n, uint64_t* bars, uint32_t count) {
+            if (lane >= from && lane < from + n) mbar_init(bars + lane - from, count);
+        };
+        init(0, kMaxSlots, c.full, 1);
+        init(0, kMaxSlots, c.empty, 1);
+        init(8, 2, c.s_full, 1);
+        init(8, 2, c.s_free, kSoftWarps);
+        init(10, 2, c.q_ready, 1);
+        init(10, 2, c.rows_free, kSoftWarps);
+        init(12, kParts, c.part_full, 1);
+        init(12, kParts, c.part_free, kSoftWarps + 3);
+        init(16, 4, c.v_ready, 1);
+        init(16, 4, c.v_fix, 1);
+        init(20, 1, &c.q_free, 1);
+        init(21, 1, &c.p_full, kSoftWarps);
+        init(22, 1, &c.o_done, 1);
+        init(23, 1, &c.done, 1);
+        if (lane == 24) c.abort = 0;
         mbar_init_fence();
     }
     if (warp == kIssuer) tc::alloc(&c.tmem_base, p.tmem_cols);
@@ -545,9 +568,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             const int32_t* row = p.table + (long long)w.b * p.width;
             // Boxes of tile i: cached rows, then nodes; one of up to 16 is this lane's.
-            auto cached = [&](int i) { return min(kKeys, max(0, w.pre - i * kKeys)) / p.box; };
+            auto cached = [&](int i) { return min(kKeys, max(0, w.pre - i * kKeys)) >> p.box_log; };
             auto ids = [&](int i) {  // its page
-                return kb < cached(i) ? row[(w.base + i * kKeys + kb * p.box) / p.page_size] : -1;
+                return kb < cached(i) ? row[p.by_page.quot(w.base + i * kKeys + kb * p.box)] : -1;
             };
             int id0 = -1, id1 = ids(w.t0), id2 = -1;
 #pragma unroll 1
@@ -566,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int at_row = old ? kb * p.box : from + (kb - nc) * kTreeBox;
                 const int x = tile * kKeys + at_row;
                 // A page id out of range is an out-of-range coordinate: the box reads as zeros.
-                const int z = old ? (w.base + x) % p.page_size : w.first + x - w.pre;
+                const int z = old ? p.by_page.rem(w.base + x) : w.first + x - w.pre;
                 const int pg = page < 0 ? p.pages : page;
                 const uint64_t map = old ? (is_v ? vd : kd) : (is_v ? vnd : knd);
                 const uint32_t bytes = (uint32_t)(from + nn * kTreeBox) * 128 * kHalves;
@@ -711,7 +734,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The group's rows r0 .. r0 + nh - 1, in eights; with few rows some groups have none.
         const int r0 = (N >> 3) * grp / 4 * 8, nh = (N >> 3) * (grp + 1) / 4 * 8 - r0;
         const uint32_t lanes = (uint32_t)(qd * 32) << 16;
-        const int gqa = p.heads / p.kv_heads;
         int tile = 0;
         float l[kNH];
         // After a wait that gave up, these warps go on (on meaningless values) to the end of the share:
@@ -903,7 +925,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             wait(&c.o_done, (tile - 1) & 1, abort);
             __syncwarp();
             tc::fence_after_sync();
-            const int held = min(nh, min(N, w.n * gqa - w.g * N) - r0);  // the group's rows that exist
+            const int held = min(nh, min(N, w.n * p.gqa - w.g * N) - r0);  // the group's rows that exist
             const uint32_t ot = tmem + lanes + o_col + r0;
             if (*(volatile int*)&c.poison[part & 1]) {
 #pragma unroll 1
@@ -950,18 +972,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ------------------------------------------------------------------ scheduler
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         // Deals the parts out, and sets up each part's rows and queries while the one before is worked on.
-        const int gqa = p.heads / p.kv_heads;
         int part = 0;
         schedule(p, c, abort, [&](const Part& w) {
-            const int par = part & 1;
+            const int par = part & 1, row0 = w.g * N, R = min(N, w.n * p.gqa - row0);
             const Rows rs = rows_of(rows_at, N, p.words, par);
-            const int R = min(N, w.n * gqa - w.g * N);
-            bool ok = part < 2 || wait(&c.rows_free[par], ((part >> 1) - 1) & 1, abort);
-            // Rows of a part: r -> node (g N + r) / gqa, query head h gqa + (g N + r) % gqa.
+            // The queries, into the MMA's K-major layout, once S of the part before has completed. Rows of
+            // a part: r -> node (g N + r) / gqa, query head h gqa + (g N + r) % gqa.
+            bool ok = part == 0 || wait(&c.q_free, (part - 1) & 1, abort);
+            constexpr int kLanes = D / 8 < 32 ? D / 8 : 32;      // lanes on one row, 16 bytes each
+            const uint32_t q_at = smem_u32(qs);
+            const int step = 32 / kLanes, ch = lane % kLanes;
+#pragma unroll 1
+            for (int r = lane / kLanes; r < N; r += step) {
+                const int dst = r * 128 + ((ch & 7) ^ (r & 7)) * 16;
+                if (r < R) {
+                    const int node = p.by_gqa.quot(row0 + r), hd = row0 + r - node * p.gqa;
+                    const char* src = p.q + 2 * ((w.first + node) * p.q_stride + (w.h * p.gqa + hd) * D + ch * 8);
+#pragma unroll
+                    for (int k = 0; k < D / 8 / kLanes; ++k)
+                        cp_async16(q_at + dst + ((ch >> 3) + k * (kLanes / 8)) * N * 128, src + k * kLanes * 16);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < D / 8 / kLanes; ++k)
+                        *reinterpret_cast<uint4*>(qs + dst + ((ch >> 3) + k * (kLanes / 8)) * N * 128) = make_uint4(0, 0, 0, 0);
+                }
+            }
+            ok = ok && (part < 2 || wait(&c.rows_free[par], ((part >> 1) - 1) & 1, abort));
+            ++part;
+            if (!__all_sync(0xffffffffu, ok)) return false;
 #pragma unroll 1
             for (int r = lane; r < N; r += 32) {
-                const int row = w.g * N + r, tok = w.first + min(row / gqa, w.n - 1);
-                rs.out[r] = tok * p.out_stride + (w.h * gqa + row % gqa) * D;
+                const int node = p.by_gqa.quot(row0 + r), hd = row0 + r - node * p.gqa, tok = w.first + min(node, w.n - 1);
+                rs.out[r] = tok * p.out_stride + (w.h * p.gqa + hd) * D;
                 rs.nref[r] = kUnset;
                 const int dep = p.window ? min(max(p.depth[tok], 0), w.n - 1) : 0;
                 rs.depth[r] = dep;
@@ -970,33 +1012,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = 0; i * 32 < w.n; ++i) rs.mask[i * N + r] = p.mask[(long long)tok * p.mask_words + i];
             }
             if (lane == 0) c.poison[par] = 0;
-            // The queries, into the MMA's K-major layout, once S of the part before has completed.
-            ok = ok && (part == 0 || wait(&c.q_free, (part - 1) & 1, abort));
-            ++part;
-            if (!__all_sync(0xffffffffu, ok)) return false;
-            constexpr int kLanes = D / 8 < 32 ? D / 8 : 32;      // lanes on one row, 16 bytes each
-            const uint32_t q_at = smem_u32(qs);
-            const int step = 32 / kLanes, ch = lane % kLanes;
-            int r = lane / kLanes, node = (w.g * N + r) / gqa, hd = (w.g * N + r) % gqa;
-#pragma unroll 1
-            for (; r < N; r += step) {
-                const uint32_t dst = q_at + r * 128 + ((ch & 7) ^ (r & 7)) * 16;
-                if (r < R) {
-                    const char* src = p.q + 2 * ((w.first + node) * p.q_stride + (w.h * gqa + hd) * D + ch * 8);
-#pragma unroll
-                    for (int k = 0; k < D / 8 / kLanes; ++k)
-                        cp_async16(dst + ((ch >> 3) + k * (kLanes / 8)) * N * 128, src + k * kLanes * 16);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < D / 8 / kLanes; ++k)
-                        *reinterpret_cast<uint4*>(qs + (dst - q_at) + ((ch >> 3) + k * (kLanes / 8)) * N * 128) = make_uint4(0, 0, 0, 0);
-                }
-                hd += step;
-                while (hd >= gqa) {
-                    hd -= gqa;
-                    ++node;
-                }
-            }
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async();
             __syncwarp();
@@ -1089,20 +1104,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-constexpr int kJoinRows = 8;
+constexpr int kJoinRows = 2;  // two warps' registers fit beside the first kernel's
 
 // Joins the parts of items that several blocks worked on: out = sum_s 2^(m_s - M) O_s over
 // sum_s 2^(m_s - M) l_s. A warp per row, kJoinRows rows a block; grid (seqs x kv_heads, row blocks).
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(32 * kJoinRows) tree_attn_join_kernel(const __grid_constant__ Params p) {
     __shared__ int red[32];
-    pdl_wait();
+    // Which parts there are follows from the inputs alone; only the parts themselves are waited for.
     const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads, lane = threadIdx.x & 31;
-    const int gqa = p.heads / p.kv_heads;
     Seq s;
-    load_seq(p, b, s);
-    if (s.n * gqa <= (int)blockIdx.y * kJoinRows) return;
+    read_seq(p, b, s);
+    derive_seq(p, s);
+    if (s.n * p.gqa <= (int)blockIdx.y * kJoinRows) return;
     int before = 0, all = 0;
+#pragma unroll 1
     for (int i = threadIdx.x; i < p.seqs; i += 32 * kJoinRows) {
         const int t = seq_units(p, i);
         all += t;
@@ -1111,23 +1127,24 @@ __global__ void __launch_bounds__(32 * kJoinRows) tree_attn_join_kernel(const __
     before = block_total(before, red);
     all = block_total(all, red);
     const int row = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
-    if (row >= s.n * gqa) return;
-    const int g = row / p.N, r = row % p.N;
+    if (row >= s.n * p.gqa) return;
+    const int g = p.by_rows.quot(row), r = row - g * p.N;
     const int item = s.tiles + kItemCost;
     const int a = before + (h * s.groups + g) * item, z = a + item;
     // Block that holds unit x: an estimate, corrected.
     const auto block_of = [&](int x) {
-        int c = min(p.grid - 1, (int)((float)x / (float)all * (float)p.grid));
-        while (c > 0 && share_begin(all, p.grid, c) > x) --c;
-        while (c + 1 < p.grid && share_begin(all, p.grid, c + 1) <= x) ++c;
+        int c = min((int)p.by_grid.d - 1, (int)((float)x / (float)all * (float)p.by_grid.d));
+        while (c > 0 && share_begin(p, all, c) > x) --c;
+        while (c + 1 < (int)p.by_grid.d && share_begin(p, all, c + 1) <= x) ++c;
         return c;
     };
     const int c0 = block_of(a + kItemCost), c1 = block_of(z - 1);  // the blocks of its first and last tile
     if (c0 == c1) return;
-    const auto slot_of = [&](int c) { return (long long)(2 * c + (share_begin(all, p.grid, c) < a ? 1 : 0)); };
+    const auto slot_of = [&](int c) { return (long long)(2 * c + (share_begin(p, all, c) < a ? 1 : 0)); };
+    pdl_wait();
     float top = -INFINITY;
     for (int c = c0 + lane; c <= c1; c += 32) {
-        if (share_begin(all, p.grid, c) == share_begin(all, p.grid, c + 1)) continue;
+        if (share_begin(p, all, c) == share_begin(p, all, c + 1)) continue;
         const float2 x = p.ml[slot_of(c) * p.N + r];
         top = fmaxf(top, x.x);
     }
@@ -1141,7 +1158,7 @@ __global__ void __launch_bounds__(32 * kJoinRows) tree_attn_join_kernel(const __
         for (int j = 0; j < kV; ++j) o[k][j] = 0.f;
 #pragma unroll 2
     for (int c = c0; c <= c1; ++c) {
-        if (share_begin(all, p.grid, c) == share_begin(all, p.grid, c + 1)) continue;
+        if (share_begin(p, all, c) == share_begin(p, all, c + 1)) continue;
         const float2 x = p.ml[slot_of(c) * p.N + r];
         if (x.x == -INFINITY) continue;  // this part's keys are all hidden from the row
         const float f = exp2_approx(x.x - top);
@@ -1157,7 +1174,8 @@ __global__ void __launch_bounds__(32 * kJoinRows) tree_attn_join_kernel(const __
         }
     }
     const float inv = sum != 0.f ? 1.f / sum : 0.f;
-    uint32_t* out = reinterpret_cast<uint32_t*>(p.out + 2 * ((s.first + row / gqa) * p.out_stride + (h * gqa + row % gqa) * D));
+    const int node = p.by_gqa.quot(row);
+    uint32_t* out = reinterpret_cast<uint32_t*>(p.out + 2 * ((s.first + node) * p.out_stride + (h * p.gqa + row - node * p.gqa) * D));
 #pragma unroll
     for (int k = 0; k < kL; ++k)
 #pragma unroll
@@ -1231,9 +1249,9 @@ cudaError_t run(const CUtensorMap* maps, const Params& p, const Shape& sh, cudaS
         if (e != cudaSuccess) return e;
         attr = true;
     }
-    cudaError_t e = launch(kern, dim3(p.grid), dim3(kThreads), sh.smem, st, false, maps[0], maps[1], maps[2], maps[3], p);
+    cudaError_t e = launch(kern, dim3(p.by_grid.d), dim3(kThreads), sh.smem, st, false, maps[0], maps[1], maps[2], maps[3], p);
     if (e != cudaSuccess || p.whole) return e;
-    const int rows = p.max_nodes * (p.heads / p.kv_heads);
+    const int rows = p.max_nodes * p.gqa;
     return launch(tree_attn_join_kernel<D, kBf16>, dim3(p.seqs * p.kv_heads, (rows + kJoinRows - 1) / kJoinRows),
                   dim3(32 * kJoinRows), 0, st, true, p);
 }
@@ -1271,9 +1289,9 @@ cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
     p.cu = a.cu;
     p.mask = a.mask;
     p.depth = a.depth;
-    p.grid = sm_count();
+    int grid = sm_count();
     p.part = static_cast<float*>(a.work);
-    p.ml = reinterpret_cast<float2*>(p.part + (size_t)2 * p.grid * sh.N * a.dim);
+    p.ml = reinterpret_cast<float2*>(p.part + (size_t)2 * grid * sh.N * a.dim);
     p.q_stride = a.q_stride;
     p.out_stride = a.out_stride;
     p.page_stride = a.page_stride;
@@ -1285,7 +1303,7 @@ cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
     p.page_size = a.page_size;
     p.width = a.width;
     p.mask_words = a.mask_words;
-    p.heads = a.heads;
+    p.gqa = a.heads / a.kv_heads;
     p.kv_heads = a.kv_heads;
     p.window = a.window;
     p.N = sh.N;
@@ -1294,11 +1312,16 @@ cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
     p.tmem_cols = sh.tmem;
     // The largest power of two that divides a page, so that a box never crosses one.
     p.box = std::min(kPageBox, a.page_size & -a.page_size);
+    while (1 << p.box_log < p.box) ++p.box_log;
     const long long tiles = ((long long)a.width * a.page_size + 2 * kPageBox + a.max_nodes + kKeys - 1) / kKeys;
     const long long items = (long long)a.seqs * a.kv_heads * ((a.max_nodes * (a.heads / a.kv_heads) + sh.N - 1) / sh.N);
     if (items * (tiles + kItemCost) > INT32_MAX) return cudaErrorInvalidConfiguration;  // units are counted in 32 bits
     p.whole = tiles <= kWholeTiles;
-    if (p.whole) p.grid = (int)std::min<long long>(p.grid, items);
+    if (p.whole) grid = (int)std::min<long long>(grid, items);
+    p.by_rows = make_div(sh.N);
+    p.by_gqa = make_div(p.gqa);
+    p.by_page = make_div(a.page_size);
+    p.by_grid = make_div(grid);
     p.c = a.scale * 1.4426950408889634f;
     const cuuint64_t row = (cuuint64_t)a.dim * 2, D = a.dim, H = a.kv_heads;
     const cuuint64_t pool_dims[4] = {D, H, (cuuint64_t)a.page_size, (cuuint64_t)a.pages};
