@@ -756,26 +756,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 tc::fence_after_sync();
                 const bool edge = w.edge(p.window, i);
-                if (edge) {
-                    // Hidden scores become -inf, in tensor memory.
-                    const int x = i * kKeys + key;
-                    const bool old = x < w.pre;
-                    const int j = old ? w.base + x : x - w.pre;
-                    const bool in = j < (old ? w.len : w.n);
-                    const int near = p.window && in && !old ? min(max(p.depth[w.first + j], 0), w.n - 1) + p.window : INT_MAX;
-                    // What a row is asked: its first position, or the node's word of its mask.
-                    const int* ask = old || !in ? rs.start + r0 : reinterpret_cast<const int*>(rs.mask) + (j >> 5) * N + r0;
-                    const int* depth = rs.depth + r0;
+                // This thread's place in the line of keys, and what a row is asked about it: its first
+                // position, or the node's word of its mask.
+                const int x = i * kKeys + key;
+                const bool old = x < w.pre;
+                const int j = old ? w.base + x : x - w.pre;
+                const bool in = j < (old ? w.len : w.n), fresh = i == w.t0;
+                const int near = edge && p.window && in && !old ? min(max(p.depth[w.first + j], 0), w.n - 1) + p.window : INT_MAX;
+                const int* ask = old || !in ? rs.start + r0 : reinterpret_cast<const int*>(rs.mask) + (j >> 5) * N + r0;
+                // First look. Hidden scores become -inf, in tensor memory too. In a part's first tile each
+                // row's maximum is taken; later it matters whether a score exceeds its row's reference by
+                // more than kLazy. The scores are read again for the exponentials, which leaves the
+                // registers to the row sums.
+                float over = -INFINITY;
 #pragma unroll 1
-                    for (int f = 0; f < nh; f += 8) {
-                        float v[8];
-                        tc::ld8(st + f, v);
+                for (int f = 0; f < nh; f += 8) {
+                    float v[8];
+                    tc::ld8(st + f, v);
+                    tc::wait_ld();
+                    if (edge) {
                         int a[8], d[8];
                         *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(ask + f);
                         *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(ask + f + 4);
-                        *reinterpret_cast<int4*>(d) = *reinterpret_cast<const int4*>(depth + f);
-                        *reinterpret_cast<int4*>(d + 4) = *reinterpret_cast<const int4*>(depth + f + 4);
-                        tc::wait_ld();
+                        *reinterpret_cast<int4*>(d) = *reinterpret_cast<const int4*>(rs.depth + r0 + f);
+                        *reinterpret_cast<int4*>(d + 4) = *reinterpret_cast<const int4*>(rs.depth + r0 + f + 4);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             const bool seen = old ? j >= a[k] : (((unsigned)a[k] >> (j & 31)) & 1u) & (unsigned)(d[k] < near);
@@ -783,40 +787,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         tc::st8(st + f, v);
                     }
-                    tc::wait_st();
+                    if (fresh) {
+                        reduce_scatter8<true>(v, lane);
+                        c.red[qd][r0 + f + (lane >> 2)] = v[0] * p.c;
+                    } else {
+                        const float4 n0 = *reinterpret_cast<const float4*>(&rs.nref[r0 + f]), n1 = *reinterpret_cast<const float4*>(&rs.nref[r0 + f + 4]);
+                        over = fmaxf(over, fmaxf(fmaf(v[0], p.c, n0.x), fmaf(v[1], p.c, n0.y)));
+                        over = fmaxf(over, fmaxf(fmaf(v[2], p.c, n0.z), fmaf(v[3], p.c, n0.w)));
+                        over = fmaxf(over, fmaxf(fmaf(v[4], p.c, n1.x), fmaf(v[5], p.c, n1.y)));
+                        over = fmaxf(over, fmaxf(fmaf(v[6], p.c, n1.z), fmaf(v[7], p.c, n1.w)));
+                    }
                 }
-                // First look: does a score exceed its row's reference by more than kLazy? The scores
-                // stay in tensor memory and are read again for the exponentials, which leaves the
-                // registers to the row sums.
-                float over = -INFINITY;
-#pragma unroll 1
-                for (int f = 0; f < nh; f += 16) {
-                    float v[16];
-                    const bool both = f + 8 < nh;
-                    load16(st + f, both, v);
-#pragma unroll
-                    for (int r = 0; r < 16; r += 4)
-                        if (r < 8 || both) {
-                            const float4 n = *reinterpret_cast<const float4*>(&rs.nref[r0 + f + r]);
-                            over = fmaxf(over, fmaxf(fmaf(v[r], p.c, n.x), fmaf(v[r + 1], p.c, n.y)));
-                            over = fmaxf(over, fmaxf(fmaf(v[r + 2], p.c, n.z), fmaf(v[r + 3], p.c, n.w)));
-                        }
-                }
+                if (edge) tc::wait_st();
                 bool waited = tile == 0;
-                if (group_or(grp, over > kLazy)) {
+                if (fresh || group_or(grp, over > kLazy)) {
 #pragma unroll 1
-                    for (int f = 0; f < nh; f += 16) {
-                        float m[2][8];
-                        const bool both = f + 8 < nh;
-                        tc::ld8(st + f, m[0]);
-                        if (both) tc::ld8(st + f + 8, m[1]);
+                    for (int f = 0; f < nh && !fresh; f += 8) {
+                        float m[8];
+                        tc::ld8(st + f, m);
                         tc::wait_ld();
-                        reduce_scatter8<true>(m[0], lane);
-                        c.red[qd][r0 + f + (lane >> 2)] = m[0][0] * p.c;
-                        if (both) {
-                            reduce_scatter8<true>(m[1], lane);
-                            c.red[qd][r0 + f + 8 + (lane >> 2)] = m[1][0] * p.c;
-                        }
+                        reduce_scatter8<true>(m, lane);
+                        c.red[qd][r0 + f + (lane >> 2)] = m[0] * p.c;
                     }
                     group_bar(grp);
                     if (gt < nh) {
@@ -833,14 +824,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     group_bar(grp);
 #pragma unroll
                     for (int r = 0; r < kNH; r += 4)
-                        if (r < nh) {
+                        if (r < nh && !fresh) {
                             const float4 f = *reinterpret_cast<const float4*>(&c.corr[r0 + r]);
                             l[r] *= f.x;
                             l[r + 1] *= f.y;
                             l[r + 2] *= f.z;
                             l[r + 3] *= f.w;
                         }
-                    if (i > w.t0) {
+                    if (!fresh) {
                         wait(&c.o_done, (tile - 1) & 1, abort);
                         __syncwarp();
                         waited = true;
@@ -949,18 +940,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + d;
                 float* dst = p.part + ((long long)slot * N + r0) * D + d;
 #pragma unroll 1
-                for (int f = 0; f < held; f += 16) {
-                    float v[16];
-                    load16(ot + ci * N + f, f + 8 < nh, v);
+                for (int f = 0; f < held; f += 8) {
+                    float v[8];
+                    tc::ld8(ot + ci * N + f, v);
+                    tc::wait_ld();
                     if (D == 64 && key >= 64) continue;
                     if (whole) {
+                        // Lanes swap so that each holds two dims of four rows: fewer, wider stores.
+                        const float4 i0 = *reinterpret_cast<const float4*>(&c.inv[r0 + f]), i1 = *reinterpret_cast<const float4*>(&c.inv[r0 + f + 4]);
+                        v[0] *= i0.x, v[1] *= i0.y, v[2] *= i0.z, v[3] *= i0.w;
+                        v[4] *= i1.x, v[5] *= i1.y, v[6] *= i1.z, v[7] *= i1.w;
+                        const bool odd = lane & 1;
+                        const int row = r0 + f + (odd ? 4 : 0);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (f + j < held) out[rs.out[r0 + f + j]] = pack1<kBf16>(v[j] * c.inv[r0 + f + j]);
+                        for (int e = 0; e < 4; ++e) {
+                            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[e] : v[e + 4], 1);
+                            const uint32_t two = odd ? pack2<kBf16>(got, v[e + 4]) : pack2<kBf16>(v[e], got);
+                            if (row + e - r0 < held) *reinterpret_cast<uint32_t*>(out + rs.out[row + e] - odd) = two;
+                        }
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (f + j < held) __stcg(dst + (f + j) * D, v[j]);
+                        for (int e = 0; e < 8; ++e)
+                            if (f + e < held) __stcg(dst + (f + e) * D, v[e]);
                     }
                 }
             }
@@ -981,22 +982,35 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = part == 0 || wait(&c.q_free, (part - 1) & 1, abort);
             constexpr int kLanes = D / 8 < 32 ? D / 8 : 32;      // lanes on one row, 16 bytes each
             const uint32_t q_at = smem_u32(qs);
-            const int step = 32 / kLanes, ch = lane % kLanes;
+            constexpr int kStep = 32 / kLanes, kBatch = 4;       // rows at once; such rounds unrolled
+            const int ch = lane % kLanes;
+            const int q_col = q_at + (ch >> 3) * N * 128, c7 = ch & 7;
+            // Row r + kStep is kStep heads on, or in a later node: no division inside the loop.
+            int r = lane / kLanes, node = p.by_gqa.quot(row0 + r), hd = row0 + r - node * p.gqa;
+            const char* src = p.q + 2 * ((w.first + node) * p.q_stride + (w.h * p.gqa + hd) * D + ch * 8);
+            const long long next_head = 2 * kStep * D, next_node = 2 * (p.q_stride - (long long)p.gqa * D);
 #pragma unroll 1
-            for (int r = lane / kLanes; r < N; r += step) {
-                const int dst = r * 128 + ((ch & 7) ^ (r & 7)) * 16;
-                if (r < R) {
-                    const int node = p.by_gqa.quot(row0 + r), hd = row0 + r - node * p.gqa;
-                    const char* src = p.q + 2 * ((w.first + node) * p.q_stride + (w.h * p.gqa + hd) * D + ch * 8);
+            for (; r - lane / kLanes < R; r += kBatch * kStep) {
 #pragma unroll
-                    for (int k = 0; k < D / 8 / kLanes; ++k)
-                        cp_async16(q_at + dst + ((ch >> 3) + k * (kLanes / 8)) * N * 128, src + k * kLanes * 16);
-                } else {
+                for (int u = 0; u < kBatch; ++u) {
+                    const int x = r + u * kStep;
+                    if (x < R)
 #pragma unroll
-                    for (int k = 0; k < D / 8 / kLanes; ++k)
-                        *reinterpret_cast<uint4*>(qs + dst + ((ch >> 3) + k * (kLanes / 8)) * N * 128) = make_uint4(0, 0, 0, 0);
+                        for (int k = 0; k < D / 8 / kLanes; ++k)
+                            cp_async16(q_col + x * 128 + ((c7 ^ (x & 7)) << 4) + k * (kLanes / 8) * N * 128, src + k * kLanes * 16);
+                    src += next_head;
+                    hd += kStep;
+                    while (hd >= p.gqa) {
+                        hd -= p.gqa;
+                        src += next_node;
+                    }
                 }
             }
+#pragma unroll 1
+            for (int x = R + lane / kLanes; x < N; x += kStep)   // rows that do not exist
+#pragma unroll
+                for (int k = 0; k < D / 8 / kLanes; ++k)
+                    *reinterpret_cast<uint4*>(qs + (q_col - q_at) + x * 128 + ((c7 ^ (x & 7)) << 4) + k * (kLanes / 8) * N * 128) = make_uint4(0, 0, 0, 0);
             ok = ok && (part < 2 || wait(&c.rows_free[par], ((part >> 1) - 1) & 1, abort));
             ++part;
             if (!__all_sync(0xffffffffu, ok)) return false;
