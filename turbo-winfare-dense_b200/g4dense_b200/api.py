@@ -6,6 +6,7 @@ point is called, the call fails loudly.
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -40,36 +41,20 @@ def lib():
     return _lib
 
 
-class TreeAttentionArgs(ctypes.Structure):
-    """g4b_tree_attention_args (include/g4dense_b200_ops.h)."""
-    _fields_ = ([(n, _vp) for n in ("q", "k_pool", "v_pool", "k_new", "v_new", "out", "table", "lens", "cu_nodes",
-                                    "mask", "depth", "workspace")] + [("workspace_bytes", ctypes.c_size_t)] +
-                [(n, ctypes.c_int64) for n in ("q_stride", "out_stride", "new_stride", "page_stride")] +
-                [(n, ctypes.c_int) for n in ("n_seqs", "n_tokens", "max_nodes", "n_pages", "page_size", "table_width",
-                                             "mask_words", "heads", "kv_heads", "head_dim", "window", "dtype")] +
-                [("scale", ctypes.c_float)])
-
-
-class PagePool(ctypes.Structure):
-    """g4b_page_pool (include/g4dense_b200_ops.h)."""
-    _fields_ = [("base", _vp), ("plane_stride", ctypes.c_int64), ("page_stride", ctypes.c_int64),
-                ("n_planes", ctypes.c_int), ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int),
-                ("row_bytes", ctypes.c_int)]
-
-
-class PageTables(ctypes.Structure):
-    """g4b_page_tables (include/g4dense_b200_ops.h)."""
-    _fields_ = ([(n, _vp) for n in ("refs", "table", "lens", "refs_out", "table_out", "lens_out")] +
-                [(n, ctypes.c_int) for n in ("n_pages", "n_seqs", "table_width", "page_size")])
+# The argument structs of the tree-verification operators (include/g4dense_b200_ops.h), packed in one
+# go: these calls are short, and setting ctypes fields one by one would cost more than the launch.
+_TREE_ATTENTION = struct.Struct("@12PN4q12if4x")  # g4b_tree_attention_args
+_PAGE_POOL = struct.Struct("@P2q4i")            # g4b_page_pool
+_PAGE_TABLES = struct.Struct("@6P4i")           # g4b_page_tables
 
 
 def _bind_tree(L):
     """Binds the tree-verification and paged-cache operators (include/g4dense_b200_ops.h)."""
     i, i64 = ctypes.c_int, ctypes.c_int64
-    pool, tables = ctypes.POINTER(PagePool), ctypes.POINTER(PageTables)
+    args = pool = tables = ctypes.c_char_p  # a packed struct
     L.g4b_tree_attention_workspace.restype = ctypes.c_size_t
     L.g4b_tree_attention_workspace.argtypes = [i, i, i, i]
-    L.g4b_tree_attention.argtypes = [ctypes.POINTER(TreeAttentionArgs), _vp]
+    L.g4b_tree_attention.argtypes = [args, _vp]
     L.g4b_tree_attention_check_error.argtypes = []
     L.g4b_sample_rows.argtypes = [_vp, i, i, i, i64] + [_vp] * 9
     L.g4b_tree_accept.argtypes = [_vp] * 4 + [i, i, _vp, i, _vp, _vp, _vp]
@@ -213,29 +198,54 @@ def sample_token(logits, temperature, top_p, top_k, seed, workspace, out, stream
     _check(lib().g4b_sample_token(_dptr(logits), logits.numel(), temperature, top_p, top_k, seed & (2**64 - 1),
                                   _dptr(workspace), _dptr(out), _stream(stream)), "g4b_sample_token")
 
-_DTYPES = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2}  # g4b_dtype
+_dtypes = {}  # torch dtype -> g4b_dtype, filled by _types()
+_i32 = _f32 = None
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+def _types():
+    """Loads torch's types and the library once; returns the library."""
+    global _i32, _f32
+    if _i32 is None:
+        import torch
+        _dtypes.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2})
+        _i32, _f32 = torch.int32, torch.float32
+    return lib()
 
 
-def _ints(name, t, shape=None, optional=False):
-    """Device pointer of a contiguous int32 CUDA tensor of the given shape."""
-    if t is None and optional:
-        return None
-    _need(t.is_cuda and str(t.dtype) == "torch.int32" and t.is_contiguous(), f"{name}: a contiguous int32 CUDA tensor")
-    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, expected {tuple(shape or ())}")
-    return _dptr(t)
+def _bad(what):
+    raise ValueError(what)
 
 
-def _floats(name, t, shape):
+def _ints(name, t, n):
+    """Device pointer of a contiguous int32 CUDA tensor of n elements."""
+    if t.dtype is not _i32 or not t.is_cuda or t.numel() != n or not t.is_contiguous():
+        _bad(f"{name}: a contiguous int32 CUDA tensor of {n} elements is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _floats(name, t, n):
+    """As _ints for float32; None stays None."""
     if t is None:
         return None
-    _need(t.is_cuda and str(t.dtype) == "torch.float32" and t.is_contiguous() and tuple(t.shape) == tuple(shape),
-          f"{name}: a contiguous float32 CUDA tensor of shape {tuple(shape)}")
-    return _dptr(t)
+    if t.dtype is not _f32 or not t.is_cuda or t.numel() != n or not t.is_contiguous():
+        _bad(f"{name}: a contiguous float32 CUDA tensor of {n} elements is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows_of(name, t, dtype, shape):
+    """(device pointer, stride of the first dimension) of a CUDA tensor contiguous but for that one."""
+    if t.dtype is not dtype or not t.is_cuda or t.shape != shape:
+        _bad(f"{name}: a {dtype} CUDA tensor of shape {tuple(shape)} is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    n, strides = 1, t.stride()
+    for k in range(len(shape) - 1, 0, -1):
+        if strides[k] != n and shape[k] != 1:
+            _bad(f"{name} has to be contiguous but for its first dimension")
+        n *= shape[k]
+    return t.data_ptr(), strides[0] if shape[0] > 1 else n
+
+
+def _at(stream):
+    return stream.cuda_stream if stream is not None else 0
 
 
 def tree_mask(parents, words=None):
@@ -246,7 +256,8 @@ def tree_mask(parents, words=None):
     words = words or max(1, (n + 31) // 32)
     mask, depth = np.zeros((n, words), np.uint32), np.zeros(n, np.int32)
     for i, p in enumerate(parents):
-        _need(-1 <= p < i, f"tree_mask: parent {p} of node {i}")
+        if not -1 <= p < i:
+            _bad(f"tree_mask: parent {p} of node {i}")
         if p >= 0:
             mask[i] = mask[p]
             depth[i] = depth[p] + 1
@@ -257,7 +268,8 @@ def tree_mask(parents, words=None):
 def tree_attention_workspace(max_nodes, heads, kv_heads, head_dim):
     """Bytes of workspace tree_attention needs (ValueError for a shape it does not support)."""
     n = int(lib().g4b_tree_attention_workspace(max_nodes, heads, kv_heads, head_dim))
-    _need(n, f"tree_attention: max_nodes {max_nodes} (1..256), heads {heads} (a multiple of {kv_heads}), head_dim "
+    if not n:
+        _bad(f"tree_attention: max_nodes {max_nodes} (1..256), heads {heads} (a multiple of {kv_heads}), head_dim "
              f"{head_dim} (64, 128, 256 or 512)")
     return n
 
@@ -269,44 +281,38 @@ def tree_attention(q, k_pool, v_pool, table, lens, k_new, v_new, cu_nodes, mask,
     [tokens][kv_heads][dim], all bf16 or all fp16 torch CUDA tensors (token and page strides
     honoured); table [seqs][width], lens [seqs], cu_nodes [seqs + 1], mask [tokens][words], depth
     [tokens] int32; workspace a byte tensor of tree_attention_workspace()."""
-    _need(q.dim() == 3 and k_pool.dim() == 4 and k_new.dim() == 3, "tree_attention: q and k_new 3-d, pools 4-d")
-    tokens, heads, dim = q.shape
-    pages, page_size, kv_heads, _ = k_pool.shape
-    dtype = _DTYPES.get(str(q.dtype), -1)
-    _need(dtype in (0, 1), f"tree_attention: dtype {q.dtype} (bfloat16 or float16)")
-    for name, t, shape in (("q", q, (tokens, heads, dim)), ("out", out, (tokens, heads, dim)),
-                           ("k_pool", k_pool, (pages, page_size, kv_heads, dim)),
-                           ("v_pool", v_pool, (pages, page_size, kv_heads, dim)),
-                           ("k_new", k_new, (tokens, kv_heads, dim)), ("v_new", v_new, (tokens, kv_heads, dim))):
-        _need(t.is_cuda and t.dtype == q.dtype and tuple(t.shape) == shape,
-              f"tree_attention: {name} has to be a {q.dtype} CUDA tensor of shape {shape}")
-        inner = t.stride()[1:]
-        want, n = [], 1
-        for size in reversed(shape[1:]):
-            want.insert(0, n)
-            n *= size
-        _need(all(w == s or d == 1 for w, s, d in zip(want, inner, shape[1:])),
-              f"tree_attention: {name} has to be contiguous but for its first dimension")
-    _need(tokens <= 1 or k_new.stride(0) == v_new.stride(0), "tree_attention: k_new and v_new differ in their strides")
-    _need(pages <= 1 or k_pool.stride(0) == v_pool.stride(0), "tree_attention: the pools differ in their strides")
-    seqs, row = lens.numel(), kv_heads * dim
-    a = TreeAttentionArgs()
-    a.table = _ints("table", table, (seqs, table.shape[-1]))
-    a.lens = _ints("lens", lens, (seqs,))
-    a.cu_nodes = _ints("cu_nodes", cu_nodes, (seqs + 1,))
-    a.mask = _ints("mask", mask, (tokens, mask.shape[-1]))
-    a.depth = _ints("depth", depth, (tokens,), optional=True)
-    _need(not window or depth is not None, "tree_attention: a window needs the nodes' depths")
-    a.q, a.k_pool, a.v_pool, a.k_new, a.v_new = map(_dptr, (q, k_pool, v_pool, k_new, v_new))
-    a.out, a.workspace, a.workspace_bytes = _dptr(out), _dptr(workspace), workspace.numel() * workspace.element_size()
-    a.q_stride = q.stride(0) if tokens > 1 else heads * dim
-    a.out_stride = out.stride(0) if tokens > 1 else heads * dim
-    a.new_stride = k_new.stride(0) if tokens > 1 else row
-    a.page_stride = k_pool.stride(0) if pages > 1 else row * page_size
-    a.n_seqs, a.n_tokens, a.max_nodes, a.n_pages, a.page_size = seqs, tokens, max_nodes, pages, page_size
-    a.table_width, a.mask_words = table.shape[1], mask.shape[1]
-    a.heads, a.kv_heads, a.head_dim, a.window, a.dtype, a.scale = heads, kv_heads, dim, window, dtype, scale
-    _check(lib().g4b_tree_attention(ctypes.byref(a), _stream(stream)), "g4b_tree_attention")
+    L = _types()
+    shape, pool, dtype = q.shape, k_pool.shape, q.dtype
+    if len(shape) != 3 or len(pool) != 4 or _dtypes.get(dtype, 2) > 1:
+        _bad(f"tree_attention: q [tokens][heads][dim] and pools [pages][page_size][kv_heads][dim] of dtype bfloat16 or "
+             f"float16 are needed, got {tuple(shape)}, {tuple(pool)}, {dtype}")
+    tokens, heads, dim = shape
+    pages, page_size, kv_heads, _ = pool
+    new = (tokens, kv_heads, dim)
+    if pool[3] != dim:
+        _bad("tree_attention: q and the pools differ in head_dim")
+    pq, q_stride = _rows_of("q", q, dtype, shape)
+    po, out_stride = _rows_of("out", out, dtype, shape)
+    pk, page_stride = _rows_of("k_pool", k_pool, dtype, pool)
+    pv, v_stride = _rows_of("v_pool", v_pool, dtype, pool)
+    pkn, new_stride = _rows_of("k_new", k_new, dtype, new)
+    pvn, vn_stride = _rows_of("v_new", v_new, dtype, new)
+    if v_stride != page_stride or vn_stride != new_stride:
+        _bad("tree_attention: K and V differ in their strides")
+    if window and depth is None:
+        _bad("tree_attention: a window needs the nodes' depths")
+    seqs, width, words = lens.numel(), table.shape[-1], mask.shape[-1]
+    if not workspace.is_cuda:
+        _bad("workspace: a CUDA tensor is needed")
+    a = _TREE_ATTENTION.pack(
+        pq, pk, pv, pkn, pvn, po, _ints("table", table, seqs * width), _ints("lens", lens, seqs),
+        _ints("cu_nodes", cu_nodes, seqs + 1), _ints("mask", mask, tokens * words),
+        0 if depth is None else _ints("depth", depth, tokens), workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), q_stride, out_stride, new_stride, page_stride, seqs, tokens,
+        max_nodes, pages, page_size, width, words, heads, kv_heads, dim, window, _dtypes[dtype], scale)
+    rc = L.g4b_tree_attention(a, _at(stream))
+    if rc:
+        _check(rc, "g4b_tree_attention")
 
 
 def tree_attention_check_error():
@@ -320,111 +326,121 @@ def sample_rows(logits, uniform, token, prob=None, kept=None, temperature=None, 
     [rows] int32, from uniform [rows] float32 in [0, 1), with per-row temperature, top_p, min_p
     (float32) and top_k (int32) where given (g4b_sample_rows). prob [rows] float32 and kept [rows]
     int32 receive the token's share of the kept mass and the number of kept entries."""
-    _need(logits.is_cuda and logits.dim() == 2 and logits.stride(1) in (1,) or logits.shape[-1] == 1,
-          "sample_rows: logits [rows][vocab] with contiguous rows")
+    L = _types()
+    if logits.dim() != 2 or logits.dtype not in _dtypes:
+        _bad(f"sample_rows: logits [rows][vocab] of dtype bfloat16, float16 or float32 are needed, got "
+             f"{tuple(logits.shape)} {logits.dtype}")
+    if uniform is None:
+        _bad("sample_rows: uniform numbers are needed")
     rows, vocab = logits.shape
-    dtype = _DTYPES.get(str(logits.dtype), -1)
-    _need(dtype >= 0, f"sample_rows: dtype {logits.dtype} (bfloat16, float16 or float32)")
-    _need(uniform is not None, "sample_rows: uniform numbers are needed")
-    _check(lib().g4b_sample_rows(_dptr(logits), dtype, rows, vocab, logits.stride(0) if rows > 1 else vocab,
-                                 _floats("uniform", uniform, (rows,)), _floats("temperature", temperature, (rows,)),
-                                 _ints("top_k", top_k, (rows,), optional=True), _floats("top_p", top_p, (rows,)),
-                                 _floats("min_p", min_p, (rows,)), _ints("token", token, (rows,)),
-                                 _floats("prob", prob, (rows,)), _ints("kept", kept, (rows,), optional=True),
-                                 _stream(stream)), "g4b_sample_rows")
+    ptr, stride = _rows_of("logits", logits, logits.dtype, logits.shape)
+    rc = L.g4b_sample_rows(ptr, _dtypes[logits.dtype], rows, vocab, stride, _floats("uniform", uniform, rows),
+                           _floats("temperature", temperature, rows), None if top_k is None else _ints("top_k", top_k, rows),
+                           _floats("top_p", top_p, rows), _floats("min_p", min_p, rows), _ints("token", token, rows),
+                           _floats("prob", prob, rows), None if kept is None else _ints("kept", kept, rows), _at(stream))
+    if rc:
+        _check(rc, "g4b_sample_rows")
 
 
 def tree_accept(tokens, parents, sampled, cu_nodes, path, count, next_token, stream=None):
     """Walks each tree along the drawn tokens (g4b_tree_accept): path [seqs][width], count [seqs] and
     next_token [seqs] from tokens, parents, sampled [nodes] and cu_nodes [seqs + 1], all int32."""
-    n, seqs = tokens.numel(), cu_nodes.numel() - 1
-    _check(lib().g4b_tree_accept(_ints("tokens", tokens, (n,)), _ints("parents", parents, (n,)),
-                                 _ints("sampled", sampled, (n,)), _ints("cu_nodes", cu_nodes, (seqs + 1,)), seqs, n,
-                                 _ints("path", path, (seqs, path.shape[-1])), path.shape[-1],
-                                 _ints("count", count, (seqs,)), _ints("next_token", next_token, (seqs,)),
-                                 _stream(stream)), "g4b_tree_accept")
+    L = _types()
+    n, seqs, width = tokens.numel(), cu_nodes.numel() - 1, path.shape[-1]
+    rc = L.g4b_tree_accept(_ints("tokens", tokens, n), _ints("parents", parents, n), _ints("sampled", sampled, n),
+                           _ints("cu_nodes", cu_nodes, seqs + 1), seqs, n, _ints("path", path, seqs * width), width,
+                           _ints("count", count, seqs), _ints("next_token", next_token, seqs), _at(stream))
+    if rc:
+        _check(rc, "g4b_tree_accept")
 
 
 def _pool(pool):
-    """g4b_page_pool of a CUDA tensor [planes][pages][page_size][...] with contiguous pages."""
-    _need(pool.is_cuda and pool.dim() >= 4, "pool: a CUDA tensor [planes][pages][page_size][row...]")
-    size = pool.element_size()
-    row = 1
-    for d in pool.shape[3:]:
-        row *= d
-    _need(pool[0, 0].is_contiguous(), "pool: the rows of a page have to be contiguous")
-    planes, pages, page_size = pool.shape[:3]
-    page_stride = (pool.stride(1) if pages > 1 else page_size * row) * size
-    plane_stride = (pool.stride(0) if planes > 1 else pages * page_size * row) * size
-    return PagePool(pool.data_ptr(), plane_stride, page_stride, planes, pages, page_size, row * size)
+    """Packed g4b_page_pool of a CUDA tensor [planes][pages][page_size][...] with contiguous pages."""
+    shape, strides, size = pool.shape, pool.stride(), pool.element_size()
+    if not pool.is_cuda or len(shape) < 4:
+        _bad("pool: a CUDA tensor [planes][pages][page_size][row...] is needed")
+    n = 1
+    for k in range(len(shape) - 1, 1, -1):
+        if strides[k] != n and shape[k] != 1:
+            _bad("pool: the rows of a page have to be contiguous")
+        n *= shape[k]
+    page = (strides[1] if shape[1] > 1 else n) * size
+    plane = (strides[0] if shape[0] > 1 else shape[1] * n) * size
+    return _PAGE_POOL.pack(pool.data_ptr(), plane, page, shape[0], shape[1], shape[2], n // max(shape[2], 1) * size)
 
 
 def _tables(refs, table, lens, refs_out, table_out, lens_out, page_size):
     pages, (seqs, width) = refs.numel(), table.shape
-    t = PageTables()
-    t.refs, t.table = _ints("refs", refs, (pages,)), _ints("table", table, (seqs, width))
-    t.refs_out, t.table_out = _ints("refs_out", refs_out, (pages,)), _ints("table_out", table_out, (seqs, width))
-    t.lens = _ints("lens", lens, (seqs,), optional=True)
-    t.lens_out = _ints("lens_out", lens_out, (seqs,), optional=True)
-    t.n_pages, t.n_seqs, t.table_width, t.page_size = pages, seqs, width, page_size
-    return t
+    return _PAGE_TABLES.pack(
+        _ints("refs", refs, pages), _ints("table", table, seqs * width), 0 if lens is None else _ints("lens", lens, seqs),
+        _ints("refs_out", refs_out, pages), _ints("table_out", table_out, seqs * width),
+        0 if lens_out is None else _ints("lens_out", lens_out, seqs), pages, seqs, width, page_size)
 
 
 def pages_reserve(refs, table, lens, grow, page_size, refs_out, table_out, status, stream=None):
     """Pages for grow[s] more tokens of every sequence (g4b_pages_reserve). int32 CUDA tensors: refs
     [pages], table [seqs][width], lens, grow [seqs], status [1]; the outputs may be the inputs."""
-    t = _tables(refs, table, lens, refs_out, table_out, None, page_size)
-    _check(lib().g4b_pages_reserve(ctypes.byref(t), _ints("grow", grow, (lens.numel(),)), _ints("status", status, (1,)),
-                                   _stream(stream)), "g4b_pages_reserve")
+    L = _types()
+    rc = L.g4b_pages_reserve(_tables(refs, table, lens, refs_out, table_out, None, page_size),
+                             _ints("grow", grow, lens.numel()), _ints("status", status, 1), _at(stream))
+    if rc:
+        _check(rc, "g4b_pages_reserve")
 
 
 def pages_fork(pool, refs, table, lens, src, dst, refs_out, table_out, lens_out, status, stream=None):
     """Sequences dst[i] become continuations of src[i] (g4b_pages_fork): full pages shared, a partial
     last page copied. pool [planes][pages][page_size][row...]."""
-    t, p = _tables(refs, table, lens, refs_out, table_out, lens_out, pool.shape[2]), _pool(pool)
-    _check(lib().g4b_pages_fork(ctypes.byref(p), ctypes.byref(t), _ints("src", src, (src.numel(),)),
-                                _ints("dst", dst, (src.numel(),)), src.numel(), _ints("status", status, (1,)),
-                                _stream(stream)), "g4b_pages_fork")
+    L, n = _types(), src.numel()
+    rc = L.g4b_pages_fork(_pool(pool), _tables(refs, table, lens, refs_out, table_out, lens_out, pool.shape[2]),
+                          _ints("src", src, n), _ints("dst", dst, n), n, _ints("status", status, 1), _at(stream))
+    if rc:
+        _check(rc, "g4b_pages_fork")
 
 
 def pages_free(refs, table, lens, seqs, page_size, refs_out, table_out, lens_out, stream=None):
     """Releases the pages of the sequences seqs[] and empties them (g4b_pages_free)."""
-    t = _tables(refs, table, lens, refs_out, table_out, lens_out, page_size)
-    _check(lib().g4b_pages_free(ctypes.byref(t), _ints("seqs", seqs, (seqs.numel(),)), seqs.numel(), _stream(stream)),
-           "g4b_pages_free")
+    L, n = _types(), seqs.numel()
+    rc = L.g4b_pages_free(_tables(refs, table, lens, refs_out, table_out, lens_out, page_size), _ints("seqs", seqs, n), n,
+                          _at(stream))
+    if rc:
+        _check(rc, "g4b_pages_free")
 
 
 def pages_compact(pool, refs, table, refs_out, table_out, moves, stream=None):
     """Moves live pages to the front of the pool (g4b_pages_compact); moves [1 + 2 * pages] int32
     receives their number and the (from, to) pairs."""
-    t, p = _tables(refs, table, None, refs_out, table_out, None, pool.shape[2]), _pool(pool)
-    _check(lib().g4b_pages_compact(ctypes.byref(p), ctypes.byref(t), _ints("moves", moves, (1 + 2 * refs.numel(),)),
-                                   _stream(stream)), "g4b_pages_compact")
+    L = _types()
+    rc = L.g4b_pages_compact(_pool(pool), _tables(refs, table, None, refs_out, table_out, None, pool.shape[2]),
+                             _ints("moves", moves, 1 + 2 * refs.numel()), _at(stream))
+    if rc:
+        _check(rc, "g4b_pages_compact")
 
 
 def pages_copy(pool, to_pool, src, dst, stream=None):
     """Page src[i] of pool to page dst[i] of to_pool, in every plane (g4b_pages_copy)."""
-    a, b = _pool(pool), _pool(to_pool)
-    _check(lib().g4b_pages_copy(ctypes.byref(a), ctypes.byref(b), _ints("src", src, (src.numel(),)),
-                                _ints("dst", dst, (src.numel(),)), src.numel(), _stream(stream)), "g4b_pages_copy")
+    L, n = _types(), src.numel()
+    rc = L.g4b_pages_copy(_pool(pool), _pool(to_pool), _ints("src", src, n), _ints("dst", dst, n), n, _at(stream))
+    if rc:
+        _check(rc, "g4b_pages_copy")
 
 
 def pages_commit(pool, table, lens, rows, cu_nodes, path, count, lens_out, status=None, stream=None):
     """Writes the accepted nodes' rows [planes][tokens][row...] into their sequences' pages and the
     new lengths into lens_out (g4b_pages_commit). path None: the first count[s] rows."""
-    p, seqs, tokens = _pool(pool), lens.numel(), rows.shape[1]
-    _need(rows.is_cuda and rows.dtype == pool.dtype and rows.shape[0] == pool.shape[0] and
-          tuple(rows.shape[2:]) == tuple(pool.shape[3:]) and (tokens == 0 or rows[0].is_contiguous()),
-          "pages_commit: rows have to be [planes][tokens][row...] of the pool's type")
-    stride = rows.stride(0) * rows.element_size() if rows.shape[0] > 1 else p.row_bytes * tokens
-    _check(lib().g4b_pages_commit(ctypes.byref(p), _ints("table", table, (seqs, table.shape[-1])), table.shape[-1],
-                                  _ints("lens", lens, (seqs,)), seqs, _dptr(rows), stride, tokens,
-                                  _ints("cu_nodes", cu_nodes, (seqs + 1,)),
-                                  None if path is None else _ints("path", path, (seqs, path.shape[-1])),
-                                  0 if path is None else path.shape[-1], _ints("count", count, (seqs,)),
-                                  _ints("status", status, (1,), optional=True), _ints("lens_out", lens_out, (seqs,)),
-                                  _stream(stream)), "g4b_pages_commit")
-
+    L = _types()
+    shape, want, seqs, width = rows.shape, pool.shape, lens.numel(), table.shape[-1]
+    tokens = shape[1]
+    if len(shape) != len(want) - 1 or shape[0] != want[0] or shape[2:] != want[3:]:
+        _bad("pages_commit: rows have to be [planes][tokens][row...] like the pool")
+    ptr, stride = _rows_of("rows", rows, pool.dtype, shape)
+    rc = L.g4b_pages_commit(_pool(pool), _ints("table", table, seqs * width), width, _ints("lens", lens, seqs), seqs, ptr,
+                            stride * rows.element_size(), tokens, _ints("cu_nodes", cu_nodes, seqs + 1),
+                            None if path is None else _ints("path", path, seqs * path.shape[-1]),
+                            0 if path is None else path.shape[-1], _ints("count", count, seqs),
+                            None if status is None else _ints("status", status, 1), _ints("lens_out", lens_out, seqs),
+                            _at(stream))
+    if rc:
+        _check(rc, "g4b_pages_commit")
 
 
 class QMat:
