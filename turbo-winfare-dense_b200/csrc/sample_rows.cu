@@ -15,12 +15,18 @@
 // descending order; this one has no bound on the kept entries, and measures top_p after the
 // temperature and top_k.
 //
-// A row is held in the registers of one cluster of 1 to 16 blocks (up to 16384 entries a block),
-// read from memory once. The prefix's end, as a 50-bit key (ordered logit bits, inverted index), is
-// found by counting: first 256 bins of 1/8 in (m - l) / T, which spread a row's likely entries
-// evenly, then 256 bins over the range of keys that is left, until one key is left. Each block
-// counts in shared memory; the blocks exchange bins through distributed shared memory, one
-// cluster barrier a step.
+// A row is one cluster of 1 to 16 blocks. Each reads its slice of up to 16384 entries from memory
+// once, into shared memory, and passes over it there; blocks exchange through distributed shared
+// memory, one cluster barrier an exchange:
+//   * the maximum;
+//   * where top_k or top_p cut, a histogram of 256 bins of 1/8 in (m - l) / T, which spreads a row's
+//     likely entries evenly (counts, and for a cut by mass the exact masses);
+//   * usual cuts leave a few hundred entries at and above the bin that is cut: these go to the first
+//     block, which ranks them all against all and finishes alone. Where they are more than kList
+//     (nucleus sampling of a flat row), the bin is split into 256 again, the part that is cut is
+//     ranked, and the threshold goes back to all blocks. Ties by the thousand end in a search over
+//     the 50-bit keys (ordered logit bits, inverted index), 8 bits a step;
+//   * without a list, the kept masses per block; the block in whose range r falls finds the token.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -37,36 +43,49 @@ namespace g4b {
 
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kPer = 16;                    // entries a thread holds
-constexpr int kSpan = kThreads * kPer;      // entries a block holds
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kSlice = 16384;               // entries a block holds
+constexpr int kRounds = kSlice / (8 * kThreads);  // a thread takes eight consecutive entries a round
 constexpr int kIndexBits = 18;              // vocabularies up to 262144
+constexpr int kIndexMask = (1 << kIndexBits) - 1;
 constexpr int kBins = 256;
+constexpr int kList = 1024;
 typedef unsigned long long u64;
 
-struct Bins {  // counts and masses; a mass is the sum of three 16-bit parts, whose sums fit 32 bits
+// Masses in three 16-bit parts of their addends, whose sums over a slice fit 32 bits.
+struct Bins {
     unsigned count[kBins], lo[kBins], mid[kBins], hi[kBins];
 };
-struct Exchange {
+struct Pair {
     u64 a, b;
 };
-struct Smem {
+struct Shared {
     Bins bins[2];
-    Exchange ex[2];
-    u64 red[2][32];
-    u64 part[4][32];
+    Pair ex[2];
+    u64 red[2][kWarps];
+    u64 part[kRounds][kWarps];
     u64 cum_count[kBins], cum_mass[kBins];
-    int bin;
+    u64 key[kList];      // the list, in the first block
+    u64 weight[kList];
+    u64 sorted[kList];
+    u64 answer;
+    int bin, list;
 };
 
-__device__ __forceinline__ unsigned order_bits(float l) {  // 0: never kept
-    if (!(l > -INFINITY)) return 0;
+__device__ __forceinline__ unsigned order_bits(float l) {
     const unsigned u = __float_as_uint(l == 0.f ? 0.f : l);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float from_order(unsigned o) {
     return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
+// Key of an entry: larger is earlier in the descending order.
+__device__ __forceinline__ u64 key_of(float l, int index) {
+    return ((u64)order_bits(l) << kIndexBits) | (u64)(kIndexMask - index);
+}
+__device__ __forceinline__ int key_index(u64 k) { return kIndexMask - (int)(k & kIndexMask); }
+__device__ __forceinline__ float key_logit(u64 k) { return from_order((unsigned)(k >> kIndexBits)); }
 
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
 #pragma unroll
@@ -79,85 +98,139 @@ __device__ __forceinline__ u64 warp_max64(u64 v) {
     return v;
 }
 
-template <class T>
-__device__ __forceinline__ float as_f32(T x) { return static_cast<float>(x); }
+// The row's numbers that turn a logit into a weight.
+struct Scale {
+    float m, t, r, bins;  // maximum, temperature, 1 / t, 8 / t
+    bool inf, simple;
+    __device__ void set(float max, float temperature) {
+        m = max;
+        t = temperature;
+        r = 1.f / t;
+        bins = 8.f / t;
+        inf = m == INFINITY;
+        // Out of this range the reciprocal or the remainder below could leave the normal numbers.
+        simple = t > 1e-18f && t < 1e18f;
+    }
+    // exp((l - m) / t). The quotient is the correctly rounded one of a division, from the correctly
+    // rounded reciprocal and one exact remainder (Markstein's theorem), as t is the same for all.
+    __device__ __forceinline__ float share(float l) const {
+        if (inf) return l == m ? 1.f : 0.f;
+        const float a = l - m;
+        float q = a * r;
+        if (simple) q = q > -200.f ? fmaf(fmaf(-q, t, a), r, q) : q;
+        else q = a / t;
+        return expf(q);
+    }
+    static __device__ __forceinline__ u64 weight(float share) { return (u64)(share * 1099511627776.f); }
+    // Bin of a live logit; bins are ordered as the logits are. +inf below +inf gives NaN, which
+    // converts to 0.
+    __device__ __forceinline__ float place(float l) const { return (m - l) * bins; }
+    __device__ __forceinline__ int bin(float l) const { return (int)fminf(place(l), 255.f); }
+    // Of 256 parts of its bin.
+    __device__ __forceinline__ int sub(float l) const {
+        const float x = place(l);
+        return (int)fminf((x - floorf(x)) * 256.f, 255.f);
+    }
+};
 
+template <class T>
+__device__ __forceinline__ void read8(const T* at, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(at);
+        const T* h = reinterpret_cast<const T*>(&a);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(h[i]);
+    }
+}
+
+// One row of one cluster.
 template <class T>
 struct Row {
-    float l[kPer];  // entry 4 k + j is index base + 4096 k + 4 tid + j
-    float m, heat;
-    int base, n;    // this block's slice of the row
-    Smem* sm;
+    Shared& sm;
+    T* data;  // the slice, padded with -inf to a multiple of eight
     cg::cluster_group cl;
-    int phase;
+    int base, n, rounds, blocks, rank, phase;
+    Scale sc;
 
-    __device__ Row(Smem* s) : sm(s), cl(cg::this_cluster()), phase(0) {}
-
-    __device__ int index(int k, int j) const { return base + 4096 * k + 4 * (int)threadIdx.x + j; }
-    __device__ u64 key(int e) const {
-        const unsigned o = order_bits(l[e]);
-        return o ? ((u64)o << kIndexBits) | (u64)((1 << kIndexBits) - 1 - index(e >> 2, e & 3)) : 0;
+    __device__ Row(Shared& s, T* d) : sm(s), data(d), cl(cg::this_cluster()), phase(0) {
+        blocks = (int)cl.num_blocks();
+        rank = (int)cl.block_rank();
     }
-    __device__ float share(int e) const { return l[e] == m ? 1.f : expf((l[e] - m) / heat); }
-    static __device__ u64 weight(float e) { return (u64)(e * 1099511627776.f); }
-
-    __device__ void barrier() {
-        if (cl.num_blocks() > 1) cl.sync();
+    __device__ __forceinline__ void barrier() {
+        if (blocks > 1) cl.sync();
         else __syncthreads();
     }
-
-    // The cluster's largest a and largest b.
-    __device__ Exchange reduce_max(u64 a, u64 b) {
+    // each(l, index, round) for this thread's live entries in index order within a round.
+    template <class Each>
+    __device__ __forceinline__ void pass(Each each) const {
+#pragma unroll 1
+        for (int j = 0; j < rounds; ++j) {
+            const int at = 8 * (j * kThreads + (int)threadIdx.x);
+            if (at >= n) continue;
+            float v[8];
+            read8(data + at, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (v[i] > -INFINITY) each(v[i], base + at + i, j);
+        }
+    }
+    __device__ Pair block_max(u64 a, u64 b) {
         const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
         a = warp_max64(a);
         b = warp_max64(b);
         __syncthreads();
-        if (lane == 0) {
-            sm->red[0][w] = a;
-            sm->red[1][w] = b;
-        }
+        if (lane == 0) sm.red[0][w] = a, sm.red[1][w] = b;
         __syncthreads();
-        if (w == 0) {
-            a = warp_max64(sm->red[0][lane]);
-            b = warp_max64(sm->red[1][lane]);
-            if (lane == 0) sm->ex[phase] = {a, b};
-        }
+        return {warp_max64(lane < kWarps ? sm.red[0][lane] : 0), warp_max64(lane < kWarps ? sm.red[1][lane] : 0)};
+    }
+    __device__ Pair block_sum(u64 a, u64 b) {
+        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+        a = warp_sum64(a);
+        b = warp_sum64(b);
+        __syncthreads();
+        if (lane == 0) sm.red[0][w] = a, sm.red[1][w] = b;
+        __syncthreads();
+        return {warp_sum64(lane < kWarps ? sm.red[0][lane] : 0), warp_sum64(lane < kWarps ? sm.red[1][lane] : 0)};
+    }
+    // Each block's pair, folded over the cluster. Two buffers in turn: a block writes one again only
+    // after the next barrier, which the readers of the last use have passed.
+    template <class Fold>
+    __device__ void exchange(Pair mine, Fold fold) {
+        if (threadIdx.x == 0) sm.ex[phase] = mine;
         barrier();
-        Exchange r{0, 0};
-        for (unsigned c = 0; c < cl.num_blocks(); ++c) {
-            const Exchange x = *cl.map_shared_rank(&sm->ex[phase], c);
-            r.a = max(r.a, x.a);
-            r.b = max(r.b, x.b);
-        }
+#pragma unroll 1
+        for (int b = 0; b < blocks; ++b) fold(b, *cl.map_shared_rank(&sm.ex[phase], b));
         phase ^= 1;
-        return r;
     }
 
-    __device__ Bins& clear_bins() {
-        Bins& b = sm->bins[phase];
-        unsigned* z = b.count;
-        z[threadIdx.x] = 0;  // 4 x 256 counters, 1024 threads
+    __device__ Bins& clear() {
+        Bins& b = sm.bins[phase];
+#pragma unroll
+        for (int i = threadIdx.x; i < 4 * kBins; i += kThreads) b.count[i] = 0;
         __syncthreads();
         return b;
     }
-    __device__ static void add(Bins& b, int i, u64 w, bool mass) {
+    static __device__ __forceinline__ void add(Bins& b, int i, u64 w, bool mass) {
         atomicAdd(&b.count[i], 1u);
-        if (mass && w) {
-            atomicAdd(&b.lo[i], (unsigned)(w & 0xffff));
-            if (w >> 16) atomicAdd(&b.mid[i], (unsigned)((w >> 16) & 0xffff));
-            if (w >> 32) atomicAdd(&b.hi[i], (unsigned)(w >> 32));
-        }
+        if (!mass) return;
+        if (w & 0xffff) atomicAdd(&b.lo[i], (unsigned)(w & 0xffff));
+        if ((w >> 16) & 0xffff) atomicAdd(&b.mid[i], (unsigned)((w >> 16) & 0xffff));
+        if (w >> 32) atomicAdd(&b.hi[i], (unsigned)(w >> 32));
     }
-    // Running counts and masses over the cluster's bins, in every block.
-    __device__ void merge() {
+    // Running counts (and masses) over the cluster's bins, in every block.
+    __device__ void merge(bool mass) {
         barrier();
         const int t = threadIdx.x, lane = t & 31, w = t >> 5;
         u64 c = 0, m = 0;
         if (t < kBins)
-            for (unsigned r = 0; r < cl.num_blocks(); ++r) {
-                const Bins* b = cl.map_shared_rank(&sm->bins[phase], r);
+#pragma unroll 4
+            for (int r = 0; r < blocks; ++r) {
+                const Bins* b = cl.map_shared_rank(&sm.bins[phase], r);
                 c += b->count[t];
-                m += b->lo[t] + ((u64)b->mid[t] << 16) + ((u64)b->hi[t] << 32);
+                if (mass) m += b->lo[t] + ((u64)b->mid[t] << 16) + ((u64)b->hi[t] << 32);
             }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -165,242 +238,446 @@ struct Row {
             if (lane >= o) c += x, m += y;
         }
         __syncthreads();
-        if (t < kBins && lane == 31) sm->red[0][w] = c, sm->red[1][w] = m;
+        if (t < kBins && lane == 31) sm.red[0][w] = c, sm.red[1][w] = m;
         __syncthreads();
         if (t < kBins) {
-            for (int i = 0; i < w; ++i) c += sm->red[0][i], m += sm->red[1][i];
-            sm->cum_count[t] = c;
-            sm->cum_mass[t] = m;
+            for (int i = 0; i < w; ++i) c += sm.red[0][i], m += sm.red[1][i];
+            sm.cum_count[t] = c;
+            sm.cum_mass[t] = m;
         }
-        if (t == 0) sm->bin = kBins;
+        if (t == 0) sm.bin = kBins - 1;
         __syncthreads();
         phase ^= 1;
     }
-
-    // Narrows the kept prefix: its last key is returned, 0 when all entries stay. With `mass`, an
-    // entry stays while the mass before it is below p times the mass of the entries at or above
-    // `from`; otherwise the `k` largest stay.
-    __device__ u64 last_kept(bool mass, u64 k, double p, u64 from) {
-        Bins& b = clear_bins();
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            const u64 c = key(e);
-            if (c && c >= from) {
-                const float x = l[e] == m ? 0.f : (m - l[e]) / heat;
-                add(b, (int)fminf(x * 8.f, 255.f), mass ? weight(share(e)) : 0, mass);
-            }
+    // The bin in which the last kept entry lies: it starts below the goal, and ends at or above it.
+    __device__ int cut_bin(bool mass, u64 before, double goal) {
+        if (threadIdx.x < kBins) {
+            const u64* cum = mass ? sm.cum_mass : sm.cum_count;
+            const int t = threadIdx.x;
+            const u64 lo = t ? cum[t - 1] : 0;
+            if (cum[t] != lo && (double)(before + lo) < goal && !((double)(before + cum[t]) < goal)) sm.bin = t;
         }
-        merge();
-        const u64 all = mass ? sm->cum_mass[kBins - 1] : sm->cum_count[kBins - 1];
-        const double goal = mass ? p * (double)all : (double)k;
-        if (!((double)all > goal)) return 0;  // k at or above the entries there are
+        __syncthreads();
+        return sm.bin;
+    }
+
+    // Entries in(l) go to the first block's list; it returns their number there (the others must not
+    // use theirs). At most kList of them.
+    template <class In>
+    __device__ int gather(In in) {
+        if (threadIdx.x == 0 && rank == 0) sm.list = 0;
+        barrier();
+        int* count = cl.map_shared_rank(&sm.list, 0);
+        u64* list = cl.map_shared_rank(sm.key, 0);
+        pass([&](float l, int index, int) {
+            if (in(l)) {
+                const int at = atomicAdd(count, 1);
+                if (at < kList) list[at] = key_of(l, index);
+            }
+        });
+        barrier();
+        return min(sm.list, kList);
+    }
+
+    // Key of the last kept entry, searched for over keys: of those at or above `from`, the k largest
+    // stay, or the ones before which less than `goal` of mass lies. The slow way, for ties.
+    __device__ __noinline__ u64 search(bool mass, double goal, u64 from) {
         u64 before = 0, lo = from, hi = ~0ull;
-        bool first = true;
-        int bin = 0;
         // Every step leaves 1/256 of a 50-bit range of keys, or less: seven steps reach one key.
-        for (int step = 0; step < 8; ++step) {
-            // The bin in which the last kept entry lies.
-            const u64* cum = mass ? sm->cum_mass : sm->cum_count;
-            if (threadIdx.x < kBins) {
-                const int t = threadIdx.x;
-                const u64 at = before + (t ? cum[t - 1] : 0);
-                if (cum[t] != (t ? cum[t - 1] : 0) && (double)at < goal && !((double)(before + cum[t]) < goal)) sm->bin = t;
-            }
-            __syncthreads();
-            bin = sm->bin;
-            before += bin ? cum[bin - 1] : 0;
-            u64 top = 0, low = 0;  // largest key and, inverted, smallest key in that bin
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                const u64 c = key(e);
-                bool in = c && c >= lo && c <= hi;
-                if (first && in) {
-                    const float x = l[e] == m ? 0.f : (m - l[e]) / heat;
-                    in = (int)fminf(x * 8.f, 255.f) == bin;
-                }
-                if (in) {
-                    top = max(top, c);
-                    low = max(low, ~c);
-                }
-            }
-            first = false;
-            const Exchange r = reduce_max(top, low);
-            hi = r.a;
-            lo = ~r.b;
-            if (hi == lo) return lo;
+        for (int step = 0; step < 9; ++step) {
+            u64 top = 0, low = 0;  // the largest key and, inverted, the smallest
+            pass([&](float l, int index, int) {
+                const u64 c = key_of(l, index);
+                if (c >= lo && c <= hi) top = max(top, c), low = max(low, ~c);
+            });
+            const Pair mine = block_max(top, low);
+            Pair all{0, 0};
+            exchange(mine, [&](int, Pair x) { all = {max(all.a, x.a), max(all.b, x.b)}; });
+            hi = all.a;
+            lo = ~all.b;
+            if (hi <= lo) return lo;
             const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 8);
-            Bins& b2 = clear_bins();
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                const u64 c = key(e);
-                if (c && c >= lo && c <= hi) add(b2, (int)((hi - c) >> shift), mass ? weight(share(e)) : 0, mass);
-            }
-            merge();
-            // The chosen bin's key range, for the next step.
-            if (threadIdx.x < kBins) {
-                const u64* cm = mass ? sm->cum_mass : sm->cum_count;
-                const int t = threadIdx.x;
-                const u64 at = before + (t ? cm[t - 1] : 0);
-                if (cm[t] != (t ? cm[t - 1] : 0) && (double)at < goal && !((double)(before + cm[t]) < goal)) sm->bin = t;
-            }
+            Bins& b = clear();
+            pass([&](float l, int index, int) {
+                const u64 c = key_of(l, index);
+                if (c >= lo && c <= hi) add(b, (int)((hi - c) >> shift), mass ? Scale::weight(sc.share(l)) : 0, mass);
+            });
+            merge(mass);
+            const int bin = cut_bin(mass, before, goal);
+            if (bin) before += (mass ? sm.cum_mass : sm.cum_count)[bin - 1];
+            const u64 first = hi - ((u64)bin << shift), span = ((u64)1 << shift) - 1;
             __syncthreads();
-            const u64 top_key = hi - ((u64)sm->bin << shift);
-            const u64 span = ((u64)1 << shift) - 1;
-            hi = top_key;
-            lo = max(lo, top_key >= span ? top_key - span : 0);
-            __syncthreads();
+            hi = first;
+            lo = max(lo, first >= span ? first - span : 0);
         }
         return lo;
     }
 };
 
-template <class T>
-__global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(SampleRowsArgs a) {
-    __shared__ Smem sm;
-    Row<T> row(&sm);
-    const int rank = (int)row.cl.block_rank(), blocks = (int)row.cl.num_blocks();
-    const int r = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const T* in = static_cast<const T*>(a.logits) + r * a.stride;
-    const int per = ((a.vocab + blocks - 1) / blocks + 7) & ~7;
-    row.base = rank * per;
-    row.n = min(per, a.vocab - row.base);
-    const bool vec = reinterpret_cast<uintptr_t>(in) % (4 * sizeof(T)) == 0;
-    u64 best = 0;
-#pragma unroll
-    for (int k = 0; k < kPer / 4; ++k) {
-        const int at = 4096 * k + 4 * tid;
-        T x[4];
-        if (vec && at + 3 < row.n) {
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(x) = __ldcs(reinterpret_cast<const uint4*>(in + row.base + at));
-            else *reinterpret_cast<uint2*>(x) = __ldcs(reinterpret_cast<const uint2*>(in + row.base + at));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) row.l[4 * k + j] = as_f32(x[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) row.l[4 * k + j] = at + j < row.n ? as_f32(in[row.base + at + j]) : -INFINITY;
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) best = max(best, row.key(e));
-    best = row.reduce_max(best, 0).a;
-    const float t = a.temperature ? a.temperature[r] : 1.f;
-    const bool lead = rank == 0 && tid == 0;
-    if (best == 0 || !(t > 0.f)) {
-        if (lead) {
-            a.token[r] = best ? (1 << kIndexBits) - 1 - (int)(best & ((1 << kIndexBits) - 1)) : -1;
-            if (a.prob) a.prob[r] = best ? 1.f : 0.f;
-            if (a.kept) a.kept[r] = best ? 1 : 0;
-        }
-        row.barrier();  // no block leaves while its shared memory is read
-        return;
-    }
-    row.m = from_order((unsigned)(best >> kIndexBits));
-    row.heat = t;
-    const int k = a.top_k ? a.top_k[r] : 0;
-    const float p = a.top_p ? a.top_p[r] : 1.f;
-    float low = a.min_p ? a.min_p[r] : 0.f;
-    low = low > 0.f ? fminf(low, 1.f) : 0.f;
-    u64 from = 1;
-    if (k > 0 && k < a.vocab) from = max(from, row.last_kept(false, k, 0.0, 1));
-    if (p < 1.f) from = max(from, p > 0.f ? row.last_kept(true, 0, (double)p, from) : best);
+__device__ __forceinline__ void write(const SampleRowsArgs& a, int r, int token, float prob, int kept) {
+    a.token[r] = token;
+    if (a.prob) a.prob[r] = prob;
+    if (a.kept) a.kept[r] = kept;
+}
 
-    // Kept mass in index order: per (4096-entry tile, warp), then block by block.
-    u64 w[4] = {0, 0, 0, 0};
-    unsigned cnt = 0;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        const u64 c = row.key(e);
-        if (c && c >= from) {
-            const float x = row.share(e);
-            if (x >= low) {
-                w[e >> 2] += Row<T>::weight(x);
-                ++cnt;
-            }
-        }
+__device__ __forceinline__ u64 draw(float u, u64 total) {
+    const double x = floor((double)u * (double)total);
+    return min(x > 0.0 ? (u64)x : 0ull, total - 1);  // also for numbers outside [0, 1)
+}
+
+// Ranks the first block's list of n keys: sm.sorted in descending order.
+__device__ void rank_list(Shared& sm, int n) {
+#pragma unroll 1
+    for (int t = threadIdx.x; t < n; t += kThreads) {
+        const u64 mine = sm.key[t];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += sm.key[j] > mine;
+        sm.sorted[rank] = mine;
     }
     __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const u64 s = warp_sum64(w[q]);
-        if (lane == 0) sm.part[q][warp] = s;
-    }
-    const u64 c = warp_sum64(cnt);
-    if (lane == 0) sm.red[0][warp] = c;
-    __syncthreads();
-    if (warp == 0) {
-        u64 s = sm.part[0][lane] + sm.part[1][lane] + sm.part[2][lane] + sm.part[3][lane];
-        s = warp_sum64(s);
-        const u64 n = warp_sum64(sm.red[0][lane]);
-        if (lane == 0) sm.ex[row.phase] = {s, n};
-    }
-    row.barrier();
-    u64 total = 0, ahead = 0, kept = 0;
-    u64 mine = 0;
-    for (int b = 0; b < blocks; ++b) {
-        const Exchange x = *row.cl.map_shared_rank(&sm.ex[row.phase], b);
-        if (b < rank) ahead += x.a;
-        if (b == rank) mine = x.a;
-        total += x.a;
-        kept += x.b;
-    }
-    row.barrier();  // no block leaves while its shared memory is read
-    const float u = a.uniform[r];
-    const double scaled = floor((double)u * (double)total);
-    u64 goal = scaled > 0.0 ? (u64)scaled : 0;
-    goal = min(goal, total - 1);
-    if (goal < ahead || goal >= ahead + mine) return;
-    goal -= ahead;
-    // The (tile, warp) part that holds it, then the thread and the entry.
-    u64 run = 0;
-    int q = 0, wv = 0;
-    for (q = 0; q < 4; ++q) {
-        u64 s = 0;
-        for (int i = 0; i < 32; ++i) s += sm.part[q][i];
-        if (goal < run + s) break;
-        run += s;
-    }
-    for (wv = 0; wv < 32; ++wv) {
-        if (goal < run + sm.part[q][wv]) break;
-        run += sm.part[q][wv];
-    }
-    if (wv != warp) return;
-    u64 part = q == 0 ? w[0] : q == 1 ? w[1] : q == 2 ? w[2] : w[3];
-    u64 incl = part;
+}
+
+// Exclusive running sum over the block's threads of one value each, and the whole.
+__device__ u64 block_scan(Shared& sm, u64 v, u64* total) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    u64 x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
+        const u64 y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
     }
-    if (goal < run + incl - part || goal >= run + incl) return;
-    run += incl - part;
+    __syncthreads();
+    if (lane == 31) sm.red[0][w] = x;
+    __syncthreads();
+    u64 ahead = 0, all = 0;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        if ((e >> 2) != q) continue;
-        const u64 ky = row.key(e);
-        const float x = row.share(e);
-        if (!ky || ky < from || !(x >= low)) continue;
-        const u64 wt = Row<T>::weight(x);
-        if (goal >= run && goal < run + wt) {
-            a.token[r] = row.index(e >> 2, e & 3);
-            if (a.prob) a.prob[r] = x / ((float)total * 9.094947017729282e-13f);  // 2^-40
-            if (a.kept) a.kept[r] = (int)kept;
-        }
-        run += wt;
+    for (int i = 0; i < kWarps; ++i) {
+        const u64 s = sm.red[0][i];
+        ahead += i < w ? s : 0;
+        all += s;
+    }
+    *total = all;
+    return ahead + x - v;
+}
+
+// The end of a row whose list (in the first block, descending in sm.sorted) holds every entry that
+// may be kept: the first k of it, then the cuts by mass and by min-p, then the draw.
+__device__ __noinline__ void finish_list(const SampleRowsArgs& a, int r, Shared& sm, const Scale& sc, int n, u64 k,
+                                         float p, double goal, float low) {
+    const int m = (int)min((u64)n, k), t = threadIdx.x;
+    // Two neighbours of the descending order a thread.
+    float e[2];
+    u64 w[2], key[2], total, mass;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int x = 2 * t + i;
+        key[i] = x < m ? sm.sorted[x] : 0;
+        e[i] = x < m ? sc.share(key_logit(key[i])) : 0.f;
+        w[i] = Scale::weight(e[i]);
+    }
+    const u64 before = block_scan(sm, w[0] + w[1], &mass);
+    if (k != ~0ull) goal = (double)p * (double)mass;
+    unsigned kept = 0;
+    u64 sum = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int x = 2 * t + i;
+        const u64 ahead = before + (i ? w[0] : 0);
+        const bool in = x < m && (x == 0 || ((p >= 1.f || (double)ahead < goal) && e[i] >= low));
+        if (!in) w[i] = 0;
+        kept += in;
+        sum += w[i];
+        if (x < m) sm.weight[x] = w[i];
+    }
+    block_scan(sm, sum, &total);
+    u64 count;
+    block_scan(sm, kept, &count);  // its barriers also make sm.weight visible
+    const u64 target = draw(a.uniform[r], total);
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+        if (w[i] == 0) continue;
+        u64 below = 0;  // kept mass of lower indices
+        const u64 index = key[i] & kIndexMask;  // inverted: a lower index is larger
+#pragma unroll 4
+        for (int j = 0; j < m; ++j) below += (sm.sorted[j] & kIndexMask) > index ? sm.weight[j] : 0;
+        if (target >= below && target < below + w[i])
+            write(a, r, key_index(key[i]), e[i] / ((float)total * 9.094947017729282e-13f), (int)count);  // 2^-40
     }
 }
 
 template <class T>
+__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs a) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    Shared& sm = *reinterpret_cast<Shared*>(raw);
+    Row<T> row(sm, reinterpret_cast<T*>(raw + sizeof(Shared)));
+    const int r = blockIdx.x / row.blocks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const T* in = static_cast<const T*>(a.logits) + r * a.stride;
+    const int per = ((a.vocab + row.blocks - 1) / row.blocks + 7) & ~7;
+    row.base = row.rank * per;
+    row.n = max(0, min(per, a.vocab - row.base));
+    row.rounds = (row.n + 8 * kThreads - 1) / (8 * kThreads);
+    const T* from = in + row.base;
+    constexpr int kWide = 16 / sizeof(T);
+    if (reinterpret_cast<uintptr_t>(from) % 16 == 0) {
+        const int whole = row.n / kWide;
+        const uint32_t at = (uint32_t)__cvta_generic_to_shared(row.data);
+#pragma unroll 4
+        for (int i = tid; i < whole; i += kThreads)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + i * 16), "l"(from + i * kWide) : "memory");
+        for (int i = whole * kWide + tid; i < row.n; i += kThreads) row.data[i] = from[i];
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+#pragma unroll 4
+        for (int i = tid; i < row.n; i += kThreads) row.data[i] = from[i];
+    }
+    if (tid < ((row.n + 7) & ~7) - row.n) row.data[row.n + tid] = static_cast<T>(-INFINITY);
+    __syncthreads();
+
+    // The maximum and the number of live entries; NaN becomes -inf on the way.
+    float m = -INFINITY;
+    unsigned live = 0;
+    bool nan = false;
+#pragma unroll 1
+    for (int j = 0; j < row.rounds; ++j) {
+        const int at = 8 * (j * kThreads + tid);
+        if (at >= row.n) continue;
+        float v[8];
+        read8(row.data + at, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            m = fmaxf(m, v[i]);
+            live += v[i] > -INFINITY;
+            nan |= v[i] != v[i];
+        }
+        if (nan) {
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i)
+                if (!(static_cast<float>(row.data[at + i]) > -INFINITY)) row.data[at + i] = static_cast<T>(-INFINITY);
+        }
+    }
+    Pair all = row.block_sum(live, 0);
+    const u64 mine_live = all.a;
+    all = row.block_max(m > -INFINITY ? order_bits(m) : 0, 0);
+    u64 top = 0, alive = 0;
+    row.exchange({all.a, mine_live}, [&](int, Pair x) { top = max(top, x.a), alive += x.b; });
+    const float t = a.temperature ? a.temperature[r] : 1.f;
+    const bool lead = row.rank == 0 && tid == 0;
+    if (top == 0) {
+        if (lead) write(a, r, -1, 0.f, 0);
+        row.barrier();  // no block leaves while its shared memory is read
+        return;
+    }
+    m = from_order((unsigned)top);
+    if (!(t > 0.f)) {
+        u64 first = 0;  // the lowest index that holds the maximum, inverted
+        row.pass([&](float l, int index, int) {
+            if (l == m) first = max(first, (u64)(kIndexMask - index) + 1);
+        });
+        first = row.block_max(first, 0).a;
+        u64 best = 0;
+        row.exchange({first, 0}, [&](int, Pair x) { best = max(best, x.a); });
+        if (lead) write(a, r, kIndexMask + 1 - (int)best, 1.f, 1);
+        row.barrier();
+        return;
+    }
+    row.sc.set(m, t);
+    const Scale sc = row.sc;
+    const int want = a.top_k ? a.top_k[r] : 0;
+    const float p = a.top_p ? a.top_p[r] : 1.f;
+    float low = a.min_p ? a.min_p[r] : 0.f;
+    low = low > 0.f ? fminf(low, 1.f) : 0.f;
+    u64 k = want > 0 && (u64)want < alive ? (u64)want : ~0ull;
+    if (p <= 0.f) k = 1;  // the first entry always stays
+    const bool by_mass = k == ~0ull && p < 1.f;
+
+    u64 from_key = 0;  // the last kept key, as far as it is known
+    if (k != ~0ull || by_mass) {
+        Bins& b = row.clear();
+        if (by_mass)
+            row.pass([&](float l, int, int) { Row<T>::add(b, sc.bin(l), Scale::weight(sc.share(l)), true); });
+        else
+            row.pass([&](float l, int, int) {
+                // The last bin is not counted: it holds what the others do not.
+                const int x = sc.bin(l);
+                if (x < kBins - 1) atomicAdd(&b.count[x], 1u);
+            });
+        row.merge(by_mass);
+        double goal = by_mass ? (double)p * (double)sm.cum_mass[kBins - 1] : (double)k;
+        const int bin = row.cut_bin(by_mass, 0, goal);
+        const u64 held = bin == kBins - 1 ? alive : sm.cum_count[bin];
+        if (held <= kList) {
+            const int n = row.gather([&](float l) { return sc.bin(l) <= bin; });
+            if (row.rank != 0) return;  // nobody reads this block's memory any more
+            rank_list(sm, n);
+            finish_list(a, r, sm, sc, n, k, p, goal, low);
+            return;
+        }
+        const u64 ahead = bin ? (by_mass ? sm.cum_mass : sm.cum_count)[bin - 1] : 0;
+        __syncthreads();
+        u64 key = 0;
+        bool found = false;
+        if (bin < kBins - 1) {  // the bin in 256 parts
+            Bins& s = row.clear();
+            row.pass([&](float l, int, int) {
+                if (sc.bin(l) == bin) Row<T>::add(s, sc.sub(l), by_mass ? Scale::weight(sc.share(l)) : 0, by_mass);
+            });
+            row.merge(by_mass);
+            const int part = row.cut_bin(by_mass, ahead, goal);
+            const u64 lo = part ? sm.cum_count[part - 1] : 0, before = ahead + (part ? (by_mass ? sm.cum_mass : sm.cum_count)[part - 1] : 0);
+            if (sm.cum_count[part] - lo <= kList) {
+                const int n = row.gather([&](float l) { return sc.bin(l) == bin && sc.sub(l) == part; });
+                if (row.rank == 0) {
+                    rank_list(sm, n);
+                    u64 w[2], whole;
+                    const u64 one = by_mass ? 0 : 1;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int x = 2 * tid + i;
+                        w[i] = x < n ? (by_mass ? Scale::weight(sc.share(key_logit(sm.sorted[x]))) : one) : 0;
+                    }
+                    u64 at = before + block_scan(sm, w[0] + w[1], &whole);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (w[i] && (double)at < goal && !((double)(at + w[i]) < goal))
+#pragma unroll 1
+                            for (int c = 0; c < row.blocks; ++c) *row.cl.map_shared_rank(&sm.answer, c) = sm.sorted[2 * tid + i];
+                        at += w[i];
+                    }
+                }
+                row.barrier();
+                key = sm.answer;
+                found = true;
+            }
+        }
+        if (!found) key = row.search(by_mass, goal, 0);
+        from_key = key;
+        if (!by_mass && p > 0.f && p < 1.f) {  // the k that stay, then the cut by their mass
+            u64 mass = 0;
+            row.pass([&](float l, int index, int) {
+                if (key_of(l, index) >= from_key) mass += Scale::weight(sc.share(l));
+            });
+            const Pair mine = row.block_sum(mass, 0);
+            u64 sum = 0;
+            row.exchange(mine, [&](int, Pair x) { sum += x.a; });
+            goal = (double)p * (double)sum;
+            from_key = max(from_key, row.search(true, goal, from_key));
+        }
+    }
+
+    // Kept mass in index order: per (round, warp), then block by block.
+    const float edge = from_key ? key_logit(from_key) : -INFINITY;
+    const float far = low > 0.f ? (0.01f - logf(low)) * 8.f * 1.001f : INFINITY;  // bins past which no share reaches low
+    const int edge_index = from_key ? key_index(from_key) : kIndexMask;
+    const auto weigh = [&](float l, int index, float& e) -> u64 {
+        if (l < edge || (l == edge && index > edge_index) || sc.place(l) > far) return ~0ull;
+        e = sc.share(l);
+        return e >= low ? Scale::weight(e) : ~0ull;
+    };
+    u64 count = 0;
+#pragma unroll 1
+    for (int j = 0; j < kRounds; ++j) {
+        const int at = 8 * (j * kThreads + tid);
+        u64 sum = 0;
+        if (j < row.rounds && at < row.n) {
+            float v[8];
+            read8(row.data + at, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (v[i] > -INFINITY) {
+                    float e;
+                    const u64 w = weigh(v[i], row.base + at + i, e);
+                    if (w != ~0ull) sum += w, ++count;
+                }
+        }
+        sum = warp_sum64(sum);
+        if (lane == 0) sm.part[j][warp] = sum;
+    }
+    __syncthreads();
+    u64 slice = 0;
+    if (tid < kRounds * kWarps) slice = sm.part[tid / kWarps][tid % kWarps];
+    const Pair mine = row.block_sum(slice, count);
+    u64 total = 0, ahead = 0, kept = 0;
+    row.exchange(mine, [&](int b, Pair x) {
+        if (b < row.rank) ahead += x.a;
+        total += x.a;
+        kept += x.b;
+    });
+    row.barrier();  // no block leaves while its shared memory is read
+    u64 goal = draw(a.uniform[r], total);
+    if (goal < ahead || goal >= ahead + mine.a) return;
+    goal -= ahead;
+    // The (round, warp) part that holds it: one warp looks, 64 parts in two.
+    if (warp == 0) {
+        const u64 w0 = sm.part[0][2 * lane], w1 = sm.part[0][2 * lane + 1];
+        u64 x = w0 + w1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        const u64 at = x - w0 - w1;
+        if (goal >= at && goal < x) {
+            const int second = goal >= at + w0;
+            sm.bin = 2 * lane + second;
+            sm.answer = goal - at - (second ? w0 : 0);
+        }
+        __syncwarp();
+        const int j = sm.bin / kWarps, at8 = 8 * (j * kThreads + (sm.bin % kWarps) * 32 + lane);
+        goal = sm.answer;
+        u64 own = 0;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = -INFINITY;
+        if (at8 < row.n) read8(row.data + at8, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (v[i] > -INFINITY) {
+                float e;
+                const u64 w = weigh(v[i], row.base + at8 + i, e);
+                if (w != ~0ull) own += w;
+            }
+        u64 upto = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        u64 run = upto - own;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (v[i] > -INFINITY) {
+                float e;
+                const u64 w = weigh(v[i], row.base + at8 + i, e);
+                if (w == ~0ull) continue;
+                if (goal >= run && goal < run + w)
+                    write(a, r, row.base + at8 + i, e / ((float)total * 9.094947017729282e-13f), (int)kept);  // 2^-40
+                run += w;
+            }
+    }
+}
+static_assert(kRounds * kWarps == 64, "the last search looks at 64 parts");
+
+template <class T>
 cudaError_t run(const SampleRowsArgs& a, cudaStream_t st) {
     int blocks = 1;
-    while (blocks * kSpan < a.vocab) blocks *= 2;
+    while (blocks * kSlice < a.vocab) blocks *= 2;
+    const int per = ((a.vocab + blocks - 1) / blocks + 7) & ~7;
+    const size_t smem = sizeof(Shared) + (size_t)per * sizeof(T);
     auto kern = sample_rows_kernel<T>;
-    if (blocks > 8) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    static bool attr = false;
+    if (!attr) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)(sizeof(Shared) + kSlice * sizeof(T)));
         if (e != cudaSuccess) return e;
+        attr = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * blocks));
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
