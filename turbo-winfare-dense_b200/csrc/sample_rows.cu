@@ -50,7 +50,8 @@ constexpr int kRounds = kSlice / (8 * kThreads);  // a thread takes eight consec
 constexpr int kIndexBits = 18;              // vocabularies up to 262144
 constexpr int kIndexMask = (1 << kIndexBits) - 1;
 constexpr int kBins = 256;
-constexpr int kList = 1024;
+constexpr int kList = 1024;                 // entries the first block ranks
+constexpr int kCand = 2048;                 // entries of one bin that a block sets aside
 typedef unsigned long long u64;
 
 // Masses in three 16-bit parts of their addends, whose sums over a slice fit 32 bits.
@@ -60,18 +61,22 @@ struct Bins {
 struct Pair {
     u64 a, b;
 };
-struct Shared {
+struct alignas(16) Shared {
     Bins bins[2];
-    Pair ex[2];
+    Pair ex[2][16];      // every block's, by rank
     u64 red[2][kWarps];
+    unsigned red32[2][kWarps];
     u64 part[kRounds][kWarps];
     u64 cum_count[kBins], cum_mass[kBins];
     u64 key[kList];      // the list, in the first block
-    u64 weight[kList];
-    u64 sorted[kList];
+    u64 weight[kList];   // by rank in the descending order, then by rank in index order
+    u64 named[kList];    // keys by rank
+    uint16_t cand[kCand];    // places in the slice of what is set aside
     u64 answer;
-    int bin, list;
+    int bin, list, cands;
 };
+
+static_assert(sizeof(Shared) % 16 == 0, "the slice behind it is read in 16-byte pieces");
 
 __device__ __forceinline__ unsigned order_bits(float l) {
     const unsigned u = __float_as_uint(l == 0.f ? 0.f : l);
@@ -87,10 +92,12 @@ __device__ __forceinline__ u64 key_of(float l, int index) {
 __device__ __forceinline__ int key_index(u64 k) { return kIndexMask - (int)(k & kIndexMask); }
 __device__ __forceinline__ float key_logit(u64 k) { return from_order((unsigned)(k >> kIndexBits)); }
 
+// Sum over the warp, in three parts whose sums fit the 32-bit reduction.
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    constexpr u64 kPart = (1u << 26) - 1;
+    return (u64)__reduce_add_sync(0xffffffffu, (unsigned)(v & kPart)) +
+           ((u64)__reduce_add_sync(0xffffffffu, (unsigned)((v >> 26) & kPart)) << 26) +
+           ((u64)__reduce_add_sync(0xffffffffu, (unsigned)(v >> 52)) << 52);
 }
 __device__ __forceinline__ u64 warp_max64(u64 v) {
 #pragma unroll
@@ -177,6 +184,17 @@ struct Row {
                 if (v[i] > -INFINITY) each(v[i], base + at + i, j);
         }
     }
+    // The block's largest a and sum of b.
+    __device__ uint2 block_max_sum(unsigned a, unsigned b) {
+        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+        a = __reduce_max_sync(0xffffffffu, a);
+        b = __reduce_add_sync(0xffffffffu, b);
+        __syncthreads();
+        if (lane == 0) sm.red32[0][w] = a, sm.red32[1][w] = b;
+        __syncthreads();
+        return {__reduce_max_sync(0xffffffffu, lane < kWarps ? sm.red32[0][lane] : 0),
+                __reduce_add_sync(0xffffffffu, lane < kWarps ? sm.red32[1][lane] : 0)};
+    }
     __device__ Pair block_max(u64 a, u64 b) {
         const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
         a = warp_max64(a);
@@ -186,23 +204,23 @@ struct Row {
         __syncthreads();
         return {warp_max64(lane < kWarps ? sm.red[0][lane] : 0), warp_max64(lane < kWarps ? sm.red[1][lane] : 0)};
     }
-    __device__ Pair block_sum(u64 a, u64 b) {
+    __device__ u64 block_sum(u64 a) {
         const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
         a = warp_sum64(a);
-        b = warp_sum64(b);
         __syncthreads();
-        if (lane == 0) sm.red[0][w] = a, sm.red[1][w] = b;
+        if (lane == 0) sm.red[0][w] = a;
         __syncthreads();
-        return {warp_sum64(lane < kWarps ? sm.red[0][lane] : 0), warp_sum64(lane < kWarps ? sm.red[1][lane] : 0)};
+        return warp_sum64(lane < kWarps ? sm.red[0][lane] : 0);
     }
-    // Each block's pair, folded over the cluster. Two buffers in turn: a block writes one again only
-    // after the next barrier, which the readers of the last use have passed.
+    // Each block's pair, folded over the cluster. A block writes its own into every block before the
+    // barrier: what is read after it is local. Two buffers in turn: one is written again only after the
+    // next barrier, which the readers of the last use have passed.
     template <class Fold>
     __device__ void exchange(Pair mine, Fold fold) {
-        if (threadIdx.x == 0) sm.ex[phase] = mine;
+        if ((int)threadIdx.x < blocks) *cl.map_shared_rank(&sm.ex[phase][rank], threadIdx.x) = mine;
         barrier();
 #pragma unroll 1
-        for (int b = 0; b < blocks; ++b) fold(b, *cl.map_shared_rank(&sm.ex[phase], b));
+        for (int b = 0; b < blocks; ++b) fold(b, sm.ex[phase][b]);
         phase ^= 1;
     }
 
@@ -220,23 +238,37 @@ struct Row {
         if ((w >> 16) & 0xffff) atomicAdd(&b.mid[i], (unsigned)((w >> 16) & 0xffff));
         if (w >> 32) atomicAdd(&b.hi[i], (unsigned)(w >> 32));
     }
-    // Running counts (and masses) over the cluster's bins, in every block.
+    // Running counts (and masses) over the cluster's bins, in every block. Each block adds up its share
+    // of the bins over all blocks, a lane a (bin, block), and hands the sums to all: reading every
+    // bin of every block everywhere would be sixteen times the traffic between SMs.
     __device__ void merge(bool mass) {
         barrier();
         const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-        u64 c = 0, m = 0;
-        if (t < kBins)
-#pragma unroll 4
-            for (int r = 0; r < blocks; ++r) {
-                const Bins* b = cl.map_shared_rank(&sm.bins[phase], r);
-                c += b->count[t];
-                if (mass) m += b->lo[t] + ((u64)b->mid[t] << 16) + ((u64)b->hi[t] << 32);
+        if (t < kBins) {
+            const int src = t & (blocks - 1), bin = (t + rank * kBins) / blocks;
+            const Bins* b = cl.map_shared_rank(&sm.bins[phase], src);
+            unsigned c = b->count[bin];
+            u64 m = mass ? b->lo[bin] + ((u64)b->mid[bin] << 16) + ((u64)b->hi[bin] << 32) : 0;
+            for (int o = blocks >> 1; o > 0; o >>= 1) {
+                c += __shfl_xor_sync(0xffffffffu, c, o);
+                if (mass) m += __shfl_xor_sync(0xffffffffu, m, o);
             }
+            *cl.map_shared_rank(&sm.cum_count[bin], src) = c;
+            if (mass) *cl.map_shared_rank(&sm.cum_mass[bin], src) = m;
+        }
+        barrier();
+        u64 c = t < kBins ? sm.cum_count[t] : 0, m = t < kBins && mass ? sm.cum_mass[t] : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const u64 x = __shfl_up_sync(0xffffffffu, c, o), y = __shfl_up_sync(0xffffffffu, m, o);
-            if (lane >= o) c += x, m += y;
+            const unsigned x = __shfl_up_sync(0xffffffffu, (unsigned)c, o);  // counts fit 32 bits
+            if (lane >= o) c += x;
         }
+        if (mass)
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 y = __shfl_up_sync(0xffffffffu, m, o);
+                if (lane >= o) m += y;
+            }
         __syncthreads();
         if (t < kBins && lane == 31) sm.red[0][w] = c, sm.red[1][w] = m;
         __syncthreads();
@@ -261,22 +293,41 @@ struct Row {
         return sm.bin;
     }
 
-    // Entries in(l) go to the first block's list; it returns their number there (the others must not
-    // use theirs). At most kList of them.
-    template <class In>
-    __device__ int gather(In in) {
+    // Entries that each(put) passes to put(l, index) go to the first block's list; their number is
+    // returned there (the others must not use theirs). At most kList of them in the cluster.
+    template <class Each>
+    __device__ int gather(Each each) {
         if (threadIdx.x == 0 && rank == 0) sm.list = 0;
         barrier();
         int* count = cl.map_shared_rank(&sm.list, 0);
         u64* list = cl.map_shared_rank(sm.key, 0);
-        pass([&](float l, int index, int) {
-            if (in(l)) {
-                const int at = atomicAdd(count, 1);
-                if (at < kList) list[at] = key_of(l, index);
-            }
+        each([&](float l, int index) {
+            const int at = atomicAdd(count, 1);
+            if (at < kList) list[at] = key_of(l, index);
         });
         barrier();
         return min(sm.list, kList);
+    }
+    // Sets a bin's entries aside, in the order they come; at most kCand of them.
+    __device__ void set_aside(int bin) {
+        if (threadIdx.x == 0) sm.cands = 0;
+        __syncthreads();
+        pass([&](float l, int index, int) {
+            if (sc.bin(l) == bin) {
+                const int at = atomicAdd(&sm.cands, 1);
+                if (at < kCand) sm.cand[at] = (uint16_t)(index - base);
+            }
+        });
+        __syncthreads();
+    }
+    template <class Each>
+    __device__ __forceinline__ void pass_aside(Each each) const {
+        const int m = min(sm.cands, kCand);
+#pragma unroll 1
+        for (int i = threadIdx.x; i < m; i += kThreads) {
+            const int at = sm.cand[i];
+            each(static_cast<float>(data[at]), base + at);
+        }
     }
 
     // Key of the last kept entry, searched for over keys: of those at or above `from`, the k largest
@@ -325,19 +376,6 @@ __device__ __forceinline__ u64 draw(float u, u64 total) {
     return min(x > 0.0 ? (u64)x : 0ull, total - 1);  // also for numbers outside [0, 1)
 }
 
-// Ranks the first block's list of n keys: sm.sorted in descending order.
-__device__ void rank_list(Shared& sm, int n) {
-#pragma unroll 1
-    for (int t = threadIdx.x; t < n; t += kThreads) {
-        const u64 mine = sm.key[t];
-        int rank = 0;
-#pragma unroll 8
-        for (int j = 0; j < n; ++j) rank += sm.key[j] > mine;
-        sm.sorted[rank] = mine;
-    }
-    __syncthreads();
-}
-
 // Exclusive running sum over the block's threads of one value each, and the whole.
 __device__ u64 block_scan(Shared& sm, u64 v, u64* total) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -361,50 +399,82 @@ __device__ u64 block_scan(Shared& sm, u64 v, u64* total) {
     return ahead + x - v;
 }
 
-// The end of a row whose list (in the first block, descending in sm.sorted) holds every entry that
-// may be kept: the first k of it, then the cuts by mass and by min-p, then the draw.
+// Ranks of a key among the list's n, in descending order of keys (x) and in index order (y). Few
+// keys have several neighbouring threads each; each(i, ranks) runs in one of them. All threads come.
+template <class Each>
+__device__ __forceinline__ void rank_list(const Shared& sm, int n, Each each) {
+    int share = 1;  // threads a key
+    while (share < 32 && 2 * share * n <= kThreads) share *= 2;
+    const int part = threadIdx.x % share, step = kThreads / share;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += step) {
+        const int i = i0 + threadIdx.x / share;
+        const u64 mine = i < n ? sm.key[i] : 0;
+        int2 r{0, 0};
+#pragma unroll 4
+        for (int j = part; j < n; j += share) {
+            const u64 k = sm.key[j];
+            r.x += k > mine;
+            r.y += (unsigned)(k & kIndexMask) > (unsigned)(mine & kIndexMask);  // inverted indices
+        }
+        for (int o = share >> 1; o > 0; o >>= 1) {
+            r.x += __shfl_xor_sync(0xffffffffu, r.x, o);
+            r.y += __shfl_xor_sync(0xffffffffu, r.y, o);
+        }
+        if (i < n && part == 0) each(i, r);
+    }
+}
+
+// The end of a row whose list (in the first block) holds every entry that may be kept: the first k
+// of it, then the cuts by mass and by min-p, then the draw.
 __device__ __noinline__ void finish_list(const SampleRowsArgs& a, int r, Shared& sm, const Scale& sc, int n, u64 k,
                                          float p, double goal, float low) {
     const int m = (int)min((u64)n, k), t = threadIdx.x;
-    // Two neighbours of the descending order a thread.
-    float e[2];
-    u64 w[2], key[2], total, mass;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int x = 2 * t + i;
-        key[i] = x < m ? sm.sorted[x] : 0;
-        e[i] = x < m ? sc.share(key_logit(key[i])) : 0.f;
-        w[i] = Scale::weight(e[i]);
-    }
-    const u64 before = block_scan(sm, w[0] + w[1], &mass);
+    // A key's owner is found again by its ranks: at most kList / kThreads keys a thread.
+    int2 ranks[kList / kThreads];
+    u64 w[kList / kThreads], key[kList / kThreads];
+    float e[kList / kThreads];
+    int mine = 0;
+    rank_list(sm, n, [&](int i, int2 x) {
+        key[mine] = sm.key[i];
+        e[mine] = sc.share(key_logit(key[mine]));
+        w[mine] = Scale::weight(e[mine]);
+        ranks[mine] = x;
+        sm.weight[x.x] = w[mine];
+        ++mine;
+    });
+    __syncthreads();
+    // Mass before each rank of the first m, two neighbouring ranks a thread.
+    const int x0 = 2 * t, x1 = 2 * t + 1;
+    const u64 w0 = x0 < m ? sm.weight[x0] : 0, w1 = x1 < m ? sm.weight[x1] : 0;
+    u64 mass, total;
+    const u64 before = block_scan(sm, w0 + w1, &mass);
     if (k != ~0ull) goal = (double)p * (double)mass;
+    if (x0 < n) sm.weight[x0] = before;
+    if (x1 < n) sm.weight[x1] = before + w0;
+    __syncthreads();
     unsigned kept = 0;
-    u64 sum = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int x = 2 * t + i;
-        const u64 ahead = before + (i ? w[0] : 0);
-        const bool in = x < m && (x == 0 || ((p >= 1.f || (double)ahead < goal) && e[i] >= low));
-        if (!in) w[i] = 0;
+    for (int i = 0; i < mine; ++i) {
+        const u64 ahead = sm.weight[ranks[i].x];
+        const bool in = ranks[i].x < m && (ranks[i].x == 0 || ((p >= 1.f || (double)ahead < goal) && e[i] >= low));
         kept += in;
-        sum += w[i];
-        if (x < m) sm.weight[x] = w[i];
+        if (!in) w[i] = 0;
     }
-    block_scan(sm, sum, &total);
-    u64 count;
-    block_scan(sm, kept, &count);  // its barriers also make sm.weight visible
+    __syncthreads();
+    for (int i = 0; i < mine; ++i) {
+        sm.weight[ranks[i].y] = w[i];
+        sm.named[ranks[i].y] = key[i];
+    }
+    const int count = __syncthreads_count(kept > 0) + __syncthreads_count(kept > 1);
+    const u64 v0 = x0 < n ? sm.weight[x0] : 0, v1 = x1 < n ? sm.weight[x1] : 0;
+    const u64 at = block_scan(sm, v0 + v1, &total);
     const u64 target = draw(a.uniform[r], total);
-#pragma unroll 1
-    for (int i = 0; i < 2; ++i) {
-        if (w[i] == 0) continue;
-        u64 below = 0;  // kept mass of lower indices
-        const u64 index = key[i] & kIndexMask;  // inverted: a lower index is larger
-#pragma unroll 4
-        for (int j = 0; j < m; ++j) below += (sm.sorted[j] & kIndexMask) > index ? sm.weight[j] : 0;
-        if (target >= below && target < below + w[i])
-            write(a, r, key_index(key[i]), e[i] / ((float)total * 9.094947017729282e-13f), (int)count);  // 2^-40
+    if (target >= at && target < at + v0 + v1) {
+        const u64 k1 = sm.named[target < at + v0 ? x0 : x1];
+        write(a, r, key_index(k1), sc.share(key_logit(k1)) / ((float)total * 9.094947017729282e-13f), count);  // 2^-40
     }
 }
+static_assert(kList == 2 * kThreads, "two list entries a thread");
 
 template <class T>
 __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs a) {
@@ -456,11 +526,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
                 if (!(static_cast<float>(row.data[at + i]) > -INFINITY)) row.data[at + i] = static_cast<T>(-INFINITY);
         }
     }
-    Pair all = row.block_sum(live, 0);
-    const u64 mine_live = all.a;
-    all = row.block_max(m > -INFINITY ? order_bits(m) : 0, 0);
+    const uint2 own = row.block_max_sum(m > -INFINITY ? order_bits(m) : 0, live);
     u64 top = 0, alive = 0;
-    row.exchange({all.a, mine_live}, [&](int, Pair x) { top = max(top, x.a), alive += x.b; });
+    row.exchange({own.x, own.y}, [&](int, Pair x) { top = max(top, x.a), alive += x.b; });
     const float t = a.temperature ? a.temperature[r] : 1.f;
     const bool lead = row.rank == 0 && tid == 0;
     if (top == 0) {
@@ -470,11 +538,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
     }
     m = from_order((unsigned)top);
     if (!(t > 0.f)) {
-        u64 first = 0;  // the lowest index that holds the maximum, inverted
+        unsigned first = 0;  // the lowest index that holds the maximum, inverted
         row.pass([&](float l, int index, int) {
-            if (l == m) first = max(first, (u64)(kIndexMask - index) + 1);
+            if (l == m) first = max(first, (unsigned)(kIndexMask - index) + 1);
         });
-        first = row.block_max(first, 0).a;
+        first = row.block_max_sum(first, 0).x;
         u64 best = 0;
         row.exchange({first, 0}, [&](int, Pair x) { best = max(best, x.a); });
         if (lead) write(a, r, kIndexMask + 1 - (int)best, 1.f, 1);
@@ -507,41 +575,48 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
         const int bin = row.cut_bin(by_mass, 0, goal);
         const u64 held = bin == kBins - 1 ? alive : sm.cum_count[bin];
         if (held <= kList) {
-            const int n = row.gather([&](float l) { return sc.bin(l) <= bin; });
+            const int n = row.gather([&](auto put) {
+                row.pass([&](float l, int index, int) {
+                    if (sc.bin(l) <= bin) put(l, index);
+                });
+            });
             if (row.rank != 0) return;  // nobody reads this block's memory any more
-            rank_list(sm, n);
             finish_list(a, r, sm, sc, n, k, p, goal, low);
             return;
         }
         const u64 ahead = bin ? (by_mass ? sm.cum_mass : sm.cum_count)[bin - 1] : 0;
+        const u64 in_bin = held - (bin ? sm.cum_count[bin - 1] : 0);
         __syncthreads();
         u64 key = 0;
         bool found = false;
         if (bin < kBins - 1) {  // the bin in 256 parts
+            row.set_aside(bin);
             Bins& s = row.clear();
-            row.pass([&](float l, int, int) {
-                if (sc.bin(l) == bin) Row<T>::add(s, sc.sub(l), by_mass ? Scale::weight(sc.share(l)) : 0, by_mass);
-            });
+            row.pass_aside([&](float l, int) { Row<T>::add(s, sc.sub(l), by_mass ? Scale::weight(sc.share(l)) : 0, by_mass); });
             row.merge(by_mass);
             const int part = row.cut_bin(by_mass, ahead, goal);
             const u64 lo = part ? sm.cum_count[part - 1] : 0, before = ahead + (part ? (by_mass ? sm.cum_mass : sm.cum_count)[part - 1] : 0);
-            if (sm.cum_count[part] - lo <= kList) {
-                const int n = row.gather([&](float l) { return sc.bin(l) == bin && sc.sub(l) == part; });
+            const u64 here = sm.cum_count[part] - lo;
+            if (sm.cum_count[kBins - 1] == in_bin && here <= kList) {  // no block had too many
+                const int n = row.gather([&](auto put) {
+                    row.pass_aside([&](float l, int index) {
+                        if (sc.sub(l) == part) put(l, index);
+                    });
+                });
                 if (row.rank == 0) {
-                    rank_list(sm, n);
-                    u64 w[2], whole;
-                    const u64 one = by_mass ? 0 : 1;
+                    rank_list(sm, n, [&](int i, int2 x) { sm.named[x.x] = sm.key[i]; });
+                    __syncthreads();
+                    u64 whole;
+                    u64 w[2], at = 0;  // two neighbours of the descending order
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int x = 2 * tid + i;
-                        w[i] = x < n ? (by_mass ? Scale::weight(sc.share(key_logit(sm.sorted[x]))) : one) : 0;
-                    }
-                    u64 at = before + block_scan(sm, w[0] + w[1], &whole);
+                    for (int i = 0; i < 2; ++i)
+                        w[i] = 2 * tid + i >= n ? 0 : by_mass ? Scale::weight(sc.share(key_logit(sm.named[2 * tid + i]))) : 1;
+                    at = before + block_scan(sm, w[0] + w[1], &whole);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         if (w[i] && (double)at < goal && !((double)(at + w[i]) < goal))
 #pragma unroll 1
-                            for (int c = 0; c < row.blocks; ++c) *row.cl.map_shared_rank(&sm.answer, c) = sm.sorted[2 * tid + i];
+                            for (int c = 0; c < row.blocks; ++c) *row.cl.map_shared_rank(&sm.answer, c) = sm.named[2 * tid + i];
                         at += w[i];
                     }
                 }
@@ -557,9 +632,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
             row.pass([&](float l, int index, int) {
                 if (key_of(l, index) >= from_key) mass += Scale::weight(sc.share(l));
             });
-            const Pair mine = row.block_sum(mass, 0);
+            const u64 mine = row.block_sum(mass);
             u64 sum = 0;
-            row.exchange(mine, [&](int, Pair x) { sum += x.a; });
+            row.exchange({mine, 0}, [&](int, Pair x) { sum += x.a; });
             goal = (double)p * (double)sum;
             from_key = max(from_key, row.search(true, goal, from_key));
         }
@@ -569,12 +644,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
     const float edge = from_key ? key_logit(from_key) : -INFINITY;
     const float far = low > 0.f ? (0.01f - logf(low)) * 8.f * 1.001f : INFINITY;  // bins past which no share reaches low
     const int edge_index = from_key ? key_index(from_key) : kIndexMask;
+    const bool some = from_key || low > 0.f;  // most entries are cut: skip their exponentials
     const auto weigh = [&](float l, int index, float& e) -> u64 {
-        if (l < edge || (l == edge && index > edge_index) || sc.place(l) > far) return ~0ull;
+        if (some && (l < edge || (l == edge && index > edge_index) || sc.place(l) > far)) return ~0ull;
         e = sc.share(l);
         return e >= low ? Scale::weight(e) : ~0ull;
     };
-    u64 count = 0;
+    unsigned count = 0;
 #pragma unroll 1
     for (int j = 0; j < kRounds; ++j) {
         const int at = 8 * (j * kThreads + tid);
@@ -582,21 +658,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
         if (j < row.rounds && at < row.n) {
             float v[8];
             read8(row.data + at, v);
+            if (!some) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (v[i] > -INFINITY) {
-                    float e;
-                    const u64 w = weigh(v[i], row.base + at + i, e);
-                    if (w != ~0ull) sum += w, ++count;
+                for (int i = 0; i < 8; ++i) {
+                    sum += Scale::weight(sc.share(v[i]));  // 0 for -inf
+                    count += v[i] > -INFINITY;
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (v[i] > -INFINITY) {
+                        float e;
+                        const u64 w = weigh(v[i], row.base + at + i, e);
+                        if (w != ~0ull) sum += w, ++count;
+                    }
+            }
         }
         sum = warp_sum64(sum);
         if (lane == 0) sm.part[j][warp] = sum;
     }
-    __syncthreads();
+    count = row.block_max_sum(0, count).y;  // its barriers also show the parts
     u64 slice = 0;
     if (tid < kRounds * kWarps) slice = sm.part[tid / kWarps][tid % kWarps];
-    const Pair mine = row.block_sum(slice, count);
+    const Pair mine{row.block_sum(slice), count};
     u64 total = 0, ahead = 0, kept = 0;
     row.exchange(mine, [&](int b, Pair x) {
         if (b < row.rank) ahead += x.a;

@@ -42,6 +42,7 @@
 #include "tree_attn.h"
 
 #include <algorithm>
+#include <cstddef>
 #include <cstring>
 
 namespace g4b {
@@ -100,6 +101,9 @@ struct alignas(16) Ctl {
     alignas(16) float inv[128];
     alignas(16) float red[4][128];
 };
+
+static_assert(offsetof(Ctl, corr) % 16 == 0 && offsetof(Ctl, inv) % 16 == 0 && alignof(Ctl) == 16,
+              "read in 16-byte pieces");
 
 // What a part's rows carry, twice: the next part's is set up before the current one is written out.
 struct Rows {
