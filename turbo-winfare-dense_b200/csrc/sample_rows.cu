@@ -15,7 +15,7 @@
 // descending order; this one has no bound on the kept entries, and measures top_p after the
 // temperature and top_k.
 //
-// A row is one cluster of 1 to 16 blocks. Each reads its slice of up to 16384 entries from memory
+// A row is one cluster of 1 to 16 blocks. Each reads its slice of up to 64 KB from memory
 // once, into shared memory, and passes over it there; blocks exchange through distributed shared
 // memory, one cluster barrier an exchange:
 //   * the maximum;
@@ -32,6 +32,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.cuh"
@@ -45,8 +46,8 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kSlice = 16384;               // entries a block holds
-constexpr int kRounds = kSlice / (8 * kThreads);  // a thread takes eight consecutive entries a round
+constexpr int kSliceBytes = 65536;          // of a row that a block holds: two blocks fit an SM
+constexpr int kRounds = kSliceBytes / 2 / (8 * kThreads);  // a thread takes eight consecutive entries a round
 constexpr int kIndexBits = 18;              // vocabularies up to 262144
 constexpr int kIndexMask = (1 << kIndexBits) - 1;
 constexpr int kBins = 256;
@@ -68,12 +69,12 @@ struct alignas(16) Shared {
     unsigned red32[2][kWarps];
     u64 part[kRounds][kWarps];
     u64 cum_count[kBins], cum_mass[kBins];
-    u64 key[kList];      // the list, in the first block
+    alignas(16) u64 key[kList + 2];  // the list, in the first block
     u64 weight[kList];   // by rank in the descending order, then by rank in index order
     u64 named[kList];    // keys by rank
     uint16_t cand[kCand];    // places in the slice of what is set aside
     u64 answer;
-    int bin, list, cands;
+    int bin, list, staged, place, cands;
 };
 
 static_assert(sizeof(Shared) % 16 == 0, "the slice behind it is read in 16-byte pieces");
@@ -107,13 +108,13 @@ __device__ __forceinline__ u64 warp_max64(u64 v) {
 
 // The row's numbers that turn a logit into a weight.
 struct Scale {
-    float m, t, r, bins;  // maximum, temperature, 1 / t, 8 / t
+    float m, t, r, bins;  // maximum, temperature, 1 / t, 32 / t
     bool inf, simple;
     __device__ void set(float max, float temperature) {
         m = max;
         t = temperature;
         r = 1.f / t;
-        bins = 8.f / t;
+        bins = 32.f / t;
         inf = m == INFINITY;
         // Out of this range the reciprocal or the remainder below could leave the normal numbers.
         simple = t > 1e-18f && t < 1e18f;
@@ -123,20 +124,27 @@ struct Scale {
     __device__ __forceinline__ float share(float l) const {
         if (inf) return l == m ? 1.f : 0.f;
         const float a = l - m;
-        float q = a * r;
-        if (simple) q = q > -200.f ? fmaf(fmaf(-q, t, a), r, q) : q;
+        float q = fmaxf(a * r, -200.f);  // below -104 the exponential is 0 either way
+        if (simple) q = fmaf(fmaf(-q, t, a), r, q);
         else q = a / t;
         return expf(q);
     }
     static __device__ __forceinline__ u64 weight(float share) { return (u64)(share * 1099511627776.f); }
-    // Bin of a live logit; bins are ordered as the logits are. +inf below +inf gives NaN, which
-    // converts to 0.
-    __device__ __forceinline__ float place(float l) const { return (m - l) * bins; }
-    __device__ __forceinline__ int bin(float l) const { return (int)fminf(place(l), 255.f); }
-    // Of 256 parts of its bin.
+    // Four times the bin of a logit, ordered as the logits are: the scaled distance from the maximum,
+    // made whole by adding 2^23 (which leaves it in the low bits) and cut to a multiple of four. -inf
+    // is in the last bin, as all that is far below; +inf below +inf gives NaN, which fminf drops.
+    __device__ __forceinline__ float place(float l) const { return (m - l) * bins; }  // in quarters of a bin
+    __device__ __forceinline__ unsigned bin4(float l) const {
+        const float x = inf && l == m ? 0.f : fminf(place(l), 1020.f);
+        return __float_as_uint(x + 8388608.f) & 0x3fcu;
+    }
+    __device__ __forceinline__ int bin(float l) const { return (int)(bin4(l) >> 2); }
+    // Cheap first test: a logit for which this is false is in a later bin.
+    __device__ __forceinline__ bool near(float l, int bin) const { return !(place(l) > (float)(4 * bin + 8)); }
+    // Which of 256 parts of its bin, from what the bin's rounding kept.
     __device__ __forceinline__ int sub(float l) const {
-        const float x = place(l);
-        return (int)fminf((x - floorf(x)) * 256.f, 255.f);
+        const float x = inf && l == m ? 0.f : place(l);
+        return (int)fminf(fmaxf((x - (float)bin4(l) + 0.5f) * 64.f, 0.f), 255.f);
     }
 };
 
@@ -153,6 +161,30 @@ __device__ __forceinline__ void read8(const T* at, float (&v)[8]) {
     }
 }
 
+// Least and largest of eight values; the least is NaN where one of them is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+template <class T>
+__device__ __forceinline__ void extremes8(const T* at, float& least, float& most) {
+    if constexpr (sizeof(T) == 4) {
+        float v[8];
+        read8(at, v);
+        least = min_nan(min_nan(min_nan(v[0], v[1]), min_nan(v[2], v[3])), min_nan(min_nan(v[4], v[5]), min_nan(v[6], v[7])));
+        most = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+    } else {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        const uint4 a = *reinterpret_cast<const uint4*>(at);
+        const T2* h = reinterpret_cast<const T2*>(&a);
+        const T2 lo = __hmin2_nan(__hmin2_nan(h[0], h[1]), __hmin2_nan(h[2], h[3]));
+        const T2 hi = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        least = min_nan(static_cast<float>(lo.x), static_cast<float>(lo.y));
+        most = fmaxf(static_cast<float>(hi.x), static_cast<float>(hi.y));
+    }
+}
+
 // One row of one cluster.
 template <class T>
 struct Row {
@@ -166,9 +198,19 @@ struct Row {
         blocks = (int)cl.num_blocks();
         rank = (int)cl.block_rank();
     }
+    // All blocks' writes before it are seen by all after it. The block meets first, so that one warp's
+    // release stands for all threads' writes, and the other warps need not wait for theirs.
     __device__ __forceinline__ void barrier() {
-        if (blocks > 1) cl.sync();
-        else __syncthreads();
+        __syncthreads();
+        if (blocks == 1) return;
+        if (threadIdx.x < 32) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        else asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    // No block leaves while its shared memory is read.
+    __device__ __forceinline__ void leave() {
+        if (blocks == 1) return;
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     // each(l, index, round) for this thread's live entries in index order within a round.
     template <class Each>
@@ -182,6 +224,39 @@ struct Row {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (v[i] > -INFINITY) each(v[i], base + at + i, j);
+        }
+    }
+    // As pass, for all entries, dead ones (and the padding) among them.
+    template <class Each>
+    __device__ __forceinline__ void pass_all(Each each) const {
+#pragma unroll 1
+        for (int j = 0; j < rounds; ++j) {
+            const int at = 8 * (j * kThreads + (int)threadIdx.x);
+            if (at >= n) continue;
+            float v[8];
+            read8(data + at, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) each(v[i], base + at + i);
+        }
+    }
+    // each(l, index) for the few entries that test(l) holds for: the tests of eight entries make one
+    // mask and one branch.
+    template <class Test, class Each>
+    __device__ __forceinline__ void pass_few(Test test, Each each) const {
+#pragma unroll 1
+        for (int j = 0; j < rounds; ++j) {
+            const int at = 8 * (j * kThreads + (int)threadIdx.x);
+            if (at >= n) continue;
+            float v[8];
+            read8(data + at, v);
+            unsigned hits = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) hits |= test(v[i]) ? 1u << i : 0u;
+#pragma unroll 1
+            for (; hits; hits &= hits - 1) {
+                const int i = __ffs(hits) - 1;
+                each(static_cast<float>(data[at + i]), base + at + i);
+            }
         }
     }
     // The block's largest a and sum of b.
@@ -294,17 +369,24 @@ struct Row {
     }
 
     // Entries that each(put) passes to put(l, index) go to the first block's list; their number is
-    // returned there (the others must not use theirs). At most kList of them in the cluster.
+    // returned there (the others must not use theirs). At most kList of them in the cluster. A block
+    // collects its own first and reserves their places at once.
     template <class Each>
     __device__ int gather(Each each) {
-        if (threadIdx.x == 0 && rank == 0) sm.list = 0;
+        if (threadIdx.x == 0) sm.staged = sm.list = 0;
         barrier();
-        int* count = cl.map_shared_rank(&sm.list, 0);
-        u64* list = cl.map_shared_rank(sm.key, 0);
         each([&](float l, int index) {
-            const int at = atomicAdd(count, 1);
-            if (at < kList) list[at] = key_of(l, index);
+            const int at = atomicAdd(&sm.staged, 1);
+            if (at < kList) sm.named[at] = key_of(l, index);
         });
+        __syncthreads();
+        const int mine = min(sm.staged, kList);
+        if (threadIdx.x == 0 && mine) sm.place = atomicAdd(cl.map_shared_rank(&sm.list, 0), mine);
+        __syncthreads();
+        u64* list = cl.map_shared_rank(sm.key, 0);
+        const int first = sm.place;
+        for (int i = threadIdx.x; i < mine; i += kThreads)
+            if (first + i < kList) list[first + i] = sm.named[i];
         barrier();
         return min(sm.list, kList);
     }
@@ -312,11 +394,9 @@ struct Row {
     __device__ void set_aside(int bin) {
         if (threadIdx.x == 0) sm.cands = 0;
         __syncthreads();
-        pass([&](float l, int index, int) {
-            if (sc.bin(l) == bin) {
-                const int at = atomicAdd(&sm.cands, 1);
-                if (at < kCand) sm.cand[at] = (uint16_t)(index - base);
-            }
+        pass_few([&](float l) { return sc.bin4(l) == 4u * bin; }, [&](float l, int index) {
+            const int at = atomicAdd(&sm.cands, 1);
+            if (at < kCand) sm.cand[at] = (uint16_t)(index - base);
         });
         __syncthreads();
     }
@@ -402,7 +482,9 @@ __device__ u64 block_scan(Shared& sm, u64 v, u64* total) {
 // Ranks of a key among the list's n, in descending order of keys (x) and in index order (y). Few
 // keys have several neighbouring threads each; each(i, ranks) runs in one of them. All threads come.
 template <class Each>
-__device__ __forceinline__ void rank_list(const Shared& sm, int n, Each each) {
+__device__ __forceinline__ void rank_list(Shared& sm, int n, Each each) {
+    if (threadIdx.x == 0 && (n & 1)) sm.key[n] = 0;
+    __syncthreads();
     int share = 1;  // threads a key
     while (share < 32 && 2 * share * n <= kThreads) share *= 2;
     const int part = threadIdx.x % share, step = kThreads / share;
@@ -411,11 +493,12 @@ __device__ __forceinline__ void rank_list(const Shared& sm, int n, Each each) {
         const int i = i0 + threadIdx.x / share;
         const u64 mine = i < n ? sm.key[i] : 0;
         int2 r{0, 0};
+        // Two keys a load; the list ends in zeros, which rank behind every key in either order.
 #pragma unroll 4
-        for (int j = part; j < n; j += share) {
-            const u64 k = sm.key[j];
-            r.x += k > mine;
-            r.y += (unsigned)(k & kIndexMask) > (unsigned)(mine & kIndexMask);  // inverted indices
+        for (int j = 2 * part; j < n; j += 2 * share) {
+            const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&sm.key[j]);
+            r.x += (k.x > mine) + (k.y > mine);
+            r.y += ((unsigned)(k.x & kIndexMask) > (unsigned)(mine & kIndexMask)) + ((unsigned)(k.y & kIndexMask) > (unsigned)(mine & kIndexMask));
         }
         for (int o = share >> 1; o > 0; o >>= 1) {
             r.x += __shfl_xor_sync(0xffffffffu, r.x, o);
@@ -504,26 +587,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
     if (tid < ((row.n + 7) & ~7) - row.n) row.data[row.n + tid] = static_cast<T>(-INFINITY);
     __syncthreads();
 
-    // The maximum and the number of live entries; NaN becomes -inf on the way.
+    // The maximum and the number of live entries. Eights with a NaN or -inf among them (their least
+    // says so) are looked at one by one, and NaN becomes -inf.
     float m = -INFINITY;
     unsigned live = 0;
-    bool nan = false;
 #pragma unroll 1
     for (int j = 0; j < row.rounds; ++j) {
         const int at = 8 * (j * kThreads + tid);
         if (at >= row.n) continue;
-        float v[8];
-        read8(row.data + at, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            m = fmaxf(m, v[i]);
-            live += v[i] > -INFINITY;
-            nan |= v[i] != v[i];
-        }
-        if (nan) {
+        float least, most;
+        extremes8(row.data + at, least, most);
+        if (least > -INFINITY) {
+            m = fmaxf(m, most);
+            live += 8;
+        } else {
 #pragma unroll 1
-            for (int i = 0; i < 8; ++i)
-                if (!(static_cast<float>(row.data[at + i]) > -INFINITY)) row.data[at + i] = static_cast<T>(-INFINITY);
+            for (int i = 0; i < 8; ++i) {
+                const float v = static_cast<float>(row.data[at + i]);
+                if (v > -INFINITY) m = fmaxf(m, v), ++live;
+                else row.data[at + i] = static_cast<T>(-INFINITY);
+            }
         }
     }
     const uint2 own = row.block_max_sum(m > -INFINITY ? order_bits(m) : 0, live);
@@ -533,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
     const bool lead = row.rank == 0 && tid == 0;
     if (top == 0) {
         if (lead) write(a, r, -1, 0.f, 0);
-        row.barrier();  // no block leaves while its shared memory is read
+        row.leave();
         return;
     }
     m = from_order((unsigned)top);
@@ -546,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
         u64 best = 0;
         row.exchange({first, 0}, [&](int, Pair x) { best = max(best, x.a); });
         if (lead) write(a, r, kIndexMask + 1 - (int)best, 1.f, 1);
-        row.barrier();
+        row.leave();
         return;
     }
     row.sc.set(m, t);
@@ -562,13 +645,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
     u64 from_key = 0;  // the last kept key, as far as it is known
     if (k != ~0ull || by_mass) {
         Bins& b = row.clear();
+        // The last bin is not counted, and has no mass: it holds what the others do not.
         if (by_mass)
-            row.pass([&](float l, int, int) { Row<T>::add(b, sc.bin(l), Scale::weight(sc.share(l)), true); });
+            row.pass_all([&](float l, int) {
+                const unsigned at = sc.bin4(l);
+                if (at == 4 * (kBins - 1)) return;
+                const u64 w = Scale::weight(sc.share(l));
+                char* c = reinterpret_cast<char*>(&b) + at;
+                atomicAdd(reinterpret_cast<unsigned*>(c), 1u);
+                atomicAdd(reinterpret_cast<unsigned*>(c + sizeof(b.count)), (unsigned)w & 0xffff);
+                atomicAdd(reinterpret_cast<unsigned*>(c + 2 * sizeof(b.count)), (unsigned)w >> 16);
+                if (w >> 32) atomicAdd(reinterpret_cast<unsigned*>(c + 3 * sizeof(b.count)), (unsigned)(w >> 32));
+            });
         else
-            row.pass([&](float l, int, int) {
-                // The last bin is not counted: it holds what the others do not.
-                const int x = sc.bin(l);
-                if (x < kBins - 1) atomicAdd(&b.count[x], 1u);
+            row.pass_all([&](float l, int) {
+                const unsigned at = sc.bin4(l);
+                if (at < 4 * (kBins - 1)) atomicAdd(reinterpret_cast<unsigned*>(reinterpret_cast<char*>(&b) + at), 1u);
             });
         row.merge(by_mass);
         double goal = by_mass ? (double)p * (double)sm.cum_mass[kBins - 1] : (double)k;
@@ -576,8 +668,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
         const u64 held = bin == kBins - 1 ? alive : sm.cum_count[bin];
         if (held <= kList) {
             const int n = row.gather([&](auto put) {
-                row.pass([&](float l, int index, int) {
-                    if (sc.bin(l) <= bin) put(l, index);
+                row.pass_few([&](float l) { return sc.near(l, bin); }, [&](float l, int index) {
+                    if (sc.bin(l) <= bin && l > -INFINITY) put(l, index);
                 });
             });
             if (row.rank != 0) return;  // nobody reads this block's memory any more
@@ -642,7 +734,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
 
     // Kept mass in index order: per (round, warp), then block by block.
     const float edge = from_key ? key_logit(from_key) : -INFINITY;
-    const float far = low > 0.f ? (0.01f - logf(low)) * 8.f * 1.001f : INFINITY;  // bins past which no share reaches low
+    const float far = low > 0.f ? (0.01f - logf(low)) * 32.f * 1.001f : INFINITY;  // places past which no share reaches low
     const int edge_index = from_key ? key_index(from_key) : kIndexMask;
     const bool some = from_key || low > 0.f;  // most entries are cut: skip their exponentials
     const auto weigh = [&](float l, int index, float& e) -> u64 {
@@ -652,10 +744,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
     };
     unsigned count = 0;
 #pragma unroll 1
-    for (int j = 0; j < kRounds; ++j) {
+    for (int j = 0; j < row.rounds; ++j) {
         const int at = 8 * (j * kThreads + tid);
         u64 sum = 0;
-        if (j < row.rounds && at < row.n) {
+        if (at < row.n) {
             float v[8];
             read8(row.data + at, v);
             if (!some) {
@@ -665,13 +757,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
                     count += v[i] > -INFINITY;
                 }
             } else {
+                unsigned hits = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (v[i] > -INFINITY) {
-                        float e;
-                        const u64 w = weigh(v[i], row.base + at + i, e);
-                        if (w != ~0ull) sum += w, ++count;
-                    }
+                for (int i = 0; i < 8; ++i) hits |= v[i] >= edge && v[i] > -INFINITY && !(sc.place(v[i]) > far) ? 1u << i : 0u;
+#pragma unroll 1
+                for (; hits; hits &= hits - 1) {
+                    const int i = __ffs(hits) - 1;
+                    float e;
+                    const u64 w = weigh(static_cast<float>(row.data[at + i]), row.base + at + i, e);
+                    if (w != ~0ull) sum += w, ++count;
+                }
             }
         }
         sum = warp_sum64(sum);
@@ -679,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
     }
     count = row.block_max_sum(0, count).y;  // its barriers also show the parts
     u64 slice = 0;
-    if (tid < kRounds * kWarps) slice = sm.part[tid / kWarps][tid % kWarps];
+    if (tid < row.rounds * kWarps) slice = sm.part[0][tid];
     const Pair mine{row.block_sum(slice), count};
     u64 total = 0, ahead = 0, kept = 0;
     row.exchange(mine, [&](int b, Pair x) {
@@ -687,24 +782,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
         total += x.a;
         kept += x.b;
     });
-    row.barrier();  // no block leaves while its shared memory is read
+    row.leave();
     u64 goal = draw(a.uniform[r], total);
     if (goal < ahead || goal >= ahead + mine.a) return;
     goal -= ahead;
-    // The (round, warp) part that holds it: one warp looks, 64 parts in two.
+    // The (round, warp) part that holds it: one warp looks, four parts a lane.
     if (warp == 0) {
-        const u64 w0 = sm.part[0][2 * lane], w1 = sm.part[0][2 * lane + 1];
-        u64 x = w0 + w1;
+        u64 w[4], x = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = 4 * lane + i < row.rounds * kWarps ? sm.part[0][4 * lane + i] : 0;
+            x += w[i];
+        }
+        u64 at = x;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const u64 y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        const u64 at = x - w0 - w1;
-        if (goal >= at && goal < x) {
-            const int second = goal >= at + w0;
-            sm.bin = 2 * lane + second;
-            sm.answer = goal - at - (second ? w0 : 0);
+        at = x - at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (goal >= at && goal < at + w[i]) {
+                sm.bin = 4 * lane + i;
+                sm.answer = goal - at;
+            }
+            at += w[i];
         }
         __syncwarp();
         const int j = sm.bin / kWarps, at8 = 8 * (j * kThreads + (sm.bin % kWarps) * 32 + lane);
@@ -740,13 +843,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
             }
     }
 }
-static_assert(kRounds * kWarps == 64, "the last search looks at 64 parts");
+static_assert(kRounds * kWarps == 128, "the last search looks at 128 parts");
 
 template <class T>
 cudaError_t run(const SampleRowsArgs& a, cudaStream_t st) {
+    // As few blocks a row as hold it, so that a row's barriers weigh little; more, down to 4096 entries
+    // each, while all rows' blocks are resident at once: then latency counts.
     int blocks = 1;
-    while (blocks * kSlice < a.vocab) blocks *= 2;
-    const int per = ((a.vocab + blocks - 1) / blocks + 7) & ~7;
+    const auto span = [&](int n) { return ((a.vocab + n - 1) / n + 7) & ~7; };
+    while (span(blocks) * sizeof(T) > kSliceBytes) blocks *= 2;
+    while (blocks < 16 && span(blocks) > 4096 && 2ll * a.rows * blocks <= 2 * 148) blocks *= 2;
+    const int per = span(blocks);
     const size_t smem = sizeof(Shared) + (size_t)per * sizeof(T);
     auto kern = sample_rows_kernel<T>;
     static bool attr = false;
@@ -754,7 +861,7 @@ cudaError_t run(const SampleRowsArgs& a, cudaStream_t st) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)(sizeof(Shared) + kSlice * sizeof(T)));
+                                     (int)(sizeof(Shared) + kSliceBytes));
         if (e != cudaSuccess) return e;
         attr = true;
     }
