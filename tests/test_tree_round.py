@@ -147,6 +147,37 @@ def test_sample_rows_special_values(built_lib):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [900, 40000, 262144])
+def test_sample_rows_wide_cuts(built_lib, vocab):
+    """Cuts that leave thousands of entries, by number and by mass, in rows with and without ties, and
+    cuts that fall far below the maximum (where most entries share the last histogram bin)."""
+    import torch
+    g = torch.Generator().manual_seed(vocab + 1)
+    settings = [(1.0, vocab // 2, 1.0, 0.0), (1.0, vocab // 3, 0.5, 0.0), (0.02, vocab // 2, 1.0, 0.0), (1.0, 0, 0.5, 0.0),
+                (4.0, 0, 0.9, 0.0), (0.01, 500, 1.0, 0.0), (50.0, 700, 0.7, 0.0), (1.0, vocab - 1, 0.999, 0.001)]
+    for kind in (torch.float32, torch.bfloat16):
+        x = (torch.randn(len(settings), vocab, generator=g) * 2).to(kind)
+        x[6] = torch.round(x[6].float() / 3).to(kind)  # ties by the thousand
+        u = torch.rand(len(settings), generator=g).tolist()
+        t, k, p, low = zip(*settings)
+        token, prob, kept = sample(x.cuda(), u, temperature=t, top_k=k, top_p=p, min_p=low)
+        for r in range(len(settings)):
+            check_row(x[r].double().numpy(), u[r], t[r], k[r], p[r], low[r], token[r], prob[r], kept[r])
+
+
+@pytest.mark.gpu
+def test_sample_rows_split_does_not_matter(built_lib):
+    """A row alone is spread over more blocks than among many: the same token, share and count."""
+    import torch
+    g = torch.Generator().manual_seed(5)
+    x = (torch.randn(1, 100000, generator=g) * 2).cuda()
+    for kw in (dict(top_p=0.97), dict(top_k=50), dict(top_k=3000, top_p=0.8), dict(min_p=0.01), dict()):
+        one = sample(x, [0.37], **{k: [v] for k, v in kw.items()})
+        many = sample(x.repeat(300, 1), [0.37] * 300, **{k: [v] * 300 for k, v in kw.items()})
+        assert all(set(m) == set(o) for m, o in zip(many, one)), kw
+
+
+@pytest.mark.gpu
 def test_sample_rows_frequencies(built_lib):
     """Evenly spaced uniform numbers hit each kept entry as often as its probability says."""
     import torch

@@ -70,11 +70,11 @@ struct alignas(16) Shared {
     u64 part[kRounds][kWarps];
     u64 cum_count[kBins], cum_mass[kBins];
     alignas(16) u64 key[kList + 2];  // the list, in the first block
-    u64 weight[kList];   // by rank in the descending order, then by rank in index order
-    u64 named[kList];    // keys by rank
+    u64 weight[kThreads];  // kept masses by index
+    u64 named[kList];      // the list sorted
     uint16_t cand[kCand];    // places in the slice of what is set aside
     u64 answer;
-    int bin, list, staged, place, cands;
+    int bin, staged, cands;
 };
 
 static_assert(sizeof(Shared) % 16 == 0, "the slice behind it is read in 16-byte pieces");
@@ -139,8 +139,10 @@ struct Scale {
         return __float_as_uint(x + 8388608.f) & 0x3fcu;
     }
     __device__ __forceinline__ int bin(float l) const { return (int)(bin4(l) >> 2); }
-    // Cheap first test: a logit for which this is false is in a later bin.
-    __device__ __forceinline__ bool near(float l, int bin) const { return !(place(l) > (float)(4 * bin + 8)); }
+    // Cheap first test: a logit for which this is false is in a later bin (the last has none).
+    __device__ __forceinline__ bool near(float l, int bin) const {
+        return !(place(l) > (bin < kBins - 1 ? (float)(4 * bin + 8) : INFINITY));
+    }
     // Which of 256 parts of its bin, from what the bin's rounding kept.
     __device__ __forceinline__ int sub(float l) const {
         const float x = inf && l == m ? 0.f : place(l);
@@ -206,11 +208,6 @@ struct Row {
         if (threadIdx.x < 32) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         else asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    }
-    // No block leaves while its shared memory is read.
-    __device__ __forceinline__ void leave() {
-        if (blocks == 1) return;
-        asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     // each(l, index, round) for this thread's live entries in index order within a round.
     template <class Each>
@@ -368,27 +365,26 @@ struct Row {
         return sm.bin;
     }
 
-    // Entries that each(put) passes to put(l, index) go to the first block's list; their number is
-    // returned there (the others must not use theirs). At most kList of them in the cluster. A block
-    // collects its own first and reserves their places at once.
+    // Entries that each(put) passes to put(l, index) go to the first block's list, block by block. Their
+    // number in the cluster is returned; over kList of them are not listed.
     template <class Each>
     __device__ int gather(Each each) {
-        if (threadIdx.x == 0) sm.staged = sm.list = 0;
-        barrier();
+        if (threadIdx.x == 0) sm.staged = 0;
+        __syncthreads();
         each([&](float l, int index) {
             const int at = atomicAdd(&sm.staged, 1);
             if (at < kList) sm.named[at] = key_of(l, index);
         });
         __syncthreads();
-        const int mine = min(sm.staged, kList);
-        if (threadIdx.x == 0 && mine) sm.place = atomicAdd(cl.map_shared_rank(&sm.list, 0), mine);
-        __syncthreads();
-        u64* list = cl.map_shared_rank(sm.key, 0);
-        const int first = sm.place;
-        for (int i = threadIdx.x; i < mine; i += kThreads)
-            if (first + i < kList) list[first + i] = sm.named[i];
+        const int mine = sm.staged;
+        int first = 0, all = 0;
+        exchange({(u64)mine, 0}, [&](int b, Pair x) { first += b < rank ? (int)x.a : 0, all += (int)x.a; });
+        if (all <= kList) {
+            u64* list = cl.map_shared_rank(sm.key, 0);
+            for (int i = threadIdx.x; i < mine; i += kThreads) list[first + i] = sm.named[i];
+        }
         barrier();
-        return min(sm.list, kList);
+        return all;
     }
     // Sets a bin's entries aside, in the order they come; at most kCand of them.
     __device__ void set_aside(int bin) {
@@ -479,97 +475,105 @@ __device__ u64 block_scan(Shared& sm, u64 v, u64* total) {
     return ahead + x - v;
 }
 
-// Ranks of a key among the list's n, in descending order of keys (x) and in index order (y). Few
-// keys have several neighbouring threads each; each(i, ranks) runs in one of them. All threads come.
-template <class Each>
-__device__ __forceinline__ void rank_list(Shared& sm, int n, Each each) {
-    if (threadIdx.x == 0 && (n & 1)) sm.key[n] = 0;
-    __syncthreads();
-    int share = 1;  // threads a key
-    while (share < 32 && 2 * share * n <= kThreads) share *= 2;
-    const int part = threadIdx.x % share, step = kThreads / share;
-#pragma unroll 1
-    for (int i0 = 0; i0 < n; i0 += step) {
-        const int i = i0 + threadIdx.x / share;
+// Puts the list's n keys into sm.named in descending order. Up to 256 keys are ranked, each against
+// all (few keys have several neighbouring threads each); more go through a bitonic network, whose
+// steps cost a barrier each but no n^2.
+__device__ __noinline__ void sort_list(Shared& sm, int n) {
+    const int t = threadIdx.x;
+    if (n <= 256) {
+        if (t == 0) sm.key[n] = 0;  // keys are loaded in pairs
+        __syncthreads();
+        int share = 2;  // threads a key
+        while (share < 32 && 2 * share * n <= kThreads) share *= 2;
+        const int part = t % share, i = t / share;
         const u64 mine = i < n ? sm.key[i] : 0;
-        int2 r{0, 0};
-        // Two keys a load; the list ends in zeros, which rank behind every key in either order.
+        int rank = 0;
 #pragma unroll 4
         for (int j = 2 * part; j < n; j += 2 * share) {
             const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&sm.key[j]);
-            r.x += (k.x > mine) + (k.y > mine);
-            r.y += ((unsigned)(k.x & kIndexMask) > (unsigned)(mine & kIndexMask)) + ((unsigned)(k.y & kIndexMask) > (unsigned)(mine & kIndexMask));
+            rank += (k.x > mine) + (k.y > mine);
         }
-        for (int o = share >> 1; o > 0; o >>= 1) {
-            r.x += __shfl_xor_sync(0xffffffffu, r.x, o);
-            r.y += __shfl_xor_sync(0xffffffffu, r.y, o);
-        }
-        if (i < n && part == 0) each(i, r);
+        for (int o = share >> 1; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        if (i < n && part == 0) sm.named[rank] = mine;
+    } else {
+        const int size = n <= 512 ? 512 : kList;
+        for (int i = n + t; i < size; i += kThreads) sm.key[i] = 0;
+        for (int k = 2; k <= size; k <<= 1)
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                __syncthreads();
+                if (t < size / 2) {
+                    const int i = 2 * t - (t & (j - 1)), o = i + j;  // the t-th pair j apart
+                    const u64 x = sm.key[i], y = sm.key[o];
+                    if ((i & k) == 0 ? x < y : x > y) sm.key[i] = y, sm.key[o] = x;
+                }
+            }
+        __syncthreads();
+        for (int i = t; i < n; i += kThreads) sm.named[i] = sm.key[i];
     }
+    __syncthreads();
 }
+static_assert(kThreads == 2 * 256 && kList == 2 * kThreads, "two threads a ranked key, a thread a sorted pair");
 
 // The end of a row whose list (in the first block) holds every entry that may be kept: the first k
 // of it, then the cuts by mass and by min-p, then the draw.
 __device__ __noinline__ void finish_list(const SampleRowsArgs& a, int r, Shared& sm, const Scale& sc, int n, u64 k,
                                          float p, double goal, float low) {
+    sort_list(sm, n);
     const int m = (int)min((u64)n, k), t = threadIdx.x;
-    // A key's owner is found again by its ranks: at most kList / kThreads keys a thread.
-    int2 ranks[kList / kThreads];
-    u64 w[kList / kThreads], key[kList / kThreads];
-    float e[kList / kThreads];
-    int mine = 0;
-    rank_list(sm, n, [&](int i, int2 x) {
-        key[mine] = sm.key[i];
-        e[mine] = sc.share(key_logit(key[mine]));
-        w[mine] = Scale::weight(e[mine]);
-        ranks[mine] = x;
-        sm.weight[x.x] = w[mine];
-        ++mine;
-    });
-    __syncthreads();
-    // Mass before each rank of the first m, two neighbouring ranks a thread.
-    const int x0 = 2 * t, x1 = 2 * t + 1;
-    const u64 w0 = x0 < m ? sm.weight[x0] : 0, w1 = x1 < m ? sm.weight[x1] : 0;
-    u64 mass, total;
-    const u64 before = block_scan(sm, w0 + w1, &mass);
+    // Two neighbours of the descending order a thread.
+    u64 key[2], w[2], mass, total;
+    float e[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        key[i] = 2 * t + i < m ? sm.named[2 * t + i] : 0;
+        e[i] = 2 * t + i < m ? sc.share(key_logit(key[i])) : 0.f;
+        w[i] = Scale::weight(e[i]);
+    }
+    const u64 before = block_scan(sm, w[0] + w[1], &mass);
     if (k != ~0ull) goal = (double)p * (double)mass;
-    if (x0 < n) sm.weight[x0] = before;
-    if (x1 < n) sm.weight[x1] = before + w0;
+    sm.weight[t] = 0;
+    if (t == 0) sm.staged = 0;
     __syncthreads();
-    unsigned kept = 0;
-    for (int i = 0; i < mine; ++i) {
-        const u64 ahead = sm.weight[ranks[i].x];
-        const bool in = ranks[i].x < m && (ranks[i].x == 0 || ((p >= 1.f || (double)ahead < goal) && e[i] >= low));
-        kept += in;
-        if (!in) w[i] = 0;
+    // The draw goes in index order: kept masses by the index's upper half, a thread a bucket of 512.
+    bool in[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int x = 2 * t + i;
+        const u64 ahead = before + (i ? w[0] : 0);
+        in[i] = x < m && (x == 0 || ((p >= 1.f || (double)ahead < goal) && e[i] >= low));
+        if (in[i]) atomicAdd(&sm.weight[key_index(key[i]) >> 9], w[i]);
     }
-    __syncthreads();
-    for (int i = 0; i < mine; ++i) {
-        sm.weight[ranks[i].y] = w[i];
-        sm.named[ranks[i].y] = key[i];
-    }
-    const int count = __syncthreads_count(kept > 0) + __syncthreads_count(kept > 1);
-    const u64 v0 = x0 < n ? sm.weight[x0] : 0, v1 = x1 < n ? sm.weight[x1] : 0;
-    const u64 at = block_scan(sm, v0 + v1, &total);
+    const int kept = __syncthreads_count(in[0]) + __syncthreads_count(in[1]);
+    const u64 bucket = sm.weight[t], at = block_scan(sm, bucket, &total);
     const u64 target = draw(a.uniform[r], total);
-    if (target >= at && target < at + v0 + v1) {
-        const u64 k1 = sm.named[target < at + v0 ? x0 : x1];
-        write(a, r, key_index(k1), sc.share(key_logit(k1)) / ((float)total * 9.094947017729282e-13f), count);  // 2^-40
+    if (target >= at && target < at + bucket) {
+        sm.bin = t;
+        sm.answer = target - at;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (in[i] && key_index(key[i]) >> 9 == sm.bin) {  // that bucket's entries
+            const int x = atomicAdd(&sm.staged, 1);
+            sm.key[x] = key[i];
+            sm.named[x] = w[i];
+        }
+    __syncthreads();
+    const int c = sm.staged;
+    for (int i = t; i < c; i += kThreads) {
+        const u64 mine = sm.key[i];
+        u64 below = 0;
+        for (int j = 0; j < c; ++j) below += key_index(sm.key[j]) < key_index(mine) ? sm.named[j] : 0;
+        if (sm.answer >= below && sm.answer < below + sm.named[i])
+            write(a, r, key_index(mine), sc.share(key_logit(mine)) / ((float)total * 9.094947017729282e-13f), kept);  // 2^-40
     }
 }
-static_assert(kList == 2 * kThreads, "two list entries a thread");
+static_assert((kIndexMask >> 9) + 1 == kThreads, "a thread a bucket");
 
 template <class T>
-__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs a) {
-    extern __shared__ __align__(16) unsigned char raw[];
-    Shared& sm = *reinterpret_cast<Shared*>(raw);
-    Row<T> row(sm, reinterpret_cast<T*>(raw + sizeof(Shared)));
-    const int r = blockIdx.x / row.blocks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__device__ __forceinline__ void sample_row(const SampleRowsArgs& a, Shared& sm, Row<T>& row, int r) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const T* in = static_cast<const T*>(a.logits) + r * a.stride;
-    const int per = ((a.vocab + row.blocks - 1) / row.blocks + 7) & ~7;
-    row.base = row.rank * per;
-    row.n = max(0, min(per, a.vocab - row.base));
-    row.rounds = (row.n + 8 * kThreads - 1) / (8 * kThreads);
     const T* from = in + row.base;
     constexpr int kWide = 16 / sizeof(T);
     if (reinterpret_cast<uintptr_t>(from) % 16 == 0) {
@@ -609,6 +613,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
             }
         }
     }
+    const float own_max = m;
     const uint2 own = row.block_max_sum(m > -INFINITY ? order_bits(m) : 0, live);
     u64 top = 0, alive = 0;
     row.exchange({own.x, own.y}, [&](int, Pair x) { top = max(top, x.a), alive += x.b; });
@@ -616,7 +621,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
     const bool lead = row.rank == 0 && tid == 0;
     if (top == 0) {
         if (lead) write(a, r, -1, 0.f, 0);
-        row.leave();
         return;
     }
     m = from_order((unsigned)top);
@@ -629,7 +633,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
         u64 best = 0;
         row.exchange({first, 0}, [&](int, Pair x) { best = max(best, x.a); });
         if (lead) write(a, r, kIndexMask + 1 - (int)best, 1.f, 1);
-        row.leave();
         return;
     }
     row.sc.set(m, t);
@@ -644,6 +647,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
 
     u64 from_key = 0;  // the last kept key, as far as it is known
     if (k != ~0ull || by_mass) {
+        // Few entries: the k-th largest of the threads' own maxima is at most the k-th largest entry, so
+        // its bin bounds a list without a count of all entries.
+        if (!by_mass && k <= kList / 2 && k <= (u64)row.blocks * kThreads / 2) {
+            Bins& b = row.clear();
+            if (own_max > -INFINITY) atomicAdd(&b.count[sc.bin(own_max)], 1u);
+            row.merge(false);
+            const int bin = row.cut_bin(false, 0, (double)k);
+            const int n = row.gather([&](auto put) {
+                row.pass_few([&](float l) { return sc.near(l, bin); }, [&](float l, int index) {
+                    if (sc.bin(l) <= bin && l > -INFINITY) put(l, index);
+                });
+            });
+            if (n <= kList) {
+                if (row.rank == 0) finish_list(a, r, sm, sc, n, k, p, 0.0, low);
+                return;
+            }
+        }
         Bins& b = row.clear();
         // The last bin is not counted, and has no mass: it holds what the others do not.
         if (by_mass)
@@ -672,8 +692,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
                     if (sc.bin(l) <= bin && l > -INFINITY) put(l, index);
                 });
             });
-            if (row.rank != 0) return;  // nobody reads this block's memory any more
-            finish_list(a, r, sm, sc, n, k, p, goal, low);
+            if (row.rank == 0) finish_list(a, r, sm, sc, n, k, p, goal, low);
             return;
         }
         const u64 ahead = bin ? (by_mass ? sm.cum_mass : sm.cum_count)[bin - 1] : 0;
@@ -696,8 +715,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
                     });
                 });
                 if (row.rank == 0) {
-                    rank_list(sm, n, [&](int i, int2 x) { sm.named[x.x] = sm.key[i]; });
-                    __syncthreads();
+                    sort_list(sm, n);
                     u64 whole;
                     u64 w[2], at = 0;  // two neighbours of the descending order
 #pragma unroll
@@ -782,7 +800,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
         total += x.a;
         kept += x.b;
     });
-    row.leave();
     u64 goal = draw(a.uniform[r], total);
     if (goal < ahead || goal >= ahead + mine.a) return;
     goal -= ahead;
@@ -842,6 +859,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
                 run += w;
             }
     }
+}
+template <class T>
+__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs a) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    Shared& sm = *reinterpret_cast<Shared*>(raw);
+    Row<T> row(sm, reinterpret_cast<T*>(raw + sizeof(Shared)));
+    const int per = ((a.vocab + row.blocks - 1) / row.blocks + 7) & ~7;
+    row.base = row.rank * per;
+    row.n = max(0, min(per, a.vocab - row.base));
+    row.rounds = (row.n + 8 * kThreads - 1) / (8 * kThreads);
+    sample_row(a, sm, row, blockIdx.x / row.blocks);
 }
 static_assert(kRounds * kWarps == 128, "the last search looks at 128 parts");
 
