@@ -486,13 +486,22 @@ __device__ __noinline__ float poison_of(const Params& p, Part w, Rows c, int dim
     return sum;
 }
 
-// Whether any of eight values is an infinity or NaN: adding one to an all-ones exponent carries into
-// the sign's place.
+// Adds 0 x each of eight values to four pairs of sums, which become NaN by an infinity or NaN.
 template <bool kBf16>
-__device__ __forceinline__ bool any_not_finite(const uint4& v) {
-    constexpr uint32_t kExp = kBf16 ? 0x7f807f80u : 0x7c007c00u, kOne = kBf16 ? 0x00800080u : 0x04000400u;
-    return (((v.x & kExp) + kOne) | ((v.y & kExp) + kOne) | ((v.z & kExp) + kOne) | ((v.w & kExp) + kOne)) & 0x80008000u;
+__device__ __forceinline__ void test_finite(const uint4& v, uint32_t (&sum)[4]) {
+    if (kBf16) {
+        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[0]) : "r"(v.x), "r"(0));
+        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[1]) : "r"(v.y), "r"(0));
+        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[2]) : "r"(v.z), "r"(0));
+        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[3]) : "r"(v.w), "r"(0));
+    } else {
+        asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum[0]) : "r"(v.x), "r"(0));
+        asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum[1]) : "r"(v.y), "r"(0));
+        asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum[2]) : "r"(v.z), "r"(0));
+        asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum[3]) : "r"(v.w), "r"(0));
+    }
 }
+
 // kNH: the most rows a softmax group takes.
 template <int D, int kNH, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -738,6 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The group's rows r0 .. r0 + nh - 1, in eights; with few rows some groups have none.
         const int r0 = (N >> 3) * grp / 4 * 8, nh = (N >> 3) * (grp + 1) / 4 * 8 - r0;
         const uint32_t lanes = (uint32_t)(qd * 32) << 16;
+        constexpr int kLook = 1;
         int tile = 0;
         float l[kNH];
         // After a wait that gave up, these warps go on (on meaningless values) to the end of the share:
@@ -774,32 +784,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // registers to the row sums.
                 float over = -INFINITY;
 #pragma unroll 1
-                for (int f = 0; f < nh; f += 8) {
-                    float v[8];
-                    tc::ld8(st + f, v);
-                    tc::wait_ld();
-                    if (edge) {
-                        int a[8], d[8];
-                        *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(ask + f);
-                        *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(ask + f + 4);
-                        *reinterpret_cast<int4*>(d) = *reinterpret_cast<const int4*>(rs.depth + r0 + f);
-                        *reinterpret_cast<int4*>(d + 4) = *reinterpret_cast<const int4*>(rs.depth + r0 + f + 4);
+                for (int f = 0; f < nh; f += 8 * kLook) {
+                    float v[kLook][8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const bool seen = old ? j >= a[k] : (((unsigned)a[k] >> (j & 31)) & 1u) & (unsigned)(d[k] < near);
-                            v[k] = in & seen ? v[k] : -INFINITY;
+                    for (int u = 0; u < kLook; ++u)
+                        if (u == 0 || f + 8 * u < nh) tc::ld8(st + f + 8 * u, v[u]);
+                    tc::wait_ld();
+#pragma unroll
+                    for (int u = 0; u < kLook; ++u) {
+                        const int g = f + 8 * u;
+                        if (u > 0 && g >= nh) break;
+                        if (edge) {
+                            int a[8];
+                            *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(ask + g);
+                            *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(ask + g + 4);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                if (!(in && (old ? j >= a[k] : ((unsigned)a[k] >> (j & 31)) & 1u))) v[u][k] = -INFINITY;
+                            if (p.window && i * kKeys + kKeys > w.pre) {  // nodes further apart than the window
+                                *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(rs.depth + r0 + g);
+                                *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(rs.depth + r0 + g + 4);
+#pragma unroll
+                                for (int k = 0; k < 8; ++k)
+                                    if (a[k] >= near) v[u][k] = -INFINITY;
+                            }
+                            tc::st8(st + g, v[u]);
                         }
-                        tc::st8(st + f, v);
-                    }
-                    if (fresh) {
-                        reduce_scatter8<true>(v, lane);
-                        c.red[qd][r0 + f + (lane >> 2)] = v[0] * p.c;
-                    } else {
-                        const float4 n0 = *reinterpret_cast<const float4*>(&rs.nref[r0 + f]), n1 = *reinterpret_cast<const float4*>(&rs.nref[r0 + f + 4]);
-                        over = fmaxf(over, fmaxf(fmaf(v[0], p.c, n0.x), fmaf(v[1], p.c, n0.y)));
-                        over = fmaxf(over, fmaxf(fmaf(v[2], p.c, n0.z), fmaf(v[3], p.c, n0.w)));
-                        over = fmaxf(over, fmaxf(fmaf(v[4], p.c, n1.x), fmaf(v[5], p.c, n1.y)));
-                        over = fmaxf(over, fmaxf(fmaf(v[6], p.c, n1.z), fmaf(v[7], p.c, n1.w)));
+                        if (fresh) {
+                            reduce_scatter8<true>(v[u], lane);
+                            c.red[qd][r0 + g + (lane >> 2)] = v[u][0] * p.c;
+                        } else {
+                            const float4 n0 = *reinterpret_cast<const float4*>(&rs.nref[r0 + g]), n1 = *reinterpret_cast<const float4*>(&rs.nref[r0 + g + 4]);
+                            over = fmaxf(over, fmaxf(fmaf(v[u][0], p.c, n0.x), fmaf(v[u][1], p.c, n0.y)));
+                            over = fmaxf(over, fmaxf(fmaf(v[u][2], p.c, n0.z), fmaf(v[u][3], p.c, n0.w)));
+                            over = fmaxf(over, fmaxf(fmaf(v[u][4], p.c, n1.x), fmaf(v[u][5], p.c, n1.y)));
+                            over = fmaxf(over, fmaxf(fmaf(v[u][6], p.c, n1.z), fmaf(v[u][7], p.c, n1.w)));
+                        }
                     }
                 }
                 if (edge) tc::wait_st();
@@ -944,28 +964,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + d;
                 float* dst = p.part + ((long long)slot * N + r0) * D + d;
 #pragma unroll 1
-                for (int f = 0; f < held; f += 8) {
-                    float v[8];
-                    tc::ld8(ot + ci * N + f, v);
+                for (int f = 0; f < held; f += 8 * kLook) {
+                    float vs[kLook][8];
+#pragma unroll
+                    for (int u = 0; u < kLook; ++u)
+                        if (u == 0 || f + 8 * u < nh) tc::ld8(ot + ci * N + f + 8 * u, vs[u]);
                     tc::wait_ld();
                     if (D == 64 && key >= 64) continue;
-                    if (whole) {
-                        // Lanes swap so that each holds two dims of four rows: fewer, wider stores.
-                        const float4 i0 = *reinterpret_cast<const float4*>(&c.inv[r0 + f]), i1 = *reinterpret_cast<const float4*>(&c.inv[r0 + f + 4]);
-                        v[0] *= i0.x, v[1] *= i0.y, v[2] *= i0.z, v[3] *= i0.w;
-                        v[4] *= i1.x, v[5] *= i1.y, v[6] *= i1.z, v[7] *= i1.w;
-                        const bool odd = lane & 1;
-                        const int row = r0 + f + (odd ? 4 : 0);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[e] : v[e + 4], 1);
-                            const uint32_t two = odd ? pack2<kBf16>(got, v[e + 4]) : pack2<kBf16>(v[e], got);
-                            if (row + e - r0 < held) *reinterpret_cast<uint32_t*>(out + rs.out[row + e] - odd) = two;
+                    for (int u = 0; u < kLook; ++u) {
+                        const int g = f + 8 * u;
+                        if (u > 0 && g >= held) break;
+                        float(&v)[8] = vs[u];
+                        if (whole) {
+                            // Lanes swap so that each holds two dims of four rows: fewer, wider stores.
+                            const float4 i0 = *reinterpret_cast<const float4*>(&c.inv[r0 + g]), i1 = *reinterpret_cast<const float4*>(&c.inv[r0 + g + 4]);
+                            v[0] *= i0.x, v[1] *= i0.y, v[2] *= i0.z, v[3] *= i0.w;
+                            v[4] *= i1.x, v[5] *= i1.y, v[6] *= i1.z, v[7] *= i1.w;
+                            const bool odd = lane & 1;
+                            const int row = r0 + g + (odd ? 4 : 0);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float got = __shfl_xor_sync(0xffffffffu, odd ? v[e] : v[e + 4], 1);
+                                const uint32_t two = odd ? pack2<kBf16>(got, v[e + 4]) : pack2<kBf16>(v[e], got);
+                                if (row + e - r0 < held) *reinterpret_cast<uint32_t*>(out + rs.out[row + e] - odd) = two;
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (g + e < held) __stcg(dst + (g + e) * D, v[e]);
                         }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (f + e < held) __stcg(dst + (f + e) * D, v[e]);
                     }
                 }
             }
@@ -1089,19 +1117,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                             v[u] = make_uint4(0, 0, 0, 0);
                             if (k < mixed || (k >= nodes && k < keys)) v[u] = *reinterpret_cast<const uint4*>(base + (cc >> 3) * kBoxBytes + k * 128 + (cc & 7) * 16);
                         }
-                        uint32_t dirty = 0;
+                        uint32_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) dirty |= (uint32_t)any_not_finite<kBf16>(v[u]) << u;
+                        for (int u = 0; u < 8; ++u) test_finite<kBf16>(v[u], sum);
+                        // The sums are zeros, of either sign, or NaN.
+                        if (!((sum[0] | sum[1] | sum[2] | sum[3]) & 0x7fff7fffu)) continue;
 #pragma unroll 1
-                        for (int u = 0; dirty; ++u, dirty >>= 1) {
-                            if (!(dirty & 1)) continue;
-                            const int x = e + u * 32;
-                            uint16_t* h = reinterpret_cast<uint16_t*>(base + (x % (8 * kHalves) >> 3) * kBoxBytes +
-                                                                      x / (8 * kHalves) * 128 + (x & 7) * 16);
+                        for (int u = 0; u < 8; ++u) {
+                            const int x = e + u * 32, k = x / (8 * kHalves);
+                            if (!(k < mixed || (k >= nodes && k < keys))) continue;
+                            uint16_t* h = reinterpret_cast<uint16_t*>(base + (x % (8 * kHalves) >> 3) * kBoxBytes + k * 128 + (x & 7) * 16);
 #pragma unroll 1
                             for (int y = 0; y < 8; ++y)
-                                if (not_finite<kBf16>(h[y])) h[y] = 0;
-                            c.poison[part & 1] = 1;
+                                if (not_finite<kBf16>(h[y])) {
+                                    h[y] = 0;
+                                    c.poison[part & 1] = 1;
+                                }
                         }
                     }
                     fence_proxy_async();
