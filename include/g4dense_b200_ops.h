@@ -104,8 +104,9 @@ G4B_API int g4b_qmat_info(const g4b_qmat* q, int* out4);
  *
  * A round needs no host synchronization: lengths, counts and tables stay on the device. All calls
  * are asynchronous on `stream`, allocate nothing, and can be captured in a CUDA graph. Array
- * arguments are device memory; indices that a call finds out of range on the device are skipped,
- * never followed. Calls that write a `status` word leave the state as it was when it is not 0. */
+ * arguments are device memory; indices that a call finds out of range on the device are never
+ * followed: what they name is skipped (in the attention, a page id out of range reads as zeros).
+ * Calls that write a `status` word leave the state as it was when it is not 0. */
 
 typedef enum { G4B_BF16 = 0, G4B_FP16 = 1, G4B_FP32 = 2 } g4b_dtype;
 

@@ -514,3 +514,24 @@ def test_tree_mask():
     assert mask.view(np.uint32)[69].tolist() == [0xFFFFFFFF, 0xFFFFFFFF, 0x3F] and depth[69] == 69
     with pytest.raises(ValueError):
         api.tree_mask([-1, 2, 0])
+
+
+def test_packed_arguments_match_the_header(tmp_path):
+    """The bindings pack argument structs by hand: their sizes and last fields have to be the header's."""
+    import ctypes
+    import subprocess
+    from pathlib import Path
+
+    from g4dense_b200 import api
+    src = tmp_path / "s.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "g4dense_b200_ops.h"\n'
+                   'int main(void) { printf("%zu %zu %zu %zu %zu %zu", sizeof(g4b_tree_attention_args), '
+                   'offsetof(g4b_tree_attention_args, scale), sizeof(g4b_page_pool), offsetof(g4b_page_pool, row_bytes), '
+                   'sizeof(g4b_page_tables), offsetof(g4b_page_tables, page_size)); return 0; }\n')
+    include = Path(__file__).resolve().parent.parent / "include"
+    subprocess.run(["gcc", "-I", str(include), str(src), "-o", str(tmp_path / "s")], check=True)
+    size = list(map(int, subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split()))
+    import struct
+    at = lambda s, f: struct.calcsize(s.format.split("f")[0] if f else s.format) - (0 if f else ctypes.sizeof(ctypes.c_int))  # noqa: E731
+    assert size == [api._TREE_ATTENTION.size, at(api._TREE_ATTENTION, True), api._PAGE_POOL.size, at(api._PAGE_POOL, False),
+                    api._PAGE_TABLES.size, at(api._PAGE_TABLES, False)]

@@ -27,6 +27,14 @@
 //     ranked, and the threshold goes back to all blocks. Ties by the thousand end in a search over
 //     the 50-bit keys (ordered logit bits, inverted index), 8 bits a step;
 //   * without a list, the kept masses per block; the block in whose range r falls finds the token.
+// A top_k of up to 512 needs no histogram of all entries: the k-th largest of the threads' own maxima
+// bounds the k-th largest entry from below.
+//
+// The floor is one read of the logits; what bounds the kernel is the instructions and barriers per
+// entry behind it: about 15 for a top-k cut, 35 with an exponential for every entry, and three shared
+// atomics on top for a cut by mass. Measured on one B200, 128 rows of 262144 bf16 logits (10 us of
+// reading): 45 us greedy, 75 with top_k 40 and top_p 0.9, 100 with the temperature alone, 285 with
+// top_p 0.95 alone, 138 for a mix; one row of 4096: 10 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -31,6 +31,14 @@
 // some nodes see and others do not is taken out of the product and added back for those that do.
 //
 // Every wait is bounded (2 s); a block that gives up records it in a device word and leaves.
+//
+// Measured on one B200 (device time; GB/s of keys, values, queries and outputs read or written once):
+// 8 sequences of up to 30000 keys, 9 nodes, 32 heads on 4 of 512: 236 us, 5870 GB/s, 0.90 of the
+// measured copy rate; one node each: 215 us. 32 sequences, 64 nodes, 32 heads on 16 of 256, a window of
+// 1024 keys: 182 us, 3110 GB/s: 512 short items of ten tiles, whose starts and ends (queries in, first
+// maxima, masks, outputs) cost about two tiles each, and at 128 rows the softmax of a tile, about 5000
+// cycles, is as long as its loads. One node of one sequence of 96 keys: 8 us, a chain of latencies:
+// launch, lengths, table, keys, two products, output.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -53,20 +61,28 @@ constexpr int kKeys = 128;           // keys per tile: the M of S^T
 constexpr int kSoftWarps = 16;       // warps 0 .. 15, four groups of four
 constexpr int kProducer = 16, kIssuer = 17, kScheduler = 18;  // and 19, the cleaner
 constexpr int kThreads = 640;
+// With two groups of twice the rows the row sums alone took 64 registers and spilled: 319 us instead of
+// 259 for 9-node trees over 30000 keys.
 // Registers a thread: 96 at launch; 512 x 104 + 128 x 64 is the same total.
 constexpr int kSoftRegs = 104, kOtherRegs = 64;
 constexpr uint32_t kBoxBytes = kKeys * 128;  // 128 keys x 64 dims of 16 bits
 constexpr int kMaxSlots = 8;
 constexpr int kParts = 4;            // parts the scheduler is ahead
 constexpr int kTreeBox = 8;          // node rows per TMA box: the swizzle's eight
-constexpr int kPageBox = 32;         // and at most so many cached rows
+// And at most so many cached rows: larger boxes leave more places empty between the cached keys and the
+// nodes, smaller ones cost more copies. 8 x 30000 keys, head dims 512 / 128: 251 / 82 us with 16 rows,
+// 237 / 65 with 32, 236 / 67 with 64.
+constexpr int kPageBox = 32;
 constexpr float kUnset = 1e30f;      // negated reference of a row that has seen no key
 constexpr float kLazy = 8.f;         // a reference moves when a score exceeds it by 2^8
 constexpr size_t kSmemLimit = 232448 - 2048;  // leaves room for a block of the second kernel
-// What starting and finishing an item costs, in tiles, when the shares are cut.
+// What starting and finishing an item costs, in tiles, when the shares are cut. Measured with 64-node
+// trees over a 1024-key window (512 items): 226 us at 1, 182 at 2 and 3, 184 at 5; at 30000 keys it
+// does not matter.
 constexpr int kItemCost = 2;
-// Items of at most this many tiles are not split, which saves the second kernel.
-constexpr int kWholeTiles = 6;
+// Items of at most this many tiles are not split, which saves the second kernel: one sequence of 300
+// keys takes 10.5 us so and 11.1 split, one of 600 (5 tiles) 13.5 and 12.2.
+constexpr int kWholeTiles = 4;
 constexpr int kFewSeqs = 64;
 
 __device__ int g_tree_err;  // set when a bounded wait gives up
