@@ -75,7 +75,7 @@ constexpr int kTreeBox = 8;          // node rows per TMA box: the swizzle's eig
 constexpr int kPageBox = 32;
 constexpr float kUnset = 1e30f;      // negated reference of a row that has seen no key
 constexpr float kLazy = 8.f;         // a reference moves when a score exceeds it by 2^8
-constexpr size_t kSmemLimit = 232448 - 2048;  // leaves room for a block of the second kernel
+constexpr size_t kSmemLimit = 232448 - 2048;  // leaves room for blocks of the second kernel
 // What starting and finishing an item costs, in tiles, when the shares are cut. Measured with 64-node
 // trees over a 1024-key window (512 items): 226 us at 1, 182 at 2 and 3, 184 at 5; at 30000 keys it
 // does not matter.
@@ -156,6 +156,12 @@ Div make_div(int d) {
     return x;
 }
 
+// An item that starts in a block and goes on in later ones, c0 .. c1 (none: c1 < c0); the first part's
+// slot is `slot`, the others' are 2 c.
+struct Split {
+    int h, g, first, n, c0, c1, slot, total;
+};
+
 struct Params {
     const char* q;
     char* out;
@@ -168,6 +174,7 @@ struct Params {
     const int32_t* depth;
     float* part;   // [2 x blocks][N][dim]
     float2* ml;    // [2 x blocks][N]
+    Split* split;  // [blocks]
     long long q_stride, out_stride, page_stride, new_stride;  // elements
     int seqs, n_tokens, max_nodes, pages, page_size, width, mask_words, kv_heads, window;
     int N, words, slots, box, box_log, tmem_cols, whole, gqa;
@@ -199,19 +206,6 @@ __device__ __forceinline__ void derive_seq(const Params& p, Seq& s) {
     }
     s.tiles = s.n ? (s.pre + s.n + kKeys - 1) / kKeys : 0;
     s.groups = p.by_rows.quot(s.n * p.gqa + p.N - 1);
-}
-
-// Sum of the block's values, to every thread.
-__device__ __forceinline__ int block_total(int v, int* red) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    v = warp_sum_int(v);
-    __syncthreads();
-    if (lane == 0) red[w] = v;
-    __syncthreads();
-    int t = 0;
-#pragma unroll 1
-    for (int i = 0; i < nw; ++i) t += red[i];
-    return t;
 }
 
 // An item is as long as its tiles and kItemCost more, ahead of them; 1 where items stay whole.
@@ -285,7 +279,8 @@ __device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* 
     for (; runs > 1 && before + c.scan[first] <= pos && first + 1 < runs; ++first) before += c.scan[first];
     first *= per;
     Seq s{};
-    int b = 0, h = 0, g = 0, u = 0;
+    int b = 0, h = 0, g = 0, u = 0, parts = 0;
+    if (lane == 0 && !p.whole) p.split[blockIdx.x] = Split{0, 0, 0, 0, 0, -1, 0, 0};
     if (pos < end) {
 #pragma unroll 1
         for (int b0 = first; b0 < p.seqs; b0 += 32) {
@@ -346,6 +341,14 @@ __device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* 
             t1 = p.whole ? s.tiles : max(0, v - kItemCost);
             u = v;
         }
+        if (!p.whole && t0 < t1 && t0 == 0 && t1 < s.tiles) {
+            // This block's last part, and the first of an item that others finish.
+            const int z = pos + item_units(p, s) - u;  // the unit behind the item
+            int last = blockIdx.x + 1;
+            while (share_begin(p, total, last + 1) < z) ++last;
+            if (lane == 0) p.split[blockIdx.x] = Split{h, g, s.first, s.n, (int)blockIdx.x, last, 2 * (int)blockIdx.x + (parts ? 1 : 0), total};
+        }
+        ++parts;
         if (!__all_sync(0xffffffffu, wait(&c.part_free[at.slot], at.phase ^ 1, abort))) return;
         const Part part{b, h, g, t0, t1, s.len, s.first, s.n, s.start, s.base, s.pre, s.tiles};
         if ((threadIdx.x & 31) == 0) {
@@ -1169,47 +1172,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-constexpr int kJoinRows = 2;  // two warps' registers fit beside the first kernel's
+constexpr int kJoinRows = 4;
 
 // Joins the parts of items that several blocks worked on: out = sum_s 2^(m_s - M) O_s over
-// sum_s 2^(m_s - M) l_s. A warp per row, kJoinRows rows a block; grid (seqs x kv_heads, row blocks).
+// sum_s 2^(m_s - M) l_s. A warp per row, kJoinRows rows a block; grid (blocks of the first kernel, row
+// blocks): an item belongs to the block it starts in, which wrote down where the others are.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(32 * kJoinRows) tree_attn_join_kernel(const __grid_constant__ Params p) {
-    __shared__ int red[32];
-    // Which parts there are follows from the inputs alone; only the parts themselves are waited for.
-    const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads, lane = threadIdx.x & 31;
-    Seq s;
-    read_seq(p, b, s);
-    derive_seq(p, s);
-    if (s.n * p.gqa <= (int)blockIdx.y * kJoinRows) return;
-    int before = 0, all = 0;
-#pragma unroll 1
-    for (int i = threadIdx.x; i < p.seqs; i += 32 * kJoinRows) {
-        const int t = seq_units(p, i);
-        all += t;
-        if (i < b) before += t;
-    }
-    before = block_total(before, red);
-    all = block_total(all, red);
-    const int row = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
-    if (row >= s.n * p.gqa) return;
-    const int g = p.by_rows.quot(row), r = row - g * p.N;
-    const int item = s.tiles + kItemCost;
-    const int a = before + (h * s.groups + g) * item, z = a + item;
-    // Block that holds unit x: an estimate, corrected.
-    const auto block_of = [&](int x) {
-        int c = min((int)p.by_grid.d - 1, (int)((float)x / (float)all * (float)p.by_grid.d));
-        while (c > 0 && share_begin(p, all, c) > x) --c;
-        while (c + 1 < (int)p.by_grid.d && share_begin(p, all, c + 1) <= x) ++c;
-        return c;
-    };
-    const int c0 = block_of(a + kItemCost), c1 = block_of(z - 1);  // the blocks of its first and last tile
-    if (c0 == c1) return;
-    const auto slot_of = [&](int c) { return (long long)(2 * c + (share_begin(p, all, c) < a ? 1 : 0)); };
+    const int lane = threadIdx.x & 31, r = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
     pdl_wait();
+    const Split s = p.split[blockIdx.x];
+    const int row = s.g * p.N + r, c0 = s.c0, c1 = s.c1, h = s.h;
+    if (c1 < c0 || r >= p.N || row >= s.n * p.gqa) return;
+    const auto slot_of = [&](int c) { return (long long)(c == c0 ? s.slot : 2 * c); };
     float top = -INFINITY;
     for (int c = c0 + lane; c <= c1; c += 32) {
-        if (share_begin(p, all, c) == share_begin(p, all, c + 1)) continue;
+        if (share_begin(p, s.total, c) == share_begin(p, s.total, c + 1)) continue;  // a block without work
         const float2 x = p.ml[slot_of(c) * p.N + r];
         top = fmaxf(top, x.x);
     }
@@ -1223,7 +1201,7 @@ __global__ void __launch_bounds__(32 * kJoinRows) tree_attn_join_kernel(const __
         for (int j = 0; j < kV; ++j) o[k][j] = 0.f;
 #pragma unroll 2
     for (int c = c0; c <= c1; ++c) {
-        if (share_begin(p, all, c) == share_begin(p, all, c + 1)) continue;
+        if (share_begin(p, s.total, c) == share_begin(p, s.total, c + 1)) continue;  // a block without work
         const float2 x = p.ml[slot_of(c) * p.N + r];
         if (x.x == -INFINITY) continue;  // this part's keys are all hidden from the row
         const float f = exp2_approx(x.x - top);
@@ -1316,8 +1294,7 @@ cudaError_t run(const CUtensorMap* maps, const Params& p, const Shape& sh, cudaS
     }
     cudaError_t e = launch(kern, dim3(p.by_grid.d), dim3(kThreads), sh.smem, st, false, maps[0], maps[1], maps[2], maps[3], p);
     if (e != cudaSuccess || p.whole) return e;
-    const int rows = p.max_nodes * p.gqa;
-    return launch(tree_attn_join_kernel<D, kBf16>, dim3(p.seqs * p.kv_heads, (rows + kJoinRows - 1) / kJoinRows),
+    return launch(tree_attn_join_kernel<D, kBf16>, dim3(p.by_grid.d, (p.N + kJoinRows - 1) / kJoinRows),
                   dim3(32 * kJoinRows), 0, st, true, p);
 }
 
@@ -1339,7 +1316,7 @@ cudaError_t run_type(const CUtensorMap* maps, const Params& p, const Shape& sh, 
 
 size_t tree_attn_workspace(int max_nodes, int heads, int kv_heads, int dim) {
     const int N = rows_per_item(max_nodes, heads / kv_heads, dim);
-    return (size_t)2 * sm_count() * N * (dim * sizeof(float) + sizeof(float2));
+    return (size_t)2 * sm_count() * N * (dim * sizeof(float) + sizeof(float2)) + sm_count() * sizeof(Split);
 }
 
 cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
@@ -1357,6 +1334,7 @@ cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
     int grid = sm_count();
     p.part = static_cast<float*>(a.work);
     p.ml = reinterpret_cast<float2*>(p.part + (size_t)2 * grid * sh.N * a.dim);
+    p.split = reinterpret_cast<Split*>(p.ml + (size_t)2 * grid * sh.N);
     p.q_stride = a.q_stride;
     p.out_stride = a.out_stride;
     p.page_stride = a.page_stride;
