@@ -22,10 +22,11 @@
 //   * where top_k or top_p cut, a histogram of 256 bins of 1/8 in (m - l) / T, which spreads a row's
 //     likely entries evenly (counts, and for a cut by mass the exact masses);
 //   * usual cuts leave a few hundred entries at and above the bin that is cut: these go to the first
-//     block, which ranks them all against all and finishes alone. Where they are more than kList
-//     (nucleus sampling of a flat row), the bin is split into 256 again, the part that is cut is
-//     ranked, and the threshold goes back to all blocks. Ties by the thousand end in a search over
-//     the 50-bit keys (ordered logit bits, inverted index), 8 bits a step;
+//     block, which ranks up to kRanked of them all against all, searches longer lists for the last
+//     key that stays, and finishes alone. Where they are more than kList (nucleus sampling of a flat
+//     row), the bin is split into 256 again, the part that is cut is searched, and the threshold goes
+//     back to all blocks. Ties by the thousand end in a search over the 50-bit keys (ordered logit
+//     bits, inverted index) of all blocks, 8 bits a step;
 //   * without a list, the kept masses per block; the block in whose range r falls finds the token.
 // A top_k of up to 512 needs no histogram of all entries: the k-th largest of the threads' own maxima
 // bounds the k-th largest entry from below.
@@ -33,8 +34,8 @@
 // The floor is one read of the logits; what bounds the kernel is the instructions and barriers per
 // entry behind it: about 15 for a top-k cut, 35 with an exponential for every entry, and three shared
 // atomics on top for a cut by mass. Measured on one B200, 128 rows of 262144 bf16 logits (10 us of
-// reading): 45 us greedy, 75 with top_k 40 and top_p 0.9, 100 with the temperature alone, 285 with
-// top_p 0.95 alone, 138 for a mix; one row of 4096: 10 us.
+// reading): 45 us greedy, 76 with top_k 40 and top_p 0.9, 100 with the temperature alone, 271 with
+// top_p 0.95 alone, 134 for a mix; one row of 4096: 10 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -59,7 +60,7 @@ constexpr int kRounds = kSliceBytes / 2 / (8 * kThreads);  // a thread takes eig
 constexpr int kIndexBits = 18;              // vocabularies up to 262144
 constexpr int kIndexMask = (1 << kIndexBits) - 1;
 constexpr int kBins = 256;
-constexpr int kList = 1024;                 // entries the first block ranks
+constexpr int kList = 1024;                 // entries the first block takes
 constexpr int kCand = 2048;                 // entries of one bin that a block sets aside
 typedef unsigned long long u64;
 
@@ -79,7 +80,7 @@ struct alignas(16) Shared {
     u64 cum_count[kBins], cum_mass[kBins];
     alignas(16) u64 key[kList + 2];  // the list, in the first block
     u64 weight[kThreads];  // kept masses by index
-    u64 named[kList];      // the list sorted
+    u64 named[kList];      // the list sorted, and what a block names for it
     uint16_t cand[kCand];    // places in the slice of what is set aside
     u64 answer;
     int bin, staged, cands;
@@ -483,74 +484,142 @@ __device__ u64 block_scan(Shared& sm, u64 v, u64* total) {
     return ahead + x - v;
 }
 
-// Puts the list's n keys into sm.named in descending order. Up to 256 keys are ranked, each against
-// all (few keys have several neighbouring threads each); more go through a bitonic network, whose
-// steps cost a barrier each but no n^2.
-__device__ __noinline__ void sort_list(Shared& sm, int n) {
+// Lists up to this long are ranked, each key against all; longer ones are searched in 8-bit steps.
+// With every list ranked, 128 rows of 262144 took 88 us at top_k 256 (85 so) and 285 at top_p 0.95 (271).
+constexpr int kRanked = 256;
+
+// Puts the list's n <= kRanked keys into sm.named in descending order, several neighbouring threads a
+// key.
+__device__ __noinline__ void rank_list(Shared& sm, int n) {
     const int t = threadIdx.x;
-    if (n <= 256) {
-        if (t == 0) sm.key[n] = 0;  // keys are loaded in pairs
-        __syncthreads();
-        int share = 2;  // threads a key
-        while (share < 32 && 2 * share * n <= kThreads) share *= 2;
-        const int part = t % share, i = t / share;
-        const u64 mine = i < n ? sm.key[i] : 0;
-        int rank = 0;
+    if (t == 0) sm.key[n] = 0;  // keys are loaded in pairs
+    __syncthreads();
+    int share = kThreads / kRanked;  // threads a key
+    while (share < 32 && 2 * share * n <= kThreads) share *= 2;
+    const int part = t % share, i = t / share;
+    const u64 mine = i < n ? sm.key[i] : 0;
+    int rank = 0;
 #pragma unroll 4
-        for (int j = 2 * part; j < n; j += 2 * share) {
-            const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&sm.key[j]);
-            rank += (k.x > mine) + (k.y > mine);
-        }
-        for (int o = share >> 1; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-        if (i < n && part == 0) sm.named[rank] = mine;
-    } else {
-        const int size = n <= 512 ? 512 : kList;
-        for (int i = n + t; i < size; i += kThreads) sm.key[i] = 0;
-        for (int k = 2; k <= size; k <<= 1)
-            for (int j = k >> 1; j > 0; j >>= 1) {
-                __syncthreads();
-                if (t < size / 2) {
-                    const int i = 2 * t - (t & (j - 1)), o = i + j;  // the t-th pair j apart
-                    const u64 x = sm.key[i], y = sm.key[o];
-                    if ((i & k) == 0 ? x < y : x > y) sm.key[i] = y, sm.key[o] = x;
-                }
-            }
-        __syncthreads();
-        for (int i = t; i < n; i += kThreads) sm.named[i] = sm.key[i];
+    for (int j = 2 * part; j < n; j += 2 * share) {
+        const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&sm.key[j]);
+        rank += (k.x > mine) + (k.y > mine);
     }
+    for (int o = share >> 1; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (i < n && part == 0) sm.named[rank] = mine;
     __syncthreads();
 }
-static_assert(kThreads == 2 * 256 && kList == 2 * kThreads, "two threads a ranked key, a thread a sorted pair");
+
+// As Row::search, over the list alone (two keys a thread, 0: none): the last of the keys at or above
+// `from` that stays. `before` is what lies ahead of the list.
+__device__ __noinline__ u64 search_list(Shared& sm, const u64 (&key)[2], const u64 (&w)[2], bool mass, u64 before,
+                                        double goal, u64 from) {
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    u64 lo = max(from, (u64)1), hi = ~0ull;
+    Bins& b = sm.bins[0];  // all remote reads of it ended before the last barrier
+    for (int step = 0; step < 9; ++step) {
+        u64 top = 0, low = 0;
+        bool in[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            in[i] = key[i] >= lo && key[i] <= hi;
+            if (in[i]) top = max(top, key[i]), low = max(low, ~key[i]);
+        }
+        top = warp_max64(top);
+        low = warp_max64(low);
+        __syncthreads();
+        if (lane == 0) sm.red[0][warp] = top, sm.red[1][warp] = low;
+        for (int i = t; i < 4 * kBins; i += kThreads) b.count[i] = 0;
+        if (t == 0) sm.bin = kBins - 1;
+        __syncthreads();
+        hi = warp_max64(lane < kWarps ? sm.red[0][lane] : 0);
+        lo = ~warp_max64(lane < kWarps ? sm.red[1][lane] : 0);
+        if (hi <= lo) return lo;
+        const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 8);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (in[i]) {
+                const int x = (int)((hi - key[i]) >> shift);
+                const u64 v = mass ? w[i] : 1;
+                atomicAdd(&b.lo[x], (unsigned)v & 0xffff);
+                if (mass) atomicAdd(&b.mid[x], (unsigned)v >> 16);
+                if (v >> 32) atomicAdd(&b.hi[x], (unsigned)(v >> 32));
+            }
+        __syncthreads();
+        u64 own = t < kBins ? b.lo[t] + ((u64)b.mid[t] << 16) + ((u64)b.hi[t] << 32) : 0, x = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) sm.red[0][warp] = x;
+        __syncthreads();
+        for (int i = 0; i < warp && i < kBins / 32; ++i) x += sm.red[0][i];
+        if (own && (double)(before + x - own) < goal && !((double)(before + x) < goal)) {
+            sm.bin = t;
+            sm.answer = before + x - own;
+        }
+        __syncthreads();
+        before = sm.answer;
+        const u64 first = hi - ((u64)sm.bin << shift), span = ((u64)1 << shift) - 1;
+        hi = first;
+        lo = max(lo, first >= span ? first - span : 0);
+    }
+    return lo;
+}
 
 // The end of a row whose list (in the first block) holds every entry that may be kept: the first k
 // of it, then the cuts by mass and by min-p, then the draw.
 __device__ __noinline__ void finish_list(const SampleRowsArgs& a, int r, Shared& sm, const Scale& sc, int n, u64 k,
                                          float p, double goal, float low) {
-    sort_list(sm, n);
-    const int m = (int)min((u64)n, k), t = threadIdx.x;
-    // Two neighbours of the descending order a thread.
+    const int t = threadIdx.x;
     u64 key[2], w[2], mass, total;
     float e[2];
+    bool in[2];
+    if (n <= kRanked) {
+        rank_list(sm, n);
+        // Two neighbours of the descending order a thread.
+        const int m = (int)min((u64)n, k);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        key[i] = 2 * t + i < m ? sm.named[2 * t + i] : 0;
-        e[i] = 2 * t + i < m ? sc.share(key_logit(key[i])) : 0.f;
-        w[i] = Scale::weight(e[i]);
+        for (int i = 0; i < 2; ++i) {
+            key[i] = 2 * t + i < m ? sm.named[2 * t + i] : 0;
+            e[i] = 2 * t + i < m ? sc.share(key_logit(key[i])) : 0.f;
+            w[i] = Scale::weight(e[i]);
+        }
+        const u64 before = block_scan(sm, w[0] + w[1], &mass);
+        if (k != ~0ull) goal = (double)p * (double)mass;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int x = 2 * t + i;
+            const u64 ahead = before + (i ? w[0] : 0);
+            in[i] = x < m && (x == 0 || ((p >= 1.f || (double)ahead < goal) && e[i] >= low));
+        }
+    } else {
+        u64 from = 1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            key[i] = t + i * kThreads < n ? sm.key[t + i * kThreads] : 0;
+            e[i] = key[i] ? sc.share(key_logit(key[i])) : 0.f;
+            w[i] = Scale::weight(e[i]);
+        }
+        if (k < (u64)n) from = search_list(sm, key, w, false, 0, (double)k, 1);
+        block_scan(sm, (key[0] >= from ? w[0] : 0) + (key[1] >= from ? w[1] : 0), &mass);
+        if (k != ~0ull) goal = (double)p * (double)mass;
+        if (p <= 0.f) from = search_list(sm, key, w, false, 0, 1.0, 1);
+        else if (p < 1.f) from = search_list(sm, key, w, true, 0, goal, from);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) in[i] = key[i] >= from && key[i] && e[i] >= low;
+        __syncthreads();
     }
-    const u64 before = block_scan(sm, w[0] + w[1], &mass);
-    if (k != ~0ull) goal = (double)p * (double)mass;
     sm.weight[t] = 0;
     if (t == 0) sm.staged = 0;
     __syncthreads();
-    // The draw goes in index order: kept masses by the index's upper half, a thread a bucket of 512.
-    bool in[2];
+    // The draw goes in index order: kept masses by the index's upper bits, a thread a bucket. (64-bit
+    // atomics in shared memory are loops, 60 to 2500 cycles a warp by how many lanes meet; so as many
+    // buckets as there are threads, and no such atomics where every entry takes part.)
+    const int shift = max(0, 23 - __clz(max(1, a.vocab - 1)));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int x = 2 * t + i;
-        const u64 ahead = before + (i ? w[0] : 0);
-        in[i] = x < m && (x == 0 || ((p >= 1.f || (double)ahead < goal) && e[i] >= low));
-        if (in[i]) atomicAdd(&sm.weight[key_index(key[i]) >> 9], w[i]);
-    }
+    for (int i = 0; i < 2; ++i)
+        if (in[i]) atomicAdd(&sm.weight[key_index(key[i]) >> shift], w[i]);
     const int kept = __syncthreads_count(in[0]) + __syncthreads_count(in[1]);
     const u64 bucket = sm.weight[t], at = block_scan(sm, bucket, &total);
     const u64 target = draw(a.uniform[r], total);
@@ -561,7 +630,7 @@ __device__ __noinline__ void finish_list(const SampleRowsArgs& a, int r, Shared&
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-        if (in[i] && key_index(key[i]) >> 9 == sm.bin) {  // that bucket's entries
+        if (in[i] && key_index(key[i]) >> shift == sm.bin) {  // that bucket's entries
             const int x = atomicAdd(&sm.staged, 1);
             sm.key[x] = key[i];
             sm.named[x] = w[i];
@@ -723,20 +792,15 @@ __device__ __forceinline__ void sample_row(const SampleRowsArgs& a, Shared& sm, 
                     });
                 });
                 if (row.rank == 0) {
-                    sort_list(sm, n);
-                    u64 whole;
-                    u64 w[2], at = 0;  // two neighbours of the descending order
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        w[i] = 2 * tid + i >= n ? 0 : by_mass ? Scale::weight(sc.share(key_logit(sm.named[2 * tid + i]))) : 1;
-                    at = before + block_scan(sm, w[0] + w[1], &whole);
+                    u64 own[2], w[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        if (w[i] && (double)at < goal && !((double)(at + w[i]) < goal))
-#pragma unroll 1
-                            for (int c = 0; c < row.blocks; ++c) *row.cl.map_shared_rank(&sm.answer, c) = sm.named[2 * tid + i];
-                        at += w[i];
+                        own[i] = tid + i * kThreads < n ? sm.key[tid + i * kThreads] : 0;
+                        w[i] = own[i] && by_mass ? Scale::weight(sc.share(key_logit(own[i]))) : 0;
                     }
+                    const u64 last = search_list(sm, own, w, by_mass, before, goal, 1);
+                    __syncthreads();
+                    if (tid < row.blocks) *row.cl.map_shared_rank(&sm.answer, tid) = last;
                 }
                 row.barrier();
                 key = sm.answer;
