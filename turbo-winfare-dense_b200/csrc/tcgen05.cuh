@@ -127,10 +127,10 @@ __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.
 // layout: rows of 64 fp16 (128 B) stored consecutively, 16-byte chunk c of row r at chunk
 // position c ^ (r % 8), 8-row atoms 1024 B apart. `addr` is the shared-memory byte address of
 // the first row, advanced by 32 B per 16-wide K slice; the tile itself is 1024-byte aligned.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t sbo = 1024) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4)  // start address, 16-byte units
            | ((uint64_t)1 << 16)               // leading byte offset (unused for swizzled K-major)
-           | ((uint64_t)(1024 >> 4) << 32)     // stride byte offset: 8-row atom pitch
+           | ((uint64_t)(sbo >> 4) << 32)      // stride byte offset: 8-row atom pitch
            | ((uint64_t)1 << 46)               // descriptor version for sm_100
            | ((uint64_t)2 << 61);              // 128-byte swizzle
 }

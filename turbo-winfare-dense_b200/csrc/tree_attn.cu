@@ -397,11 +397,11 @@ __device__ __forceinline__ void tma_3d(void* dst, uint64_t map, int x, int y, in
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
-__device__ __forceinline__ void tma_4d(void* dst, uint64_t map, int x, int y, int z, int w, uint64_t* bar) {
+__device__ __forceinline__ void tma_5d(void* dst, uint64_t map, int x, int y, int z, int w, int v, uint64_t* bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-        "[%6];" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
+        "[%7];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(smem_u32(bar))
         : "memory");
 }
 
@@ -530,6 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kHalves = D == 64 ? 1 : 2;                // 64-dim boxes per slot
     constexpr int kChunks = D == 64 ? 1 : D / 128;          // slots per K or V tile
     constexpr uint32_t kSlotBytes = kHalves * kBoxBytes;
+    constexpr uint32_t kRows8 = kHalves * 1024;             // eight keys of a slot: [64-dim block][key][64 dims]
     extern __shared__ unsigned char smem_raw[];
     // An offset, not a rounded pointer: the compiler still sees shared memory, and uses its 32-bit
     // addresses and instructions.
@@ -589,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         Place at, list;
         int used = 0;
         bool ok = true;
-        const int kb = lane & 15, half = lane >> 4;  // up to 16 key boxes, two halves of 64 dims
+        const int kb = lane;  // up to 16 key boxes
         const uint64_t kd = reinterpret_cast<uint64_t>(&kmap), vd = reinterpret_cast<uint64_t>(&vmap);
         const uint64_t knd = reinterpret_cast<uint64_t>(&knmap), vnd = reinterpret_cast<uint64_t>(&vnmap);
 #pragma unroll 1
@@ -617,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (tile < w.t0 || tile >= w.t1) continue;
                 const int nc = cached(tile), from = nc * p.box, nn = max(0, w.keys(tile) - from + kTreeBox - 1) / kTreeBox;
-                const bool old = kb < nc, mine = kb < nc + nn && half < kHalves;
+                const bool old = kb < nc, mine = kb < nc + nn;
                 const int at_row = old ? kb * p.box : from + (kb - nc) * kTreeBox;
                 const int x = tile * kKeys + at_row;
                 // A page id out of range is an out-of-range coordinate: the box reads as zeros.
@@ -633,10 +634,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) mbar_expect_tx(&c.full[at.slot], bytes);
                     __syncwarp();
                     if (mine) {
-                        unsigned char* dst = ring + at.slot * kSlotBytes + half * kBoxBytes + at_row * 128;
-                        const int d = 128 * ci + 64 * half;
-                        if (old) tma_4d(dst, map, d, w.h, z, pg, &c.full[at.slot]);
-                        else tma_3d(dst, map, d, w.h, z, &c.full[at.slot]);
+                        unsigned char* dst = ring + at.slot * kSlotBytes + (at_row >> 3) * kRows8;
+                        const int block = w.h * (D / 64) + ci * kHalves;
+                        if (old) tma_5d(dst, map, 0, 0, block, z >> 3, pg, &c.full[at.slot]);
+                        else tma_3d(dst, map, 0, z, block, &c.full[at.slot]);
                     }
                     at.step(slots);
                     ++used;
@@ -661,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t id_o = tc::idesc_16(128, N, kBf16, true, true);
         // Descriptors of the ring's first slot, of Q and of P; other places add their distance in
         // 16-byte units.
-        const uint64_t k_desc = tc::desc_sw128(smem_u32(ring)), v_desc = tc::desc_sw128_mn(smem_u32(ring), kBoxBytes, 1024);
+        const uint64_t k_desc = tc::desc_sw128(smem_u32(ring), kRows8), v_desc = tc::desc_sw128_mn(smem_u32(ring), 1024, kRows8);
         const uint64_t q_desc = tc::desc_sw128(smem_u32(qs)), p_desc = tc::desc_sw128_mn(smem_u32(ps), kBoxBytes, 1024);
         const uint32_t blk = (uint32_t)N * 8;  // one 64-dim block of Q
         // V chunks that fit the ring beside nothing else: the cleaning of an edge tile's first ones
@@ -694,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (leader) {
 #pragma unroll
                             for (int kk = 0; kk < 4 * kHalves; ++kk)
-                                tc::mma_ss(tmem + b * N, a + (kk >> 2) * (kBoxBytes >> 4) + (kk & 3) * 2,
+                                tc::mma_ss(tmem + b * N, a + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2,
                                            q + (kk >> 2) * blk + (kk & 3) * 2, id_s, (ci | kk) ? 1u : 0u);
                             tc::commit(&c.empty[at.slot]);
                         }
@@ -729,17 +730,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc::fence_after_sync();
                         const uint64_t a = v_desc + at.slot * (kSlotBytes >> 4);
                         const uint32_t d = tmem + o_col + ci * N, more = i - 1 > t0 ? 1u : 0u;
-                        // V^T rows are the slot's dims, two 64-dim boxes apart (with D = 64 the lanes
-                        // 64 .. 127 multiply whatever follows in shared memory, and are never read).
+                        // V^T rows are the slot's dims (with D = 64 the lanes 64 .. 127 multiply whatever
+                        // follows in shared memory, and are never read).
                         if (leader) {
                             if (steps == 8) {
 #pragma unroll
                                 for (int kk = 0; kk < 8; ++kk)
-                                    tc::mma_ss(d, a + kk * 128, p_desc + kk * 128, id_o, kk ? 1u : more);
+                                    tc::mma_ss(d, a + kk * (2 * kRows8 >> 4), p_desc + kk * 128, id_o, kk ? 1u : more);
                             } else {
 #pragma unroll 1
                                 for (int kk = 0; kk < steps; ++kk)
-                                    tc::mma_ss(d, a + kk * 128, p_desc + kk * 128, id_o, kk ? 1u : more);
+                                    tc::mma_ss(d, a + kk * (2 * kRows8 >> 4), p_desc + kk * 128, id_o, kk ? 1u : more);
                             }
                             tc::commit(&c.empty[at.slot]);
                         }
@@ -766,7 +767,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The group's rows r0 .. r0 + nh - 1, in eights; with few rows some groups have none.
         const int r0 = (N >> 3) * grp / 4 * 8, nh = (N >> 3) * (grp + 1) / 4 * 8 - r0;
         const uint32_t lanes = (uint32_t)(qd * 32) << 16;
-        constexpr int kLook = 1;
         int tile = 0;
         float l[kNH];
         // After a wait that gave up, these warps go on (on meaningless values) to the end of the share:
@@ -803,42 +803,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // registers to the row sums.
                 float over = -INFINITY;
 #pragma unroll 1
-                for (int f = 0; f < nh; f += 8 * kLook) {
-                    float v[kLook][8];
-#pragma unroll
-                    for (int u = 0; u < kLook; ++u)
-                        if (u == 0 || f + 8 * u < nh) tc::ld8(st + f + 8 * u, v[u]);
+                for (int g = 0; g < nh; g += 8) {
+                    float v[8];
+                    tc::ld8(st + g, v);
                     tc::wait_ld();
+                    if (edge) {
+                        int a[8];
+                        *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(ask + g);
+                        *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(ask + g + 4);
 #pragma unroll
-                    for (int u = 0; u < kLook; ++u) {
-                        const int g = f + 8 * u;
-                        if (u > 0 && g >= nh) break;
-                        if (edge) {
-                            int a[8];
-                            *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(ask + g);
-                            *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(ask + g + 4);
+                        for (int k = 0; k < 8; ++k)
+                            if (!(in && (old ? j >= a[k] : ((unsigned)a[k] >> (j & 31)) & 1u))) v[k] = -INFINITY;
+                        if (p.window && i * kKeys + kKeys > w.pre) {  // nodes further apart than the window
+                            *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(rs.depth + r0 + g);
+                            *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(rs.depth + r0 + g + 4);
 #pragma unroll
                             for (int k = 0; k < 8; ++k)
-                                if (!(in && (old ? j >= a[k] : ((unsigned)a[k] >> (j & 31)) & 1u))) v[u][k] = -INFINITY;
-                            if (p.window && i * kKeys + kKeys > w.pre) {  // nodes further apart than the window
-                                *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(rs.depth + r0 + g);
-                                *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(rs.depth + r0 + g + 4);
-#pragma unroll
-                                for (int k = 0; k < 8; ++k)
-                                    if (a[k] >= near) v[u][k] = -INFINITY;
-                            }
-                            tc::st8(st + g, v[u]);
+                                if (a[k] >= near) v[k] = -INFINITY;
                         }
-                        if (fresh) {
-                            reduce_scatter8<true>(v[u], lane);
-                            c.red[qd][r0 + g + (lane >> 2)] = v[u][0] * p.c;
-                        } else {
-                            const float4 n0 = *reinterpret_cast<const float4*>(&rs.nref[r0 + g]), n1 = *reinterpret_cast<const float4*>(&rs.nref[r0 + g + 4]);
-                            over = fmaxf(over, fmaxf(fmaf(v[u][0], p.c, n0.x), fmaf(v[u][1], p.c, n0.y)));
-                            over = fmaxf(over, fmaxf(fmaf(v[u][2], p.c, n0.z), fmaf(v[u][3], p.c, n0.w)));
-                            over = fmaxf(over, fmaxf(fmaf(v[u][4], p.c, n1.x), fmaf(v[u][5], p.c, n1.y)));
-                            over = fmaxf(over, fmaxf(fmaf(v[u][6], p.c, n1.z), fmaf(v[u][7], p.c, n1.w)));
-                        }
+                        tc::st8(st + g, v);
+                    }
+                    if (fresh) {
+                        reduce_scatter8<true>(v, lane);
+                        c.red[qd][r0 + g + (lane >> 2)] = v[0] * p.c;
+                    } else {
+                        const float4 n0 = *reinterpret_cast<const float4*>(&rs.nref[r0 + g]), n1 = *reinterpret_cast<const float4*>(&rs.nref[r0 + g + 4]);
+                        over = fmaxf(over, fmaxf(fmaf(v[0], p.c, n0.x), fmaf(v[1], p.c, n0.y)));
+                        over = fmaxf(over, fmaxf(fmaf(v[2], p.c, n0.z), fmaf(v[3], p.c, n0.w)));
+                        over = fmaxf(over, fmaxf(fmaf(v[4], p.c, n1.x), fmaf(v[5], p.c, n1.y)));
+                        over = fmaxf(over, fmaxf(fmaf(v[6], p.c, n1.z), fmaf(v[7], p.c, n1.w)));
                     }
                 }
                 if (edge) tc::wait_st();
@@ -983,36 +976,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + d;
                 float* dst = p.part + ((long long)slot * N + r0) * D + d;
 #pragma unroll 1
-                for (int f = 0; f < held; f += 8 * kLook) {
-                    float vs[kLook][8];
-#pragma unroll
-                    for (int u = 0; u < kLook; ++u)
-                        if (u == 0 || f + 8 * u < nh) tc::ld8(ot + ci * N + f + 8 * u, vs[u]);
+                for (int g = 0; g < held; g += 8) {
+                    float v[8];
+                    tc::ld8(ot + ci * N + g, v);
                     tc::wait_ld();
                     if (D == 64 && key >= 64) continue;
+                    if (whole) {
+                        // Lanes swap so that each holds two dims of four rows: fewer, wider stores.
+                        const float4 i0 = *reinterpret_cast<const float4*>(&c.inv[r0 + g]), i1 = *reinterpret_cast<const float4*>(&c.inv[r0 + g + 4]);
+                        v[0] *= i0.x, v[1] *= i0.y, v[2] *= i0.z, v[3] *= i0.w;
+                        v[4] *= i1.x, v[5] *= i1.y, v[6] *= i1.z, v[7] *= i1.w;
+                        const bool odd = lane & 1;
+                        const int row = r0 + g + (odd ? 4 : 0);
 #pragma unroll
-                    for (int u = 0; u < kLook; ++u) {
-                        const int g = f + 8 * u;
-                        if (u > 0 && g >= held) break;
-                        float(&v)[8] = vs[u];
-                        if (whole) {
-                            // Lanes swap so that each holds two dims of four rows: fewer, wider stores.
-                            const float4 i0 = *reinterpret_cast<const float4*>(&c.inv[r0 + g]), i1 = *reinterpret_cast<const float4*>(&c.inv[r0 + g + 4]);
-                            v[0] *= i0.x, v[1] *= i0.y, v[2] *= i0.z, v[3] *= i0.w;
-                            v[4] *= i1.x, v[5] *= i1.y, v[6] *= i1.z, v[7] *= i1.w;
-                            const bool odd = lane & 1;
-                            const int row = r0 + g + (odd ? 4 : 0);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float got = __shfl_xor_sync(0xffffffffu, odd ? v[e] : v[e + 4], 1);
-                                const uint32_t two = odd ? pack2<kBf16>(got, v[e + 4]) : pack2<kBf16>(v[e], got);
-                                if (row + e - r0 < held) *reinterpret_cast<uint32_t*>(out + rs.out[row + e] - odd) = two;
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (g + e < held) __stcg(dst + (g + e) * D, v[e]);
+                        for (int e = 0; e < 4; ++e) {
+                            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[e] : v[e + 4], 1);
+                            const uint32_t two = odd ? pack2<kBf16>(got, v[e + 4]) : pack2<kBf16>(v[e], got);
+                            if (row + e - r0 < held) *reinterpret_cast<uint32_t*>(out + rs.out[row + e] - odd) = two;
                         }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (g + e < held) __stcg(dst + (g + e) * D, v[e]);
                     }
                 }
             }
@@ -1117,11 +1102,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     unsigned char* base = ring + (vq + ci) % slots * kSlotBytes;
+                    // Sixteen bytes of key x / (8 kHalves).
+                    const auto piece = [&](int x) {
+                        const int k = x / (8 * kHalves);
+                        return base + (k >> 3) * kRows8 + (x % (8 * kHalves) >> 3) * 1024 + (k & 7) * 128 + (x & 7) * 16;
+                    };
                     const auto zero = [&](int k0, int k1) {
 #pragma unroll 1
                         for (int e = k0 * 8 * kHalves + lane; e < k1 * 8 * kHalves; e += 32)
-                            *reinterpret_cast<uint4*>(base + (e % (8 * kHalves) >> 3) * kBoxBytes + e / (8 * kHalves) * 128 +
-                                                      (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(piece(e)) = make_uint4(0, 0, 0, 0);
                     };
                     zero(0, lead);
                     zero(held, nodes);
@@ -1132,9 +1121,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         uint4 v[8];
 #pragma unroll
                         for (int u = 0; u < 8; ++u) {
-                            const int x = e + u * 32, k = x / (8 * kHalves), cc = x % (8 * kHalves);
+                            const int x = e + u * 32, k = x / (8 * kHalves);
                             v[u] = make_uint4(0, 0, 0, 0);
-                            if (k < mixed || (k >= nodes && k < keys)) v[u] = *reinterpret_cast<const uint4*>(base + (cc >> 3) * kBoxBytes + k * 128 + (cc & 7) * 16);
+                            if (k < mixed || (k >= nodes && k < keys)) v[u] = *reinterpret_cast<const uint4*>(piece(x));
                         }
                         uint32_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -1145,7 +1134,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int u = 0; u < 8; ++u) {
                             const int x = e + u * 32, k = x / (8 * kHalves);
                             if (!(k < mixed || (k >= nodes && k < keys))) continue;
-                            uint16_t* h = reinterpret_cast<uint16_t*>(base + (x % (8 * kHalves) >> 3) * kBoxBytes + k * 128 + (x & 7) * 16);
+                            uint16_t* h = reinterpret_cast<uint16_t*>(piece(x));
 #pragma unroll 1
                             for (int y = 0; y < 8; ++y)
                                 if (not_finite<kBf16>(h[y])) {
@@ -1276,7 +1265,7 @@ cudaError_t make_map(CUtensorMap* m, const void* base, int rank, const cuuint64_
         if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn) return cudaErrorNotSupported;
         encode = reinterpret_cast<EncodeFn>(fn);
     }
-    const cuuint32_t one[4] = {1, 1, 1, 1};
+    const cuuint32_t one[5] = {1, 1, 1, 1, 1};
     const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, const_cast<void*>(base), dims, strides, box, one,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1366,17 +1355,20 @@ cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
     p.by_page = make_div(a.page_size);
     p.by_grid = make_div(grid);
     p.c = a.scale * 1.4426950408889634f;
-    const cuuint64_t row = (cuuint64_t)a.dim * 2, D = a.dim, H = a.kv_heads;
-    const cuuint64_t pool_dims[4] = {D, H, (cuuint64_t)a.page_size, (cuuint64_t)a.pages};
-    const cuuint64_t pool_strides[3] = {row, row * H, (cuuint64_t)a.page_stride * 2};
-    const cuuint32_t pool_box[4] = {64, 1, (cuuint32_t)p.box, 1};
-    const cuuint64_t new_dims[3] = {D, H, (cuuint64_t)a.n_tokens};
-    const cuuint64_t new_strides[2] = {row, (cuuint64_t)a.new_stride * 2};
-    const cuuint32_t new_box[3] = {64, 1, kTreeBox};
+    // A row is H D / 64 blocks of 64 dims; a box takes up to two of them, of eight rows each, so that one
+    // copy lays a slot's rows out in the MMA's eights whatever the number of rows.
+    const cuuint64_t row = (cuuint64_t)a.dim * a.kv_heads * 2, blocks = (cuuint64_t)a.kv_heads * (a.dim / 64);
+    const cuuint32_t wide = a.dim == 64 ? 1 : 2;
+    const cuuint64_t pool_dims[5] = {64, 8, blocks, (cuuint64_t)a.page_size / 8, (cuuint64_t)a.pages};
+    const cuuint64_t pool_strides[4] = {row, 128, row * 8, (cuuint64_t)a.page_stride * 2};
+    const cuuint32_t pool_box[5] = {64, 8, wide, (cuuint32_t)p.box / 8, 1};
+    const cuuint64_t new_dims[3] = {64, (cuuint64_t)a.n_tokens, blocks};
+    const cuuint64_t new_strides[2] = {(cuuint64_t)a.new_stride * 2, 128};
+    const cuuint32_t new_box[3] = {64, kTreeBox, wide};
     CUtensorMap m[4];
     cudaError_t e;
-    if ((e = make_map(&m[0], a.k_pool, 4, pool_dims, pool_strides, pool_box)) != cudaSuccess) return e;
-    if ((e = make_map(&m[1], a.v_pool, 4, pool_dims, pool_strides, pool_box)) != cudaSuccess) return e;
+    if ((e = make_map(&m[0], a.k_pool, 5, pool_dims, pool_strides, pool_box)) != cudaSuccess) return e;
+    if ((e = make_map(&m[1], a.v_pool, 5, pool_dims, pool_strides, pool_box)) != cudaSuccess) return e;
     if ((e = make_map(&m[2], a.k_new, 3, new_dims, new_strides, new_box)) != cudaSuccess) return e;
     if ((e = make_map(&m[3], a.v_new, 3, new_dims, new_strides, new_box)) != cudaSuccess) return e;
     switch (a.dim) {
