@@ -69,10 +69,11 @@ constexpr uint32_t kBoxBytes = kKeys * 128;  // 128 keys x 64 dims of 16 bits
 constexpr int kMaxSlots = 8;
 constexpr int kParts = 4;            // parts the scheduler is ahead
 constexpr int kTreeBox = 8;          // node rows per TMA box: the swizzle's eight
-// And at most so many cached rows: larger boxes leave more places empty between the cached keys and the
-// nodes, smaller ones cost more copies. 8 x 30000 keys, head dims 512 / 128: 251 / 82 us with 16 rows,
-// 237 / 65 with 32, 236 / 67 with 64.
-constexpr int kPageBox = 32;
+// And at most 8 KB of cached rows: larger boxes leave more places empty between the cached keys and the
+// nodes, smaller ones cost more copies. 8 x 30000 keys in 64-row pages, one node each, head dims 512 /
+// 128 / 64: 227 / 79 / 81 us with 8 rows a box, 213 / 64 / 62 with 16, 211 / 66 / 53 with 32, 212 / 66 /
+// 48 with 64.
+constexpr int kBoxCopy = 8192;
 constexpr float kUnset = 1e30f;      // negated reference of a row that has seen no key
 constexpr float kLazy = 8.f;         // a reference moves when a score exceeds it by 2^8
 constexpr size_t kSmemLimit = 232448 - 2048;  // leaves room for blocks of the second kernel
@@ -1343,9 +1344,9 @@ cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
     p.slots = sh.slots;
     p.tmem_cols = sh.tmem;
     // The largest power of two that divides a page, so that a box never crosses one.
-    p.box = std::min(kPageBox, a.page_size & -a.page_size);
+    p.box = std::min(kBoxCopy / (a.dim == 64 ? 128 : 256), a.page_size & -a.page_size);
     while (1 << p.box_log < p.box) ++p.box_log;
-    const long long tiles = ((long long)a.width * a.page_size + 2 * kPageBox + a.max_nodes + kKeys - 1) / kKeys;
+    const long long tiles = ((long long)a.width * a.page_size + 2 * p.box + a.max_nodes + kKeys - 1) / kKeys;
     const long long items = (long long)a.seqs * a.kv_heads * ((a.max_nodes * (a.heads / a.kv_heads) + sh.N - 1) / sh.N);
     if (items * (tiles + kItemCost) > INT32_MAX) return cudaErrorInvalidConfiguration;  // units are counted in 32 bits
     p.whole = tiles <= kWholeTiles;
