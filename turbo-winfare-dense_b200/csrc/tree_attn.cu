@@ -18,8 +18,14 @@
 // Per tile, S^T[key][row] = K Q^T and O^T[dim][row] += V^T P^T: with the keys and the dimensions on
 // the 128-lane side of the MMA the row count is its N, so a tree of 5 nodes costs N = 16 and not a
 // padded 128. Roles:
+//   * one warp deals the block's share out in parts and sets their rows up, one brings their queries in
+//     (as its own warp it is done before the part ahead is: with one warp for both, which took 18000
+//     cycles over 128 rows of 256, 64-node trees took 160 us instead of 137);
 //   * one warp streams K of tile t + 1, then V of tile t, through a ring of 32 KB slots (128 keys x
-//     128 dims) by TMA: one box per (page part, 64 dims), swizzled as the MMA reads it;
+//     128 dims) by TMA: one box per page part, both 64-dim blocks of it, laid out in eights of keys as the
+//     MMA reads them (a copy per block was the limit at 16-row pages: 106 us instead of 87 for 1-node
+//     trees over a 1024-key window; slots of 16 KB, which use what is left of shared memory, need more
+//     copies and are no faster);
 //   * one thread of another issues the MMAs, S^T into two alternating TMEM buffers;
 //   * four groups of four warps take a quarter of the rows each, a thread one key of all its rows: they
 //     hold the softmax in fp32, write P^T (rounded to the cache's type, 8 rows a store) and, when a
@@ -27,18 +33,19 @@
 //     reference and rescale that row of O^T in TMEM. In between only a vote of the group is needed,
 //     so most tiles run without any reduction over keys; the sums are reduced once per part.
 // What a node must not see never reaches the MMA: scores are replaced, not added to, and in tiles
-// that hold hidden keys the rows of V past the end are zeroed; an infinity or NaN in a V row that
-// some nodes see and others do not is taken out of the product and added back for those that do.
+// that hold hidden keys the softmax warps clean V before it is used: rows that no node sees are zeroed; an
+// infinity or NaN in a V row that some nodes see and others do not is taken out of the product and added
+// back for those that do.
 //
 // Every wait is bounded (2 s); a block that gives up records it in a device word and leaves.
 //
 // Measured on one B200 (device time; GB/s of keys, values, queries and outputs read or written once):
-// 8 sequences of up to 30000 keys, 9 nodes, 32 heads on 4 of 512: 236 us, 5870 GB/s, 0.90 of the
-// measured copy rate; one node each: 215 us. 32 sequences, 64 nodes, 32 heads on 16 of 256, a window of
-// 1024 keys: 182 us, 3110 GB/s: 512 short items of ten tiles, whose starts and ends (queries in, first
-// maxima, masks, outputs) cost about two tiles each, and at 128 rows the softmax of a tile, about 5000
-// cycles, is as long as its loads. One node of one sequence of 96 keys: 8 us, a chain of latencies:
-// launch, lengths, table, keys, two products, output.
+// 8 sequences of up to 30000 keys, 9 nodes, 32 heads on 4 of 512: 235 us, 5900 GB/s, 0.90 of the
+// measured copy rate; one node each: 213 us. 32 sequences, 64 nodes, 32 heads on 16 of 256, a window of
+// 1024 keys: 131 us, 4300 GB/s: 512 short items of ten tiles, whose starts and ends (first maxima, sums,
+// outputs) cost about three tiles each, and at 128 rows the softmax of a tile, about 4500 cycles, is as
+// long as its loads; with 32 nodes 100 us, with one 85. One node of one sequence of 96 keys: 8 us, a chain
+// of latencies: launch, lengths, table, keys, two products, output.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -59,10 +66,11 @@ namespace {
 
 constexpr int kKeys = 128;           // keys per tile: the M of S^T
 constexpr int kSoftWarps = 16;       // warps 0 .. 15, four groups of four
-constexpr int kProducer = 16, kIssuer = 17, kScheduler = 18;  // and 19, the cleaner
+constexpr int kProducer = 16, kIssuer = 17, kScheduler = 18;  // and 19, the queries
 constexpr int kThreads = 640;
 // With two groups of twice the rows the row sums alone took 64 registers and spilled: 319 us instead of
-// 259 for 9-node trees over 30000 keys.
+// 259 for 9-node trees over 30000 keys. Scores held in registers from the look at their maxima to their
+// exponentials spill too (193 us instead of 157 with 64-node trees): they are read from TMEM twice.
 // Registers a thread: 96 at launch; 512 x 104 + 128 x 64 is the same total.
 constexpr int kSoftRegs = 104, kOtherRegs = 64;
 constexpr uint32_t kBoxBytes = kKeys * 128;  // 128 keys x 64 dims of 16 bits
@@ -77,10 +85,10 @@ constexpr int kBoxCopy = 8192;
 constexpr float kUnset = 1e30f;      // negated reference of a row that has seen no key
 constexpr float kLazy = 8.f;         // a reference moves when a score exceeds it by 2^8
 constexpr size_t kSmemLimit = 232448 - 2048;  // leaves room for blocks of the second kernel
-// What starting and finishing an item costs, in tiles, when the shares are cut. Measured with 64-node
-// trees over a 1024-key window (512 items): 226 us at 1, 182 at 2 and 3, 184 at 5; at 30000 keys it
-// does not matter.
-constexpr int kItemCost = 2;
+// What starting and finishing an item costs, in tiles, when the shares are cut: it grows with the rows,
+// the tiles' time less so. 128 rows an item, dim 256: 131 us over a 1024-key window and 282 over up to
+// 4096 keys at 3, 137 and 303 at 2; 64 rows, 12-node trees, dim 128: 22.9 us at 3, 21.4 at 2.
+__host__ __device__ constexpr int item_cost(int rows) { return rows > 64 ? 3 : 2; }
 // Items of at most this many tiles are not split, which saves the second kernel: one sequence of 300
 // keys takes 10.5 us so and 11.1 split, one of 600 (5 tiles) 13.5 and 12.2.
 constexpr int kWholeTiles = 4;
@@ -113,6 +121,7 @@ struct alignas(16) Ctl {
     uint64_t q_ready[2], q_free, rows_free[2], p_full, o_done, v_ready[4], v_fix[4], done;
     uint32_t tmem_base;
     int abort, poison[2];
+    int v_at[4];                  // slot and phase of an edge tile's V, 128 dims each
     int scan[kThreads / 32];      // units of each warp's run of sequences
     alignas(16) float corr[128];  // factor of a row's sum and output when its reference moves
     alignas(16) float inv[128];
@@ -209,8 +218,8 @@ __device__ __forceinline__ void derive_seq(const Params& p, Seq& s) {
     s.groups = p.by_rows.quot(s.n * p.gqa + p.N - 1);
 }
 
-// An item is as long as its tiles and kItemCost more, ahead of them; 1 where items stay whole.
-__device__ __forceinline__ int item_units(const Params& p, const Seq& s) { return p.whole ? 1 : s.tiles + kItemCost; }
+// An item is as long as its tiles and item_cost(p.N) more, ahead of them; 1 where items stay whole.
+__device__ __forceinline__ int item_units(const Params& p, const Seq& s) { return p.whole ? 1 : s.tiles + item_cost(p.N); }
 __device__ __forceinline__ int seq_units(const Params& p, const Seq& s) {
     return s.tiles ? item_units(p, s) * s.groups * p.kv_heads : 0;
 }
@@ -338,8 +347,8 @@ __device__ __forceinline__ void schedule(const Params& p, Ctl& c, volatile int* 
             }
             const int v = min(item, u + (end - pos));
             pos += v - u;
-            t0 = p.whole ? 0 : max(0, u - kItemCost);
-            t1 = p.whole ? s.tiles : max(0, v - kItemCost);
+            t0 = p.whole ? 0 : max(0, u - item_cost(p.N));
+            t1 = p.whole ? s.tiles : max(0, v - item_cost(p.N));
             u = v;
         }
         if (!p.whole && t0 < t1 && t0 == 0 && t1 < s.tiles) {
@@ -406,19 +415,9 @@ __device__ __forceinline__ void tma_5d(void* dst, uint64_t map, int x, int y, in
         : "memory");
 }
 
-// 8 or 16 consecutive tensor-memory columns of this thread's lane.
-__device__ __forceinline__ void load16(uint32_t ta, bool both, float (&v)[16]) {
-    if (both) {
-        tc::ld16(ta, v);
-    } else {
-        float h[8];
-        tc::ld8(ta, h);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = h[j];
-    }
-    tc::wait_ld();
+__device__ __forceinline__ void st_shared_zero(uint32_t dst) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
 }
-
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -477,6 +476,45 @@ __device__ __forceinline__ bool sees(const Params& p, const Part& w, const Rows&
     return !p.window || c.depth[r] - min(max(p.depth[w.first + j], 0), w.n - 1) < p.window;
 }
 
+__device__ __forceinline__ unsigned low_bits(int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1; }
+
+// Bit j of lane i's word becomes bit i of lane j's.
+__device__ __forceinline__ unsigned transpose_bits(unsigned x, int lane) {
+    unsigned m = 0x0000ffff;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1, m ^= m << o) {
+        const unsigned y = __shfl_xor_sync(0xffffffffu, x, o);
+        x = lane & o ? (x & ~m) | ((y >> o) & m) : (x & m) | ((y << o) & ~m);
+    }
+    return x;
+}
+
+// Which rows of a group (up to 32) see this lane's key: cached position at + lane, or node j0 + lane from
+// there on. A lane puts one row's view of the 32 keys together, from its `start` and its words of `mask`
+// (N apart), and the warp turns the words over. Not inlined: the callers' sums stay in registers.
+__device__ __forceinline__ unsigned seen_by(const int* start, const uint32_t* mask, int N, int at, int len, int j0, int n, int lane) {
+    unsigned word = low_bits(len - at) & ~low_bits(*start - at);
+    if (j0 > -32 && j0 < n) {
+        unsigned low = mask[(max(j0, 0) >> 5) * N], high = 0;
+        if (j0 < 0) low <<= -j0;
+        else {
+            if ((j0 | 31) + 1 < n) high = mask[((j0 >> 5) + 1) * N];
+            low = __funnelshift_r(low, high, j0 & 31);
+        }
+        word |= low & low_bits(n - j0);
+    }
+    return transpose_bits(word, lane);
+}
+// Takes out the rows whose nodes are `window` or more levels below node j.
+__device__ __forceinline__ unsigned within(unsigned seen, const int* row_depth, int rows, const int* depth, int j, int n, int window) {
+    if (j < 0 || j >= n) return seen;
+    const int near = min(max(depth[j], 0), n - 1) + window;
+#pragma unroll 1
+    for (int k = 0; k < rows; ++k)
+        if (row_depth[k] >= near) seen &= ~(1u << k);
+    return seen;
+}
+
 // V's row at place x (null: no such row).
 __device__ const uint16_t* v_row(const Params& p, const Part& w, int x, int dim) {
     if (x < w.pre) {
@@ -506,19 +544,27 @@ __device__ __noinline__ float poison_of(const Params& p, Part w, Rows c, int dim
     return sum;
 }
 
-// Adds 0 x each of eight values to four pairs of sums, which become NaN by an infinity or NaN.
-template <bool kBf16>
-__device__ __forceinline__ void test_finite(const uint4& v, uint32_t (&sum)[4]) {
-    if (kBf16) {
-        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[0]) : "r"(v.x), "r"(0));
-        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[1]) : "r"(v.y), "r"(0));
-        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[2]) : "r"(v.z), "r"(0));
-        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum[3]) : "r"(v.w), "r"(0));
-    } else {
-        asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum[0]) : "r"(v.x), "r"(0));
-        asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum[1]) : "r"(v.y), "r"(0));
-        asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum[2]) : "r"(v.z), "r"(0));
-        asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum[3]) : "r"(v.w), "r"(0));
+// V of an edge tile, 64 x kHalves dims of it: keys 0 .. lead - 1, held .. nodes - 1 and from `keys` to the
+// MMA's next step of 16 are nobody's and become zeros; keys lead .. mixed - 1 and nodes .. keys - 1 lose
+// their infinities and NaN, which is noted in *found. All softmax warps.
+template <int kHalves, bool kBf16>
+__device__ __forceinline__ void clean_v(unsigned char* slot, int lead, int mixed, int held, int nodes, int keys, volatile int* found) {
+#pragma unroll 1
+    for (int x = threadIdx.x; x < ((keys + 15) & ~15) * 8 * kHalves; x += kSoftWarps * 32) {
+        const int k = x / (8 * kHalves);  // sixteen bytes of this key
+        uint4* at = reinterpret_cast<uint4*>(slot + (k >> 3) * (kHalves * 1024) + (x % (8 * kHalves) >> 3) * 1024 + (k & 7) * 128 + (x & 7) * 16);
+        if (k < lead || (k >= held && k < nodes) || k >= keys) {
+            *at = make_uint4(0, 0, 0, 0);
+        } else if (k < mixed || k >= nodes) {
+            const uint4 v = *at;
+            const uint32_t bits = kBf16 ? 0x7f807f80u : 0x7c007c00u;  // the exponents
+            if (!(__vcmpeq2(v.x & bits, bits) | __vcmpeq2(v.y & bits, bits) | __vcmpeq2(v.z & bits, bits) | __vcmpeq2(v.w & bits, bits))) continue;
+            uint16_t* h = reinterpret_cast<uint16_t*>(at);
+#pragma unroll 1
+            for (int y = 0; y < 8; ++y)
+                if (not_finite<kBf16>(h[y])) h[y] = 0;
+            *found = 1;
+        }
     }
 }
 
@@ -553,12 +599,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         init(0, kMaxSlots, c.empty, 1);
         init(8, 2, c.s_full, 1);
         init(8, 2, c.s_free, kSoftWarps);
-        init(10, 2, c.q_ready, 1);
+        init(10, 2, c.q_ready, 2);
         init(10, 2, c.rows_free, kSoftWarps);
         init(12, kParts, c.part_full, 1);
         init(12, kParts, c.part_free, kSoftWarps + 3);
         init(16, 4, c.v_ready, 1);
-        init(16, 4, c.v_fix, 1);
+        init(16, 4, c.v_fix, kSoftWarps);
         init(20, 1, &c.q_free, 1);
         init(21, 1, &c.p_full, kSoftWarps);
         init(22, 1, &c.o_done, 1);
@@ -669,6 +715,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         // V chunks that fit the ring beside nothing else: the cleaning of an edge tile's first ones
         // can start before its P is there.
         const int ahead = min(kChunks, slots);
+        const auto show_v = [&](int ci, const Place& x) {
+            *(volatile int*)&c.v_at[ci] = 2 * x.slot + x.phase;
+            mbar_arrive(&c.v_ready[ci]);
+        };
         Place at;
         int tile = 0, otile = 0, part = 0, fix = 0;
         bool ok = true;
@@ -715,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                     for (int ci = 0; ci < ahead && edge; ++ci) {
                         ok = ok && wait(&c.full[look.slot], look.phase, abort);
-                        if (leader) mbar_arrive(&c.v_ready[ci]);
+                        if (leader) show_v(ci, look);
                         look.step(slots);
                     }
                     ok = ok && wait(&c.p_full, otile & 1, abort);
@@ -723,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int ci = 0; ci < kChunks; ++ci) {
                         ok = ok && wait(&c.full[at.slot], at.phase, abort);
                         if (edge) {  // cleaned first
-                            if (ci >= ahead && leader) mbar_arrive(&c.v_ready[ci]);
+                            if (ci >= ahead && leader) show_v(ci, at);
                             ok = ok && wait(&c.v_fix[ci], fix & 1, abort);
                         }
                         ok = __all_sync(0xffffffffu, ok);
@@ -768,7 +818,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The group's rows r0 .. r0 + nh - 1, in eights; with few rows some groups have none.
         const int r0 = (N >> 3) * grp / 4 * 8, nh = (N >> 3) * (grp + 1) / 4 * 8 - r0;
         const uint32_t lanes = (uint32_t)(qd * 32) << 16;
-        int tile = 0;
+        int tile = 0, fix = 0;
         float l[kNH];
         // After a wait that gave up, these warps go on (on meaningless values) to the end of the share:
         // none of them may leave while others stand at a barrier of the group.
@@ -790,14 +840,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 tc::fence_after_sync();
                 const bool edge = w.edge(p.window, i);
-                // This thread's place in the line of keys, and what a row is asked about it: its first
-                // position, or the node's word of its mask.
-                const int x = i * kKeys + key;
-                const bool old = x < w.pre;
-                const int j = old ? w.base + x : x - w.pre;
-                const bool in = j < (old ? w.len : w.n), fresh = i == w.t0;
-                const int near = edge && p.window && in && !old ? min(max(p.depth[w.first + j], 0), w.n - 1) + p.window : INT_MAX;
-                const int* ask = old || !in ? rs.start + r0 : reinterpret_cast<const int*>(rs.mask) + (j >> 5) * N + r0;
+                const bool fresh = i == w.t0;
+                unsigned seen = ~0u;
+                if (edge) {
+                    const int x0 = i * kKeys + qd * 32, r = min(r0 + lane, N - 1);
+                    seen = seen_by(rs.start + r, rs.mask + r, N, w.base + x0, w.len, x0 - w.pre, w.n, lane);
+                    if (p.window && p.window < w.n) seen = within(seen, rs.depth + r0, nh, p.depth + w.first, x0 - w.pre + lane, w.n, p.window);
+                }
                 // First look. Hidden scores become -inf, in tensor memory too. In a part's first tile each
                 // row's maximum is taken; later it matters whether a score exceeds its row's reference by
                 // more than kLazy. The scores are read again for the exponentials, which leaves the
@@ -809,19 +858,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc::ld8(st + g, v);
                     tc::wait_ld();
                     if (edge) {
-                        int a[8];
-                        *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(ask + g);
-                        *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(ask + g + 4);
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            if (!(in && (old ? j >= a[k] : ((unsigned)a[k] >> (j & 31)) & 1u))) v[k] = -INFINITY;
-                        if (p.window && i * kKeys + kKeys > w.pre) {  // nodes further apart than the window
-                            *reinterpret_cast<int4*>(a) = *reinterpret_cast<const int4*>(rs.depth + r0 + g);
-                            *reinterpret_cast<int4*>(a + 4) = *reinterpret_cast<const int4*>(rs.depth + r0 + g + 4);
-#pragma unroll
-                            for (int k = 0; k < 8; ++k)
-                                if (a[k] >= near) v[k] = -INFINITY;
-                        }
+                            if (!((seen >> g >> k) & 1)) v[k] = -INFINITY;
                         tc::st8(st + g, v);
                     }
                     if (fresh) {
@@ -890,43 +929,64 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc::wait_st();
                     }
                 }
-                uint32_t pk[kNH / 2];
+                // P V of the tile before has read the buffer.
+                if (!waited) wait(&c.o_done, (tile - 1) & 1, abort);
+                unsigned char* const prow = ps + key * 128;
 #pragma unroll
-                for (int f = 0; f < kNH; f += 16)
+                for (int f = 0; f < kNH; f += 8)
                     if (f < nh) {
-                        float v[16];
-                        load16(st + f, kNH > 8 && f + 8 < nh, v);
+                        float v[8];
+                        tc::ld8(st + f, v);
+                        tc::wait_ld();
+                        uint32_t pk[4];
 #pragma unroll
-                        for (int r = 0; r < 16; r += 4)
-                            if (f + r < kNH && f + r < nh) {
-                                const float4 n = *reinterpret_cast<const float4*>(&rs.nref[r0 + f + r]);
-                                const float e0 = exp2_approx(fmaf(v[r], p.c, n.x)), e1 = exp2_approx(fmaf(v[r + 1], p.c, n.y));
-                                const float e2 = exp2_approx(fmaf(v[r + 2], p.c, n.z)), e3 = exp2_approx(fmaf(v[r + 3], p.c, n.w));
-                                l[f + r] += e0;
-                                l[f + r + 1] += e1;
-                                l[f + r + 2] += e2;
-                                l[f + r + 3] += e3;
-                                pk[(f + r) / 2] = pack2<kBf16>(e0, e1);
-                                pk[(f + r) / 2 + 1] = pack2<kBf16>(e2, e3);
-                            }
+                        for (int r = 0; r < 8; r += 4) {
+                            const float4 n = *reinterpret_cast<const float4*>(&rs.nref[r0 + f + r]);
+                            const float e0 = exp2_approx(fmaf(v[r], p.c, n.x)), e1 = exp2_approx(fmaf(v[r + 1], p.c, n.y));
+                            const float e2 = exp2_approx(fmaf(v[r + 2], p.c, n.z)), e3 = exp2_approx(fmaf(v[r + 3], p.c, n.w));
+                            l[f + r] += e0;
+                            l[f + r + 1] += e1;
+                            l[f + r + 2] += e2;
+                            l[f + r + 3] += e3;
+                            pk[r / 2] = pack2<kBf16>(e0, e1);
+                            pk[r / 2 + 1] = pack2<kBf16>(e2, e3);
+                        }
+                        const int r = r0 + f;
+                        *reinterpret_cast<uint4*>(prow + (r >> 6) * kBoxBytes + ((((r & 63) >> 3) ^ (key & 7)) << 4)) =
+                            make_uint4(pk[0], pk[1], pk[2], pk[3]);
                     }
                 tc::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.s_free[b]);
-                // P V of the tile before has read the buffer.
-                if (!waited) wait(&c.o_done, (tile - 1) & 1, abort);
-                const uint32_t prow = key * 128;
-#pragma unroll
-                for (int e = 0; e < kNH / 8; ++e)
-                    if (8 * e < nh) {
-                        const int r = r0 + 8 * e;
-                        *reinterpret_cast<uint4*>(ps + (r >> 6) * kBoxBytes + prow + ((((r & 63) >> 3) ^ (key & 7)) << 4)) =
-                            make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
-                    }
                 fence_proxy_async();
                 tc::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.p_full);
+
+                if (edge) {
+                    // V's rows that no row may see become zeros (they may hold anything, and 0 x NaN is NaN);
+                    // rows that only some see lose their infinities and NaN, which are noted and added to those
+                    // rows' outputs. Nobody's rows: before every window, from the sequence's end to its first
+                    // node, past the last node. Rows that some see and others do not: where windows start, and
+                    // the nodes.
+                    const int keys = w.keys(i), at = w.base + i * kKeys, nodes = min(kKeys, max(0, w.pre - i * kKeys));
+                    const int held = min(nodes, max(0, w.len - at));
+                    const int lead = max(0, min(held, w.start - at));
+                    const int mixed = p.window ? min(held, max(lead, w.start + w.n - 1 - at)) : lead;
+#pragma unroll 1
+                    for (int ci = 0; ci < kChunks; ++ci) {
+                        // The issuing warp shows where V is once it is there: the slot might still be a use
+                        // behind, and a parity cannot tell a phase from the one two before it.
+                        bool ok = wait(&c.v_ready[ci], fix & 1, abort);
+                        const int v_at = *(volatile int*)&c.v_at[ci];
+                        ok = ok && wait(&c.full[v_at >> 1], v_at & 1, abort);
+                        if (ok) clean_v<kHalves, kBf16>(ring + (v_at >> 1) * kSlotBytes, lead, mixed, held, nodes, keys, &c.poison[part & 1]);
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&c.v_fix[ci]);
+                    }
+                    ++fix;
+                }
             }
 
             // The part's result: sums over the keys, then O^T.
@@ -1009,46 +1069,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == kScheduler) {
         // ------------------------------------------------------------------ scheduler
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        // Deals the parts out, and sets up each part's rows and queries while the one before is worked on.
+        // Deals the parts out, and sets up each part's rows while the one before is worked on.
         int part = 0;
         schedule(p, c, abort, [&](const Part& w) {
-            const int par = part & 1, row0 = w.g * N, R = min(N, w.n * p.gqa - row0);
+            const int par = part & 1, row0 = w.g * N;
             const Rows rs = rows_of(rows_at, N, p.words, par);
-            // The queries, into the MMA's K-major layout, once S of the part before has completed. Rows of
-            // a part: r -> node (g N + r) / gqa, query head h gqa + (g N + r) % gqa.
-            bool ok = part == 0 || wait(&c.q_free, (part - 1) & 1, abort);
-            constexpr int kLanes = D / 8 < 32 ? D / 8 : 32;      // lanes on one row, 16 bytes each
-            const uint32_t q_at = smem_u32(qs);
-            constexpr int kStep = 32 / kLanes, kBatch = 4;       // rows at once; such rounds unrolled
-            const int ch = lane % kLanes;
-            const int q_col = q_at + (ch >> 3) * N * 128, c7 = ch & 7;
-            // Row r + kStep is kStep heads on, or in a later node: no division inside the loop.
-            int r = lane / kLanes, node = p.by_gqa.quot(row0 + r), hd = row0 + r - node * p.gqa;
-            const char* src = p.q + 2 * ((w.first + node) * p.q_stride + (w.h * p.gqa + hd) * D + ch * 8);
-            const long long next_head = 2 * kStep * D, next_node = 2 * (p.q_stride - (long long)p.gqa * D);
-#pragma unroll 1
-            for (; r - lane / kLanes < R; r += kBatch * kStep) {
-#pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    const int x = r + u * kStep;
-                    if (x < R)
-#pragma unroll
-                        for (int k = 0; k < D / 8 / kLanes; ++k)
-                            cp_async16(q_col + x * 128 + ((c7 ^ (x & 7)) << 4) + k * (kLanes / 8) * N * 128, src + k * kLanes * 16);
-                    src += next_head;
-                    hd += kStep;
-                    while (hd >= p.gqa) {
-                        hd -= p.gqa;
-                        src += next_node;
-                    }
-                }
-            }
-#pragma unroll 1
-            for (int x = R + lane / kLanes; x < N; x += kStep)   // rows that do not exist
-#pragma unroll
-                for (int k = 0; k < D / 8 / kLanes; ++k)
-                    *reinterpret_cast<uint4*>(qs + (q_col - q_at) + x * 128 + ((c7 ^ (x & 7)) << 4) + k * (kLanes / 8) * N * 128) = make_uint4(0, 0, 0, 0);
-            ok = ok && (part < 2 || wait(&c.rows_free[par], ((part >> 1) - 1) & 1, abort));
+            // Rows of a part: r -> node (g N + r) / gqa, query head h gqa + (g N + r) % gqa.
+            const bool ok = part < 2 || wait(&c.rows_free[par], ((part >> 1) - 1) & 1, abort);
             ++part;
             if (!__all_sync(0xffffffffu, ok)) return false;
 #pragma unroll 1
@@ -1063,94 +1090,47 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = 0; i * 32 < w.n; ++i) rs.mask[i * N + r] = p.mask[(long long)tok * p.mask_words + i];
             }
             if (lane == 0) c.poison[par] = 0;
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&c.q_ready[par]);
             return true;
         });
     } else {
-        // ------------------------------------------------------------------ cleaner
+        // ------------------------------------------------------------------ queries
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        // In tiles with hidden keys, V's rows that no row may see become zeros (they may hold anything,
-        // and 0 x NaN is NaN); rows that only some see lose their infinities and NaN, which are noted and
-        // added to those rows' outputs.
+        // Each part's queries into the MMA's K-major layout, once S of the part before has completed.
+        constexpr int kLanes = D / 8 < 32 ? D / 8 : 32, kStep = 32 / kLanes;  // lanes on one row, 16 bytes each; rows at once
+        const int ch = lane % kLanes, sub = lane / kLanes;
+        const uint32_t q_at = smem_u32(qs) + (ch >> 3) * N * 128;
         Part w;
         Place list;
-        int q = 0, fix = 0;  // ring slots, as the producer counts them, and edge tiles so far
-        bool ok = true;
 #pragma unroll 1
-        for (int part = 0; ok; ++part) {
-            ok = __all_sync(0xffffffffu, next_part(c, list, w, false, abort));
+        for (int part = 0;; ++part) {
+            bool ok = __all_sync(0xffffffffu, next_part(c, list, w, false, abort));
             if (lane == 0) mbar_arrive(&c.part_free[(list.slot + kParts - 1) % kParts]);
-            if (!ok) break;
+            ok = ok && (part == 0 || wait(&c.q_free, (part - 1) & 1, abort));
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const int row0 = w.g * N, R = min(N, w.n * p.gqa - row0);
 #pragma unroll 1
-            for (int i = w.t0; i < w.t1; ++i) {
-                if (!w.edge(p.window, i)) continue;
-                // V(i) comes after K(t0) .. K(i + 1) and V(t0) .. V(i - 1).
-                const int vq = q + (i - w.t0) * 2 * kChunks + (i + 1 < w.t1 ? 2 : 1) * kChunks;
-                // Nobody's rows: before every window, from the sequence's end to its first node, past the
-                // last node. Rows that some see and others do not: where windows start, and the nodes.
-                const int keys = w.keys(i), at = w.base + i * kKeys, nodes = min(kKeys, max(0, w.pre - i * kKeys));
-                const int held = min(nodes, max(0, w.len - at));
-                const int lead = max(0, min(held, w.start - at));
-                const int mixed = p.window ? min(held, max(lead, w.start + w.n - 1 - at)) : lead;
-#pragma unroll 1
-                for (int ci = 0; ci < kChunks && ok; ++ci) {
-                    // v_ready first: the slot may still be a use behind, and a parity cannot tell a phase
-                    // from the one two before it.
-                    ok = wait(&c.v_ready[ci], fix & 1, abort) && wait(&c.full[(vq + ci) % slots], ((vq + ci) / slots) & 1, abort);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    unsigned char* base = ring + (vq + ci) % slots * kSlotBytes;
-                    // Sixteen bytes of key x / (8 kHalves).
-                    const auto piece = [&](int x) {
-                        const int k = x / (8 * kHalves);
-                        return base + (k >> 3) * kRows8 + (x % (8 * kHalves) >> 3) * 1024 + (k & 7) * 128 + (x & 7) * 16;
-                    };
-                    const auto zero = [&](int k0, int k1) {
-#pragma unroll 1
-                        for (int e = k0 * 8 * kHalves + lane; e < k1 * 8 * kHalves; e += 32)
-                            *reinterpret_cast<uint4*>(piece(e)) = make_uint4(0, 0, 0, 0);
-                    };
-                    zero(0, lead);
-                    zero(held, nodes);
-                    zero(keys, (keys + 15) & ~15);
-#pragma unroll 1
-                    for (int e = lead * 8 * kHalves + lane; e < keys * 8 * kHalves; e += 8 * 32) {
-                        if (e >= mixed * 8 * kHalves && e + 7 * 32 < nodes * 8 * kHalves) continue;
-                        uint4 v[8];
+            for (int r = 0; r < N; r += 32) {
+                // A row's place is worked out by one lane and handed to those that copy it.
+                const int node = p.by_gqa.quot(row0 + r + lane), hd = row0 + r + lane - node * p.gqa;
+                const long long mine = (w.first + node) * p.q_stride + (w.h * p.gqa + hd) * D;
+#pragma unroll 4
+                for (int u = sub; u < 32; u += kStep) {
+                    const long long from = __shfl_sync(0xffffffffu, mine, u);
+                    const int x = r + u;
+                    const uint32_t to = q_at + x * 128 + (((ch ^ x) & 7) << 4);
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            const int x = e + u * 32, k = x / (8 * kHalves);
-                            v[u] = make_uint4(0, 0, 0, 0);
-                            if (k < mixed || (k >= nodes && k < keys)) v[u] = *reinterpret_cast<const uint4*>(piece(x));
-                        }
-                        uint32_t sum[4] = {0, 0, 0, 0};
-#pragma unroll
-                        for (int u = 0; u < 8; ++u) test_finite<kBf16>(v[u], sum);
-                        // The sums are zeros, of either sign, or NaN.
-                        if (!((sum[0] | sum[1] | sum[2] | sum[3]) & 0x7fff7fffu)) continue;
-#pragma unroll 1
-                        for (int u = 0; u < 8; ++u) {
-                            const int x = e + u * 32, k = x / (8 * kHalves);
-                            if (!(k < mixed || (k >= nodes && k < keys))) continue;
-                            uint16_t* h = reinterpret_cast<uint16_t*>(piece(x));
-#pragma unroll 1
-                            for (int y = 0; y < 8; ++y)
-                                if (not_finite<kBf16>(h[y])) {
-                                    h[y] = 0;
-                                    c.poison[part & 1] = 1;
-                                }
-                        }
+                    for (int k = 0; k < D / 8 / kLanes; ++k) {
+                        if (x < R) cp_async16(to + k * (kLanes / 8) * N * 128, p.q + 2 * (from + ch * 8 + k * kLanes * 8));
+                        else if (x < N) st_shared_zero(to + k * (kLanes / 8) * N * 128);
                     }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&c.v_fix[ci]);
                 }
-                ++fix;
             }
-            q += (w.t1 - w.t0) * 2 * kChunks;
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c.q_ready[part & 1]);
         }
     }
     tc::fence_before_sync();
@@ -1348,7 +1328,7 @@ cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
     while (1 << p.box_log < p.box) ++p.box_log;
     const long long tiles = ((long long)a.width * a.page_size + 2 * p.box + a.max_nodes + kKeys - 1) / kKeys;
     const long long items = (long long)a.seqs * a.kv_heads * ((a.max_nodes * (a.heads / a.kv_heads) + sh.N - 1) / sh.N);
-    if (items * (tiles + kItemCost) > INT32_MAX) return cudaErrorInvalidConfiguration;  // units are counted in 32 bits
+    if (items * (tiles + item_cost(sh.N)) > INT32_MAX) return cudaErrorInvalidConfiguration;  // units are counted in 32 bits
     p.whole = tiles <= kWholeTiles;
     if (p.whole) grid = (int)std::min<long long>(grid, items);
     p.by_rows = make_div(sh.N);
