@@ -42,8 +42,8 @@
 // Measured on one B200 (device time; GB/s of keys, values, queries and outputs read or written once):
 // 8 sequences of up to 30000 keys, 9 nodes, 32 heads on 4 of 512: 235 us, 5900 GB/s, 0.90 of the
 // measured copy rate; one node each: 213 us. 32 sequences, 64 nodes, 32 heads on 16 of 256, a window of
-// 1024 keys: 131 us, 4300 GB/s: 512 short items of ten tiles, whose starts and ends (first maxima, sums,
-// outputs) cost about three tiles each, and at 128 rows the softmax of a tile, about 4500 cycles, is as
+// 1024 keys: 126 us, 4470 GB/s: 512 short items of ten tiles, whose starts and ends (first maxima, sums,
+// outputs) cost three tiles each, and at 128 rows the softmax of a tile, about 4500 cycles, is as
 // long as its loads; with 32 nodes 100 us, with one 85. One node of one sequence of 96 keys: 8 us, a chain
 // of latencies: launch, lengths, table, keys, two products, output.
 #include <cuda.h>
@@ -1098,9 +1098,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ------------------------------------------------------------------ queries
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         // Each part's queries into the MMA's K-major layout, once S of the part before has completed.
-        constexpr int kLanes = D / 8 < 32 ? D / 8 : 32, kStep = 32 / kLanes;  // lanes on one row, 16 bytes each; rows at once
-        const int ch = lane % kLanes, sub = lane / kLanes;
-        const uint32_t q_at = smem_u32(qs) + (ch >> 3) * N * 128;
+        // Eight rows at once, four lanes on 64 bytes of each: a lane's rows all have its place in the swizzle.
+        const int sub = lane >> 2, q4 = lane & 3;
+        const uint32_t q_at = smem_u32(qs), even = (q4 ^ sub) << 4, odd = ((q4 + 4) ^ sub) << 4;
         Part w;
         Place list;
 #pragma unroll 1
@@ -1110,20 +1110,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = ok && (part == 0 || wait(&c.q_free, (part - 1) & 1, abort));
             if (!__all_sync(0xffffffffu, ok)) break;
             const int row0 = w.g * N, R = min(N, w.n * p.gqa - row0);
-#pragma unroll 1
-            for (int r = 0; r < N; r += 32) {
-                // A row's place is worked out by one lane and handed to those that copy it.
-                const int node = p.by_gqa.quot(row0 + r + lane), hd = row0 + r + lane - node * p.gqa;
-                const long long mine = (w.first + node) * p.q_stride + (w.h * p.gqa + hd) * D;
-#pragma unroll 4
-                for (int u = sub; u < 32; u += kStep) {
-                    const long long from = __shfl_sync(0xffffffffu, mine, u);
-                    const int x = r + u;
-                    const uint32_t to = q_at + x * 128 + (((ch ^ x) & 7) << 4);
+#pragma unroll 2
+            for (int r = sub; r < N; r += 8) {
+                const int node = p.by_gqa.quot(row0 + r), hd = row0 + r - node * p.gqa;
+                const char* from = p.q + 2 * ((w.first + node) * p.q_stride + (w.h * p.gqa + hd) * D + q4 * 8);
+                uint32_t to = q_at + r * 128;
 #pragma unroll
-                    for (int k = 0; k < D / 8 / kLanes; ++k) {
-                        if (x < R) cp_async16(to + k * (kLanes / 8) * N * 128, p.q + 2 * (from + ch * 8 + k * kLanes * 8));
-                        else if (x < N) st_shared_zero(to + k * (kLanes / 8) * N * 128);
+                for (int k = 0; k < D / 32; k += 2, to += N * 128) {
+                    if (r < R) {
+                        cp_async16(to + even, from + k * 64);
+                        cp_async16(to + odd, from + k * 64 + 64);
+                    } else {
+                        st_shared_zero(to + even);
+                        st_shared_zero(to + odd);
                     }
                 }
             }
