@@ -342,3 +342,23 @@ def test_refusals(built_lib):
         api.tree_attention_workspace(3, 4, 2, 96)
     with pytest.raises(ValueError, match="multiple"):
         api.tree_attention_workspace(3, 5, 2, 64)
+
+
+@pytest.mark.parametrize("dim,nodes", [(256, 64), (512, 9), (64, 256)])
+def test_windows_shorter_than_the_tree(built_lib, dim, nodes):
+    """Chains of nodes longer than the window, whose first node falls anywhere in a group of 32 keys, with
+    values that are not numbers in every row of the pages that no sequence holds; and nothing timed out."""
+    import torch
+    from g4dense_b200 import api
+    lens = [0, 5, 31, 63, 104, 127]
+    chain = [-1] + list(range(nodes - 1))
+    c = make(lens, [nodes] * len(lens), 2, 1, dim, 8, "bf16", seed=dim, parents=[chain] * len(lens))
+    held = torch.zeros(c["k_pool"].shape[:2], dtype=torch.bool, device="cuda")
+    for s, n in enumerate(lens):
+        for j in range(n):
+            held[c["table"][s, j // 8], j % 8] = True
+    c["k_pool"][~held] = float("inf")
+    c["v_pool"][~held] = float("nan")
+    for window in (1, nodes // 2, nodes - 1, nodes, nodes + 40):
+        check(c, window)
+    api.tree_attention_check_error()

@@ -166,6 +166,23 @@ def test_sample_rows_wide_cuts(built_lib, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [1500, 262144])
+@pytest.mark.parametrize("p", [1.0, 0.9, 1e-6])
+def test_sample_rows_list_lengths(built_lib, vocab, p):
+    """Short cuts by number around the lengths at which a list is ranked, searched or left to all blocks,
+    without ties and with hundreds of entries in a tie across the cut."""
+    import torch
+    g = torch.Generator().manual_seed(vocab + 2)
+    ks = [254, 255, 256, 257, 511, 512, 513, 600, 1022, 1023, 1024, 1025]
+    x = torch.randn(2 * len(ks), vocab, generator=g) * 2
+    x[len(ks):, :300] = x[len(ks):].median(1, keepdim=True).values + 9
+    u = torch.rand(2 * len(ks), generator=g).tolist()
+    token, prob, kept = sample(x.cuda(), u, top_k=ks * 2, top_p=[p] * len(u))
+    for r, k in enumerate(ks * 2):
+        check_row(x[r].double().numpy(), u[r], 1.0, k, p, 0.0, token[r], prob[r], kept[r])
+
+
+@pytest.mark.gpu
 def test_sample_rows_split_does_not_matter(built_lib):
     """A row alone is spread over more blocks than among many: the same token, share and count."""
     import torch
