@@ -87,7 +87,7 @@ constexpr float kLazy = 8.f;         // a reference moves when a score exceeds i
 constexpr size_t kSmemLimit = 232448 - 2048;  // leaves room for blocks of the second kernel
 // What starting and finishing an item costs, in tiles, when the shares are cut: it grows with the rows,
 // the tiles' time less so. 128 rows an item, dim 256: 131 us over a 1024-key window and 282 over up to
-// 4096 keys at 3, 137 and 303 at 2; 64 rows, 12-node trees, dim 128: 22.9 us at 3, 21.4 at 2.
+// 4096 keys at 3, 137 and 303 at 2; 64 rows, 13-node trees, dim 128: 22.9 us at 3, 21.4 at 2.
 __host__ __device__ constexpr int item_cost(int rows) { return rows > 64 ? 3 : 2; }
 // Items of at most this many tiles are not split, which saves the second kernel: one sequence of 300
 // keys takes 10.5 us so and 11.1 split, one of 600 (5 tiles) 13.5 and 12.2.
