@@ -305,15 +305,14 @@ def plain_sample(s):
     by_index = torch.zeros_like(w).scatter_(1, order, w)
     r = torch.floor(s["uniform"].double() * total.double()).long()
     token = (by_index.cumsum(1) <= r[:, None]).sum(1).clamp(max=vocab - 1)
-    share = torch.zeros_like(x).scatter_(1, order, e).gather(1, token[:, None])[:, 0]
-    prob = share / (total.float() * 2.0 ** -40)
+    prob = by_index.gather(1, token[:, None])[:, 0].float() / total.float()
     return dict(token=token.int(), prob=prob, kept=keep.sum(1).int())
 
 
 def plain_reserve(refs, table, lens, grow, page):
     have, want = (lens + page - 1) // page, (lens + grow + page - 1) // page
     col = torch.arange(table.shape[1], device=table.device)[None]
-    fresh = (col >= have[:, None]) & (col < want[:, None]) & (table < 0)
+    fresh = (col >= have[:, None]) & (col < want[:, None])
     rank = fresh.reshape(-1).long().cumsum(0) - 1
     free = torch.sort((refs != 0).long(), stable=True)[1]
     ids = free[rank.clamp(min=0)].reshape(fresh.shape).int()
