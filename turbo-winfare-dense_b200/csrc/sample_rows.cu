@@ -209,6 +209,15 @@ struct Row {
         blocks = (int)cl.num_blocks();
         rank = (int)cl.block_rank();
     }
+    // A block's shared memory may be reached from others only once that block has started. Every block says so at
+    // its entry, started(), and waits for the others' word ahead of the first exchange, meet(): the slice is read
+    // in between, so the wait costs nothing where the blocks start together.
+    __device__ __forceinline__ void started() const {
+        if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    }
+    __device__ __forceinline__ void meet() const {
+        if (blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
     // All blocks' writes before it are seen by all after it. The block meets first, so that one warp's
     // release stands for all threads' writes, and the other warps need not wait for theirs.
     __device__ __forceinline__ void barrier() {
@@ -293,8 +302,8 @@ struct Row {
         __syncthreads();
         return warp_sum64(lane < kWarps ? sm.red[0][lane] : 0);
     }
-    // Each block's pair, folded over the cluster. A block writes its own into every block before the
-    // barrier: what is read after it is local. Two buffers in turn: one is written again only after the
+    // Each block's pair, folded over the cluster, after meet(). A block writes its own into every block before
+    // the barrier: what is read after it is local. Two buffers in turn: one is written again only after the
     // next barrier, which the readers of the last use have passed.
     template <class Fold>
     __device__ void exchange(Pair mine, Fold fold) {
@@ -693,6 +702,7 @@ __device__ __forceinline__ void sample_row(const SampleRowsArgs& a, Shared& sm, 
     const float own_max = m;
     const uint2 own = row.block_max_sum(m > -INFINITY ? order_bits(m) : 0, live);
     u64 top = 0, alive = 0;
+    row.meet();
     row.exchange({own.x, own.y}, [&](int, Pair x) { top = max(top, x.a), alive += x.b; });
     const float t = a.temperature ? a.temperature[r] : 1.f;
     const bool lead = row.rank == 0 && tid == 0;
@@ -937,6 +947,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(SampleRowsArgs
     extern __shared__ __align__(16) unsigned char raw[];
     Shared& sm = *reinterpret_cast<Shared*>(raw);
     Row<T> row(sm, reinterpret_cast<T*>(raw + sizeof(Shared)));
+    row.started();
     const int per = ((a.vocab + row.blocks - 1) / row.blocks + 7) & ~7;
     row.base = row.rank * per;
     row.n = max(0, min(per, a.vocab - row.base));
