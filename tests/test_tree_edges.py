@@ -9,8 +9,9 @@ from __future__ import annotations
 import re
 from pathlib import Path
 
-import numpy as np
 import pytest
+
+from test_tree_round import check_row, sample
 
 CSRC = Path(__file__).resolve().parent.parent / "turbo-winfare-dense_b200" / "csrc"
 
@@ -57,3 +58,30 @@ def test_sampling_beside_other_work(built_lib, rows, vocab):
         api.sample_rows(x, u, token[0], top_k=k)
         api.sample_rows(x, u, token[1], temperature=cold)
         assert torch.equal(token[0], want) and torch.equal(token[1], best)
+
+
+CUTS = [(0, 1.0, 0.0), (5, 1.0, 0.0), (0, 0.5, 0.0), (0, 1.0, 0.3), (700, 0.6, 0.0), (2000, 1.0, 0.0), (3, 0.9, 0.2)]
+
+
+def logits_with_masks(rows, vocab, seed):
+    """Rows of whole numbers (ties all over) whose entries are masked here and there, ends included."""
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(-3, 4, (rows, vocab), generator=g).float()
+    x[torch.rand(rows, vocab, generator=g) < 0.2] = -float("inf")
+    x[:, 0], x[:, -1], x[:, vocab // 2] = -float("inf"), -float("inf"), 3.0
+    return x, torch.rand(rows, generator=g).tolist()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [3, 1003, 40000, 262144])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_infinite_temperature(built_lib, vocab, dtype):
+    """Every entry that is not masked weighs the same; a masked one, or the padding behind the row, nothing."""
+    import torch
+    x, u = logits_with_masks(len(CUTS), vocab, vocab)
+    k, p, low = zip(*CUTS)
+    token, prob, kept = sample(x.to(getattr(torch, dtype)).cuda(), u, temperature=[float("inf")] * len(u), top_k=k, top_p=p,
+                               min_p=low)
+    for r in range(len(CUTS)):  # 1e30 leaves weights of 1 - 1e-29
+        check_row(x[r].double().numpy(), u[r], 1e30, k[r], p[r], low[r], token[r], prob[r], kept[r])

@@ -135,7 +135,7 @@ struct Scale {
         const float a = l - m;
         float q = fmaxf(a * r, -200.f);  // below -104 the exponential is 0 either way
         if (simple) q = fmaf(fmaf(-q, t, a), r, q);
-        else q = a / t;
+        else q = a > -INFINITY ? a / t : a;  // and nothing at -inf, also by an infinite t
         return expf(q);
     }
     static __device__ __forceinline__ u64 weight(float share) { return (u64)(share * 1099511627776.f); }
