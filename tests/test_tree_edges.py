@@ -85,3 +85,15 @@ def test_infinite_temperature(built_lib, vocab, dtype):
                                min_p=low)
     for r in range(len(CUTS)):  # 1e30 leaves weights of 1 - 1e-29
         check_row(x[r].double().numpy(), u[r], 1e30, k[r], p[r], low[r], token[r], prob[r], kept[r])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [3, 1003, 40000])
+@pytest.mark.parametrize("temperature", [1e-36, 1e-38, 1e-40, 1.5e-45])
+def test_tiny_temperatures(built_lib, vocab, temperature):
+    """All that is below the maximum weighs nothing, and the maxima that tie share the mass, whatever cuts."""
+    x, u = logits_with_masks(len(CUTS), vocab, vocab + 1)
+    k, p, low = zip(*CUTS)
+    token, prob, kept = sample(x.cuda(), u, temperature=[temperature] * len(u), top_k=k, top_p=p, min_p=low)
+    for r in range(len(CUTS)):  # 1e-3 leaves exp(-1000) of the next logit
+        check_row(x[r].double().numpy(), u[r], 1e-3, k[r], p[r], low[r], token[r], prob[r], kept[r])

@@ -41,6 +41,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "common.cuh"
@@ -117,13 +118,13 @@ __device__ __forceinline__ u64 warp_max64(u64 v) {
 
 // The row's numbers that turn a logit into a weight.
 struct Scale {
-    float m, t, r, bins;  // maximum, temperature, 1 / t, 32 / t
+    float m, t, r, bins;  // maximum, temperature, 1 / t, 32 / t (at most FLT_MAX)
     bool inf, simple;
     __device__ void set(float max, float temperature) {
         m = max;
         t = temperature;
         r = 1.f / t;
-        bins = 32.f / t;
+        bins = fminf(32.f / t, FLT_MAX);  // finite: a distance of 0 stays in the first bin
         inf = m == INFINITY;
         // Out of this range the reciprocal or the remainder below could leave the normal numbers.
         simple = t > 1e-18f && t < 1e18f;
