@@ -158,8 +158,8 @@ G4B_API int g4b_tree_attention_check_error(void);
  * times the whole. temperature <= 0 picks the maximum. NaN and -inf are never kept; a row without
  * any other entry gives token -1, probability 0. prob (may be NULL) receives the token's share of
  * the kept mass, kept (may be NULL) their number. Any of temperature, top_k, top_p and min_p may
- * be NULL (1, 0, 1, 0). Differs from g4b_sample_token, which keeps the reference's order and its
- * 256-entry bound. vocab 1..262144; stride in elements; dtype any g4b_dtype. One kernel launch. */
+ * be NULL (1, 0, 1, 0); a top_p or min_p of NaN is off, a temperature of NaN picks the maximum. Differs
+ * from g4b_sample_token, which keeps the reference's order and its 256-entry bound. vocab 1..262144; stride in elements; dtype any g4b_dtype. One kernel launch. */
 G4B_API int g4b_sample_rows(const void* logits, int dtype, int rows, int vocab, int64_t stride,
                             const float* uniform, const float* temperature, const int32_t* top_k,
                             const float* top_p, const float* min_p, int32_t* token, float* prob, int32_t* kept,

@@ -97,3 +97,18 @@ def test_tiny_temperatures(built_lib, vocab, temperature):
     token, prob, kept = sample(x.cuda(), u, temperature=[temperature] * len(u), top_k=k, top_p=p, min_p=low)
     for r in range(len(CUTS)):  # 1e-3 leaves exp(-1000) of the next logit
         check_row(x[r].double().numpy(), u[r], 1e-3, k[r], p[r], low[r], token[r], prob[r], kept[r])
+
+
+@pytest.mark.gpu
+def test_settings_that_are_not_numbers(built_lib):
+    """A NaN top_p or min_p is off, whichever way the row takes; a NaN temperature picks the maximum."""
+    import torch
+    nan = float("nan")
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(5, 5000, generator=g)
+    k = [20, 300, 2000, 0, 20]
+    t = [1.0, 1.0, 1.0, 1.0, nan]
+    token, prob, kept = sample(x.cuda(), [0.4] * 5, temperature=t, top_k=k, top_p=[nan] * 5, min_p=[nan] * 5)
+    for r in range(4):
+        check_row(x[r].double().numpy(), 0.4, 1.0, k[r], 1.0, 0.0, token[r], prob[r], kept[r])
+    assert (token[4], prob[4], kept[4]) == (int(x[4].argmax()), 1.0, 1)

@@ -726,7 +726,8 @@ __device__ __forceinline__ void sample_row(const SampleRowsArgs& a, Shared& sm, 
     row.sc.set(m, t);
     const Scale sc = row.sc;
     const int want = a.top_k ? a.top_k[r] : 0;
-    const float p = a.top_p ? a.top_p[r] : 1.f;
+    float p = a.top_p ? a.top_p[r] : 1.f;
+    if (!(p < 1.f)) p = 1.f;  // a NaN setting is off
     float low = a.min_p ? a.min_p[r] : 0.f;
     low = low > 0.f ? fminf(low, 1.f) : 0.f;
     u64 k = want > 0 && (u64)want < alive ? (u64)want : ~0ull;
