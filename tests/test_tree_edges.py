@@ -112,3 +112,160 @@ def test_settings_that_are_not_numbers(built_lib):
     for r in range(4):
         check_row(x[r].double().numpy(), 0.4, 1.0, k[r], 1.0, 0.0, token[r], prob[r], kept[r])
     assert (token[4], prob[4], kept[4]) == (int(x[4].argmax()), 1.0, 1)
+
+
+# -------------------------------------------------------------------------------------- streams
+
+class Stand:
+    """What the bindings look at in a tensor, without a device."""
+
+    def __init__(self, shape, dtype=None, device=0):
+        import torch
+        self.shape, self.dtype, self.device = tuple(shape), dtype or torch.int32, device
+        self.is_cuda = True
+
+    def numel(self):
+        n = 1
+        for k in self.shape:
+            n *= k
+        return n
+
+    def stride(self):
+        out, n = [], 1
+        for k in reversed(self.shape):
+            out.insert(0, n)
+            n *= k
+        return tuple(out)
+
+    dim = lambda self: len(self.shape)  # noqa: E731
+    is_contiguous = lambda self: True  # noqa: E731
+    data_ptr = lambda self: 4096  # noqa: E731
+    element_size = lambda self: self.dtype.itemsize  # noqa: E731
+    get_device = lambda self: self.device  # noqa: E731
+
+
+def operator_calls(api, device=None, **kw):
+    """One call of every operator on stand-ins; `device` names the tensors that are elsewhere."""
+    import torch
+    bf, f32 = torch.bfloat16, torch.float32
+    t = lambda *shape, dtype=None: Stand(shape, dtype)  # noqa: E731
+    q, pool, new = t(6, 4, 64, dtype=bf), t(9, 16, 2, 64, dtype=bf), t(6, 2, 64, dtype=bf)
+    planes, state = t(2, 9, 16, 2, 64, dtype=bf), (t(9), t(3, 4), t(3))
+    n = Stand((3,), device=1) if device else t(3)
+    return {
+        "tree_attention": lambda: api.tree_attention(q, pool, pool, t(3, 4), n, new, new, t(4), t(6, 1), q, t(1 << 20, dtype=torch.uint8),
+                                                     max_nodes=6, scale=1.0, **kw),
+        "sample_rows": lambda: api.sample_rows(t(3, 50, dtype=f32), t(3, dtype=f32), n, **kw),
+        "tree_accept": lambda: api.tree_accept(t(6), t(6), t(6), t(4), t(3, 6), n, t(3), **kw),
+        "pages_reserve": lambda: api.pages_reserve(*state, n, 16, *state[:2], t(1), **kw),
+        "pages_fork": lambda: api.pages_fork(planes, *state, n, t(3), *state, t(1), **kw),
+        "pages_free": lambda: api.pages_free(*state, n, 16, *state, **kw),
+        "pages_compact": lambda: api.pages_compact(planes, *state[:2], *state[:2], t(19) if not device else Stand((19,), device=1), **kw),
+        "pages_copy": lambda: api.pages_copy(planes, planes, n, t(3), **kw),
+        "pages_commit": lambda: api.pages_commit(planes, t(3, 4), t(3), t(2, 6, 2, 64, dtype=bf), t(4), t(3, 6), n, t(3), **kw),
+    }
+
+
+OPERATORS = ["tree_attention", "sample_rows", "tree_accept", "pages_reserve", "pages_fork", "pages_free", "pages_compact",
+             "pages_copy", "pages_commit"]
+
+
+class Calls:
+    """A library that takes down the stream, the last argument, of every call."""
+
+    def __init__(self):
+        self.streams = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.streams.append(args[-1])
+            return 0
+        return call
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The bindings over a stand-in library, current device 0 and current stream 1234."""
+    import torch
+    from g4dense_b200 import api
+    calls = Calls()
+    monkeypatch.setattr(api, "lib", lambda: calls)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: type("S", (), {"cuda_stream": 1234}))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    return calls
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_calls_go_to_the_current_stream(calls, name):
+    from g4dense_b200 import api
+    operator_calls(api)[name]()
+    assert calls.streams == [1234]
+    operator_calls(api, stream=type("S", (), {"cuda_stream": 77}))[name]()
+    assert calls.streams == [1234, 77]
+
+
+def test_decoder_products_go_to_the_current_stream(calls):
+    import torch
+    from g4dense_b200 import tree_decode as T
+    got = []
+
+    class Matrix:
+        N = 5
+
+        def gemm(self, x, out, stream=None):
+            got.append((x.shape[0], stream.cuda_stream))
+    T._product(Matrix(), torch.zeros(130, 8))
+    assert got == [(128, 1234), (2, 1234)]
+
+
+@pytest.mark.gpu
+def test_calls_wait_for_the_current_stream(built_lib):
+    """Inputs that a side stream is still to make, outputs that it reads next, no stream given."""
+    import torch
+    from g4dense_b200 import api
+    from test_tree_attention import make, run
+    c = make([300, 40], [5, 3], 4, 2, 64, 16, "bf16", seed=1)
+    want = run(c)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x, u = torch.randn(40, 3000, generator=g, device="cuda"), torch.rand(40, generator=g, device="cuda")
+    token = torch.empty(40, dtype=torch.int32, device="cuda")
+    api.sample_rows(x, u, token)
+    dev = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool = torch.randn(3, 6, 8, 16, generator=g, device="cuda")
+    there, src, dst = torch.zeros_like(pool), dev([0, 5, 2]), dev([4, 1, 3])
+    late, side = [torch.zeros_like(t) for t in (c["q"], x, pool)], torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        for a, b in zip(late, (c["q"], x, pool)):
+            a.copy_(b)
+        out = run(dict(c, q=late[0])).clone()
+        drawn = torch.empty_like(token)
+        api.sample_rows(late[1], u, drawn)
+        drawn = drawn.clone()
+        api.pages_copy(late[2], there, src, dst)
+        moved = there.clone()
+    side.synchronize()
+    assert torch.equal(out, want) and torch.equal(drawn, token)
+    assert all(torch.equal(moved[:, d], pool[:, s]) for s, d in ((0, 4), (5, 1), (2, 3)))
+
+
+@pytest.mark.gpu
+def test_decoder_on_a_side_stream(built_lib):
+    import torch
+    from g4dense_b200 import tree_decode as T
+
+    def go():
+        d = T.Decoder(T.Model(3), 2)
+        d.prompt([[5] * 40, [9, 8, 7]])
+        uniform = torch.rand(2, 300, generator=torch.Generator().manual_seed(5)).cuda()
+        got = [d.round([([1, 2, 3], [-1, 0, 0]), ([4], [-1])], uniform) for _ in range(3)]
+        return got, d.pool.clone()
+    want, pool = go()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        got, other = go()
+        side.synchronize()
+    assert got == want and torch.equal(pool, other)

@@ -199,16 +199,17 @@ def sample_token(logits, temperature, top_p, top_k, seed, workspace, out, stream
                                   _dptr(workspace), _dptr(out), _stream(stream)), "g4b_sample_token")
 
 _dtypes = {}  # torch dtype -> g4b_dtype, filled by _types()
-_i32 = _f32 = None
+_i32 = _f32 = _cuda = None
 
 
 def _types():
     """Loads torch's types and the library once; returns the library."""
-    global _i32, _f32
+    global _i32, _f32, _cuda
     if _i32 is None:
         import torch
         _dtypes.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2})
-        _i32, _f32 = torch.int32, torch.float32
+        _f32, _cuda = torch.float32, torch.cuda
+        _i32 = torch.int32
     return lib()
 
 
@@ -245,7 +246,8 @@ def _rows_of(name, t, dtype, shape):
 
 
 def _at(stream):
-    return stream.cuda_stream if stream is not None else 0
+    """Handle of the stream given, else of torch's current one: what made the inputs is ordered before."""
+    return (_cuda.current_stream() if stream is None else stream).cuda_stream
 
 
 def tree_mask(parents, words=None):

@@ -35,7 +35,8 @@ class Model:
             words = torch.randint(-2 ** 31, 2 ** 31, (n, k // 8), generator=g, dtype=torch.int64).to(torch.int32)
             scale = torch.full((n, k // 64), 0.25 * k ** -0.5).to(torch.bfloat16)
             bias = (-7.5 * scale.float()).to(torch.bfloat16)  # nibbles 0..15, centred
-            return api.QMat(words.cuda(), scale.view(torch.int16).cuda(), bias.view(torch.int16).cuda())
+            return api.QMat(words.cuda(), scale.view(torch.int16).cuda(), bias.view(torch.int16).cuda(),
+                            torch.cuda.current_stream())
 
         q, kv = self.heads * self.head_dim, self.kv_heads * self.head_dim
         self.embed = torch.randn(self.vocab, self.dim, generator=g).cuda()
@@ -49,9 +50,9 @@ class Model:
 def _product(m, x):
     """x [rows][K] fp32 through a prepared matrix, 128 rows a call."""
     import torch
-    out = torch.empty(x.shape[0], m.N, device="cuda")
+    out, stream = x.new_empty(x.shape[0], m.N), torch.cuda.current_stream()
     for i in range(0, x.shape[0], 128):
-        m.gemm(x[i:i + 128].contiguous(), out[i:i + 128])
+        m.gemm(x[i:i + 128].contiguous(), out[i:i + 128], stream)
     return out
 
 
