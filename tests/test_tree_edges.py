@@ -204,6 +204,15 @@ def test_calls_go_to_the_current_stream(calls, name):
     assert calls.streams == [1234, 77]
 
 
+@pytest.mark.parametrize("name", OPERATORS)
+def test_tensors_of_another_device_are_refused(calls, name):
+    """A kernel runs on the current device: an array of another one would be a bad address there."""
+    from g4dense_b200 import api
+    with pytest.raises(ValueError, match="current device"):
+        operator_calls(api, device=1)[name]()
+    assert calls.streams == []
+
+
 def test_decoder_products_go_to_the_current_stream(calls):
     import torch
     from g4dense_b200 import tree_decode as T

@@ -217,26 +217,34 @@ def _bad(what):
     raise ValueError(what)
 
 
-def _ints(name, t, n):
-    """Device pointer of a contiguous int32 CUDA tensor of n elements."""
-    if t.dtype is not _i32 or not t.is_cuda or t.numel() != n or not t.is_contiguous():
-        _bad(f"{name}: a contiguous int32 CUDA tensor of {n} elements is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _here():
+    """Index of the current device, on which every tensor of a call has to be: kernels launch there."""
+    return _cuda.current_device()
+
+
+def _ints(name, t, n, dev):
+    """Device pointer of a contiguous int32 tensor of n elements on device `dev`."""
+    if t.dtype is not _i32 or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+        _bad(f"{name}: a contiguous int32 CUDA tensor of {n} elements on the current device, {dev}, is needed, got "
+             f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _floats(name, t, n):
+def _floats(name, t, n, dev):
     """As _ints for float32; None stays None."""
     if t is None:
         return None
-    if t.dtype is not _f32 or not t.is_cuda or t.numel() != n or not t.is_contiguous():
-        _bad(f"{name}: a contiguous float32 CUDA tensor of {n} elements is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.dtype is not _f32 or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+        _bad(f"{name}: a contiguous float32 CUDA tensor of {n} elements on the current device, {dev}, is needed, got "
+             f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _rows_of(name, t, dtype, shape):
-    """(device pointer, stride of the first dimension) of a CUDA tensor contiguous but for that one."""
-    if t.dtype is not dtype or not t.is_cuda or t.shape != shape:
-        _bad(f"{name}: a {dtype} CUDA tensor of shape {tuple(shape)} is needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _rows_of(name, t, dtype, shape, dev):
+    """(device pointer, stride of the first dimension) of a tensor on device `dev`, contiguous but for that one."""
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
+        _bad(f"{name}: a {dtype} CUDA tensor of shape {tuple(shape)} on the current device, {dev}, is needed, got "
+             f"{t.dtype} {tuple(t.shape)} on {t.device}")
     n, strides = 1, t.stride()
     for k in range(len(shape) - 1, 0, -1):
         if strides[k] != n and shape[k] != 1:
@@ -283,7 +291,7 @@ def tree_attention(q, k_pool, v_pool, table, lens, k_new, v_new, cu_nodes, mask,
     [tokens][kv_heads][dim], all bf16 or all fp16 torch CUDA tensors (token and page strides
     honoured); table [seqs][width], lens [seqs], cu_nodes [seqs + 1], mask [tokens][words], depth
     [tokens] int32; workspace a byte tensor of tree_attention_workspace()."""
-    L = _types()
+    L, dev = _types(), _here()
     shape, pool, dtype = q.shape, k_pool.shape, q.dtype
     if len(shape) != 3 or len(pool) != 4 or _dtypes.get(dtype, 2) > 1:
         _bad(f"tree_attention: q [tokens][heads][dim] and pools [pages][page_size][kv_heads][dim] of dtype bfloat16 or "
@@ -293,23 +301,23 @@ def tree_attention(q, k_pool, v_pool, table, lens, k_new, v_new, cu_nodes, mask,
     new = (tokens, kv_heads, dim)
     if pool[3] != dim:
         _bad("tree_attention: q and the pools differ in head_dim")
-    pq, q_stride = _rows_of("q", q, dtype, shape)
-    po, out_stride = _rows_of("out", out, dtype, shape)
-    pk, page_stride = _rows_of("k_pool", k_pool, dtype, pool)
-    pv, v_stride = _rows_of("v_pool", v_pool, dtype, pool)
-    pkn, new_stride = _rows_of("k_new", k_new, dtype, new)
-    pvn, vn_stride = _rows_of("v_new", v_new, dtype, new)
+    pq, q_stride = _rows_of("q", q, dtype, shape, dev)
+    po, out_stride = _rows_of("out", out, dtype, shape, dev)
+    pk, page_stride = _rows_of("k_pool", k_pool, dtype, pool, dev)
+    pv, v_stride = _rows_of("v_pool", v_pool, dtype, pool, dev)
+    pkn, new_stride = _rows_of("k_new", k_new, dtype, new, dev)
+    pvn, vn_stride = _rows_of("v_new", v_new, dtype, new, dev)
     if v_stride != page_stride or vn_stride != new_stride:
         _bad("tree_attention: K and V differ in their strides")
     if window and depth is None:
         _bad("tree_attention: a window needs the nodes' depths")
     seqs, width, words = lens.numel(), table.shape[-1], mask.shape[-1]
-    if not workspace.is_cuda:
-        _bad("workspace: a CUDA tensor is needed")
+    if workspace.get_device() != dev:
+        _bad(f"workspace: a CUDA tensor on the current device, {dev}, is needed")
     a = _TREE_ATTENTION.pack(
-        pq, pk, pv, pkn, pvn, po, _ints("table", table, seqs * width), _ints("lens", lens, seqs),
-        _ints("cu_nodes", cu_nodes, seqs + 1), _ints("mask", mask, tokens * words),
-        0 if depth is None else _ints("depth", depth, tokens), workspace.data_ptr(),
+        pq, pk, pv, pkn, pvn, po, _ints("table", table, seqs * width, dev), _ints("lens", lens, seqs, dev),
+        _ints("cu_nodes", cu_nodes, seqs + 1, dev), _ints("mask", mask, tokens * words, dev),
+        0 if depth is None else _ints("depth", depth, tokens, dev), workspace.data_ptr(),
         workspace.numel() * workspace.element_size(), q_stride, out_stride, new_stride, page_stride, seqs, tokens,
         max_nodes, pages, page_size, width, words, heads, kv_heads, dim, window, _dtypes[dtype], scale)
     rc = L.g4b_tree_attention(a, _at(stream))
@@ -328,18 +336,18 @@ def sample_rows(logits, uniform, token, prob=None, kept=None, temperature=None, 
     [rows] int32, from uniform [rows] float32 in [0, 1), with per-row temperature, top_p, min_p
     (float32) and top_k (int32) where given (g4b_sample_rows). prob [rows] float32 and kept [rows]
     int32 receive the token's share of the kept mass and the number of kept entries."""
-    L = _types()
+    L, dev = _types(), _here()
     if logits.dim() != 2 or logits.dtype not in _dtypes:
         _bad(f"sample_rows: logits [rows][vocab] of dtype bfloat16, float16 or float32 are needed, got "
              f"{tuple(logits.shape)} {logits.dtype}")
     if uniform is None:
         _bad("sample_rows: uniform numbers are needed")
     rows, vocab = logits.shape
-    ptr, stride = _rows_of("logits", logits, logits.dtype, logits.shape)
-    rc = L.g4b_sample_rows(ptr, _dtypes[logits.dtype], rows, vocab, stride, _floats("uniform", uniform, rows),
-                           _floats("temperature", temperature, rows), None if top_k is None else _ints("top_k", top_k, rows),
-                           _floats("top_p", top_p, rows), _floats("min_p", min_p, rows), _ints("token", token, rows),
-                           _floats("prob", prob, rows), None if kept is None else _ints("kept", kept, rows), _at(stream))
+    ptr, stride = _rows_of("logits", logits, logits.dtype, logits.shape, dev)
+    rc = L.g4b_sample_rows(ptr, _dtypes[logits.dtype], rows, vocab, stride, _floats("uniform", uniform, rows, dev),
+                           _floats("temperature", temperature, rows, dev), None if top_k is None else _ints("top_k", top_k, rows, dev),
+                           _floats("top_p", top_p, rows, dev), _floats("min_p", min_p, rows, dev), _ints("token", token, rows, dev),
+                           _floats("prob", prob, rows, dev), None if kept is None else _ints("kept", kept, rows, dev), _at(stream))
     if rc:
         _check(rc, "g4b_sample_rows")
 
@@ -347,20 +355,20 @@ def sample_rows(logits, uniform, token, prob=None, kept=None, temperature=None, 
 def tree_accept(tokens, parents, sampled, cu_nodes, path, count, next_token, stream=None):
     """Walks each tree along the drawn tokens (g4b_tree_accept): path [seqs][width], count [seqs] and
     next_token [seqs] from tokens, parents, sampled [nodes] and cu_nodes [seqs + 1], all int32."""
-    L = _types()
+    L, dev = _types(), _here()
     n, seqs, width = tokens.numel(), cu_nodes.numel() - 1, path.shape[-1]
-    rc = L.g4b_tree_accept(_ints("tokens", tokens, n), _ints("parents", parents, n), _ints("sampled", sampled, n),
-                           _ints("cu_nodes", cu_nodes, seqs + 1), seqs, n, _ints("path", path, seqs * width), width,
-                           _ints("count", count, seqs), _ints("next_token", next_token, seqs), _at(stream))
+    rc = L.g4b_tree_accept(_ints("tokens", tokens, n, dev), _ints("parents", parents, n, dev), _ints("sampled", sampled, n, dev),
+                           _ints("cu_nodes", cu_nodes, seqs + 1, dev), seqs, n, _ints("path", path, seqs * width, dev), width,
+                           _ints("count", count, seqs, dev), _ints("next_token", next_token, seqs, dev), _at(stream))
     if rc:
         _check(rc, "g4b_tree_accept")
 
 
-def _pool(pool):
+def _pool(pool, dev):
     """Packed g4b_page_pool of a CUDA tensor [planes][pages][page_size][...] with contiguous pages."""
     shape, strides, size = pool.shape, pool.stride(), pool.element_size()
-    if not pool.is_cuda or len(shape) < 4:
-        _bad("pool: a CUDA tensor [planes][pages][page_size][row...] is needed")
+    if pool.get_device() != dev or len(shape) < 4:
+        _bad(f"pool: a CUDA tensor [planes][pages][page_size][row...] on the current device, {dev}, is needed")
     n = 1
     for k in range(len(shape) - 1, 1, -1):
         if strides[k] != n and shape[k] != 1:
@@ -371,20 +379,20 @@ def _pool(pool):
     return _PAGE_POOL.pack(pool.data_ptr(), plane, page, shape[0], shape[1], shape[2], n // max(shape[2], 1) * size)
 
 
-def _tables(refs, table, lens, refs_out, table_out, lens_out, page_size):
+def _tables(refs, table, lens, refs_out, table_out, lens_out, page_size, dev):
     pages, (seqs, width) = refs.numel(), table.shape
     return _PAGE_TABLES.pack(
-        _ints("refs", refs, pages), _ints("table", table, seqs * width), 0 if lens is None else _ints("lens", lens, seqs),
-        _ints("refs_out", refs_out, pages), _ints("table_out", table_out, seqs * width),
-        0 if lens_out is None else _ints("lens_out", lens_out, seqs), pages, seqs, width, page_size)
+        _ints("refs", refs, pages, dev), _ints("table", table, seqs * width, dev), 0 if lens is None else _ints("lens", lens, seqs, dev),
+        _ints("refs_out", refs_out, pages, dev), _ints("table_out", table_out, seqs * width, dev),
+        0 if lens_out is None else _ints("lens_out", lens_out, seqs, dev), pages, seqs, width, page_size)
 
 
 def pages_reserve(refs, table, lens, grow, page_size, refs_out, table_out, status, stream=None):
     """Pages for grow[s] more tokens of every sequence (g4b_pages_reserve). int32 CUDA tensors: refs
     [pages], table [seqs][width], lens, grow [seqs], status [1]; the outputs may be the inputs."""
-    L = _types()
-    rc = L.g4b_pages_reserve(_tables(refs, table, lens, refs_out, table_out, None, page_size),
-                             _ints("grow", grow, lens.numel()), _ints("status", status, 1), _at(stream))
+    L, dev = _types(), _here()
+    rc = L.g4b_pages_reserve(_tables(refs, table, lens, refs_out, table_out, None, page_size, dev),
+                             _ints("grow", grow, lens.numel(), dev), _ints("status", status, 1, dev), _at(stream))
     if rc:
         _check(rc, "g4b_pages_reserve")
 
@@ -392,17 +400,17 @@ def pages_reserve(refs, table, lens, grow, page_size, refs_out, table_out, statu
 def pages_fork(pool, refs, table, lens, src, dst, refs_out, table_out, lens_out, status, stream=None):
     """Sequences dst[i] become continuations of src[i] (g4b_pages_fork): full pages shared, a partial
     last page copied. pool [planes][pages][page_size][row...]."""
-    L, n = _types(), src.numel()
-    rc = L.g4b_pages_fork(_pool(pool), _tables(refs, table, lens, refs_out, table_out, lens_out, pool.shape[2]),
-                          _ints("src", src, n), _ints("dst", dst, n), n, _ints("status", status, 1), _at(stream))
+    L, dev, n = _types(), _here(), src.numel()
+    rc = L.g4b_pages_fork(_pool(pool, dev), _tables(refs, table, lens, refs_out, table_out, lens_out, pool.shape[2], dev),
+                          _ints("src", src, n, dev), _ints("dst", dst, n, dev), n, _ints("status", status, 1, dev), _at(stream))
     if rc:
         _check(rc, "g4b_pages_fork")
 
 
 def pages_free(refs, table, lens, seqs, page_size, refs_out, table_out, lens_out, stream=None):
     """Releases the pages of the sequences seqs[] and empties them (g4b_pages_free)."""
-    L, n = _types(), seqs.numel()
-    rc = L.g4b_pages_free(_tables(refs, table, lens, refs_out, table_out, lens_out, page_size), _ints("seqs", seqs, n), n,
+    L, dev, n = _types(), _here(), seqs.numel()
+    rc = L.g4b_pages_free(_tables(refs, table, lens, refs_out, table_out, lens_out, page_size, dev), _ints("seqs", seqs, n, dev), n,
                           _at(stream))
     if rc:
         _check(rc, "g4b_pages_free")
@@ -411,17 +419,17 @@ def pages_free(refs, table, lens, seqs, page_size, refs_out, table_out, lens_out
 def pages_compact(pool, refs, table, refs_out, table_out, moves, stream=None):
     """Moves live pages to the front of the pool (g4b_pages_compact); moves [1 + 2 * pages] int32
     receives their number and the (from, to) pairs."""
-    L = _types()
-    rc = L.g4b_pages_compact(_pool(pool), _tables(refs, table, None, refs_out, table_out, None, pool.shape[2]),
-                             _ints("moves", moves, 1 + 2 * refs.numel()), _at(stream))
+    L, dev = _types(), _here()
+    rc = L.g4b_pages_compact(_pool(pool, dev), _tables(refs, table, None, refs_out, table_out, None, pool.shape[2], dev),
+                             _ints("moves", moves, 1 + 2 * refs.numel(), dev), _at(stream))
     if rc:
         _check(rc, "g4b_pages_compact")
 
 
 def pages_copy(pool, to_pool, src, dst, stream=None):
     """Page src[i] of pool to page dst[i] of to_pool, in every plane (g4b_pages_copy)."""
-    L, n = _types(), src.numel()
-    rc = L.g4b_pages_copy(_pool(pool), _pool(to_pool), _ints("src", src, n), _ints("dst", dst, n), n, _at(stream))
+    L, dev, n = _types(), _here(), src.numel()
+    rc = L.g4b_pages_copy(_pool(pool, dev), _pool(to_pool, dev), _ints("src", src, n, dev), _ints("dst", dst, n, dev), n, _at(stream))
     if rc:
         _check(rc, "g4b_pages_copy")
 
@@ -429,17 +437,17 @@ def pages_copy(pool, to_pool, src, dst, stream=None):
 def pages_commit(pool, table, lens, rows, cu_nodes, path, count, lens_out, status=None, stream=None):
     """Writes the accepted nodes' rows [planes][tokens][row...] into their sequences' pages and the
     new lengths into lens_out (g4b_pages_commit). path None: the first count[s] rows."""
-    L = _types()
+    L, dev = _types(), _here()
     shape, want, seqs, width = rows.shape, pool.shape, lens.numel(), table.shape[-1]
     tokens = shape[1]
     if len(shape) != len(want) - 1 or shape[0] != want[0] or shape[2:] != want[3:]:
         _bad("pages_commit: rows have to be [planes][tokens][row...] like the pool")
-    ptr, stride = _rows_of("rows", rows, pool.dtype, shape)
-    rc = L.g4b_pages_commit(_pool(pool), _ints("table", table, seqs * width), width, _ints("lens", lens, seqs), seqs, ptr,
-                            stride * rows.element_size(), tokens, _ints("cu_nodes", cu_nodes, seqs + 1),
-                            None if path is None else _ints("path", path, seqs * path.shape[-1]),
-                            0 if path is None else path.shape[-1], _ints("count", count, seqs),
-                            None if status is None else _ints("status", status, 1), _ints("lens_out", lens_out, seqs),
+    ptr, stride = _rows_of("rows", rows, pool.dtype, shape, dev)
+    rc = L.g4b_pages_commit(_pool(pool, dev), _ints("table", table, seqs * width, dev), width, _ints("lens", lens, seqs, dev), seqs, ptr,
+                            stride * rows.element_size(), tokens, _ints("cu_nodes", cu_nodes, seqs + 1, dev),
+                            None if path is None else _ints("path", path, seqs * path.shape[-1], dev),
+                            0 if path is None else path.shape[-1], _ints("count", count, seqs, dev),
+                            None if status is None else _ints("status", status, 1, dev), _ints("lens_out", lens_out, seqs, dev),
                             _at(stream))
     if rc:
         _check(rc, "g4b_pages_commit")
