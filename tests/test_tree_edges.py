@@ -213,6 +213,20 @@ def test_tensors_of_another_device_are_refused(calls, name):
     assert calls.streams == []
 
 
+def test_expanded_workspace_is_refused(calls):
+    """A view with more elements than memory behind it."""
+    import torch
+    from g4dense_b200 import api
+
+    class Wide(Stand):
+        is_contiguous = lambda self: False  # noqa: E731
+    q, pool, new = (Stand(n, torch.bfloat16) for n in ((6, 4, 64), (9, 16, 2, 64), (6, 2, 64)))
+    with pytest.raises(ValueError, match="workspace"):
+        api.tree_attention(q, pool, pool, Stand((3, 4)), Stand((3,)), new, new, Stand((4,)), Stand((6, 1)), q,
+                           Wide((1 << 20,), torch.uint8), max_nodes=6, scale=1.0)
+    assert calls.streams == []
+
+
 def test_decoder_products_go_to_the_current_stream(calls):
     import torch
     from g4dense_b200 import tree_decode as T

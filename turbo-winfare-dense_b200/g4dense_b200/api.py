@@ -312,8 +312,8 @@ def tree_attention(q, k_pool, v_pool, table, lens, k_new, v_new, cu_nodes, mask,
     if window and depth is None:
         _bad("tree_attention: a window needs the nodes' depths")
     seqs, width, words = lens.numel(), table.shape[-1], mask.shape[-1]
-    if workspace.get_device() != dev:
-        _bad(f"workspace: a CUDA tensor on the current device, {dev}, is needed")
+    if workspace.get_device() != dev or not workspace.is_contiguous():
+        _bad(f"workspace: a contiguous CUDA tensor on the current device, {dev}, is needed")
     a = _TREE_ATTENTION.pack(
         pq, pk, pv, pkn, pvn, po, _ints("table", table, seqs * width, dev), _ints("lens", lens, seqs, dev),
         _ints("cu_nodes", cu_nodes, seqs + 1, dev), _ints("mask", mask, tokens * words, dev),
