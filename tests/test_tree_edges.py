@@ -7,6 +7,7 @@ through bindings whose library and tensors are stand-ins.
 from __future__ import annotations
 
 import re
+import subprocess
 from pathlib import Path
 
 import pytest
@@ -292,3 +293,38 @@ def test_decoder_on_a_side_stream(built_lib):
         got, other = go()
         side.synchronize()
     assert got == want and torch.equal(pool, other)
+
+
+# -------------------------------------------------------------------------------------- devices
+
+def test_once_per_device(tmp_path):
+    """csrc/per_device.h on the host, with a stand-in for the runtime's current device."""
+    out = tmp_path / "test_per_device"
+    r = subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-I", str(CSRC), "-I", "/usr/local/cuda/include",
+                        str(Path(__file__).resolve().parent / "cpp" / "test_per_device.cpp"), "-o", str(out)],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-4000:]
+    r = subprocess.run([str(out)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout
+
+
+@pytest.mark.parametrize("name", ["tree_attn.cu", "sample_rows.cu"])
+def test_attributes_are_set_on_every_device(name):
+    """cudaFuncSetAttribute holds for the current device: no flag of the whole process may stand for it."""
+    code = code_of(name)
+    assert "static bool" not in code and "static int n" not in code
+    assert code.count("cudaFuncSetAttribute") and "static OncePerDevice" in code
+
+
+@pytest.mark.gpu
+def test_two_devices_in_one_process(built_lib):
+    import torch
+    from test_tree_attention import check, make
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    for d in (0, 1):
+        with torch.cuda.device(d):
+            check(make([900, 40], [5, 3], 8, 2, 128, 16, "bf16", seed=1))
+            x = torch.randn(2, 262144, device="cuda")
+            token, _, _ = sample(x, [0.5, 0.5], temperature=[0.0, 0.0])
+            assert token == x.argmax(1).tolist()

@@ -46,6 +46,7 @@
 
 #include "common.cuh"
 #include "launch.cuh"
+#include "per_device.h"
 #include "sample_rows.h"
 
 namespace cg = cooperative_groups;
@@ -969,15 +970,14 @@ cudaError_t run(const SampleRowsArgs& a, cudaStream_t st) {
     const int per = span(blocks);
     const size_t smem = sizeof(Shared) + (size_t)per * sizeof(T);
     auto kern = sample_rows_kernel<T>;
-    static bool attr = false;
-    if (!attr) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)(sizeof(Shared) + kSliceBytes));
-        if (e != cudaSuccess) return e;
-        attr = true;
-    }
+    static OncePerDevice attributes;
+    const cudaError_t e = attributes([&] {
+        const cudaError_t x = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (x != cudaSuccess) return x;
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (int)(sizeof(Shared) + kSliceBytes));
+    });
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * blocks));
     cfg.blockDim = dim3(kThreads);

@@ -52,11 +52,13 @@
 
 #include "common.cuh"
 #include "launch.cuh"
+#include "per_device.h"
 #include "tcgen05.cuh"
 #include "tma.cuh"
 #include "tree_attn.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cstddef>
 #include <cstring>
 
@@ -1195,14 +1197,15 @@ __global__ void __launch_bounds__(32 * kJoinRows) tree_attn_join_kernel(const __
             out[(k * 32 + lane) * (kV / 2) + j / 2] = pack2<kBf16>(o[k][j] * inv, o[k][j + 1] * inv);
 }
 
+// Multiprocessors of the current device.
 int sm_count() {
-    static int n = 0;
-    if (!n) {
-        int dev = 0;
-        cudaGetDevice(&dev);
-        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-        if (n <= 0) n = 148;
-    }
+    static std::atomic<int> known[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    const bool kept = dev >= 0 && dev < 64;
+    if (kept && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    if (kept) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 
@@ -1255,13 +1258,12 @@ cudaError_t make_map(CUtensorMap* m, const void* base, int rank, const cuuint64_
 template <int D, int kNH, bool kBf16>
 cudaError_t run(const CUtensorMap* maps, const Params& p, const Shape& sh, cudaStream_t st) {
     auto kern = tree_attn_kernel<D, kNH, kBf16>;
-    static bool attr = false;
-    if (!attr) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit);
-        if (e != cudaSuccess) return e;
-        attr = true;
-    }
-    cudaError_t e = launch(kern, dim3(p.by_grid.d), dim3(kThreads), sh.smem, st, false, maps[0], maps[1], maps[2], maps[3], p);
+    static OncePerDevice attributes;
+    cudaError_t e = attributes([&] {
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit);
+    });
+    if (e != cudaSuccess) return e;
+    e = launch(kern, dim3(p.by_grid.d), dim3(kThreads), sh.smem, st, false, maps[0], maps[1], maps[2], maps[3], p);
     if (e != cudaSuccess || p.whole) return e;
     return launch(tree_attn_join_kernel<D, kBf16>, dim3(p.by_grid.d, (p.N + kJoinRows - 1) / kJoinRows),
                   dim3(32 * kJoinRows), 0, st, true, p);
