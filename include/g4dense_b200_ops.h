@@ -145,8 +145,8 @@ typedef struct g4b_tree_attention_args {
 /* 0 when the shape is not supported. */
 G4B_API size_t g4b_tree_attention_workspace(int max_nodes, int heads, int kv_heads, int head_dim);
 G4B_API int g4b_tree_attention(const g4b_tree_attention_args* args, void* stream);
-/* Synchronizes and reports whether a launch on this device hit a bounded-wait timeout since the
- * last call. */
+/* Waits for all streams of the current device and reports whether a launch on it hit a bounded-wait
+ * timeout since the last call. */
 G4B_API int g4b_tree_attention_check_error(void);
 
 /* One token per logits row. With l the row, m its maximum and T = temperature[r], entries are

@@ -328,3 +328,23 @@ def test_two_devices_in_one_process(built_lib):
             x = torch.randn(2, 262144, device="cuda")
             token, _, _ = sample(x, [0.5, 0.5], temperature=[0.0, 0.0])
             assert token == x.argmax(1).tolist()
+
+
+# ----------------------------------------------------------------------------------- attention
+
+@pytest.mark.gpu
+def test_check_error_waits_for_every_stream(built_lib):
+    """The launch that is reported on may run on a stream that the default one does not wait for."""
+    import torch
+    from g4dense_b200 import api
+    from test_tree_attention import make, run
+    c = make([300, 40], [5, 3], 4, 2, 64, 16, "bf16", seed=1)
+    run(c)
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        run(c)
+        done.record()
+    api.tree_attention_check_error()
+    assert done.query()

@@ -1364,6 +1364,8 @@ cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
 int tree_attn_error() {
     int h = 0;
     const int zero = 0;
+    // The copies go to the legacy stream, which does not wait for non-blocking ones.
+    if (cudaDeviceSynchronize() != cudaSuccess) return -1;
     if (cudaMemcpyFromSymbol(&h, g_tree_err, sizeof(int)) != cudaSuccess) return -1;
     if (h) cudaMemcpyToSymbol(g_tree_err, &zero, sizeof(int));
     return h;
