@@ -348,3 +348,17 @@ def test_check_error_waits_for_every_stream(built_lib):
         done.record()
     api.tree_attention_check_error()
     assert done.query()
+
+
+# ------------------------------------------------------------------------------------- decoder
+
+@pytest.mark.gpu
+def test_prompt_chunks_that_do_not_fit(built_lib):
+    """A first chunk without pages must not be forgotten when a later, smaller one finds some."""
+    import torch
+    from g4dense_b200 import tree_decode as T
+    d = T.Decoder(T.Model(), 2, pages=1)
+    before = [t.clone() for t in (d.refs, d.table, d.lens, d.pool)]
+    with pytest.raises(RuntimeError, match="status 1"):
+        d.prompt([[5] * (d.max_nodes + 5), None])
+    assert all(torch.equal(a, b) for a, b in zip(before, (d.refs, d.table, d.lens, d.pool)))

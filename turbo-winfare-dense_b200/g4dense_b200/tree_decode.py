@@ -130,7 +130,7 @@ class Decoder:
             self.count.copy_(torch.tensor([len(p) for p in parts], dtype=torch.int32))
             self._grow()
             self._commit(rows, cu, None)
-        self.check()
+            self.check()  # before the next chunk, whose status replaces this one's
 
     def round(self, trees, uniform, temperature=0.0, top_k=0, top_p=1.0):
         """One verification round. trees[s]: (tokens, parents) with the pending token first, or None;
