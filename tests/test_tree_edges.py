@@ -362,3 +362,31 @@ def test_prompt_chunks_that_do_not_fit(built_lib):
     with pytest.raises(RuntimeError, match="status 1"):
         d.prompt([[5] * (d.max_nodes + 5), None])
     assert all(torch.equal(a, b) for a, b in zip(before, (d.refs, d.table, d.lens, d.pool)))
+
+
+@pytest.mark.parametrize("tree,match", [(([1, 2], [-1, 0]), "position 30"), (([-1], [-1]), "vocabulary"),
+                                        (([4096], [-1]), "vocabulary"), (([1] * 33, [-1] + [0] * 32), "at most 32"),
+                                        (([1, 2], [-1]), "1 parents")])
+def test_decoder_refuses_what_it_cannot_index(tree, match):
+    """A position without a uniform number, a token outside the vocabulary and a tree too large would be
+    indexes out of range on the device; they are refused before anything is queued."""
+    import torch
+    from g4dense_b200 import tree_decode as T
+    d = object.__new__(T.Decoder)
+    d.m, d.seqs, d.max_nodes, d.held = T.Model, 2, 32, [0, 29]
+    with pytest.raises(ValueError, match=match):
+        d.round([None, tree], torch.zeros(2, 30))
+
+
+@pytest.mark.gpu
+def test_decoder_knows_its_lengths(built_lib):
+    import torch
+    from g4dense_b200 import tree_decode as T
+    d = T.Decoder(T.Model(), 3)
+    uniform = torch.rand(3, 60, generator=torch.Generator().manual_seed(5)).cuda()
+    d.prompt([[5] * 40, None, [1, 2]])
+    d.round([([1, 2, 3], [-1, 0, 0]), None, ([7], [-1])], uniform)
+    d.fork([0], [1])
+    assert d.held == d.lens.tolist() and d.held[0] > 40 and d.held[2] == 3
+    d.finish([0])
+    assert d.held == d.lens.tolist() and d.held[0] == 0

@@ -72,6 +72,7 @@ class Decoder:
         self.refs, self.table = torch.zeros(pages, **i32), torch.full((seqs, width), -1, **i32)
         self.lens, self.status = torch.zeros(seqs, **i32), torch.zeros(1, **i32)
         self.path, self.count, self.next = torch.zeros(seqs, max_nodes, **i32), torch.zeros(seqs, **i32), torch.zeros(seqs, **i32)
+        self.held = [0] * seqs  # lens as the host knows them
         self.workspace = torch.empty(api.tree_attention_workspace(max_nodes, model.heads, model.kv_heads, model.head_dim),
                                      dtype=torch.uint8, device="cuda")
 
@@ -101,6 +102,19 @@ class Decoder:
             h = h + _product(b["down"], torch.nn.functional.gelu(gate, approximate="tanh") * up)
         return 4.0 * _product(m.head, _norm(h)), rows
 
+    def _fits(self, trees, positions):
+        """Refuses trees whose tokens, nodes or positions lie outside the arrays that they index on the device."""
+        for s, t in enumerate(trees):
+            if t is None:
+                continue
+            if len(t[0]) != len(t[1]) or len(t[0]) > self.max_nodes:
+                raise ValueError(f"sequence {s}: {len(t[0])} tokens, {len(t[1])} parents, at most {self.max_nodes} nodes")
+            if any(not 0 <= x < self.m.vocab for x in t[0]):
+                raise ValueError(f"sequence {s}: a token outside the vocabulary of {self.m.vocab}")
+            deepest = self.held[s] + int(api.tree_mask(t[1])[1].max(initial=0))
+            if positions is not None and deepest >= positions:
+                raise ValueError(f"sequence {s}: no uniform number for position {deepest}")
+
     def _nodes(self, trees):
         """Device arrays of the sequences' trees, each a (tokens, parents) pair (None: no nodes)."""
         import torch
@@ -125,18 +139,22 @@ class Decoder:
         import torch
         for at in range(0, max(len(p) for p in prompts if p), self.max_nodes):
             parts = [p[at:at + self.max_nodes] if p else [] for p in prompts]
-            tokens, _, cu, mask, depth, owner = self._nodes([(p, list(range(-1, len(p) - 1))) for p in parts])
+            trees = [(p, list(range(-1, len(p) - 1))) for p in parts]
+            self._fits(trees, None)
+            tokens, _, cu, mask, depth, owner = self._nodes(trees)
             _, rows = self._forward(tokens, cu, mask, depth, self.lens[owner] + depth)
             self.count.copy_(torch.tensor([len(p) for p in parts], dtype=torch.int32))
             self._grow()
             self._commit(rows, cu, None)
             self.check()  # before the next chunk, whose status replaces this one's
+            self.held = [n + len(p) for n, p in zip(self.held, parts)]
 
     def round(self, trees, uniform, temperature=0.0, top_k=0, top_p=1.0):
         """One verification round. trees[s]: (tokens, parents) with the pending token first, or None;
-        uniform [seqs][max_nodes + context]: the number that decides the token after each position.
+        uniform [seqs][positions]: the number that decides the token after each position.
         Returns per sequence the accepted drafts and the token drawn after them."""
         import torch
+        self._fits(trees, uniform.shape[1])
         tokens, parents, cu, mask, depth, owner = self._nodes(trees)
         position = self.lens[owner] + depth
         logits, rows = self._forward(tokens, cu, mask, depth, position)
@@ -153,6 +171,7 @@ class Decoder:
         # The host drafter's read; everything above was queued without one.
         count, path, nxt = self.count.tolist(), self.path.tolist(), self.next.tolist()
         self.check()
+        self.held = [n + c for n, c in zip(self.held, count)]
         return [None if trees[s] is None else [trees[s][0][i] for i in path[s][1:count[s]]] + [nxt[s]]
                 for s in range(self.seqs)]
 
@@ -161,11 +180,16 @@ class Decoder:
         ids = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (src, dst)]
         api.pages_fork(self.pool, self.refs, self.table, self.lens, *ids, self.refs, self.table, self.lens, self.status)
         self.check()
+        for a, b in zip(src, dst):
+            self.held[b] = self.held[a]
 
     def finish(self, seqs):
         import torch
         api.pages_free(self.refs, self.table, self.lens, torch.tensor(seqs, dtype=torch.int32, device="cuda"), self.page,
                        self.refs, self.table, self.lens)
+        for s in seqs:
+            if 0 <= s < self.seqs:
+                self.held[s] = 0
 
     def compact(self):
         import torch
