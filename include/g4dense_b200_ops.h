@@ -215,8 +215,10 @@ G4B_API int g4b_pages_copy(const g4b_page_pool* from, const g4b_page_pool* to, c
                            const int32_t* dst, int n, void* stream);
 /* Writes rows [n_planes][n_tokens][row_bytes] (plane stride rows_plane_stride bytes) of sequence s's
  * nodes path[s][0 .. count[s]) (NULL path: the first count[s]) at positions lens[s] onwards of its
- * pages, and lens_out[s] = lens[s] + count[s]. status (may be NULL) is g4b_pages_reserve's: nothing
- * is committed unless it is 0. */
+ * pages, and lens_out[s] = lens[s] + count[s]. A row whose node is not one of the sequence's own, or
+ * whose position has no page, ends that sequence's commit: the rows ahead of it are written, and the
+ * length grows by those alone. status (may be NULL) is g4b_pages_reserve's: nothing is committed
+ * unless it is 0. */
 G4B_API int g4b_pages_commit(const g4b_page_pool* pool, const int32_t* table, int table_width, const int32_t* lens,
                              int n_seqs, const void* rows, int64_t rows_plane_stride, int n_tokens,
                              const int32_t* cu_nodes, const int32_t* path, int path_width, const int32_t* count,

@@ -10,6 +10,7 @@ import re
 import subprocess
 from pathlib import Path
 
+import numpy as np
 import pytest
 
 from test_tree_round import check_row, sample
@@ -390,3 +391,42 @@ def test_decoder_knows_its_lengths(built_lib):
     assert d.held == d.lens.tolist() and d.held[0] > 40 and d.held[2] == 3
     d.finish([0])
     assert d.held == d.lens.tolist() and d.held[0] == 0
+
+
+# ----------------------------------------------------------------------------------------- pages
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [True, False])
+def test_commit_stops_at_the_first_row_without_a_place(built_lib, in_place):
+    """A path entry that is not one of the sequence's nodes, a count above them, a position past the table
+    or without a page: the rows ahead of it are committed, and the length grows by those alone."""
+    import torch
+    from g4dense_b200 import api
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    planes, page, sizes = 3, 4, [3, 2, 0, 40, 5, 1, 4]
+    lens = [2, 7, 0, 1, 5, 3, -4]
+    table = [[0, 1, 2] + [-1] * 9, [3, 4, -1] + [-1] * 9, [5] + [-1] * 11, list(range(6, 18)), [18, 19, 99] + [-1] * 9,
+             [20, -1, -1] + [-1] * 9, [21] * 12]
+    cu = np.concatenate([[0], np.cumsum(sizes)])
+    width = 41
+    for kind in ("path", "first"):
+        path = [[0, 3, 1], [0, 1, 2, -1], [0], list(range(40)) + [40], [0, 2, 4, 1, 3], [0, 0, 0], [0, 1]]
+        count = [3, 2, 1, 41, 5, 3, 2]
+        if kind == "first":
+            path, count = [list(range(60)) for _ in sizes], [3, 5, 1, 2 ** 31 - 1, 3, -2, 4]
+        g = torch.Generator(device="cuda").manual_seed(1)
+        pool = torch.randn(planes, 22, page, 8, generator=g, device="cuda")
+        rows = torch.randn(planes, int(cu[-1]), 8, generator=g, device="cuda")
+        want, grown = pool.clone(), list(lens)
+        for s, n in enumerate(lens):
+            for i in range(min(max(count[s], 0), len(path[s]))):
+                col = (n + i) // page
+                if n < 0 or not 0 <= path[s][i] < sizes[s] or col >= 12 or not 0 <= table[s][col] < 22:
+                    break
+                want[:, table[s][col], (n + i) % page] = rows[:, cu[s] + path[s][i]]
+                grown[s] += 1
+        old = dev(lens)
+        new = old if in_place else torch.full_like(old, 9)
+        api.pages_commit(pool, dev(table), old, rows, dev(cu.tolist()),
+                         dev([(p + [-1] * width)[:width] for p in path]) if kind == "path" else None, dev(count), new)
+        assert new.tolist() == grown and torch.equal(pool, want), kind

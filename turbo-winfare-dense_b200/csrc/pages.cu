@@ -362,36 +362,65 @@ __global__ void __launch_bounds__(kCopyThreads)
     });
 }
 
-// One warp per (sequence, plane) moves the accepted rows into the sequence's pages.
-__global__ void __launch_bounds__(kCopyThreads)
-    commit_kernel(PagePool pool, const int32_t* __restrict__ table, int width, const int32_t* __restrict__ lens,
-                  const char* __restrict__ rows, long long rows_plane_stride, int n_tokens,
-                  const int32_t* __restrict__ cu_nodes, const int32_t* __restrict__ path, int path_width,
-                  const int32_t* __restrict__ count, const int32_t* __restrict__ status, int32_t* lens_out) {
-    const int s = blockIdx.x, lane = threadIdx.x & 31;
-    const int plane = blockIdx.y * (kCopyThreads / 32) + (threadIdx.x >> 5);
-    const bool go = !status || *status == kPagesOk;
-    const int len = lens[s], n = go ? min(max(count[s], 0), path ? path_width : INT_MAX) : 0;
-    if (blockIdx.y == 0 && threadIdx.x == 0 && lens_out) lens_out[s] = len + n;
-    if (plane >= pool.planes || len < 0) return;
-    const int first = cu_nodes[s];
-    for (int i = 0; i < n; ++i) {
-        const int node = path ? path[(long long)s * path_width + i] : i;
-        const long long token = (long long)first + node;
-        const int pos = len + i, col = pos / pool.page_size;
-        if (node < 0 || token < 0 || token >= n_tokens || col >= width) continue;
-        const int page = table[(long long)s * width + col];
-        if (page < 0 || page >= pool.pages) continue;
-        copy_bytes<32>(pool.base + plane * pool.plane_stride + page * pool.page_stride +
-                           (long long)(pos % pool.page_size) * pool.row_bytes,
-                       rows + plane * rows_plane_stride + token * pool.row_bytes, pool.row_bytes, lane);
+struct Commit {
+    const int32_t* table;
+    const int32_t* lens;
+    const int32_t* cu_nodes;
+    const int32_t* path;
+    const int32_t* count;
+    const int32_t* status;
+    int width, path_width, n_tokens, pages, page_size;
+};
+
+// Calls use(token, page, row) for each of sequence s's accepted rows, up to the first whose node is not one
+// of the sequence's own or whose position has no page, and returns their number. A whole warp: a lane
+// looks one of 32 rows up, then all take them one by one.
+template <class Use>
+__device__ __forceinline__ int commit_rows(const Commit& c, int s, int lane, Use use) {
+    const int len = c.lens[s];
+    const unsigned n = c.status && *c.status != kPagesOk ? 0 : max(0, min(c.count[s], c.path ? c.path_width : INT_MAX));
+    const long long first = c.cu_nodes[s], nodes = c.cu_nodes[s + 1] - first;
+    for (unsigned b = 0; b < n; b += 32) {
+        const unsigned i = b + lane;
+        const long long pos = (long long)len + i, col = pos / c.page_size;
+        int node = -1, page = -1;
+        if (i < n && len >= 0) {
+            node = c.path ? c.path[(long long)s * c.path_width + i] : (int)i;
+            if (col < c.width) page = c.table[(long long)s * c.width + col];
+        }
+        const bool good = node >= 0 && node < nodes && first >= 0 && first + node < c.n_tokens && page >= 0 && page < c.pages;
+        const unsigned bad = ~__ballot_sync(0xffffffffu, good);
+        const int m = bad ? __ffs(bad) - 1 : 32;
+        for (int k = 0; k < m; ++k)
+            use(first + __shfl_sync(0xffffffffu, node, k), __shfl_sync(0xffffffffu, page, k),
+                (int)(((long long)len + b + k) % c.page_size));
+        if (bad) return (int)b + m;
     }
+    return (int)n;
 }
 
-__global__ void commit_lens_kernel(int32_t* lens, int seqs, const int32_t* count, const int32_t* status,
-                                   int path_width) {
-    const int s = blockIdx.x * blockDim.x + threadIdx.x;
-    if (s < seqs && (!status || *status == kPagesOk)) lens[s] += min(max(count[s], 0), path_width);
+// One warp per (sequence, plane) moves the accepted rows into the sequence's pages.
+__global__ void __launch_bounds__(kCopyThreads)
+    commit_kernel(PagePool pool, Commit c, const char* __restrict__ rows, long long rows_plane_stride, int32_t* lens_out) {
+    const int s = blockIdx.x, lane = threadIdx.x & 31;
+    const int plane = blockIdx.y * (kCopyThreads / 32) + (threadIdx.x >> 5);
+    if (plane >= pool.planes) return;
+    char* to = pool.base + plane * pool.plane_stride;
+    const char* from = rows + plane * rows_plane_stride;
+    const int n = commit_rows(c, s, lane, [&](long long token, int page, int row) {
+        copy_bytes<32>(to + page * pool.page_stride + (long long)row * pool.row_bytes, from + token * pool.row_bytes,
+                       pool.row_bytes, lane);
+    });
+    if (plane == 0 && lane == 0 && lens_out) lens_out[s] = c.lens[s] + n;
+}
+
+// One warp per sequence.
+__global__ void __launch_bounds__(kCopyThreads) commit_lens_kernel(Commit c, int32_t* lens, int seqs) {
+    const int s = blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (s >= seqs) return;
+    const int n = commit_rows(c, s, lane, [](long long, int, int) {});
+    __syncwarp();  // every lane has read the length
+    if (lane == 0) lens[s] += n;
 }
 
 int copy_blocks(long long units) { return (int)std::min<long long>(std::max<long long>(units, 1), 148 * 8); }
@@ -439,14 +468,13 @@ cudaError_t pages_commit(const PagePool& pool, const int32_t* table, int width, 
                          const int32_t* path, int path_width, const int32_t* count, const int32_t* status,
                          int32_t* lens_out, cudaStream_t st) {
     const dim3 grid(seqs, (pool.planes + kCopyThreads / 32 - 1) / (kCopyThreads / 32));
+    const Commit c{table, lens, cu_nodes, path, count, status, width, path_width, n_tokens, pool.pages, pool.page_size};
     // With one array for both, other blocks still read the old lengths: they change afterwards.
     const bool apart = lens_out != lens;
-    commit_kernel<<<grid, kCopyThreads, 0, st>>>(pool, table, width, lens, rows, rows_plane_stride, n_tokens, cu_nodes,
-                                                 path, path_width, count, status, apart ? lens_out : nullptr);
+    commit_kernel<<<grid, kCopyThreads, 0, st>>>(pool, c, rows, rows_plane_stride, apart ? lens_out : nullptr);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || apart) return e;
-    commit_lens_kernel<<<(seqs + 255) / 256, 256, 0, st>>>(lens_out, seqs, count, status,
-                                                           path ? path_width : INT_MAX);
+    commit_lens_kernel<<<(seqs + kCopyThreads / 32 - 1) / (kCopyThreads / 32), kCopyThreads, 0, st>>>(c, lens_out, seqs);
     return cudaGetLastError();
 }
 
