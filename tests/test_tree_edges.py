@@ -430,3 +430,41 @@ def test_commit_stops_at_the_first_row_without_a_place(built_lib, in_place):
         api.pages_commit(pool, dev(table), old, rows, dev(cu.tolist()),
                          dev([(p + [-1] * width)[:width] for p in path]) if kind == "path" else None, dev(count), new)
         assert new.tolist() == grown and torch.equal(pool, want), kind
+
+
+def test_fork_checks_do_not_depend_on_timing():
+    """Whether a warp looks at its sources' pages may not depend on what other warps have found by then: the
+    word they raise is read between two barriers of the block, once, for all of them."""
+    code = code_of("pages.cu")
+    body = code[code.index("fork_kernel(PageTables t"):code.index("compact_kernel(PageTables t")]
+    reads = [m.start() for m in re.finditer(r"code == kPagesOk", body)]
+    marks = [m.start() for m in re.finditer(r"__syncthreads\(\)", body)]
+    raises = [m.start() for m in re.finditer(r"atomicMax\(&code", body)]
+    between = lambda a, b: any(a < m < b for m in marks)  # noqa: E731
+    assert len(reads) >= 2
+    for r in reads:
+        assert all(between(w, r) if w < r else between(r, w) for w in raises)
+
+
+@pytest.mark.gpu
+def test_fork_with_several_faults(built_lib):
+    """The largest code of all faults, whichever warp meets which first."""
+    import torch
+    from g4dense_b200 import api
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    seqs, width, n = 400, 64, 200
+    table = torch.full((seqs, width), -1, dtype=torch.int32)
+    table[:n] = torch.arange(n * width).reshape(n, width)
+    lens = dev([4 * width] * n + [0] * (seqs - n))
+    refs, status = torch.ones(n * width + 8, dtype=torch.int32, device="cuda"), dev([9])
+    pool = torch.zeros(1, n * width + 8, 4, 4, device="cuda")
+    for bad_page, bad_seq in ((0, 150), (150, 0), (37, 38), (199, 1)):
+        t = table.clone()
+        t[bad_page, width - 1] = 10 ** 6  # found in the last round of its warp
+        t[n + bad_seq, 0] = 3             # a destination that holds a page
+        t = t.cuda()
+        for _ in range(20):
+            outs = [torch.full_like(x, 5) for x in (refs, t, lens)]
+            api.pages_fork(pool, refs, t, lens, dev(list(range(n))), dev(list(range(n, 2 * n))), *outs, status)
+            assert status.item() == 4
+            assert all(torch.equal(a, b) for a, b in zip(outs, (refs, t, lens)))

@@ -194,8 +194,10 @@ __global__ void __launch_bounds__(kMetaThreads)
         need += tot;
     }
     __syncthreads();
+    const bool sound = code == kPagesOk;
+    __syncthreads();  // all have read it before one raises it again
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (code == kPagesOk)  // every page that a source holds has to exist, and a destination to hold none
+    if (sound)  // every page that a source holds has to exist, and a destination to hold none
         for (int i = warp; i < n; i += kMetaThreads / 32) {
             const int held = pages_for(t.lens[src[i]], t.page_size);
             const int32_t* row = t.table + (long long)src[i] * t.width;
