@@ -183,13 +183,14 @@ typedef struct g4b_page_pool {
     int n_planes, n_pages, page_size, row_bytes;
 } g4b_page_pool;
 
-/* The keeping of n_seqs (up to 4096) sequences' pages: refs [n_pages] counts how many sequences hold
- * a page (0: free), table [n_seqs][table_width] lists each sequence's pages (-1: none), lens
- * [n_seqs] its tokens. Each call reads refs, table and lens and writes refs_out, table_out and
- * lens_out (those it changes), which may be the same arrays. New pages are the free pages of lowest
- * id, in (sequence, position) order: results depend on the state alone. status: 0 done, 1 too few
- * free pages, 2 more pages than the table row holds (or a negative length), 3 a bad sequence index,
- * 4 a page id out of range in the table; the outputs then equal the inputs. */
+/* The keeping of n_seqs (up to 4096) sequences' pages: refs [n_pages] (up to 2^24) counts how many
+ * sequences hold a page (0: free), table [n_seqs][table_width] (below 2^31 cells) lists each sequence's
+ * pages (-1: none), lens [n_seqs] its tokens. Each call reads refs, table and lens and writes refs_out,
+ * table_out and lens_out (those it changes), which may be the same arrays. New pages are the free pages
+ * of lowest id, in (sequence, position) order: results depend on the state alone. status: 0 done, 1 too
+ * few free pages, 2 more pages than the table row holds (or a negative length), 3 a bad sequence index,
+ * 4 a page id out of range in the table, the largest where several hold; the outputs then equal the
+ * inputs. */
 typedef struct g4b_page_tables {
     const int32_t *refs, *table, *lens;
     int32_t *refs_out, *table_out, *lens_out;

@@ -468,3 +468,14 @@ def test_fork_with_several_faults(built_lib):
             api.pages_fork(pool, refs, t, lens, dev(list(range(n))), dev(list(range(n, 2 * n))), *outs, status)
             assert status.item() == 4
             assert all(torch.equal(a, b) for a, b in zip(outs, (refs, t, lens)))
+
+
+def test_tables_beyond_whole_number_counts_are_refused(built_lib):
+    """Page counts of a call are summed in 32 bits: a table of 2^31 cells or more could wrap them, and a
+    reserve would report success without a page. Refused on the host."""
+    from g4dense_b200 import api
+    pack = lambda seqs, width: api._PAGE_TABLES.pack(*[4096] * 6, 1 << 20, seqs, width, 1)  # noqa: E731
+    L = api.lib()
+    for seqs, width in ((4096, 1 << 19), (2, 1 << 30)):
+        assert L.g4b_pages_reserve(pack(seqs, width), 4096, 4096, None) == 1
+        assert b"2^31 cells" in L.g4b_last_error()

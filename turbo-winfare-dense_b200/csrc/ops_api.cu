@@ -419,6 +419,7 @@ const char* bad_tables(const g4b_page_tables* t, bool lens, bool lens_out) {
     if (t->n_pages < 1 || t->n_pages > (1 << 24) || t->n_seqs < 1 || t->n_seqs > g4b::kMaxPageSeqs ||
         t->table_width < 1 || t->page_size < 1 || (int64_t)t->table_width * t->page_size > INT32_MAX)
         return "sizes out of range (1..4096 sequences, at most 2^24 pages, table_width * page_size in 31 bits)";
+    if ((int64_t)t->n_seqs * t->table_width > INT32_MAX) return "a table of 2^31 cells or more";  // counts are 32 bits
     return nullptr;
 }
 g4b::PagePool pool_of(const g4b_page_pool* p) {
