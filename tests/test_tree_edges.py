@@ -479,3 +479,28 @@ def test_tables_beyond_whole_number_counts_are_refused(built_lib):
     for seqs, width in ((4096, 1 << 19), (2, 1 << 30)):
         assert L.g4b_pages_reserve(pack(seqs, width), 4096, 4096, None) == 1
         assert b"2^31 cells" in L.g4b_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("ahead", [5.4, 18.0, 21.0])
+@pytest.mark.parametrize("place", [0, 200])
+def test_many_small_probabilities(built_lib, dtype, ahead, place):
+    """One key, with no value, `ahead` nats above 299 others: the others' small probabilities make up the
+    output. A probability is held to u of itself or, where fp16 is subnormal (below 2^-21 of the row's
+    reference, its numbers being held 2^7 times), to 2^-32; the output to u, or to 2^-25 where it is
+    subnormal. Scores are at most 21: fp32 adds 2 units in the last place of 32 and a few of the sums."""
+    import torch
+    from test_tree_attention import UNIT, make, run
+    c = make([300], [2], 1, 1, 64, 16, dtype, seed=1)
+    c["q"][:] = 1.0
+    c["k_pool"][:], c["v_pool"][:], c["k_new"][:], c["v_new"][:] = 0, 1000.0, 0, 0
+    p = c["table"][0, place // 16].long()
+    c["k_pool"][p, place % 16], c["v_pool"][p, place % 16] = ahead / 8, 0
+    score = float(c["k_pool"][p, place % 16, 0, 0]) * 8
+    seen = 300 + (c["depth"].double() + 1)  # keys a node sees, itself and its parent among them
+    small = np.exp(-score)
+    want = (299 * 1000.0 * small) / (1 + (seen - 1) * small)
+    u, err = UNIT[dtype], (run(c).double() - want[:, None, None]).abs()
+    tol = want * (2.1 * u + 2.0 ** -18) + (299 * 1000 * 2.0 ** -32 + 2.0 ** -25 if dtype == "fp16" else 0)
+    assert (err <= tol[:, None, None]).all(), (err.max().item(), tol.min().item(), want.tolist())

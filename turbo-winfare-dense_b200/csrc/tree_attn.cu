@@ -29,7 +29,7 @@
 //   * one thread of another issues the MMAs, S^T into two alternating TMEM buffers;
 //   * four groups of four warps take a quarter of the rows each, a thread one key of all its rows: they
 //     hold the softmax in fp32, write P^T (rounded to the cache's type, 8 rows a store) and, when a
-//     row's score exceeds its reference maximum by more than 8 (in powers of two), move the
+//     row's score exceeds the maximum it last took by more than 8 (in powers of two), move the
 //     reference and rescale that row of O^T in TMEM. In between only a vote of the group is needed,
 //     so most tiles run without any reduction over keys; the sums are reduced once per part.
 // What a node must not see never reaches the MMA: scores are replaced, not added to, and in tiles
@@ -85,7 +85,14 @@ constexpr int kTreeBox = 8;          // node rows per TMA box: the swizzle's eig
 // 48 with 64.
 constexpr int kBoxCopy = 8192;
 constexpr float kUnset = 1e30f;      // negated reference of a row that has seen no key
-constexpr float kLazy = 8.f;         // a reference moves when a score exceeds it by 2^8
+constexpr float kLazy = 8.f;         // a reference moves when a score exceeds the maximum it was set to by 2^8
+// A row's reference lies this far below that maximum, in powers of two: its probabilities, sum and output
+// carry the factor until the end. fp16 is subnormal below 2^-14 and stops at 65504; with numbers of up to
+// 2^(7 + 8) a probability keeps its 11 bits down to 2^-21 of the maximum and is lost below 2^-32, where
+// without the factor a long row's tail was lost below 2^-25 (while the sum still counted it). bf16 has
+// the exponents of fp32.
+template <bool kBf16>
+constexpr float kLift = kBf16 ? 0.f : 7.f;
 constexpr size_t kSmemLimit = 232448 - 2048;  // leaves room for blocks of the second kernel
 // What starting and finishing an item costs, in tiles, when the shares are cut: it grows with the rows,
 // the tiles' time less so. 128 rows an item, dim 256: 131 us over a 1024-key window and 282 over up to
@@ -136,7 +143,7 @@ static_assert(offsetof(Ctl, corr) % 16 == 0 && offsetof(Ctl, inv) % 16 == 0 && a
 // What a part's rows carry, twice: the next part's is set up before the current one is written out.
 struct Rows {
     long long* out;   // offset of the row's output in elements
-    float* nref;      // negated reference maximum of a row, in powers of two
+    float* nref;      // negated reference of a row, in powers of two
     int* start;       // first cached position a row sees
     int* depth;
     uint32_t* mask;   // [words][N]
@@ -878,7 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (edge) tc::wait_st();
                 bool waited = tile == 0;
-                if (fresh || group_or(grp, over > kLazy)) {
+                if (fresh || group_or(grp, over > kLazy + kLift<kBf16>)) {
 #pragma unroll 1
                     for (int f = 0; f < nh && !fresh; f += 8) {
                         float m[8];
@@ -893,9 +900,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float top = fmaxf(fmaxf(c.red[0][r], c.red[1][r]), fmaxf(c.red[2][r], c.red[3][r]));
                         const float old = rs.nref[r];
                         float f = 1.f;
-                        if (top > -INFINITY && (old == kUnset || top + old > kLazy)) {
-                            f = old == kUnset ? 0.f : exp2_approx(-old - top);
-                            rs.nref[r] = -top;
+                        if (top > -INFINITY && (old == kUnset || top + old > kLazy + kLift<kBf16>)) {
+                            f = old == kUnset ? 0.f : exp2_approx(kLift<kBf16> - old - top);
+                            rs.nref[r] = kLift<kBf16> - top;
                         }
                         c.corr[r] = f;
                     }
