@@ -504,3 +504,118 @@ def test_many_small_probabilities(built_lib, dtype, ahead, place):
     u, err = UNIT[dtype], (run(c).double() - want[:, None, None]).abs()
     tol = want * (2.1 * u + 2.0 ** -18) + (299 * 1000 * 2.0 ** -32 + 2.0 ** -25 if dtype == "fp16" else 0)
     assert (err <= tol[:, None, None]).all(), (err.max().item(), tol.min().item(), want.tolist())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [33, 64, 65, 100, 333])
+@pytest.mark.parametrize("longest", [40, 900])
+@pytest.mark.parametrize("window", [0, 30])
+def test_many_sequences(built_lib, seqs, longest, window):
+    """More sequences than a warp has lanes, and than the scheduling warp adds up by itself; whole runs of
+    them without nodes, at both ends too; items that stay whole (tables of up to 4 tiles) and that are cut."""
+    import random
+    from test_tree_attention import check, make
+    rng = random.Random(seqs + longest)
+    lens = [rng.choice([0, 1, rng.randrange(longest), longest]) for _ in range(seqs)]
+    nodes = [rng.choice([0, 1, 2, 4]) for _ in range(seqs)]
+    for a, b in ((0, 3), (seqs // 2, seqs // 2 + 18), (seqs - 2, seqs)):
+        nodes[a:min(b, seqs)] = [0] * (min(b, seqs) - a)
+    lens[4] = longest
+    check(make(lens, nodes, 4, 2, 64, 16, "bf16", seed=seqs), window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128, 512])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
+def test_hidden_values_in_items_that_are_cut(built_lib, dtype, dim, poison):
+    """Infinities and NaN in values that some nodes see and others do not, in the first and last tiles of an
+    item that several blocks work on."""
+    import torch
+    from test_tree_attention import formula, make, run
+    chain = [-1, 0, 1, 2, 3, 4, 5, 6]
+    c = make([3000, 2100], [8, 5], 4, 2, dim, 16, dtype, seed=dim, parents=[chain, chain])
+    want = run(c, 1000)
+    key = 3000 + 3 - 1000  # seen by depths 0..2 of the first sequence
+    c["v_pool"][c["table"][0, key // 16].long(), key % 16, :, 5] = poison
+    c["v_new"][6, 0, 9] = poison  # by nodes 6 and 7, in the heads of K/V head 0
+    got, (o, _, _) = run(c, 1000), formula(c, 1000)
+    strange = torch.zeros_like(got, dtype=torch.bool)
+    strange[:3, :, 5] = True
+    strange[6:8, :2, 9] = True
+    assert torch.equal(~torch.isfinite(got), strange) and torch.equal(~torch.isfinite(o), strange)
+    assert torch.equal(got[~strange], want[~strange])
+    assert torch.equal(torch.nan_to_num(got[strange].double(), nan=3.0), torch.nan_to_num(o[strange].to(got.dtype).double(), nan=3.0))
+
+
+@pytest.mark.gpu
+def test_bad_pages_and_lengths_give_the_formula_without_them(built_lib):
+    """A page id out of range reads as zeros, a length past the table is the table's."""
+    import torch
+    from test_tree_attention import UNIT, formula, make, run
+    c = make([50, 10, 30], [3, 2, 1], 4, 2, 64, 16, "bf16", seed=2)
+    c["table"][0, 1], c["table"][1, 0], c["lens"][0], c["lens"][2] = 10 ** 6, -5, 10 ** 9, -7
+    got = run(c)
+    zero = c["k_pool"].shape[0]
+    d = dict(c, k_pool=torch.cat([c["k_pool"], torch.zeros_like(c["k_pool"][:1])]),
+             v_pool=torch.cat([c["v_pool"], torch.zeros_like(c["v_pool"][:1])]), table=c["table"].clone(), lens=c["lens"].clone())
+    d["table"][0, 1], d["table"][1, 0], d["lens"][0], d["lens"][2] = zero, zero, 16 * c["table"].shape[1], 0
+    o, a, _ = formula(d)
+    assert ((got.double() - o).abs() <= UNIT["bf16"] * (o.abs() + a) * 1.05 + 4e-5 * a).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [True, False])
+def test_large_pools(built_lib, in_place):
+    """Reserve, fork, free and compaction in a pool of 70000 pages, nearly full, its free pages far in."""
+    import torch
+    from g4dense_b200 import api
+    from test_tree_round import Plain
+    rng = np.random.default_rng(3)
+    pages, seqs, width = 70001, 90, 1500
+    plain = Plain(rng.integers(0, 2 ** 15, (1, pages, 2, 8)).astype(np.int16), seqs, width)
+    dev = lambda x: torch.from_numpy(np.array(x, dtype=np.int32)).cuda()  # noqa: E731
+    pool = torch.from_numpy(plain.pool.copy()).cuda()
+    state, status = [dev(plain.refs), dev(plain.table), dev(plain.lens)], dev([9])
+
+    def step(what, call, expect):
+        new = state if in_place else [torch.full_like(t, 77) for t in state]
+        call(new)
+        code = expect()
+        assert code is None or status.item() == code, what
+        state[:] = new
+        for name, a, b in zip(("refs", "table", "lens"), state, (plain.refs, plain.table, plain.lens)):
+            assert np.array_equal(a.cpu().numpy(), b), (what, name)
+        assert np.array_equal(pool.cpu().numpy(), plain.pool), what
+
+    def reserve(grow):
+        def call(new):
+            api.pages_reserve(*state, dev(grow), 2, new[0], new[1], status)
+            if not in_place:
+                new[2] = state[2]
+            ok = 1 - status.clamp(max=1)
+            new[2] = new[2] + dev(grow) * ok
+
+        def expect():
+            code = plain.reserve(grow.tolist())
+            if code == 0:
+                plain.lens += grow.astype(np.int32)
+            return code
+        step("reserve", call, expect)
+
+    reserve(np.array([1801] * 76 + [0] * 14))           # 68476 pages
+    reserve(np.array([1000] + [0] * 89))                 # the rest is far in
+    reserve(np.array([0] * 76 + [400] * 14))             # too many
+    src, dst = list(range(0, 20)), list(range(76, 90))
+    step("fork", lambda new: api.pages_fork(pool, *state, dev(src[:14]), dev(dst), *new, status),
+         lambda: plain.fork(src[:14], dst))
+    gone = [0, 3, 4, 5, 40, 41, 76, 80]
+    step("free", lambda new: api.pages_free(*state, dev(gone), 2, *new), lambda: plain.free(gone))
+    moves = dev([0] * (1 + 2 * pages))
+
+    def compact(new):
+        api.pages_compact(pool, state[0], state[1], new[0], new[1], moves)
+        new[2] = state[2]
+    step("compact", compact, lambda: (plain.compact(), None)[1])
+    assert moves[0].item() > 1000
+    reserve(np.array([0] * 76 + [3] + [0] * 13))
