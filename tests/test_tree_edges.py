@@ -191,9 +191,11 @@ def calls(monkeypatch):
     import torch
     from g4dense_b200 import api
     calls = Calls()
+    api._types()
     monkeypatch.setattr(api, "lib", lambda: calls)
+    monkeypatch.setattr(api, "_here", lambda: 0)
+    monkeypatch.setattr(api, "_stream_of", lambda dev: 1234)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: type("S", (), {"cuda_stream": 1234}))
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     return calls
 
 

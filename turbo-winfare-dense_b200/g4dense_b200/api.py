@@ -199,27 +199,27 @@ def sample_token(logits, temperature, top_p, top_k, seed, workspace, out, stream
                                   _dptr(workspace), _dptr(out), _stream(stream)), "g4b_sample_token")
 
 _dtypes = {}  # torch dtype -> g4b_dtype, filled by _types()
-_i32 = _f32 = _cuda = None
+_i32 = _f32 = _here = _stream_of = None
 
 
 def _types():
     """Loads torch's types and the library once; returns the library."""
-    global _i32, _f32, _cuda
+    global _i32, _f32, _here, _stream_of
     if _i32 is None:
         import torch
         _dtypes.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2})
-        _f32, _cuda = torch.float32, torch.cuda
+        _f32 = torch.float32
+        # The current device, on which every tensor of a call has to be (kernels launch there), and the handle
+        # of its current stream: torch.cuda.current_stream() makes an object of it, 3 us a call.
+        _here = torch.cuda.current_device
+        _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
         _i32 = torch.int32
     return lib()
 
 
 def _bad(what):
     raise ValueError(what)
-
-
-def _here():
-    """Index of the current device, on which every tensor of a call has to be: kernels launch there."""
-    return _cuda.current_device()
 
 
 def _ints(name, t, n, dev):
@@ -253,9 +253,9 @@ def _rows_of(name, t, dtype, shape, dev):
     return t.data_ptr(), strides[0] if shape[0] > 1 else n
 
 
-def _at(stream):
+def _at(stream, dev):
     """Handle of the stream given, else of torch's current one: what made the inputs is ordered before."""
-    return (_cuda.current_stream() if stream is None else stream).cuda_stream
+    return _stream_of(dev) if stream is None else stream.cuda_stream
 
 
 def tree_mask(parents, words=None):
@@ -320,7 +320,7 @@ def tree_attention(q, k_pool, v_pool, table, lens, k_new, v_new, cu_nodes, mask,
         0 if depth is None else _ints("depth", depth, tokens, dev), workspace.data_ptr(),
         workspace.numel() * workspace.element_size(), q_stride, out_stride, new_stride, page_stride, seqs, tokens,
         max_nodes, pages, page_size, width, words, heads, kv_heads, dim, window, _dtypes[dtype], scale)
-    rc = L.g4b_tree_attention(a, _at(stream))
+    rc = L.g4b_tree_attention(a, _at(stream, dev))
     if rc:
         _check(rc, "g4b_tree_attention")
 
@@ -347,7 +347,7 @@ def sample_rows(logits, uniform, token, prob=None, kept=None, temperature=None, 
     rc = L.g4b_sample_rows(ptr, _dtypes[logits.dtype], rows, vocab, stride, _floats("uniform", uniform, rows, dev),
                            _floats("temperature", temperature, rows, dev), None if top_k is None else _ints("top_k", top_k, rows, dev),
                            _floats("top_p", top_p, rows, dev), _floats("min_p", min_p, rows, dev), _ints("token", token, rows, dev),
-                           _floats("prob", prob, rows, dev), None if kept is None else _ints("kept", kept, rows, dev), _at(stream))
+                           _floats("prob", prob, rows, dev), None if kept is None else _ints("kept", kept, rows, dev), _at(stream, dev))
     if rc:
         _check(rc, "g4b_sample_rows")
 
@@ -359,7 +359,7 @@ def tree_accept(tokens, parents, sampled, cu_nodes, path, count, next_token, str
     n, seqs, width = tokens.numel(), cu_nodes.numel() - 1, path.shape[-1]
     rc = L.g4b_tree_accept(_ints("tokens", tokens, n, dev), _ints("parents", parents, n, dev), _ints("sampled", sampled, n, dev),
                            _ints("cu_nodes", cu_nodes, seqs + 1, dev), seqs, n, _ints("path", path, seqs * width, dev), width,
-                           _ints("count", count, seqs, dev), _ints("next_token", next_token, seqs, dev), _at(stream))
+                           _ints("count", count, seqs, dev), _ints("next_token", next_token, seqs, dev), _at(stream, dev))
     if rc:
         _check(rc, "g4b_tree_accept")
 
@@ -392,7 +392,7 @@ def pages_reserve(refs, table, lens, grow, page_size, refs_out, table_out, statu
     [pages], table [seqs][width], lens, grow [seqs], status [1]; the outputs may be the inputs."""
     L, dev = _types(), _here()
     rc = L.g4b_pages_reserve(_tables(refs, table, lens, refs_out, table_out, None, page_size, dev),
-                             _ints("grow", grow, lens.numel(), dev), _ints("status", status, 1, dev), _at(stream))
+                             _ints("grow", grow, lens.numel(), dev), _ints("status", status, 1, dev), _at(stream, dev))
     if rc:
         _check(rc, "g4b_pages_reserve")
 
@@ -402,7 +402,7 @@ def pages_fork(pool, refs, table, lens, src, dst, refs_out, table_out, lens_out,
     last page copied. pool [planes][pages][page_size][row...]."""
     L, dev, n = _types(), _here(), src.numel()
     rc = L.g4b_pages_fork(_pool(pool, dev), _tables(refs, table, lens, refs_out, table_out, lens_out, pool.shape[2], dev),
-                          _ints("src", src, n, dev), _ints("dst", dst, n, dev), n, _ints("status", status, 1, dev), _at(stream))
+                          _ints("src", src, n, dev), _ints("dst", dst, n, dev), n, _ints("status", status, 1, dev), _at(stream, dev))
     if rc:
         _check(rc, "g4b_pages_fork")
 
@@ -411,7 +411,7 @@ def pages_free(refs, table, lens, seqs, page_size, refs_out, table_out, lens_out
     """Releases the pages of the sequences seqs[] and empties them (g4b_pages_free)."""
     L, dev, n = _types(), _here(), seqs.numel()
     rc = L.g4b_pages_free(_tables(refs, table, lens, refs_out, table_out, lens_out, page_size, dev), _ints("seqs", seqs, n, dev), n,
-                          _at(stream))
+                          _at(stream, dev))
     if rc:
         _check(rc, "g4b_pages_free")
 
@@ -421,7 +421,7 @@ def pages_compact(pool, refs, table, refs_out, table_out, moves, stream=None):
     receives their number and the (from, to) pairs."""
     L, dev = _types(), _here()
     rc = L.g4b_pages_compact(_pool(pool, dev), _tables(refs, table, None, refs_out, table_out, None, pool.shape[2], dev),
-                             _ints("moves", moves, 1 + 2 * refs.numel(), dev), _at(stream))
+                             _ints("moves", moves, 1 + 2 * refs.numel(), dev), _at(stream, dev))
     if rc:
         _check(rc, "g4b_pages_compact")
 
@@ -429,7 +429,7 @@ def pages_compact(pool, refs, table, refs_out, table_out, moves, stream=None):
 def pages_copy(pool, to_pool, src, dst, stream=None):
     """Page src[i] of pool to page dst[i] of to_pool, in every plane (g4b_pages_copy)."""
     L, dev, n = _types(), _here(), src.numel()
-    rc = L.g4b_pages_copy(_pool(pool, dev), _pool(to_pool, dev), _ints("src", src, n, dev), _ints("dst", dst, n, dev), n, _at(stream))
+    rc = L.g4b_pages_copy(_pool(pool, dev), _pool(to_pool, dev), _ints("src", src, n, dev), _ints("dst", dst, n, dev), n, _at(stream, dev))
     if rc:
         _check(rc, "g4b_pages_copy")
 
@@ -448,7 +448,7 @@ def pages_commit(pool, table, lens, rows, cu_nodes, path, count, lens_out, statu
                             None if path is None else _ints("path", path, seqs * path.shape[-1], dev),
                             0 if path is None else path.shape[-1], _ints("count", count, seqs, dev),
                             None if status is None else _ints("status", status, 1, dev), _ints("lens_out", lens_out, seqs, dev),
-                            _at(stream))
+                            _at(stream, dev))
     if rc:
         _check(rc, "g4b_pages_commit")
 
