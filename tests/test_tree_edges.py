@@ -621,3 +621,43 @@ def test_large_pools(built_lib, in_place):
     step("compact", compact, lambda: (plain.compact(), None)[1])
     assert moves[0].item() > 1000
     reserve(np.array([0] * 76 + [3] + [0] * 13))
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(built_lib):
+    """Pages and logits rows that lie gigabytes apart: element and byte offsets above 2^32."""
+    import torch
+    from g4dense_b200 import api
+    from test_tree_attention import make, run
+    c = make([300, 40], [5, 3], 4, 2, 64, 16, "bf16", seed=1)
+    c["v_new"][3, 1, 7] = float("inf")  # values looked up one by one too
+    want = run(c)
+    pages, apart = c["k_pool"].shape[0], 1 << 28
+    far = torch.empty(pages * apart, dtype=torch.bfloat16, device="cuda").view(pages, apart)
+    assert (pages - 1) * apart > 1 << 32
+    wide = [far[:, i * 4096:i * 4096 + 2048].view(pages, 16, 2, 64) for i in range(3)]
+    wide[0].copy_(c["k_pool"])
+    wide[1].copy_(c["v_pool"])
+    got = run(dict(c, k_pool=wide[0], v_pool=wide[1]))
+    assert torch.equal(torch.nan_to_num(got.double(), nan=1e9), torch.nan_to_num(want.double(), nan=1e9))
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    api.pages_copy(wide[0][None], wide[2][None], dev([0, pages - 1]), dev([pages - 1, 0]))
+    assert torch.equal(wide[2][pages - 1], c["k_pool"][0]) and torch.equal(wide[2][0], c["k_pool"][pages - 1])
+    rows, lens = torch.randn(1, 3, 2, 64, device="cuda").bfloat16(), dev([20])
+    api.pages_commit(wide[2][None], dev([[0, pages - 2]]), lens, rows, dev([0, 3]), None, dev([3]), lens)
+    assert torch.equal(wide[2][pages - 2, 4:7], rows[0]) and lens.item() == 23
+    x = far[:, 8192:8192 + 5000]
+    x.copy_(torch.randn(pages, 5000, generator=torch.Generator().manual_seed(3)))
+    token, _, _ = sample(x, [0.5] * pages, temperature=[0.0] * pages)
+    best = x.float().max(1, keepdim=True).values
+    assert token == [int((r == b).nonzero()[0]) for r, b in zip(x.float(), best)]
+
+
+def test_refusal_of_too_many_tiles_says_why(built_lib):
+    """Tiles are counted in 32 bits over all sequences and heads; a call beyond that names the sizes."""
+    from g4dense_b200 import api
+    L = api.lib()
+    args = api._TREE_ATTENTION.pack(*[4096] * 12, 1 << 40, 1024, 1024, 1024, 1 << 18, 1 << 20, 1 << 20, 1, 1000, 16,
+                                    1 << 26, 1, 16, 16, 64, 0, 0, 1.0)
+    assert L.g4b_tree_attention(args, None) != 0
+    assert b"32 bits" in L.g4b_last_error() and b"n_seqs" in L.g4b_last_error()

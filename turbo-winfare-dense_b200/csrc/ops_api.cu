@@ -363,6 +363,9 @@ int g4b_tree_attention(const g4b_tree_attention_args* x, void* stream) {
     a.window = x->window;
     a.bf16 = x->dtype == G4B_BF16;
     a.scale = x->scale;
+    if (!g4b::tree_attn_countable(a))
+        return fail_msg("g4b_tree_attention: 128-key tiles are counted in 32 bits: n_seqs * kv_heads * page_size * "
+                        "table_width is too large");
     const cudaError_t e = g4b::tree_attn_launch(a, (cudaStream_t)stream);
     return e == cudaSuccess ? 0 : fail(e, "g4b_tree_attention");
 }

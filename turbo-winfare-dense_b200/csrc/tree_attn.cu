@@ -1242,6 +1242,18 @@ Shape shape_for(int max_nodes, int gqa, int dim) {
     return s;
 }
 
+// Rows of a TMA box: the largest power of two that divides a page, so that a box never crosses one.
+int box_rows(const TreeAttnArgs& a) {
+    return std::min(kBoxCopy / (a.dim == 64 ? 128 : 256), a.page_size & -a.page_size);
+}
+// The most tiles an item can have, and the most items.
+long long most_tiles(const TreeAttnArgs& a) {
+    return ((long long)a.width * a.page_size + 2 * box_rows(a) + a.max_nodes + kKeys - 1) / kKeys;
+}
+long long most_items(const TreeAttnArgs& a, int N) {
+    return (long long)a.seqs * a.kv_heads * ((a.max_nodes * (a.heads / a.kv_heads) + N - 1) / N);
+}
+
 cudaError_t make_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
                      const cuuint32_t* box) {
     using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -1297,6 +1309,11 @@ size_t tree_attn_workspace(int max_nodes, int heads, int kv_heads, int dim) {
     return (size_t)2 * sm_count() * N * (dim * sizeof(float) + sizeof(float2)) + sm_count() * sizeof(Split);
 }
 
+bool tree_attn_countable(const TreeAttnArgs& a) {
+    const int N = rows_per_item(a.max_nodes, a.heads / a.kv_heads, a.dim);
+    return most_items(a, N) <= INT32_MAX && most_items(a, N) * (most_tiles(a) + item_cost(N)) <= INT32_MAX;
+}
+
 cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
     const Shape sh = shape_for(a.max_nodes, a.heads / a.kv_heads, a.dim);
     Params p{};
@@ -1331,12 +1348,9 @@ cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
     p.words = sh.words;
     p.slots = sh.slots;
     p.tmem_cols = sh.tmem;
-    // The largest power of two that divides a page, so that a box never crosses one.
-    p.box = std::min(kBoxCopy / (a.dim == 64 ? 128 : 256), a.page_size & -a.page_size);
+    p.box = box_rows(a);
     while (1 << p.box_log < p.box) ++p.box_log;
-    const long long tiles = ((long long)a.width * a.page_size + 2 * p.box + a.max_nodes + kKeys - 1) / kKeys;
-    const long long items = (long long)a.seqs * a.kv_heads * ((a.max_nodes * (a.heads / a.kv_heads) + sh.N - 1) / sh.N);
-    if (items * (tiles + item_cost(sh.N)) > INT32_MAX) return cudaErrorInvalidConfiguration;  // units are counted in 32 bits
+    const long long tiles = most_tiles(a), items = most_items(a, sh.N);
     p.whole = tiles <= kWholeTiles;
     if (p.whole) grid = (int)std::min<long long>(grid, items);
     p.by_rows = make_div(sh.N);

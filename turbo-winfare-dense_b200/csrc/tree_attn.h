@@ -26,6 +26,7 @@ struct TreeAttnArgs {
 };
 
 size_t tree_attn_workspace(int max_nodes, int heads, int kv_heads, int dim);
+bool tree_attn_countable(const TreeAttnArgs& a);  // whether 32 bits count the tiles of all sequences and heads
 cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st);
 int tree_attn_error();  // synchronizes; nonzero when a bounded wait gave up since the last call
 
