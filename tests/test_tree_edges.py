@@ -661,3 +661,12 @@ def test_refusal_of_too_many_tiles_says_why(built_lib):
                                     1 << 26, 1, 16, 16, 64, 0, 0, 1.0)
     assert L.g4b_tree_attention(args, None) != 0
     assert b"32 bits" in L.g4b_last_error() and b"n_seqs" in L.g4b_last_error()
+
+
+def test_head_counts_beyond_32_bits_are_refused(built_lib):
+    """A row's offset of heads * head_dim elements, and a group of max_nodes * heads rows, are 32-bit numbers."""
+    from g4dense_b200 import api
+    L = api.lib()
+    assert L.g4b_tree_attention_workspace(256, 1 << 14, 1 << 14, 512) > 0
+    assert L.g4b_tree_attention_workspace(1, 1 << 22, 1, 512) == 0
+    assert L.g4b_tree_attention_workspace(256, 1 << 23, 1, 64) == 0

@@ -299,7 +299,8 @@ int g4b_sample_token(const float* logits, int vocab, float temperature, float to
 
 size_t g4b_tree_attention_workspace(int max_nodes, int heads, int kv_heads, int head_dim) {
     if (max_nodes < 1 || max_nodes > 256 || kv_heads < 1 || heads < kv_heads || heads % kv_heads ||
-        (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512))
+        (head_dim != 64 && head_dim != 128 && head_dim != 256 && head_dim != 512) ||
+        (int64_t)heads * (head_dim > max_nodes ? head_dim : max_nodes) > INT32_MAX - 256)  // 32-bit offsets and rows
         return 0;
     return g4b::tree_attn_workspace(max_nodes, heads, kv_heads, head_dim);
 }
