@@ -384,18 +384,18 @@ __device__ __forceinline__ int commit_rows(const Commit& c, int s, int lane, Use
     const long long first = c.cu_nodes[s], nodes = c.cu_nodes[s + 1] - first;
     for (unsigned b = 0; b < n; b += 32) {
         const unsigned i = b + lane;
-        const long long pos = (long long)len + i, col = pos / c.page_size;
+        const unsigned pos = (unsigned)len + i, col = pos / (unsigned)c.page_size, row = pos - col * (unsigned)c.page_size;
         int node = -1, page = -1;
-        if (i < n && len >= 0) {
+        if (i < n && len >= 0) {  // so pos is below 2^32
             node = c.path ? c.path[(long long)s * c.path_width + i] : (int)i;
-            if (col < c.width) page = c.table[(long long)s * c.width + col];
+            if (col < (unsigned)c.width) page = c.table[(long long)s * c.width + col];
         }
         const bool good = node >= 0 && node < nodes && first >= 0 && first + node < c.n_tokens && page >= 0 && page < c.pages;
         const unsigned bad = ~__ballot_sync(0xffffffffu, good);
         const int m = bad ? __ffs(bad) - 1 : 32;
         for (int k = 0; k < m; ++k)
             use(first + __shfl_sync(0xffffffffu, node, k), __shfl_sync(0xffffffffu, page, k),
-                (int)(((long long)len + b + k) % c.page_size));
+                __shfl_sync(0xffffffffu, (int)row, k));
         if (bad) return (int)b + m;
     }
     return (int)n;
