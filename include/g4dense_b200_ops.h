@@ -103,7 +103,8 @@ G4B_API int g4b_qmat_info(const g4b_qmat* q, int* out4);
  *   g4b_pages_fork / _free / _compact / _copy   sharing, releasing and moving pages
  *
  * A round needs no host synchronization: lengths, counts and tables stay on the device. All calls
- * are asynchronous on `stream`, allocate nothing, and can be captured in a CUDA graph. Array
+ * are asynchronous on `stream`, a stream of the current device, on which all arrays have to be; they
+ * allocate nothing, and can be captured in a CUDA graph. Array
  * arguments are device memory; indices that a call finds out of range on the device are never
  * followed: what they name is skipped (in the attention, a page id out of range reads as zeros).
  * Calls that write a `status` word leave the state as it was when it is not 0. */

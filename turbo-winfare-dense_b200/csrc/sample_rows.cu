@@ -7,7 +7,8 @@
 // of them; of those, the ones before which less than top_p of their mass lies; of those, the ones
 // with exp((l_i - m) / T) >= min_p. With W the kept mass and r = floor(u W), the token is the first
 // kept entry in index order at which the running mass exceeds r. NaN and -inf are never kept, a
-// temperature <= 0 keeps the maximum alone, and a row without a finite entry (or +inf) gives -1.
+// temperature <= 0 (or NaN) keeps the maximum alone, and a row without a finite entry or +inf gives -1.
+// T may be anything else, infinite or tiny: differences that overflow fp32 count as infinite.
 // Whole-number weights make every sum exact, so the token does not depend on how the row is split
 // or in which order the parts are added.
 //
@@ -31,11 +32,13 @@
 // A top_k of up to 512 needs no histogram of all entries: the k-th largest of the threads' own maxima
 // bounds the k-th largest entry from below.
 //
-// The floor is one read of the logits; what bounds the kernel is the instructions and barriers per
-// entry behind it: about 15 for a top-k cut, 35 with an exponential for every entry, and three shared
-// atomics on top for a cut by mass. Measured on one B200, 128 rows of 262144 bf16 logits (10 us of
-// reading): 45 us greedy, 76 with top_k 40 and top_p 0.9, 100 with the temperature alone, 271 with
-// top_p 0.95 alone, 134 for a mix; one row of 4096: 10 us.
+// The floor is one read of the logits. What bounds the kernel behind it: for greedy rows and top-k cuts,
+// that a block brings its whole slice in, waits for it and then passes over it, two blocks an SM in
+// three and a half rounds that hardly overlap; with an exponential for every entry about 35
+// instructions an entry, and three shared atomics on top for a cut by mass. Measured on one B200, 128 rows of
+// 262144 bf16 logits (10 us of reading): 46 us greedy, 76 with top_k 40 and top_p 0.9, 101 with the
+// temperature alone, 272 with top_p 0.95 alone, 135 for a mix; fp16 a little less (44, 74, 100, 263, 132),
+// fp32 (21 us of reading) 90, 139, 157, 425 and 200; one row of 4096: 10 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

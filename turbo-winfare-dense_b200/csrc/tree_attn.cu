@@ -31,7 +31,11 @@
 //     hold the softmax in fp32, write P^T (rounded to the cache's type, 8 rows a store) and, when a
 //     row's score exceeds the maximum it last took by more than 8 (in powers of two), move the
 //     reference and rescale that row of O^T in TMEM. In between only a vote of the group is needed,
-//     so most tiles run without any reduction over keys; the sums are reduced once per part.
+//     so most tiles run without any reduction over keys; the sums are reduced once per part. P is one 16-bit
+//     number because both of the MMA's operands have V's type: a second term for the rest would double the
+//     P V products and P's shared memory, at 128 rows of 256 at the cost of one of the ring's three slots.
+//     The rounding adds at most u sum_j p_j |v_j|, of either sign, to an output that is itself rounded to u;
+//     the row sums take the unrounded numbers;
 // What a node must not see never reaches the MMA: scores are replaced, not added to, and in tiles
 // that hold hidden keys the softmax warps clean V before it is used: rows that no node sees are zeroed; an
 // infinity or NaN in a V row that some nodes see and others do not is taken out of the product and added

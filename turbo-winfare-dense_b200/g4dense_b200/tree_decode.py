@@ -10,8 +10,8 @@ attention, random weights); what it shows is the round:
     -> g4b_sample_rows for every node -> g4b_tree_accept -> g4b_pages_reserve -> g4b_pages_commit
 
 Prompts go through the same attention as chains of nodes; `fork` shares a prompt's pages between
-continuations, `finish` releases them. Nothing in a round waits for the device: the accepted tokens
-are read for the drafter, which here lives on the host, after the round is queued.
+continuations, `finish` releases them. The operators of a round wait for nothing on the host. This decoder
+does: its drafter lives there, so that every round uploads the trees and reads the accepted tokens back.
 """
 from __future__ import annotations
 
@@ -168,7 +168,7 @@ class Decoder:
         api.tree_accept(tokens, parents, drawn, cu, self.path, self.count, self.next)
         self._grow()
         self._commit(rows, cu, self.path)
-        # The host drafter's read; everything above was queued without one.
+        # The host drafter's read; no operator above needed one.
         count, path, nxt = self.count.tolist(), self.path.tolist(), self.next.tolist()
         self.check()
         self.held = [n + c for n, c in zip(self.held, count)]
